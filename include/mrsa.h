@@ -42,6 +42,7 @@ enum {
 };
 
 enum { MRSA_BF16 = 0, MRSA_F32 = 1 };                 /* cos/sin and score dtypes */
+enum { MRSA_F16 = 2 };                                /* with the two above: tensors of the rotary and paged ops */
 enum { MRSA_WEIGHTS_AFFINE = 0, MRSA_WEIGHTS_SOFTMAX = 1 };
 enum { MRSA_GEMM_PLAIN = 0, MRSA_GEMM_SWIGLU = 1, MRSA_GEMM_RESIDUAL = 2 };   /* mrsa_gemm_bf16 epilogues */
 
@@ -421,6 +422,114 @@ int mrsa_probe_tile_gather(const void* k, const void* v, const void* q, int64_t 
  * Replaces ops/hils_bidir_output_fusion_tilelang.py:138 fuse_hils_outputs. */
 int mrsa_fuse_outputs(const void* remote, const void* local, const void* local_w, void* out,
                       int64_t rows, int64_t head_dim, mrsa_stream_t stream);
+
+/* ------------------------------------------------- rotary positions and pages
+ * These operators have no counterpart in the reference.  They take any of the
+ * types named at them, tensors with any strides but a contiguous last
+ * dimension, and argument structs instead of long lists. */
+
+typedef struct {
+  const void* q;              /* [batch, len, q_heads, head_dim]; may be NULL with q_heads = 0 */
+  void* q_out;                /* [batch, len, q_heads, head_dim], contiguous */
+  const void* k;              /* [batch, len, k_heads, head_dim]; may be NULL with k_heads = 0 (mrsa_rotary) */
+  void* k_out;                /* contiguous; unused by mrsa_paged_append */
+  const int64_t* position_ids;/* [batch, len], contiguous */
+  const float* inv_freq;      /* [pairs] */
+  int64_t q_batch_stride, q_token_stride, q_head_stride;   /* in elements */
+  int64_t k_batch_stride, k_token_stride, k_head_stride;
+  int64_t batch, len, q_heads, k_heads, head_dim;
+  int64_t pairs;              /* the first 2 * pairs dims of a head turn; at most 128 */
+  float attention_factor;     /* cos and sin are multiplied by it */
+  int32_t dtype;              /* MRSA_BF16, MRSA_F16 or MRSA_F32 */
+  int32_t interleaved;        /* 0: pairs (i, i + pairs); 1: pairs (2i, 2i + 1) */
+  int32_t inverse;            /* 1: by minus the angle (the gradient) */
+} mrsa_rotary_args;
+
+/* Rotary positions of q and k: the angle is the fp32 product
+ * position * inv_freq, as in mrsa_rope; fp32 arithmetic, one rounding. */
+int mrsa_rotary(const mrsa_rotary_args* a, mrsa_stream_t stream);
+
+/* Bits of a page table's status word (the bits of a call are or-ed in). */
+enum {
+  MRSA_PAGE_BAD_SEQUENCE = 1,  /* a sequence number out of range, or twice in one call */
+  MRSA_PAGE_NO_PAGES = 2,      /* the pool has not enough free pages */
+  MRSA_PAGE_TOO_LONG = 4,      /* a sequence would outgrow its table row, or its length was negative */
+  MRSA_PAGE_OUTSIDE = 8,       /* a token outside its sequence, or a page number out of range */
+  MRSA_PAGE_SHARED = 16        /* a write to a page that several sequences hold */
+};
+#define MRSA_PAGE_MAX_SEQS 1024   /* sequences per call of the page operators */
+
+typedef struct {
+  int32_t* table;             /* [max_seqs, max_pages] page numbers, -1: none */
+  int32_t* lengths;           /* [max_seqs] tokens */
+  int32_t* refcount;          /* [pages] sequences that hold each page; 0: free */
+  int32_t* status;            /* [1] or NULL */
+  int64_t max_seqs, max_pages, pages;
+  int64_t page_size;          /* 16, 32, 64, 128 or 256 tokens */
+} mrsa_page_table;
+
+/* A pool of pages: `layers` x 2 (keys, values) planes of table->pages pages,
+ * each page one contiguous block of page_size tokens x heads x row_bytes
+ * (tokens outside or heads outside).  Strides in bytes; everything 16-byte
+ * aligned. */
+typedef struct {
+  void* data;
+  int64_t layers;
+  int64_t layer_stride, kv_stride, page_stride, token_stride, head_stride;
+  int64_t heads, row_bytes;
+} mrsa_page_pool;
+
+typedef struct {
+  void* k_pages;              /* [pages, page_size, k_heads, head_dim] */
+  void* v_pages;
+  const void* v;              /* [batch, len, k_heads, head_dim] */
+  const int32_t* seqs;        /* [batch] */
+  const int32_t* start;       /* [batch] cache position of the first token; NULL: the sequence's last len */
+  int64_t k_page_stride, k_slot_stride, k_head_stride;     /* in elements */
+  int64_t v_page_stride, v_slot_stride, vp_head_stride;
+  int64_t v_batch_stride, v_token_stride, v_head_stride;
+  int32_t check_shared;       /* 1: a write to a page with refcount > 1 is refused and reported */
+} mrsa_paged_append_args;
+
+/* q and k turned as in mrsa_rotary (position_ids NULL: the cache positions;
+ * pairs 0: not turned), q to q_out, k and v into their sequences' pages.  A
+ * token that has no page is reported in the status word and not written. */
+int mrsa_paged_append(const mrsa_rotary_args* r, const mrsa_page_table* t, const mrsa_paged_append_args* p,
+                      mrsa_stream_t stream);
+
+/* Device workspace of the page operators below for n sequences. */
+size_t mrsa_page_workspace(const mrsa_page_table* t, int64_t n);
+
+/* The sequences seqs [n] give up their pages: rows -1, lengths 0.  A sequence
+ * number out of range or given twice is reported, and nothing is done. */
+int mrsa_page_free(const mrsa_page_table* t, const int32_t* seqs, int64_t n, mrsa_stream_t stream);
+
+/* Sequence seqs[i] grows by tokens[i] (tokens NULL: by all) tokens, on the
+ * lowest free pages in the order of seqs and positions.  All or nothing: if
+ * one does not fit, that is reported and none grows. */
+int mrsa_page_extend(const mrsa_page_table* t, const int32_t* seqs, const int32_t* tokens, int64_t all, int64_t n,
+                     void* workspace, size_t ws_bytes, mrsa_stream_t stream);
+
+/* Sequence dst[i] gives up its pages and becomes src[i]: whole pages below
+ * min(share[i], length) tokens (share NULL: length) are held in common, the
+ * others are copied, in every plane, to the lowest free pages.  dst are
+ * distinct and none is a src.  If the pool does not hold the copies, that is
+ * reported and every dst is left empty. */
+int mrsa_page_fork(const mrsa_page_table* t, const mrsa_page_pool* pool, const int32_t* src, const int32_t* dst,
+                   const int32_t* share, int64_t n, void* workspace, size_t ws_bytes, mrsa_stream_t stream);
+
+/* Sequence seqs[i] keeps the tokens whose keep[i][position] (uint8, [n,
+ * max_pages * page_size], contiguous, 16-byte aligned) is not zero, in order.
+ * Its pages before the first dropped token stay; the kept tokens after them
+ * are gathered, in every plane, into the lowest pages that were free before
+ * the call, and the old pages are given up.  All or nothing as in extend. */
+int mrsa_page_compact(const mrsa_page_table* t, const mrsa_page_pool* pool, const int32_t* seqs, const uint8_t* keep,
+                      int64_t n, void* workspace, size_t ws_bytes, mrsa_stream_t stream);
+
+/* Page src[i] copied to page dst[i] in every plane (i < n); a page number out
+ * of range is reported and skipped.  dst are distinct and none is a src. */
+int mrsa_page_copy(const mrsa_page_table* t, const mrsa_page_pool* pool, const int32_t* src, const int32_t* dst,
+                   int64_t n, mrsa_stream_t stream);
 
 /* ---------------------------------------------------------------- layers */
 typedef struct {

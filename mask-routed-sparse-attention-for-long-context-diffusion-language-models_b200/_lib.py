@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 
 import torch
 
@@ -15,7 +16,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libmrsa_b200.so")
 
 ERR_NULL, ERR_SHAPE, ERR_ALIGN, ERR_LAUNCH, ERR_ARG, ERR_WORKSPACE = -1, -2, -3, -4, -5, -6
-BF16, F32 = 0, 1
+BF16, F32, F16 = 0, 1, 2
 WEIGHTS_AFFINE, WEIGHTS_SOFTMAX = 0, 1
 GEMM_PLAIN, GEMM_SWIGLU, GEMM_RESIDUAL = 0, 1, 2
 
@@ -77,6 +78,14 @@ _SIGS = {
     "mrsa_local_attention_backward": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _i64, _int,
                                       _i64, _f32, _i64, _i64, _i64, _i64, _i64, _vp],
     "mrsa_local_attention_backward_workspace": [_i64, _i64, _i64],
+    "mrsa_rotary": [_vp, _vp],
+    "mrsa_paged_append": [_vp, _vp, _vp, _vp],
+    "mrsa_page_workspace": [_vp, _i64],
+    "mrsa_page_free": [_vp, _vp, _i64, _vp],
+    "mrsa_page_extend": [_vp, _vp, _vp, _i64, _i64, _vp, _sz, _vp],
+    "mrsa_page_fork": [_vp, _vp, _vp, _vp, _vp, _i64, _vp, _sz, _vp],
+    "mrsa_page_compact": [_vp, _vp, _vp, _vp, _i64, _vp, _sz, _vp],
+    "mrsa_page_copy": [_vp, _vp, _vp, _vp, _i64, _vp],
     "mrsa_device_error_flags": [_int],
     "mrsa_wait_selftest": [_vp, _int, _vp],
     "mrsa_route_layer_workspace_size": [_vp],
@@ -86,7 +95,7 @@ _SIGS = {
 _RESTYPE = {"mrsa_strerror": C.c_char_p, "mrsa_last_error": C.c_char_p, "mrsa_route_layer_workspace_size": _sz,
             "mrsa_route_topk_workspace_size": _sz, "mrsa_selected_token_attention_smem": _sz,
             "mrsa_selected_attention_backward_workspace": _sz, "mrsa_route_scores_backward_workspace": _sz,
-            "mrsa_local_attention_backward_workspace": _sz}
+            "mrsa_local_attention_backward_workspace": _sz, "mrsa_page_workspace": _sz}
 
 EXPORTED = tuple(_SIGS)
 
@@ -131,6 +140,21 @@ def ptr(t: torch.Tensor | None):
 
 def stream_of(t: torch.Tensor):
     return C.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+
+
+def raw_stream(device: torch.device) -> int:
+    """Handle of the device's current stream."""
+    return torch._C._cuda_getCurrentRawStream(device.index if device.index is not None else
+                                              torch.cuda.current_device())
+
+
+# The argument structs of the rotary and paged operators, packed as bytes: a
+# call then converts two or three pointers instead of thirty arguments (about
+# 1 us instead of 6 us, which counts where a step is a few microseconds long).
+ROTARY_ARGS = struct.Struct("@6P6q6qf3i")            # mrsa_rotary_args
+PAGE_TABLE = struct.Struct("@4P4q")                  # mrsa_page_table
+PAGE_POOL = struct.Struct("@P8q")                    # mrsa_page_pool
+APPEND_ARGS = struct.Struct("@5P9qi4x")              # mrsa_paged_append_args
 
 
 def call(name: str, *args):
