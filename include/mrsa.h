@@ -531,6 +531,35 @@ int mrsa_page_compact(const mrsa_page_table* t, const mrsa_page_pool* pool, cons
 int mrsa_page_copy(const mrsa_page_table* t, const mrsa_page_pool* pool, const int32_t* src, const int32_t* dst,
                    int64_t n, mrsa_stream_t stream);
 
+typedef struct {
+  const void* q;              /* [batch, len, q_heads, head_dim] */
+  const void* k_pages;        /* [pages, page_size, kv_heads, head_dim] */
+  const void* v_pages;
+  void* out;                  /* [batch, len, q_heads, head_dim], contiguous */
+  float* lse;                 /* [batch, len, q_heads] natural log, or NULL */
+  const uint8_t* key_valid;   /* [batch, max_pages * page_size], 0: token masked; NULL: none is */
+  const int32_t* seqs;        /* [batch] */
+  int64_t q_batch_stride, q_token_stride, q_head_stride;   /* in elements, multiples of 8 */
+  int64_t k_page_stride, k_slot_stride, k_head_stride;
+  int64_t v_page_stride, v_slot_stride, v_head_stride;
+  int64_t batch, len, q_heads, kv_heads, head_dim;         /* head_dim 64 or 128 */
+  float scale;
+  int32_t dtype;              /* MRSA_BF16 or MRSA_F16 */
+  int32_t causal;             /* 1: query i sees positions up to length - len + i; 0: the whole sequence */
+} mrsa_paged_attention_args;
+
+/* Device workspace of mrsa_paged_attention. */
+size_t mrsa_paged_attention_workspace(const mrsa_paged_attention_args* a);
+
+/* Attention of len query tokens per sequence over its cached tokens, read
+ * from their pages; the query tokens' own keys are in the cache already.
+ * Masked tokens, and slots past a sequence's length, may hold anything (NaN
+ * included).  A query that sees no token gets zeros and an lse of -inf.  A
+ * bad sequence or page number is reported in the status word and reads as no
+ * tokens. */
+int mrsa_paged_attention(const mrsa_paged_attention_args* a, const mrsa_page_table* t, void* workspace,
+                         size_t ws_bytes, mrsa_stream_t stream);
+
 /* ---------------------------------------------------------------- layers */
 typedef struct {
   /* inputs (device) */

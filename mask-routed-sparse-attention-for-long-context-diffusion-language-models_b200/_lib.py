@@ -86,6 +86,8 @@ _SIGS = {
     "mrsa_page_fork": [_vp, _vp, _vp, _vp, _vp, _i64, _vp, _sz, _vp],
     "mrsa_page_compact": [_vp, _vp, _vp, _vp, _i64, _vp, _sz, _vp],
     "mrsa_page_copy": [_vp, _vp, _vp, _vp, _i64, _vp],
+    "mrsa_paged_attention_workspace": [_vp],
+    "mrsa_paged_attention": [_vp, _vp, _vp, _sz, _vp],
     "mrsa_device_error_flags": [_int],
     "mrsa_wait_selftest": [_vp, _int, _vp],
     "mrsa_route_layer_workspace_size": [_vp],
@@ -95,7 +97,8 @@ _SIGS = {
 _RESTYPE = {"mrsa_strerror": C.c_char_p, "mrsa_last_error": C.c_char_p, "mrsa_route_layer_workspace_size": _sz,
             "mrsa_route_topk_workspace_size": _sz, "mrsa_selected_token_attention_smem": _sz,
             "mrsa_selected_attention_backward_workspace": _sz, "mrsa_route_scores_backward_workspace": _sz,
-            "mrsa_local_attention_backward_workspace": _sz, "mrsa_page_workspace": _sz}
+            "mrsa_local_attention_backward_workspace": _sz, "mrsa_page_workspace": _sz,
+            "mrsa_paged_attention_workspace": _sz}
 
 EXPORTED = tuple(_SIGS)
 
@@ -154,6 +157,7 @@ def raw_stream(device: torch.device) -> int:
 ROTARY_ARGS = struct.Struct("@6P6q6qf3i")            # mrsa_rotary_args
 PAGE_TABLE = struct.Struct("@4P4q")                  # mrsa_page_table
 PAGE_POOL = struct.Struct("@P8q")                    # mrsa_page_pool
+PAGED_ATTENTION_ARGS = struct.Struct("@7P14qf2i4x")  # mrsa_paged_attention_args
 APPEND_ARGS = struct.Struct("@5P9qi4x")              # mrsa_paged_append_args
 
 

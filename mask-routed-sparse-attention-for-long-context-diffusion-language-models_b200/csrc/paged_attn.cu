@@ -1,0 +1,601 @@
+// Attention over a paged key-value cache: few query rows per KV head (one new
+// token of each sequence, above all), split over the cache's length.
+//
+//   o = softmax(scale q K^T) V,  lse = ln sum exp(scale q k)
+//
+// over a sequence's cached tokens (masked tokens and, when causal, tokens past
+// the query's own position have weight zero; a row that sees nothing gets
+// zeros and -inf).  With R query rows per KV head a key's 4 D bytes (K and V)
+// meet 4 D R products and sums: R flops per byte, so up to some 40 rows the
+// cache's bytes bound it.
+//
+// Four warps per CTA, each on 16 keys of a 64-key tile, as if alone: its own
+// ring of cp.async stages, its own running maximum, sum and output, no barrier
+// until a unit ends.  16 keys lie in one page whatever its size, so a warp
+// looks up one page per tile, one tile ahead.  The products run with the keys
+// as the long side of the MMA: S^T = K Q^T (16 keys x 8 rows a step), and O^T
+// += V^T P^T, so a group of 7 heads wastes one column in eight, where the
+// usual order would waste nine rows in sixteen.  P^T gets from accumulator to
+// operand layout by transposing 8 x 8 blocks in registers.  P enters as a high
+// and a low 16-bit part (16 bits of it count): the second product costs
+// nothing where bytes bound, and the output is then as exact as its rounding.
+#include "paged_attn.cuh"
+
+#include <cuda_fp16.h>
+
+using namespace mrsa;
+
+namespace {
+
+using paged::Args;
+
+constexpr int A_WARPS = 4, A_THREADS = 32 * A_WARPS;
+constexpr int A_KEYS = 16;                  // keys per warp and tile
+constexpr int A_TILE = A_KEYS * A_WARPS;    // keys per tile
+constexpr int A_STAGES = 3;
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
+  return y;
+}
+
+template <bool kF16> __device__ __forceinline__ void mma(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  if constexpr (kF16) mma_f16(c, a, b0, b1);
+  else mma_bf16(c, a, b0, b1);
+}
+
+// (x, y) as a pair of 16-bit values, and what the pair leaves over.
+template <bool kF16> __device__ __forceinline__ uint32_t split_pair(float x, float y, uint32_t& low) {
+  if constexpr (kF16) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+    low = *reinterpret_cast<const uint32_t*>(&l);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const uint32_t h = pack_bf16x2(x, y);
+    const float2 f = unpack_bf16x2(h);
+    low = pack_bf16x2(x - f.x, y - f.y);
+    return h;
+  }
+}
+
+template <bool kF16> __device__ __forceinline__ void store_out(char* p, float v) {
+  if constexpr (kF16) *reinterpret_cast<__half*>(p) = __float2half_rn(v);
+  else *reinterpret_cast<__nv_bfloat16*>(p) = f2bf(v);
+}
+
+template <int kD, int kNT>
+struct TokenSmem {
+  // a warp's ring: [stage][K, V][16 keys][kD], 16-byte pieces swizzled by key;
+  // its start holds the warp's output rows when a unit ends
+  alignas(128) unsigned char ring[A_WARPS][A_STAGES][2][A_KEYS * kD * 2];
+  uint32_t mask[A_WARPS][A_STAGES];        // keys of the stage that count
+  float m[A_WARPS][8 * kNT], l[A_WARPS][8 * kNT];
+  int prefix[paged::kMaxBatch + 1];
+  int warp_sums[A_WARPS];
+  int64_t total;
+};
+
+template <int kD, int kNT, bool kF16>
+__global__ void __launch_bounds__(A_THREADS) paged_token_kernel(const __grid_constant__ Args a) {
+  extern __shared__ __align__(128) unsigned char smem_raw[];
+  auto& sm = *reinterpret_cast<TokenSmem<kD, kNT>*>(smem_raw);
+  constexpr int kRows = 8 * kNT;
+  constexpr int kPieces = kD / 8;          // 16-byte pieces of a key
+  constexpr int kSteps = kD / 16;
+  constexpr int kRowBytes = kD * 2;
+  static_assert(A_STAGES * 2 * A_KEYS * kRowBytes >= kRows * kD * 4, "a warp's output rows must fit its ring");
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+
+  // ---- tiles before each batch row (per head and row tile)
+  {
+    int run = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += A_THREADS) {
+      const int b = b0 + tid;
+      const int t = b < a.batch ? (paged::cached_tokens(a, b) + A_TILE - 1) / A_TILE : 0;
+      int x = t;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      if (lane == 31) sm.warp_sums[warp] = x;
+      __syncthreads();
+      int before = run;
+#pragma unroll
+      for (int w = 0; w < A_WARPS; ++w) {
+        if (w < warp) before += sm.warp_sums[w];
+        run += sm.warp_sums[w];
+      }
+      if (b < a.batch) sm.prefix[b] = before + x - t;
+      __syncthreads();
+    }
+    if (tid == 0) sm.prefix[a.batch] = run;
+    __syncthreads();
+  }
+  if (blockIdx.x == 0)
+    for (int i = tid; i <= a.batch; i += A_THREADS) a.prefix[i] = sm.prefix[i];
+  const int per = a.kv_heads * a.row_tiles;            // units per batch row
+  const int64_t total = static_cast<int64_t>(sm.prefix[a.batch]) * per;
+  const int64_t grid = paged::dealt(a, total);
+  const int64_t t_begin = blockIdx.x < grid ? paged::stretch(blockIdx.x, total, grid) : 0;
+  const int64_t t_end = blockIdx.x < grid ? paged::stretch(blockIdx.x + 1, total, grid) : 0;
+
+  for (int64_t t_now = t_begin; t_now < t_end;) {
+    // ---- the unit that holds tile t_now: the last batch row whose tiles begin at or before it
+    int lo = 0, hi = a.batch - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (static_cast<int64_t>(sm.prefix[mid]) * per <= t_now) lo = mid; else hi = mid - 1;
+    }
+    const int b = lo;
+    const int tiles = sm.prefix[b + 1] - sm.prefix[b];
+    const int64_t in_row = t_now - static_cast<int64_t>(sm.prefix[b]) * per;
+    const int unit = static_cast<int>(in_row / tiles);
+    const int tile0 = static_cast<int>(in_row - static_cast<int64_t>(unit) * tiles);
+    const int64_t room = t_end - t_now;
+    const int tile1 = room < tiles - tile0 ? tile0 + static_cast<int>(room) : tiles;
+    const int h = unit / a.row_tiles, rt = unit - h * a.row_tiles;
+    const int seq = a.seqs[b];
+    const int n = a.lengths[seq];
+    const int r0 = rt * kRows;
+    const int nrows = a.rows - r0 < kRows ? a.rows - r0 : kRows;
+
+    // ---- this thread's part of Q^T: column lane / 4 of each 8-row block
+    uint32_t qf[kNT][kSteps][2];
+#pragma unroll
+    for (int nt = 0; nt < kNT; ++nt) {
+      const int r = r0 + nt * 8 + (lane >> 2);
+      const bool ok = r < a.rows;
+      const int i = ok ? r / a.group : 0, g = ok ? r - i * a.group : 0;
+      const char* q = a.q + b * a.qb + i * a.qt + (h * a.group + g) * a.qh + (lane & 3) * 4;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        qf[nt][s][0] = ok ? *reinterpret_cast<const uint32_t*>(q + s * 32) : 0u;
+        qf[nt][s][1] = ok ? *reinterpret_cast<const uint32_t*>(q + s * 32 + 16) : 0u;
+      }
+    }
+    // the last key that this thread's two rows of each block may see
+    int last[kNT][2];
+#pragma unroll
+    for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = r0 + nt * 8 + (lane & 3) * 2 + e;
+        last[nt][e] = a.causal ? n - a.len + r / a.group : n - 1;
+      }
+
+    float o[kSteps][kNT][4], m[kNT][2], l[kNT][2];
+#pragma unroll
+    for (int nt = 0; nt < kNT; ++nt) {
+      m[nt][0] = m[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+      for (int d = 0; d < kSteps; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[d][nt][e] = 0.f;
+    }
+
+    // ---- the warp's stream of 16-key pieces; what a copy needs is fetched one tile ahead
+    const int32_t* row_pages = a.table + static_cast<int64_t>(seq) * a.max_pages;
+    const uint8_t* valid = a.valid != nullptr ? a.valid + static_cast<int64_t>(b) * a.max_pages * a.page_size : nullptr;
+    auto fetch = [&](int t, int& page, uint4& vb) {
+      const int key0 = t * A_TILE + warp * A_KEYS;
+      page = -1;
+      vb = make_uint4(~0u, ~0u, ~0u, ~0u);
+      if (t < tile1 && key0 < n) {
+        page = row_pages[key0 >> a.page_shift];
+        if (valid != nullptr) vb = *reinterpret_cast<const uint4*>(valid + key0);
+      }
+    };
+    auto copy = [&](int t, int page, const uint4& vb) {
+      const int st = (t - tile0) % A_STAGES;
+      const int key0 = t * A_TILE + warp * A_KEYS;
+      if (t < tile1 && key0 < n) {
+        uint32_t mask = n - key0 >= 16 ? 0xffffu : (1u << (n - key0)) - 1u;
+        if (valid != nullptr) {
+          const uint32_t w[4] = {vb.x, vb.y, vb.z, vb.w};
+          uint32_t keep = 0;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) keep |= ((w[i >> 2] >> (8 * (i & 3))) & 0xffu) ? 1u << i : 0u;
+          mask &= keep;
+        }
+        if (page < 0 || page >= a.pages) {
+          if (lane == 0) report(a.status, MRSA_PAGE_OUTSIDE);
+          mask = 0;
+          page = 0;
+        }
+        // keys that do not count are filled with zeros: what their slots hold may not be a number
+        const int slot = key0 & (a.page_size - 1);
+        const char* k = a.k + page * a.kp + slot * a.ks + h * a.kh;
+        const char* v = a.v + page * a.vp + slot * a.vs + h * a.vh;
+        const int piece = lane % kPieces;
+#pragma unroll
+        for (int i = 0; i < A_KEYS * kPieces / 32; ++i) {
+          const int key = i * (32 / kPieces) + lane / kPieces;
+          const int at = key * kRowBytes + ((piece ^ (key & 7)) * 16);
+          const bool on = (mask >> key) & 1u;
+          cp_async16_zfill(&sm.ring[warp][st][0][at], k + (on ? key : 0) * a.ks + piece * 16, on);
+          cp_async16_zfill(&sm.ring[warp][st][1][at], v + (on ? key : 0) * a.vs + piece * 16, on);
+        }
+        if (lane == 0) sm.mask[warp][st] = mask;
+      } else if (lane == 0) {
+        sm.mask[warp][st] = 0;
+      }
+      cp_async_commit();
+    };
+    int page_next;
+    uint4 valid_next;
+#pragma unroll
+    for (int s = 0; s < A_STAGES - 1; ++s) {
+      fetch(tile0 + s, page_next, valid_next);
+      copy(tile0 + s, page_next, valid_next);
+    }
+    fetch(tile0 + A_STAGES - 1, page_next, valid_next);
+
+    for (int t = tile0; t < tile1; ++t) {
+      const int st = (t - tile0) % A_STAGES;
+      cp_async_wait<A_STAGES - 2>();
+      __syncwarp();          // every lane's copies of this stage are in, and its reads of the last one done
+      {
+        const int page = page_next;
+        const uint4 vb = valid_next;
+        fetch(t + A_STAGES, page_next, valid_next);
+        copy(t + A_STAGES - 1, page, vb);
+      }
+      const uint32_t mask = sm.mask[warp][st];
+      if (mask == 0) continue;
+      const unsigned char* ksm = sm.ring[warp][st][0];
+      const unsigned char* vsm = sm.ring[warp][st][1];
+      float s[kNT][4];
+#pragma unroll
+      for (int nt = 0; nt < kNT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < kSteps; ++kk) {
+        uint32_t f[4];
+        const int key = lane & 15, piece = kk * 2 + (lane >> 4);
+        ldsm_x4(f[0], f[1], f[2], f[3], ksm + key * kRowBytes + ((piece ^ (key & 7)) * 16));
+#pragma unroll
+        for (int nt = 0; nt < kNT; ++nt) mma<kF16>(s[nt], f, qf[nt][kk][0], qf[nt][kk][1]);
+      }
+      const int key0 = t * A_TILE + warp * A_KEYS;
+      const bool on0 = (mask >> (lane >> 2)) & 1u, on1 = (mask >> ((lane >> 2) + 8)) & 1u;
+      const int at0 = key0 + (lane >> 2), at1 = at0 + 8;
+      uint32_t ph[kNT][2], pl[kNT][2];
+#pragma unroll
+      for (int nt = 0; nt < kNT; ++nt) {
+        float x[4];
+        x[0] = on0 && at0 <= last[nt][0] ? s[nt][0] * a.scale_log2 : -INFINITY;
+        x[1] = on0 && at0 <= last[nt][1] ? s[nt][1] * a.scale_log2 : -INFINITY;
+        x[2] = on1 && at1 <= last[nt][0] ? s[nt][2] * a.scale_log2 : -INFINITY;
+        x[3] = on1 && at1 <= last[nt][1] ? s[nt][3] * a.scale_log2 : -INFINITY;
+        float top[2] = {fmaxf(x[0], x[2]), fmaxf(x[1], x[3])};
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+          for (int w = 4; w < 32; w <<= 1) top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], w));
+        }
+        // the reference moves, and the output is scaled, only for a maximum 2^8 above it
+        if (__any_sync(0xffffffffu, top[0] > m[nt][0] + 8.f || top[1] > m[nt][1] + 8.f)) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            if (top[e] > m[nt][e] + 8.f) {
+              const float c = m[nt][e] == -INFINITY ? 0.f : fast_exp2(m[nt][e] - top[e]);
+              m[nt][e] = top[e];
+              l[nt][e] *= c;
+#pragma unroll
+              for (int d = 0; d < kSteps; ++d) {
+                o[d][nt][e] *= c;
+                o[d][nt][e + 2] *= c;
+              }
+            }
+          }
+        }
+        float p[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float ref = m[nt][e & 1];
+          p[e] = ref == -INFINITY ? 0.f : fast_exp2(x[e] - ref);
+          l[nt][e & 1] += p[e];
+        }
+        uint32_t lo0, lo1;
+        const uint32_t hi0 = split_pair<kF16>(p[0], p[1], lo0), hi1 = split_pair<kF16>(p[2], p[3], lo1);
+        ph[nt][0] = transpose8x8(hi0);
+        ph[nt][1] = transpose8x8(hi1);
+        pl[nt][0] = transpose8x8(lo0);
+        pl[nt][1] = transpose8x8(lo1);
+      }
+#pragma unroll
+      for (int d = 0; d < kSteps; ++d) {
+        uint32_t f[4];
+        const int key = (lane & 7) + (lane >> 4) * 8, piece = d * 2 + ((lane >> 3) & 1);
+        ldsm_x4_t(f[0], f[1], f[2], f[3], vsm + key * kRowBytes + ((piece ^ (key & 7)) * 16));
+#pragma unroll
+        for (int nt = 0; nt < kNT; ++nt) {
+          mma<kF16>(o[d][nt], f, ph[nt][0], ph[nt][1]);
+          mma<kF16>(o[d][nt], f, pl[nt][0], pl[nt][1]);
+        }
+      }
+    }
+
+    // ---- the warps' rows joined: each leaves its own in its ring, which its copies no longer use
+    cp_async_wait<0>();
+    __syncwarp();
+    float* own = reinterpret_cast<float*>(sm.ring[warp][0][0]);
+#pragma unroll
+    for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float sum = l[nt][e];
+#pragma unroll
+        for (int w = 4; w < 32; w <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+        const int r = nt * 8 + (lane & 3) * 2 + e;
+        if (lane < 4) {
+          sm.m[warp][r] = m[nt][e];
+          sm.l[warp][r] = sum;
+        }
+#pragma unroll
+        for (int d = 0; d < kSteps; ++d) {
+          own[r * kD + d * 16 + (lane >> 2)] = o[d][nt][e];
+          own[r * kD + d * 16 + 8 + (lane >> 2)] = o[d][nt][e + 2];
+        }
+      }
+    __syncthreads();
+    const bool whole = tile0 == 0 && tile1 == tiles;
+    const int slot = 2 * blockIdx.x + (t_now == t_begin ? 0 : 1);
+    for (int e = tid; e < nrows * kD; e += A_THREADS) {
+      const int r = e / kD, d = e - r * kD;
+      float top = sm.m[0][r];
+#pragma unroll
+      for (int w = 1; w < A_WARPS; ++w) top = fmaxf(top, sm.m[w][r]);
+      float sum = 0.f, acc = 0.f;
+#pragma unroll
+      for (int w = 0; w < A_WARPS; ++w) {
+        const float c = sm.m[w][r] == -INFINITY ? 0.f : fast_exp2(sm.m[w][r] - top);
+        sum += c * sm.l[w][r];
+        acc += c * reinterpret_cast<const float*>(sm.ring[w][0][0])[r * kD + d];
+      }
+      if (whole) {
+        const int i = (r0 + r) / a.group, g = (r0 + r) - i * a.group;
+        const int64_t at = (static_cast<int64_t>(b) * a.len + i) * a.q_heads + h * a.group + g;
+        store_out<kF16>(a.out + (at * kD + d) * 2, sum > 0.f ? acc / sum : 0.f);
+        if (d == 0 && a.lse != nullptr) a.lse[at] = sum > 0.f ? (top + log2f(sum)) * kLn2 : -INFINITY;
+      } else {
+        a.part_o[(static_cast<int64_t>(slot) * a.row_tile + r) * kD + d] = acc;
+        if (d == 0) {
+          float* ml = a.part_ml + (static_cast<int64_t>(slot) * a.row_tile + r) * 2;
+          ml[0] = top;
+          ml[1] = sum;
+        }
+      }
+    }
+    __syncthreads();
+    t_now += tile1 - tile0;
+  }
+}
+
+// One block per (batch row, KV head, query row): nothing to do for a unit that
+// one CTA finished, zeros for one without keys, else its pieces joined, eight
+// warps on every eighth piece.
+constexpr int J_WARPS = 8;
+
+template <int kD, bool kF16>
+__global__ void __launch_bounds__(32 * J_WARPS) paged_join_kernel(const __grid_constant__ Args a) {
+  constexpr int kV = kD / 32;
+  __shared__ float acc_s[J_WARPS][kD], m_s[J_WARPS], l_s[J_WARPS];
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int r = blockIdx.x % a.rows, bh = blockIdx.x / a.rows, h = bh % a.kv_heads, b = bh / a.kv_heads;
+  const int per = a.kv_heads * a.row_tiles;
+  const int p0 = a.prefix[b], tiles = a.prefix[b + 1] - p0;
+  const int64_t total = static_cast<int64_t>(a.prefix[a.batch]) * per;
+  const int rt = r / a.row_tile, rr = r - rt * a.row_tile;
+  const int i = r / a.group, g = r - i * a.group;
+  const int64_t at = (static_cast<int64_t>(b) * a.len + i) * a.q_heads + h * a.group + g;
+  if (tiles == 0) {
+    for (int d = threadIdx.x; d < kD; d += 32 * J_WARPS) store_out<kF16>(a.out + (at * kD + d) * 2, 0.f);
+    if (threadIdx.x == 0 && a.lse != nullptr) a.lse[at] = -INFINITY;
+    return;
+  }
+  const int64_t first = static_cast<int64_t>(p0) * per + static_cast<int64_t>(h * a.row_tiles + rt) * tiles;
+  const int64_t grid = paged::dealt(a, total);
+  const int c0 = paged::holder(first, total, grid), c1 = paged::holder(first + tiles - 1, total, grid);
+  if (c0 == c1) return;
+  float m = -INFINITY, l = 0.f, acc[kV];
+#pragma unroll
+  for (int e = 0; e < kV; ++e) acc[e] = 0.f;
+#pragma unroll 4
+  for (int c = c0 + warp; c <= c1; c += J_WARPS) {
+    const int64_t slot = paged::slot_of(c, c0, first, total, grid);
+    const float* ml = a.part_ml + (slot * a.row_tile + rr) * 2;
+    const float* o = a.part_o + (slot * a.row_tile + rr) * kD + lane * kV;
+    const float pm = ml[0], pl = ml[1];
+    float x[kV];
+#pragma unroll
+    for (int e = 0; e < kV; ++e) x[e] = o[e];
+    const float top = fmaxf(m, pm);
+    const float cm = m == -INFINITY ? 0.f : fast_exp2(m - top), cp = pm == -INFINITY ? 0.f : fast_exp2(pm - top);
+    m = top;
+    l = l * cm + pl * cp;
+#pragma unroll
+    for (int e = 0; e < kV; ++e) acc[e] = acc[e] * cm + x[e] * cp;
+  }
+#pragma unroll
+  for (int e = 0; e < kV; ++e) acc_s[warp][lane * kV + e] = acc[e];
+  if (lane == 0) {
+    m_s[warp] = m;
+    l_s[warp] = l;
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < kD; d += 32 * J_WARPS) {
+    float top = m_s[0];
+#pragma unroll
+    for (int w = 1; w < J_WARPS; ++w) top = fmaxf(top, m_s[w]);
+    float sum = 0.f, v = 0.f;
+#pragma unroll
+    for (int w = 0; w < J_WARPS; ++w) {
+      const float c = m_s[w] == -INFINITY ? 0.f : fast_exp2(m_s[w] - top);
+      sum += c * l_s[w];
+      v += c * acc_s[w][d];
+    }
+    store_out<kF16>(a.out + (at * kD + d) * 2, sum > 0.f ? v / sum : 0.f);
+    if (d == 0 && a.lse != nullptr) a.lse[at] = sum > 0.f ? (top + log2f(sum)) * kLn2 : -INFINITY;
+  }
+}
+
+template <int kD, int kNT, bool kF16>
+int launch_token(const Args& a, cudaStream_t s) {
+  const auto kernel = paged_token_kernel<kD, kNT, kF16>;
+  const int smem = static_cast<int>(sizeof(TokenSmem<kD, kNT>));
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    return MRSA_ERR_LAUNCH;
+  kernel<<<static_cast<unsigned>(a.grid), A_THREADS, smem, s>>>(a);
+  MRSA_CHECK_LAUNCH();
+  return MRSA_OK;
+}
+
+template <int kD, bool kF16>
+int launch_token_rows(const Args& a, cudaStream_t s) {
+  switch (a.row_tile) {
+    case 8: return launch_token<kD, 1, kF16>(a, s);
+    case 16: return launch_token<kD, 2, kF16>(a, s);
+    default: return launch_token<kD, 4, kF16>(a, s);
+  }
+}
+
+int token_row_tile(int64_t rows) { return rows <= 8 ? 8 : (rows <= 16 ? 16 : 32); }
+
+int sm_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1)
+    return 148;
+  return n;
+}
+
+bool sizes_ok(const mrsa_paged_attention_args* p) {
+  return p->batch >= 0 && p->len >= 0 && p->kv_heads >= 1 && p->q_heads >= p->kv_heads &&
+         p->q_heads % p->kv_heads == 0 && p->q_heads <= 4096 && p->len <= (1 << 20) &&
+         p->len * (p->q_heads / p->kv_heads) <= (1 << 24) && p->batch <= (1 << 24) &&
+         (p->head_dim == 64 || p->head_dim == 128);
+}
+
+}  // namespace
+
+namespace mrsa {
+namespace paged {
+
+size_t workspace(int64_t grid, int64_t row_tile, int64_t head_dim) {
+  return static_cast<size_t>(2 * grid * row_tile * (head_dim + 2) + kMaxBatch + 64) * 4;
+}
+
+int launch_join(const Args& a, int dtype, int head_dim, cudaStream_t s) {
+  const int64_t blocks = static_cast<int64_t>(a.batch) * a.kv_heads * a.rows;
+  if (blocks > 0x7fffffffLL) return MRSA_ERR_SHAPE;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+  cfg.blockDim = dim3(32 * J_WARPS);
+  cfg.stream = s;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const bool f16 = dtype == MRSA_F16;
+  const cudaError_t e =
+      head_dim == 128 ? (f16 ? cudaLaunchKernelEx(&cfg, paged_join_kernel<128, true>, a)
+                             : cudaLaunchKernelEx(&cfg, paged_join_kernel<128, false>, a))
+                      : (f16 ? cudaLaunchKernelEx(&cfg, paged_join_kernel<64, true>, a)
+                             : cudaLaunchKernelEx(&cfg, paged_join_kernel<64, false>, a));
+  if (e != cudaSuccess) {
+    note_cuda_error(e, __func__);
+    (void)cudaGetLastError();
+    return MRSA_ERR_LAUNCH;
+  }
+  return MRSA_OK;
+}
+
+}  // namespace paged
+}  // namespace mrsa
+
+extern "C" size_t mrsa_paged_attention_workspace(const mrsa_paged_attention_args* p) {
+  if (p == nullptr || !sizes_ok(p)) return 0;
+  const int64_t rows = p->len * (p->q_heads / p->kv_heads);
+  return paged::workspace(2 * static_cast<int64_t>(sm_count()), token_row_tile(rows), p->head_dim);
+}
+
+extern "C" int mrsa_paged_attention(const mrsa_paged_attention_args* p, const mrsa_page_table* t, void* workspace,
+                                    size_t ws_bytes, mrsa_stream_t stream) {
+  if (p == nullptr || t == nullptr) return MRSA_ERR_NULL;
+  if (int rc = mrsa::check_page_table(t)) return rc;
+  if (!sizes_ok(p)) return MRSA_ERR_SHAPE;
+  if (p->dtype != MRSA_BF16 && p->dtype != MRSA_F16) return MRSA_ERR_ARG;
+  if (!(p->scale > 0.f)) return MRSA_ERR_ARG;
+  if (p->batch * p->len == 0) return MRSA_OK;
+  if (!p->q || !p->k_pages || !p->v_pages || !p->out || !p->seqs) return MRSA_ERR_NULL;
+  const int64_t strides[9] = {p->q_batch_stride, p->q_token_stride, p->q_head_stride, p->k_page_stride,
+                              p->k_slot_stride, p->k_head_stride, p->v_page_stride, p->v_slot_stride,
+                              p->v_head_stride};
+  uintptr_t odd = reinterpret_cast<uintptr_t>(p->q) | reinterpret_cast<uintptr_t>(p->k_pages) |
+                  reinterpret_cast<uintptr_t>(p->v_pages) | reinterpret_cast<uintptr_t>(p->out) |
+                  reinterpret_cast<uintptr_t>(p->key_valid);
+  for (int64_t s : strides) odd |= static_cast<uintptr_t>(s * 2);
+  if (odd & 15) return MRSA_ERR_ALIGN;
+  mrsa::DeviceScope device_scope(t->table);
+  if (!workspace || ws_bytes < mrsa_paged_attention_workspace(p)) return MRSA_ERR_WORKSPACE;
+  if (reinterpret_cast<uintptr_t>(workspace) & 15) return MRSA_ERR_ALIGN;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+
+  Args a = {};
+  a.table = t->table;
+  a.lengths = t->lengths;
+  a.status = t->status;
+  a.max_seqs = static_cast<int>(t->max_seqs);
+  a.max_pages = static_cast<int>(t->max_pages);
+  a.pages = static_cast<int>(t->pages);
+  a.page_size = static_cast<int>(t->page_size);
+  a.page_shift = log2_int(t->page_size);
+  a.k = static_cast<const char*>(p->k_pages);
+  a.v = static_cast<const char*>(p->v_pages);
+  a.qb = p->q_batch_stride * 2;
+  a.qt = p->q_token_stride * 2;
+  a.qh = p->q_head_stride * 2;
+  a.kp = p->k_page_stride * 2;
+  a.ks = p->k_slot_stride * 2;
+  a.kh = p->k_head_stride * 2;
+  a.vp = p->v_page_stride * 2;
+  a.vs = p->v_slot_stride * 2;
+  a.vh = p->v_head_stride * 2;
+  a.len = static_cast<int>(p->len);
+  a.q_heads = static_cast<int>(p->q_heads);
+  a.kv_heads = static_cast<int>(p->kv_heads);
+  a.group = a.q_heads / a.kv_heads;
+  a.rows = a.len * a.group;
+  a.causal = p->causal != 0;
+  a.scale_log2 = p->scale * kLog2e;
+  a.row_tile = token_row_tile(a.rows);
+  a.row_tiles = (a.rows + a.row_tile - 1) / a.row_tile;
+  a.grid = 2 * sm_count();
+  const int64_t slots = 2 * static_cast<int64_t>(a.grid) * a.row_tile;
+  a.part_o = static_cast<float*>(workspace);
+  a.part_ml = a.part_o + slots * p->head_dim;
+  a.prefix = reinterpret_cast<int32_t*>(a.part_ml + slots * 2);
+  // more batch rows than a CTA keeps tile counts of: one stretch of them after another
+  for (int64_t b0 = 0; b0 < p->batch; b0 += paged::kMaxBatch) {
+    a.batch = static_cast<int>(p->batch - b0 < paged::kMaxBatch ? p->batch - b0 : paged::kMaxBatch);
+    a.q = static_cast<const char*>(p->q) + b0 * a.qb;
+    a.out = static_cast<char*>(p->out) + b0 * p->len * p->q_heads * p->head_dim * 2;
+    a.lse = p->lse != nullptr ? p->lse + b0 * p->len * p->q_heads : nullptr;
+    a.valid = p->key_valid != nullptr ? p->key_valid + b0 * t->max_pages * t->page_size : nullptr;
+    a.seqs = p->seqs + b0;
+    int rc;
+    if (p->dtype == MRSA_F16) rc = p->head_dim == 128 ? launch_token_rows<128, true>(a, s) : launch_token_rows<64, true>(a, s);
+    else rc = p->head_dim == 128 ? launch_token_rows<128, false>(a, s) : launch_token_rows<64, false>(a, s);
+    if (rc) return rc;
+    if ((rc = paged::launch_join(a, p->dtype, static_cast<int>(p->head_dim), s))) return rc;
+  }
+  return MRSA_OK;
+}

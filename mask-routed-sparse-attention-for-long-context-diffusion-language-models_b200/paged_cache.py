@@ -94,6 +94,11 @@ def _workspace(pt: bytes, n: int, device) -> tuple[torch.Tensor, int]:
     return torch.empty(size, dtype=torch.uint8, device=device), size
 
 
+def _aligned(x: torch.Tensor) -> torch.Tensor:
+    """``x``, or a copy that begins on 16 bytes."""
+    return x if x.data_ptr() % 16 == 0 else x.clone()
+
+
 def _count(x: torch.Tensor, name: str) -> int:
     n = x.shape[0]
     if n > MAX_SEQS:
@@ -178,9 +183,7 @@ def page_compact(pool, table, lengths, refcount, seqs, keep, *, status=None) -> 
     pt = _page_table(table, lengths, refcount, status, pool.shape[2], pool.shape[3])
     if n == 0:
         return
-    keep = keep.contiguous()
-    if keep.data_ptr() % 16:
-        keep = keep.clone()
+    keep = _aligned(keep.contiguous())
     ws, size = _workspace(pt, n, dev)
     _lib.call("mrsa_page_compact", pt, pp, seqs.data_ptr(), keep.data_ptr(), n, ws.data_ptr(), size,
               _lib.raw_stream(dev))
@@ -276,6 +279,61 @@ def paged_append(k_pages, v_pages, table, lengths, seqs, k, v, *, q=None, positi
     return qo
 
 
+def paged_attention(q, k_pages, v_pages, table, lengths, seqs, *, causal: bool = False, key_valid=None,
+                    scale: float | None = None, return_lse: bool = False, status=None):
+    """Attention of ``q [B, L, Hq, D]`` (bf16 or fp16, D 64 or 128) over the
+    cached tokens of the sequences ``seqs`` ``[B]`` in one layer's pages.
+
+    The queries are a sequence's newest L tokens, whose keys and values the
+    cache already holds: every query sees the whole sequence, as a block that
+    is denoised does, or with ``causal`` the tokens up to its own position,
+    ``length - L + i``.  ``key_valid`` (bool ``[B, max_pages * page_size]``)
+    masks cached tokens; what masked tokens and unused slots hold does not
+    matter.  Returns ``o [B, L, Hq, D]``, with ``return_lse`` also the
+    natural-log LSE ``[B, L, Hq]`` in fp32; a query that sees no token gets
+    zeros and -inf.  ``scale`` defaults to ``D ** -0.5``.  Forward only: it
+    raises under autograd rather than return an output without a gradient."""
+    check_heads(q, "q")
+    _check_pages(k_pages, v_pages)
+    b, l, hq, d = q.shape
+    dev = q.device
+    pages, page_size, hkv, dk = k_pages.shape
+    if q.dtype not in (torch.bfloat16, torch.float16) or k_pages.dtype != q.dtype or k_pages.device != dev:
+        raise ValueError("q and the pages must share a type (BF16 or FP16) and a device")
+    if d not in (64, 128) or dk != d or hkv < 1 or hq < hkv or hq % hkv:
+        raise ValueError(f"heads must be of 64 or 128 dims, Hq a multiple of Hkv; got q {tuple(q.shape)}, "
+                         f"pages {tuple(k_pages.shape)}")
+    if torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad):
+        raise NotImplementedError("paged_attention is forward-only")
+    seqs = _ints(seqs, "seqs", 1, table.device)
+    if seqs.shape[0] != b or table.device != dev:
+        raise ValueError("seqs must name one sequence per batch row, on the tensors' device")
+    scale = d ** -0.5 if scale is None else float(scale)
+    if not scale > 0:
+        raise ValueError("scale must be positive")
+    vp = 0
+    if key_valid is not None:
+        if key_valid.dtype != torch.bool or key_valid.shape != (b, table.shape[1] * page_size) or \
+                key_valid.device != dev:
+            raise ValueError(f"key_valid must be bool {(b, table.shape[1] * page_size)} on the tensors' device")
+        key_valid = _aligned(key_valid.contiguous())
+        vp = key_valid.data_ptr()
+    if q.stride(3) != 1 or q.data_ptr() % 16 or any(s % 8 for s in q.stride()[:3]):
+        q = _aligned(q.contiguous())
+    pt = _page_table(table, lengths, None, status, pages, page_size)
+    out = torch.empty((b, l, hq, d), dtype=q.dtype, device=dev)
+    lse = torch.empty((b, l, hq), dtype=torch.float32, device=dev) if return_lse else None
+    qs, ks, vs = q.stride(), k_pages.stride(), v_pages.stride()
+    args = _lib.PAGED_ATTENTION_ARGS.pack(
+        q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(), vp,
+        seqs.data_ptr(), qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], b, l, hq, hkv, d, scale,
+        DTYPES[q.dtype], causal)
+    size = _lib.load().mrsa_paged_attention_workspace(args)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    _lib.call("mrsa_paged_attention", args, pt, ws.data_ptr(), size, _lib.raw_stream(dev))
+    return (out, lse) if return_lse else out
+
+
 class PagedKVCache:
     """A pool of pages for ``layers`` layers and the bookkeeping of at most
     ``sequences`` sequences of at most ``max_len`` tokens.  The methods are
@@ -319,6 +377,11 @@ class PagedKVCache:
         return paged_append(self.pool[layer, 0], self.pool[layer, 1], self.table, self.lengths, seqs, k, v,
                             refcount=self.refcount, status=self.status, **kw)
 
+    def attend(self, layer: int, seqs, q, **kw):
+        """:func:`paged_attention` over one layer."""
+        return paged_attention(q, self.pool[layer, 0], self.pool[layer, 1], self.table, self.lengths, seqs,
+                               status=self.status, **kw)
+
     def check(self) -> None:
         """Waits for the device, clears the status word, and raises if a call
         since the last check could not be carried out."""
@@ -330,4 +393,4 @@ class PagedKVCache:
 
 
 __all__ = ["PAGE_SIZES", "PagedKVCache", "page_compact", "page_copy", "page_extend", "page_fork", "page_free",
-           "paged_append"]
+           "paged_append", "paged_attention"]
