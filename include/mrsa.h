@@ -401,8 +401,8 @@ int mrsa_wait_selftest(int* result, int rounds, mrsa_stream_t stream);
  * bit 3 = mrsa_convert_bf16_to_f16 saturated a value; bit 4 = a CTA of the
  * selected-attention backward gave up on a wait (its gradients are then
  * incomplete); bit 5 = a GEMM CTA did; bit 6 = a CTA of the local-window
- * backward did.  Synchronises the current device; with
- * clear != 0 also resets the mask.  Negative on a CUDA error.  Replaces the
+ * backward did; bit 7 = a CTA of mrsa_paged_attention did.  Synchronises the
+ * current device; with clear != 0 also resets the mask.  Negative on a CUDA error.  Replaces the
  * reference's host-side kernel-fallback reporting (dream_dllm_hils/attention.py:932-940). */
 int mrsa_device_error_flags(int clear);
 

@@ -102,28 +102,6 @@ __device__ __forceinline__ void row_band(const LocalArgs& a, int64_t pos, int64_
 
 __device__ int g_local_error;
 
-// 2^y for a pair on the FMA pipe, taking load off the special-function unit:
-// Cody-Waite reduction y = n + f (n = round(y) through the 1.5 * 2^23 shift,
-// |f| <= 1/2), 2^f by a degree-4 polynomial whose coefficients were fitted
-// for this kernel by Remez exchange on [-1/2, 1/2] (relative error 2.7e-6
-// evaluated in fp32, below fp16 P's rounding), and 2^n added to the exponent
-// field.  y is clamped to >= -126, so -inf gives 2^-126 rather than 0: only
-// for tiles without masked columns, where every row's sum is >= 1.
-__device__ __forceinline__ float2 exp2_poly2(float2 y) {
-  constexpr float kShift = 12582912.0f;   // 1.5 * 2^23
-  y.x = fmaxf(y.x, -126.0f);
-  y.y = fmaxf(y.y, -126.0f);
-  const float2 r = fadd2(y, make_float2(kShift, kShift));
-  const float2 n = fadd2(r, make_float2(-kShift, -kShift));
-  const float2 f = ffma2(n, make_float2(-1.0f, -1.0f), y);
-  float2 p = ffma2(make_float2(0.009570102f, 0.009570102f), f, make_float2(0.05591786f, 0.05591786f));
-  p = ffma2(p, f, make_float2(0.24024744f, 0.24024744f));
-  p = ffma2(p, f, make_float2(0.69312179f, 0.69312179f));
-  p = ffma2(p, f, make_float2(0.99999928f, 0.99999928f));
-  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(r.x) << 23)),
-                     __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(r.y) << 23)));
-}
-
 // kF16: V arrives in fp16 and P (values up to 2^8 under the lazy rescale) is
 // one fp16 tile, one P.V MMA per k-step; otherwise P is bf16 hi + lo.
 template <bool kF16>

@@ -33,6 +33,7 @@ constexpr int A_WARPS = 4, A_THREADS = 32 * A_WARPS;
 constexpr int A_KEYS = 16;                  // keys per warp and tile
 constexpr int A_TILE = A_KEYS * A_WARPS;    // keys per tile
 constexpr int A_STAGES = 3;
+constexpr int kTokenRows = 32;              // more query rows per KV head go to the tensor cores (paged_block.cu)
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
@@ -75,7 +76,6 @@ struct TokenSmem {
   float m[A_WARPS][8 * kNT], l[A_WARPS][8 * kNT];
   int prefix[paged::kMaxBatch + 1];
   int warp_sums[A_WARPS];
-  int64_t total;
 };
 
 template <int kD, int kNT, bool kF16>
@@ -90,32 +90,7 @@ __global__ void __launch_bounds__(A_THREADS) paged_token_kernel(const __grid_con
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
 
-  // ---- tiles before each batch row (per head and row tile)
-  {
-    int run = 0;
-    for (int b0 = 0; b0 < a.batch; b0 += A_THREADS) {
-      const int b = b0 + tid;
-      const int t = b < a.batch ? (paged::cached_tokens(a, b) + A_TILE - 1) / A_TILE : 0;
-      int x = t;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-      }
-      if (lane == 31) sm.warp_sums[warp] = x;
-      __syncthreads();
-      int before = run;
-#pragma unroll
-      for (int w = 0; w < A_WARPS; ++w) {
-        if (w < warp) before += sm.warp_sums[w];
-        run += sm.warp_sums[w];
-      }
-      if (b < a.batch) sm.prefix[b] = before + x - t;
-      __syncthreads();
-    }
-    if (tid == 0) sm.prefix[a.batch] = run;
-    __syncthreads();
-  }
+  paged::count_tiles<A_THREADS>(a, A_TILE, sm.prefix, sm.warp_sums);
   if (blockIdx.x == 0)
     for (int i = tid; i <= a.batch; i += A_THREADS) a.prefix[i] = sm.prefix[i];
   const int per = a.kv_heads * a.row_tiles;            // units per batch row
@@ -125,24 +100,8 @@ __global__ void __launch_bounds__(A_THREADS) paged_token_kernel(const __grid_con
   const int64_t t_end = blockIdx.x < grid ? paged::stretch(blockIdx.x + 1, total, grid) : 0;
 
   for (int64_t t_now = t_begin; t_now < t_end;) {
-    // ---- the unit that holds tile t_now: the last batch row whose tiles begin at or before it
-    int lo = 0, hi = a.batch - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (static_cast<int64_t>(sm.prefix[mid]) * per <= t_now) lo = mid; else hi = mid - 1;
-    }
-    const int b = lo;
-    const int tiles = sm.prefix[b + 1] - sm.prefix[b];
-    const int64_t in_row = t_now - static_cast<int64_t>(sm.prefix[b]) * per;
-    const int unit = static_cast<int>(in_row / tiles);
-    const int tile0 = static_cast<int>(in_row - static_cast<int64_t>(unit) * tiles);
-    const int64_t room = t_end - t_now;
-    const int tile1 = room < tiles - tile0 ? tile0 + static_cast<int>(room) : tiles;
-    const int h = unit / a.row_tiles, rt = unit - h * a.row_tiles;
-    const int seq = a.seqs[b];
-    const int n = a.lengths[seq];
-    const int r0 = rt * kRows;
-    const int nrows = a.rows - r0 < kRows ? a.rows - r0 : kRows;
+    const paged::Piece pc = paged::piece_at(a, sm.prefix, t_now, t_end);
+    const int b = pc.b, h = pc.h, n = pc.n, r0 = pc.r0, nrows = pc.nrows, tile0 = pc.tile0, tile1 = pc.tile1;
 
     // ---- this thread's part of Q^T: column lane / 4 of each 8-row block
     uint32_t qf[kNT][kSteps][2];
@@ -180,7 +139,7 @@ __global__ void __launch_bounds__(A_THREADS) paged_token_kernel(const __grid_con
     }
 
     // ---- the warp's stream of 16-key pieces; what a copy needs is fetched one tile ahead
-    const int32_t* row_pages = a.table + static_cast<int64_t>(seq) * a.max_pages;
+    const int32_t* row_pages = a.table + static_cast<int64_t>(pc.seq) * a.max_pages;
     const uint8_t* valid = a.valid != nullptr ? a.valid + static_cast<int64_t>(b) * a.max_pages * a.page_size : nullptr;
     auto fetch = [&](int t, int& page, uint4& vb) {
       const int key0 = t * A_TILE + warp * A_KEYS;
@@ -344,7 +303,7 @@ __global__ void __launch_bounds__(A_THREADS) paged_token_kernel(const __grid_con
         }
       }
     __syncthreads();
-    const bool whole = tile0 == 0 && tile1 == tiles;
+    const bool whole = pc.whole();
     const int slot = 2 * blockIdx.x + (t_now == t_begin ? 0 : 1);
     for (int e = tid; e < nrows * kD; e += A_THREADS) {
       const int r = e / kD, d = e - r * kD;
@@ -359,8 +318,7 @@ __global__ void __launch_bounds__(A_THREADS) paged_token_kernel(const __grid_con
         acc += c * reinterpret_cast<const float*>(sm.ring[w][0][0])[r * kD + d];
       }
       if (whole) {
-        const int i = (r0 + r) / a.group, g = (r0 + r) - i * a.group;
-        const int64_t at = (static_cast<int64_t>(b) * a.len + i) * a.q_heads + h * a.group + g;
+        const int64_t at = paged::out_row(a, pc, r);
         store_out<kF16>(a.out + (at * kD + d) * 2, sum > 0.f ? acc / sum : 0.f);
         if (d == 0 && a.lse != nullptr) a.lse[at] = sum > 0.f ? (top + log2f(sum)) * kLn2 : -INFINITY;
       } else {
@@ -466,7 +424,11 @@ int launch_token_rows(const Args& a, cudaStream_t s) {
   }
 }
 
-int token_row_tile(int64_t rows) { return rows <= 8 ? 8 : (rows <= 16 ? 16 : 32); }
+// Query rows per KV head that a unit holds.
+int row_tile_of(int64_t rows) {
+  if (rows > kTokenRows) return paged::kBlockRows;
+  return rows <= 8 ? 8 : (rows <= 16 ? 16 : 32);
+}
 
 int sm_count() {
   int dev = 0, n = 0;
@@ -475,6 +437,9 @@ int sm_count() {
     return 148;
   return n;
 }
+
+// CTAs that fill the machine: two of the small ones per SM.
+int grid_of(int64_t rows) { return rows > kTokenRows ? sm_count() : 2 * sm_count(); }
 
 bool sizes_ok(const mrsa_paged_attention_args* p) {
   return p->batch >= 0 && p->len >= 0 && p->kv_heads >= 1 && p->q_heads >= p->kv_heads &&
@@ -524,7 +489,7 @@ int launch_join(const Args& a, int dtype, int head_dim, cudaStream_t s) {
 extern "C" size_t mrsa_paged_attention_workspace(const mrsa_paged_attention_args* p) {
   if (p == nullptr || !sizes_ok(p)) return 0;
   const int64_t rows = p->len * (p->q_heads / p->kv_heads);
-  return paged::workspace(2 * static_cast<int64_t>(sm_count()), token_row_tile(rows), p->head_dim);
+  return paged::workspace(grid_of(rows), row_tile_of(rows), p->head_dim);
 }
 
 extern "C" int mrsa_paged_attention(const mrsa_paged_attention_args* p, const mrsa_page_table* t, void* workspace,
@@ -576,9 +541,9 @@ extern "C" int mrsa_paged_attention(const mrsa_paged_attention_args* p, const mr
   a.rows = a.len * a.group;
   a.causal = p->causal != 0;
   a.scale_log2 = p->scale * kLog2e;
-  a.row_tile = token_row_tile(a.rows);
+  a.row_tile = row_tile_of(a.rows);
   a.row_tiles = (a.rows + a.row_tile - 1) / a.row_tile;
-  a.grid = 2 * sm_count();
+  a.grid = grid_of(a.rows);
   const int64_t slots = 2 * static_cast<int64_t>(a.grid) * a.row_tile;
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = a.part_o + slots * p->head_dim;
@@ -592,7 +557,8 @@ extern "C" int mrsa_paged_attention(const mrsa_paged_attention_args* p, const mr
     a.valid = p->key_valid != nullptr ? p->key_valid + b0 * t->max_pages * t->page_size : nullptr;
     a.seqs = p->seqs + b0;
     int rc;
-    if (p->dtype == MRSA_F16) rc = p->head_dim == 128 ? launch_token_rows<128, true>(a, s) : launch_token_rows<64, true>(a, s);
+    if (a.rows > kTokenRows) rc = paged::launch_block(a, p->dtype, static_cast<int>(p->head_dim), s);
+    else if (p->dtype == MRSA_F16) rc = p->head_dim == 128 ? launch_token_rows<128, true>(a, s) : launch_token_rows<64, true>(a, s);
     else rc = p->head_dim == 128 ? launch_token_rows<128, false>(a, s) : launch_token_rows<64, false>(a, s);
     if (rc) return rc;
     if ((rc = paged::launch_join(a, p->dtype, static_cast<int>(p->head_dim), s))) return rc;

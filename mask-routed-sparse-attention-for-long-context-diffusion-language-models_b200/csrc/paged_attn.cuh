@@ -70,6 +70,77 @@ __device__ __forceinline__ int slot_of(int c, int c0, int64_t first, int64_t tot
   return 2 * c + ((c == c0 && stretch(c, total, grid) != first) ? 1 : 0);
 }
 
+// A CTA's part of one unit.
+struct Piece {
+  int b, h, r0, nrows;          // batch row, KV head, first query row, query rows
+  int seq, n;                   // the sequence's row of the table, its cached tokens
+  int tile0, tile1, tiles;      // this part's key tiles, and all of the unit's
+  __device__ __forceinline__ bool whole() const { return tile0 == 0 && tile1 == tiles; }
+};
+
+// The part that begins at tile `t` and ends with its unit or at `end`.
+__device__ __forceinline__ Piece piece_at(const Args& a, const int* prefix, int64_t t, int64_t end) {
+  const int per = a.kv_heads * a.row_tiles;            // units per batch row
+  int lo = 0, hi = a.batch - 1;                        // the last batch row whose tiles begin at or before t
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (static_cast<int64_t>(prefix[mid]) * per <= t) lo = mid; else hi = mid - 1;
+  }
+  Piece p;
+  p.b = lo;
+  p.tiles = prefix[lo + 1] - prefix[lo];
+  const int64_t in_row = t - static_cast<int64_t>(prefix[lo]) * per;
+  const int unit = static_cast<int>(in_row / p.tiles);
+  p.tile0 = static_cast<int>(in_row - static_cast<int64_t>(unit) * p.tiles);
+  p.tile1 = end - t < p.tiles - p.tile0 ? p.tile0 + static_cast<int>(end - t) : p.tiles;
+  p.h = unit / a.row_tiles;
+  p.r0 = (unit - p.h * a.row_tiles) * a.row_tile;
+  p.nrows = a.rows - p.r0 < a.row_tile ? a.rows - p.r0 : a.row_tile;
+  p.seq = a.seqs[lo];
+  p.n = a.lengths[p.seq];
+  return p;
+}
+
+// Tiles of `tile` keys before each batch row (per head and row tile), by all
+// threads of the CTA.
+template <int kThreads>
+__device__ __forceinline__ void count_tiles(const Args& a, int tile, int* prefix, int* warp_sums) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int run = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += kThreads) {
+    const int b = b0 + static_cast<int>(threadIdx.x);
+    const int t = b < a.batch ? (cached_tokens(a, b) + tile - 1) / tile : 0;
+    int x = t;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) warp_sums[warp] = x;
+    __syncthreads();
+    int before = run;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) {
+      if (w < warp) before += warp_sums[w];
+      run += warp_sums[w];
+    }
+    if (b < a.batch) prefix[b] = before + x - t;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) prefix[a.batch] = run;
+  __syncthreads();
+}
+
+// The output row of query row r of a piece.
+__device__ __forceinline__ int64_t out_row(const Args& a, const Piece& p, int r) {
+  const int i = (p.r0 + r) / a.group, g = (p.r0 + r) - i * a.group;
+  return (static_cast<int64_t>(p.b) * a.len + i) * a.q_heads + p.h * a.group + g;
+}
+
+// paged_block.cu: the units of a.row_tile = kBlockRows rows on a.grid CTAs, one per SM.
+constexpr int kBlockRows = 256;
+int launch_block(const Args& a, int dtype, int head_dim, cudaStream_t s);
+
 size_t workspace(int64_t grid, int64_t row_tile, int64_t head_dim);
 int launch_join(const Args& a, int dtype, int head_dim, cudaStream_t s);
 

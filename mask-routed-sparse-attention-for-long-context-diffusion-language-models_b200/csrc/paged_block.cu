@@ -1,0 +1,533 @@
+// Attention over a paged key-value cache: many query rows per KV head (a block
+// of tokens that is denoised, a prompt) on the tcgen05 tensor cores.
+//
+// With R rows per KV head a key costs R flops per cached byte: 32 tokens of a
+// 7-head group are 224, near the machine's ridge, so the products have to run
+// at tensor-core rate and each K and V tile has to serve all rows that fit.
+// One CTA holds 256 rows of one KV head as two MMA tiles of 128 and walks its
+// stretch of the key tiles (paged_attn.cuh) in tiles of 64:
+//   S[128 x 64]  = Q . K_t^T              (UMMA M=128, N=64,  TMEM)
+//   P            = exp2(S scale log2e - m)  (one thread per row, lazy maximum)
+//   O[128 x D]  += P . V_t                (UMMA M=128, N=D, A = P in TMEM)
+// P is rounded once to the type of V (8 or 11 bits; the sum of the
+// probabilities is of the unrounded ones), written over its own S and read
+// from there.  Warps 0-3 and 4-7: softmax, Q tile and epilogue of row tiles 0
+// and 1; warp 8: K tiles and key masks, warp 11: V tiles, both by TMA, one box
+// per page part and 64 dims, straight from the pages the table names; warps 9
+// and 10: MMA issue.  Rings and buffers run on from one unit of the stretch to
+// the next.  Masked keys leave the softmax; their V rows are zeroed in shared
+// memory first, since what a masked or unused slot holds may not be a number.
+// Every wait is bounded: a CTA that gives up unwinds and sets bit 7 of
+// mrsa_device_error_flags.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <mutex>
+
+#include "paged_attn.cuh"
+#include "tc.cuh"
+
+#include <cuda_fp16.h>
+
+using namespace mrsa;
+
+namespace {
+
+using paged::Args;
+using paged::Piece;
+
+constexpr int B_TILE = 64;         // keys per tile
+constexpr int B_ROWS = 128;        // rows per MMA tile; two per CTA
+constexpr int NKS = 4, NVS = 4;    // K and V stages
+constexpr int NMS = 8;             // key-mask slots
+constexpr int B_THREADS = 384;
+constexpr int W_K = 8, W_MMA = 9, W_V = 11;
+constexpr uint32_t kOCol = 256;    // S buffer i at [64 i, 64 i + 64), O of group g at 256 + 128 g
+
+template <int kD>
+struct __align__(1024) BlockSmem {
+  unsigned char q[2][kD / 64][B_ROWS * 128];     // [row tile][64 dims][row], 128-byte swizzled
+  unsigned char k[NKS][kD / 64][B_TILE * 128];
+  unsigned char v[NVS][kD / 64][B_TILE * 128];   // the MN-major B operand of P.V
+  unsigned long long kmask[NMS];                 // bit j: key j of the tile counts
+  uint64_t qfull[2], kfull[NKS], kfree[NKS], vfull[NVS], vfree[NVS], mfull[NMS];
+  uint64_t sfull[4], pready[4], pfree[4], drain[2];
+  uint32_t tmem_base;
+  int abort_flag;
+  int prefix[paged::kMaxBatch + 1];
+  int warp_sums[B_THREADS / 32];
+};
+static_assert(sizeof(BlockSmem<128>) + 1024 <= 232448, "paged attention shared memory over budget");
+
+__device__ int g_paged_error;
+
+// Pages of a tile's keys: lane j < parts looks up part j (page_size keys, or
+// the whole tile where a page holds it).  -1: no keys there to read.
+struct TilePages {
+  int parts, part_keys;
+  __device__ __forceinline__ explicit TilePages(const Args& a)
+      : parts(a.page_size < B_TILE ? B_TILE / a.page_size : 1), part_keys(a.page_size < B_TILE ? a.page_size : B_TILE) {}
+  __device__ __forceinline__ int look_up(const Args& a, const Piece& p, int tile, int lane) const {
+    const int key = tile * B_TILE + lane * part_keys;
+    if (lane >= parts || tile >= p.tile1 || key >= p.n) return -1;
+    const int page = a.table[static_cast<int64_t>(p.seq) * a.max_pages + (key >> a.page_shift)];
+    if (page < 0 || page >= a.pages) {
+      report(a.status, MRSA_PAGE_OUTSIDE);
+      return -1;
+    }
+    return page;
+  }
+};
+
+template <int kD, bool kF16>
+__global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_constant__ CUtensorMap tm_k,
+                                                                   const __grid_constant__ CUtensorMap tm_v,
+                                                                   const __grid_constant__ Args a) {
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  auto& sm = *reinterpret_cast<BlockSmem<kD>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  constexpr int kHalves = kD / 64, kQHalf = B_ROWS * 128, kKHalf = B_TILE * 128, kStage = kHalves * kKHalf;
+  volatile int* abort_flag = &sm.abort_flag;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+
+  if (tid == 0) {
+    for (int s = 0; s < NKS; ++s) {
+      tc::mbar_init(tc::smem_addr(&sm.kfull[s]), 1);
+      tc::mbar_init(tc::smem_addr(&sm.kfree[s]), 2);
+    }
+    for (int s = 0; s < NVS; ++s) {
+      tc::mbar_init(tc::smem_addr(&sm.vfull[s]), 1);
+      tc::mbar_init(tc::smem_addr(&sm.vfree[s]), 2);
+    }
+    for (int s = 0; s < NMS; ++s) tc::mbar_init(tc::smem_addr(&sm.mfull[s]), 1);
+    for (int s = 0; s < 4; ++s) {
+      tc::mbar_init(tc::smem_addr(&sm.sfull[s]), 1);
+      tc::mbar_init(tc::smem_addr(&sm.pready[s]), 4);
+      tc::mbar_init(tc::smem_addr(&sm.pfree[s]), 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      tc::mbar_init(tc::smem_addr(&sm.qfull[s]), 4);
+      tc::mbar_init(tc::smem_addr(&sm.drain[s]), 1);
+    }
+    sm.abort_flag = 0;
+    tc::fence_mbar_init();
+  }
+  if (warp == 0) {
+    tc::tmem_alloc(tc::smem_addr(&sm.tmem_base), 512);
+    tc::tmem_relinquish();
+  }
+  paged::count_tiles<B_THREADS>(a, B_TILE, sm.prefix, sm.warp_sums);
+  if (blockIdx.x == 0)
+    for (int i = tid; i <= a.batch; i += B_THREADS) a.prefix[i] = sm.prefix[i];
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tbase = sm.tmem_base;
+  const int64_t total = static_cast<int64_t>(sm.prefix[a.batch]) * a.kv_heads * a.row_tiles;
+  const int64_t grid = paged::dealt(a, total);
+  const int64_t t_begin = blockIdx.x < grid ? paged::stretch(blockIdx.x, total, grid) : 0;
+  const int64_t t_end = blockIdx.x < grid ? paged::stretch(blockIdx.x + 1, total, grid) : 0;
+  bool ok = true;
+
+  if (warp == W_K || warp == W_V) {
+    // ============================ K tiles and key masks; V tiles =============
+    const bool is_k = warp == W_K;
+    const CUtensorMap* map = is_k ? &tm_k : &tm_v;
+    uint64_t* full = is_k ? sm.kfull : sm.vfull;
+    uint64_t* freed = is_k ? sm.kfree : sm.vfree;
+    unsigned char* ring = is_k ? sm.k[0][0] : sm.v[0][0];
+    static_assert(NKS == NVS, "K and V stages share their index");
+    if (lane == 0) tc::prefetch_tensormap(map);
+    const TilePages tp(a);
+    int e = 0;                                   // tiles of the stretch so far
+    for (int64_t t_now = t_begin; ok && t_now < t_end;) {
+      const Piece p = paged::piece_at(a, sm.prefix, t_now, t_end);
+      const uint8_t* valid = a.valid != nullptr && is_k
+                                 ? a.valid + static_cast<int64_t>(p.b) * a.max_pages * a.page_size : nullptr;
+      // the next tile's page numbers and mask bytes are requested a tile ahead
+      auto valid_bytes = [&](int tile, uint32_t (&vb)[2]) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int key = tile * B_TILE + 32 * i + lane;
+          vb[i] = (valid != nullptr && tile < p.tile1 && key < p.n) ? valid[key] : 1u;
+        }
+      };
+      int page_next = tp.look_up(a, p, p.tile0, lane);
+      uint32_t vb_next[2];
+      valid_bytes(p.tile0, vb_next);
+      for (int t = p.tile0; t < p.tile1; ++t, ++e) {
+        const int st = e % NKS;
+        const int page = page_next;
+        const uint32_t vb[2] = {vb_next[0], vb_next[1]};
+        page_next = tp.look_up(a, p, t + 1, lane);
+        valid_bytes(t + 1, vb_next);
+        // the stage was released by both groups for tile e - NKS; the mask slot
+        // was last read by the softmax of tile e - NMS, before that release
+        if (e >= NKS && !(ok = tc::wait_bounded_warp(tc::smem_addr(&freed[st]), ((e / NKS) - 1) & 1, abort_flag))) break;
+        const unsigned has = __ballot_sync(0xffffffffu, page >= 0);
+        if (is_k) {
+          uint32_t mk[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int in = 32 * i + lane, key = t * B_TILE + in;
+            mk[i] = __ballot_sync(0xffffffffu, key < p.n && vb[i] != 0u && ((has >> (in / tp.part_keys)) & 1u));
+          }
+          if (lane == 0) {
+            sm.kmask[e % NMS] = static_cast<unsigned long long>(mk[0]) | (static_cast<unsigned long long>(mk[1]) << 32);
+            tc::mbar_arrive(tc::smem_addr(&sm.mfull[e % NMS]));
+          }
+        }
+        const uint32_t bar = tc::smem_addr(&full[st]);
+        if (lane == 0) tc::mbar_arrive_expect_tx(bar, __popc(has) * tp.part_keys * kD * 2);
+        __syncwarp();
+        if (page >= 0) {
+          const int slot = (t * B_TILE + lane * tp.part_keys) & (a.page_size - 1);
+#pragma unroll
+          for (int hf = 0; hf < kHalves; ++hf)
+            tc::tma_load_5d(tc::smem_addr(ring + st * kStage + hf * kKHalf + lane * tp.part_keys * 128), map, 0, slot, hf,
+                            p.h, page, bar);
+        }
+        __syncwarp();
+      }
+      t_now += p.tile1 - p.tile0;
+    }
+    // wait (bounded, even after an abort) for the copies in flight
+    if (lane == 0)
+      for (int tt = e - NKS < 0 ? 0 : e - NKS; tt < e; ++tt)
+        tc::mbar_wait(tc::smem_addr(&full[tt % NKS]), (tt / NKS) & 1);
+    __syncwarp();
+  } else if (warp >= W_MMA) {
+    // ============================ MMA issue (one warp per row tile) ==========
+    const int g = warp - W_MMA;
+    // kind::f16: the bf16 format bits cleared for fp16 operands
+    constexpr uint32_t kType = kF16 ? ~((1u << 7) | (1u << 10)) : ~0u;
+    constexpr uint32_t id_s = tc::idesc_bf16_f32(128, B_TILE, 0, 0) & kType;
+    constexpr uint32_t id_o = tc::idesc_bf16_f32(128, kD, 0, 1) & kType;
+    const uint64_t dq = tc::smem_desc_sw128(tc::smem_addr(sm.q[g][0]), 16, 1024);
+    const uint64_t dk0 = tc::smem_desc_sw128(tc::smem_addr(sm.k[0][0]), 16, 1024);
+    const uint64_t dv0 = tc::smem_desc_sw128(tc::smem_addr(sm.v[0][0]), kKHalf, 1024);
+    int e = 0, k = 0, units = 0;                  // tiles of the stretch, tiles and units of this group, so far
+    // S of the stretch's tile ee, the group's tile kk, into buffer 2g + (kk & 1),
+    // once the P that was there has been read
+    auto issue_s = [&](int ee, int kk) -> bool {
+      const int sb = 2 * g + (kk & 1), st = ee % NKS;
+      if (kk >= 2 && !tc::wait_bounded_warp(tc::smem_addr(&sm.pfree[sb]), ((kk - 2) >> 1) & 1, abort_flag)) return false;
+      if (!tc::wait_bounded_warp(tc::smem_addr(&sm.kfull[st]), (ee / NKS) & 1, abort_flag)) return false;
+      tc::fence_after_sync();
+      const uint64_t db = tc::desc_adv(dk0, st * kStage);
+      const uint32_t dS = tbase + B_TILE * sb;
+      if (tc::elect_one()) {
+        tc::mma_bf16<false>(dS, dq, db, id_s);
+#pragma unroll
+        for (int i = 1; i < kD / 16; ++i)
+          tc::mma_bf16<true>(dS, tc::desc_adv(dq, (i >> 2) * kQHalf + (i & 3) * 32),
+                             tc::desc_adv(db, (i >> 2) * kKHalf + (i & 3) * 32), id_s);
+        tc::mma_commit(tc::smem_addr(&sm.sfull[sb]));
+        tc::mma_commit(tc::smem_addr(&sm.kfree[st]));
+      }
+      __syncwarp();
+      return true;
+    };
+    for (int64_t t_now = t_begin; ok && t_now < t_end;) {
+      const Piece p = paged::piece_at(a, sm.prefix, t_now, t_end);
+      const int nt = p.tile1 - p.tile0;
+      if (p.nrows <= g * B_ROWS) {
+        // no rows for this group: the unit's stages released unused, in order
+        for (int i = 0; ok && i < nt; ++i, ++e) {
+          ok = tc::wait_bounded_warp(tc::smem_addr(&sm.kfull[e % NKS]), (e / NKS) & 1, abort_flag) &&
+               tc::wait_bounded_warp(tc::smem_addr(&sm.vfull[e % NVS]), (e / NVS) & 1, abort_flag);
+          if (ok && lane == 0) {
+            tc::mbar_arrive(tc::smem_addr(&sm.kfree[e % NKS]));
+            tc::mbar_arrive(tc::smem_addr(&sm.vfree[e % NVS]));
+          }
+          __syncwarp();
+        }
+      } else {
+        ok = tc::wait_bounded_warp(tc::smem_addr(&sm.qfull[g]), units & 1, abort_flag);
+        ++units;
+        if (ok) ok = issue_s(e, k);
+        if (ok && nt > 1) ok = issue_s(e + 1, k + 1);
+        for (int i = 0; ok && i < nt; ++i, ++e, ++k) {
+          const int sb = 2 * g + (k & 1), sv = e % NVS;
+          if (!(ok = tc::wait_bounded_warp(tc::smem_addr(&sm.pready[sb]), (k >> 1) & 1, abort_flag))) break;
+          if (!(ok = tc::wait_bounded_warp(tc::smem_addr(&sm.vfull[sv]), (e / NVS) & 1, abort_flag))) break;
+          tc::fence_after_sync();
+          const uint64_t dv = tc::desc_adv(dv0, sv * kStage);
+          const uint32_t dO = tbase + kOCol + 128 * g, aP = tbase + B_TILE * sb;
+          if (tc::elect_one()) {
+            // the unit's first tile overwrites O; 16 keys (8 columns of pairs) per step
+            if (i == 0) tc::mma_f16_ts<false>(dO, aP, dv, id_o);
+            else tc::mma_f16_ts<true>(dO, aP, dv, id_o);
+#pragma unroll
+            for (int kk = 1; kk < B_TILE / 16; ++kk)
+              tc::mma_f16_ts<true>(dO, aP + 8 * kk, tc::desc_adv(dv, kk * 2048), id_o);
+            tc::mma_commit(tc::smem_addr(&sm.pfree[sb]));
+            tc::mma_commit(tc::smem_addr(&sm.vfree[sv]));
+          }
+          __syncwarp();
+          if (i + 2 < nt) ok = issue_s(e + 2, k + 2);
+        }
+      }
+      t_now += nt;
+    }
+    if (tc::elect_one()) {
+      tc::mma_commit(tc::smem_addr(&sm.drain[g]));
+      tc::mbar_wait(tc::smem_addr(&sm.drain[g]), 0);
+    }
+    __syncwarp();
+  } else {
+    // ============================ Q, softmax and epilogue (warps 0-7) ========
+    const int g = warp >> 2, r = (warp & 3) * 32 + lane;      // row tile; row = TMEM lane
+    const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t t_o = tbase + lane_off + kOCol + 128 * g;
+    int e0 = 0, k = 0;            // tiles of the stretch before this unit; tiles of this group so far
+    for (int64_t t_now = t_begin; ok && t_now < t_end;) {
+      const Piece p = paged::piece_at(a, sm.prefix, t_now, t_end);
+      const int nt = p.tile1 - p.tile0;
+      if (p.nrows > g * B_ROWS) {
+        // ---- this row of Q (the S products of the unit before are done: the last S was read)
+        const int row = g * B_ROWS + r;
+        const bool row_ok = row < p.nrows;
+        const int qi = (p.r0 + (row_ok ? row : 0)) / a.group, qg = (p.r0 + (row_ok ? row : 0)) - qi * a.group;
+        {
+          const char* src = a.q + p.b * a.qb + qi * a.qt + (p.h * a.group + qg) * a.qh;
+          uint4 x[kD / 8];
+#pragma unroll
+          for (int j = 0; j < kD / 8; ++j)
+            x[j] = row_ok ? *reinterpret_cast<const uint4*>(src + j * 16) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+          for (int j = 0; j < kD / 8; ++j)
+            *reinterpret_cast<uint4*>(sm.q[g][j / 8] + r * 128 + (((j & 7) ^ (r & 7)) * 16)) = x[j];
+        }
+        tc::fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(tc::smem_addr(&sm.qfull[g]));
+        const int last = a.causal ? p.n - a.len + qi : p.n - 1;   // the last key this row may see
+        float m_run = -INFINITY, l_run = 0.f;
+        for (int i = 0; i < nt; ++i, ++k) {
+          const int sb = 2 * g + (k & 1), e = e0 + i;
+          const int j0 = (p.tile0 + i) * B_TILE;
+          if (!(ok = tc::wait_bounded_warp(tc::smem_addr(&sm.sfull[sb]), (k >> 1) & 1, abort_flag))) break;
+          tc::fence_after_sync();
+          uint32_t x[64];
+          const uint32_t t_s = tbase + lane_off + B_TILE * sb;
+#pragma unroll
+          for (int c = 0; c < 64; c += 16) tc::tmem_ld16(t_s + c, *reinterpret_cast<uint32_t(*)[16]>(&x[c]));
+          tc::tmem_wait_ld();
+          if (!(ok = tc::wait_bounded_warp(tc::smem_addr(&sm.mfull[e % NMS]), (e / NMS) & 1, abort_flag))) break;
+          const unsigned long long km = sm.kmask[e % NMS];
+          const int seen = last - j0;              // columns past it are out of this row's sight
+          const bool full = km == ~0ull && seen >= B_TILE - 1;
+          if (km != ~0ull) {
+#pragma unroll
+            for (int c = 0; c < B_TILE; ++c)
+              if (!((km >> c) & 1ull)) x[c] = __float_as_uint(-INFINITY);
+          }
+          if (seen < B_TILE - 1) {
+#pragma unroll
+            for (int c = 0; c < B_TILE; ++c)
+              if (c > seen) x[c] = __float_as_uint(-INFINITY);
+          }
+          float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int c = 0; c < B_TILE; c += 8)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              m4[j] = fmax3(m4[j], __uint_as_float(x[c + 2 * j]), __uint_as_float(x[c + 2 * j + 1]));
+          const float tmax = fmax3(m4[0], m4[1], fmaxf(m4[2], m4[3])) * a.scale_log2;
+          // the reference moves, and O is scaled, only for a maximum 2^8 above it
+          float corr = 1.f;
+          bool rescale = false;
+          if (tmax > m_run + 8.f) {
+            corr = m_run == -INFINITY ? 0.f : fast_exp2(m_run - tmax);
+            rescale = m_run != -INFINITY;
+            l_run *= corr;
+            m_run = tmax;
+          }
+          const float nbase = m_run == -INFINITY ? 0.f : -m_run;
+          const float2 sl2 = make_float2(a.scale_log2, a.scale_log2), nb2 = make_float2(nbase, nbase);
+          float2 s2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+          uint32_t pk[32];
+          // a quarter of a full tile's exponentials on the FMA pipe (the choice is the row's own)
+          if (full) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              const float2 y = ffma2(make_float2(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1])), sl2, nb2);
+              const float2 w = (j % 4 == 3) ? exp2_poly2(y) : make_float2(fast_exp2(y.x), fast_exp2(y.y));
+              s2[j & 1] = fadd2(s2[j & 1], w);
+              pk[j] = kF16 ? pack_f16x2(w.x, w.y) : pack_bf16x2(w.x, w.y);
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              const float2 y = ffma2(make_float2(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1])), sl2, nb2);
+              const float2 w = make_float2(fast_exp2(y.x), fast_exp2(y.y));
+              s2[j & 1] = fadd2(s2[j & 1], w);
+              pk[j] = kF16 ? pack_f16x2(w.x, w.y) : pack_bf16x2(w.x, w.y);
+            }
+          }
+          __syncwarp();
+          l_run += (s2[0].x + s2[1].x) + (s2[0].y + s2[1].y);
+          tc::tmem_st16(t_s, &pk[0]);
+          tc::tmem_st16(t_s + 16, &pk[16]);
+          tc::tmem_wait_st();
+          if (km != ~0ull) {
+            // V rows of keys that do not count: zeroed (by both groups alike), seen by the tensor core
+            const int sv = e % NVS, key = r >> 1;
+            if (!(ok = tc::wait_bounded_warp(tc::smem_addr(&sm.vfull[sv]), (e / NVS) & 1, abort_flag))) break;
+            if (!((km >> key) & 1ull)) {
+#pragma unroll
+              for (int hf = 0; hf < kHalves; ++hf)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                  *reinterpret_cast<uint4*>(sm.v[sv][hf] + key * 128 + (r & 1) * 64 + j * 16) = make_uint4(0u, 0u, 0u, 0u);
+            }
+            tc::fence_proxy_async();
+            __syncwarp();
+          }
+          if (__any_sync(0xffffffffu, rescale)) {
+            // O holds every earlier tile of the unit once the P.V before this one is done
+            if (!(ok = tc::wait_bounded_warp(tc::smem_addr(&sm.pfree[2 * g + ((k - 1) & 1)]), ((k - 1) >> 1) & 1, abort_flag)))
+              break;
+            tc::fence_after_sync();
+#pragma unroll
+            for (int cc = 0; cc < kD; cc += 16) {
+              uint32_t o[16];
+              tc::tmem_ld16(t_o + cc, o);
+              tc::tmem_wait_ld();
+#pragma unroll
+              for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr);
+              tc::tmem_st16(t_o + cc, o);
+            }
+            tc::tmem_wait_st();
+          }
+          tc::fence_before_sync();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(tc::smem_addr(&sm.pready[sb]));
+        }
+        // ---- the unit's rows: finished, or a part for the join
+        if (ok) ok = tc::wait_bounded_warp(tc::smem_addr(&sm.pfree[2 * g + ((k - 1) & 1)]), ((k - 1) >> 1) & 1, abort_flag);
+        if (!ok) break;
+        tc::fence_after_sync();
+        const bool whole = p.whole();
+        const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
+        const int64_t orow = paged::out_row(a, p, row_ok ? row : 0);
+        const int64_t prow = static_cast<int64_t>(2 * blockIdx.x + (t_now == t_begin ? 0 : 1)) * a.row_tile + row;
+#pragma unroll
+        for (int cc = 0; cc < kD; cc += 16) {
+          uint32_t o[16];
+          tc::tmem_ld16(t_o + cc, o);
+          tc::tmem_wait_ld();
+          if (row_ok) {
+            if (whole) {
+              uint32_t w[8];
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                // a row that saw nothing has P = 0 throughout, and its O is 0
+                const float f0 = __uint_as_float(o[2 * j]) * inv, f1 = __uint_as_float(o[2 * j + 1]) * inv;
+                if constexpr (kF16) {
+                  const __half2 hv = __floats2half2_rn(f0, f1);
+                  w[j] = *reinterpret_cast<const uint32_t*>(&hv);
+                } else {
+                  w[j] = pack_bf16x2(f0, f1);
+                }
+              }
+              uint4* dst = reinterpret_cast<uint4*>(a.out + (orow * kD + cc) * 2);
+              dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
+              dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
+            } else {
+              uint4* dst = reinterpret_cast<uint4*>(a.part_o + prow * kD + cc);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) dst[j] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+            }
+          }
+          __syncwarp();
+        }
+        if (row_ok) {
+          if (whole) {
+            if (a.lse != nullptr) a.lse[orow] = l_run > 0.f ? (m_run + log2f(l_run)) * kLn2 : -INFINITY;
+          } else {
+            a.part_ml[prow * 2] = m_run;
+            a.part_ml[prow * 2 + 1] = l_run;
+          }
+        }
+        tc::fence_before_sync();       // O was read before the next unit's first P is announced
+        __syncwarp();
+      }
+      e0 += nt;
+      t_now += nt;
+    }
+  }
+
+  tc::fence_before_sync();
+  __syncthreads();
+  if (tid == 0 && sm.abort_flag) atomicOr(&g_paged_error, 1);
+  if (warp == 0) {
+    tc::fence_after_sync();
+    tc::tmem_dealloc(tbase, 512);
+  }
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
+std::once_flag g_encode_once;
+
+// Pages as (dim of 64, slot, 64 dims, head, page); one box: 64 dims of the
+// slots of one page that a tile covers.
+bool page_map(CUtensorMap* m, const void* base, int64_t page, int64_t slot, int64_t head, const Args& a, int head_dim,
+              bool f16) {
+  std::call_once(g_encode_once, [] {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      g_encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+  });
+  if (g_encode == nullptr) return false;
+  const cuuint64_t dims[5] = {64, static_cast<cuuint64_t>(a.page_size), static_cast<cuuint64_t>(head_dim / 64),
+                              static_cast<cuuint64_t>(a.kv_heads), static_cast<cuuint64_t>(a.pages)};
+  const cuuint64_t strides[4] = {static_cast<cuuint64_t>(slot), 128, static_cast<cuuint64_t>(head),
+                                 static_cast<cuuint64_t>(page)};
+  const cuuint32_t box[5] = {64, static_cast<cuuint32_t>(a.page_size < B_TILE ? a.page_size : B_TILE), 1, 1, 1};
+  const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  return g_encode(m, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(base),
+                  dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int kD, bool kF16>
+int launch(const Args& a, cudaStream_t s) {
+  CUtensorMap tk, tv;
+  if (!page_map(&tk, a.k, a.kp, a.ks, a.kh, a, kD, kF16) || !page_map(&tv, a.v, a.vp, a.vs, a.vh, a, kD, kF16)) {
+    note_cuda_error(cudaErrorInvalidValue, "page tensor map");
+    return MRSA_ERR_LAUNCH;
+  }
+  const int smem = static_cast<int>(sizeof(BlockSmem<kD>) + 1024);
+  if (cudaFuncSetAttribute(paged_block_kernel<kD, kF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    return MRSA_ERR_LAUNCH;
+  paged_block_kernel<kD, kF16><<<static_cast<unsigned>(a.grid), B_THREADS, smem, s>>>(tk, tv, a);
+  MRSA_CHECK_LAUNCH();
+  return MRSA_OK;
+}
+
+}  // namespace
+
+namespace mrsa {
+namespace paged {
+
+int launch_block(const Args& a, int dtype, int head_dim, cudaStream_t s) {
+  if (dtype == MRSA_F16) return head_dim == 128 ? launch<128, true>(a, s) : launch<64, true>(a, s);
+  return head_dim == 128 ? launch<128, false>(a, s) : launch<64, false>(a, s);
+}
+
+}  // namespace paged
+
+int paged_error_flags(int clear) {
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, g_paged_error, sizeof(int)) != cudaSuccess) return -1;
+  if (clear) {
+    const int z = 0;
+    if (cudaMemcpyToSymbol(g_paged_error, &z, sizeof(int)) != cudaSuccess) return -1;
+  }
+  return v;
+}
+}  // namespace mrsa
