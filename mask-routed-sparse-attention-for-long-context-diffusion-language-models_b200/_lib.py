@@ -147,8 +147,7 @@ def stream_of(t: torch.Tensor):
 
 def raw_stream(device: torch.device) -> int:
     """Handle of the device's current stream."""
-    return torch._C._cuda_getCurrentRawStream(device.index if device.index is not None else
-                                              torch.cuda.current_device())
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 # The argument structs of the rotary and paged operators, packed as bytes: a
@@ -163,6 +162,19 @@ APPEND_ARGS = struct.Struct("@5P9qi4x")              # mrsa_paged_append_args
 
 def call(name: str, *args):
     check(getattr(load(), name)(*args), name)
+
+
+_entries: dict = {}
+
+
+def call_packed(name: str, *args):
+    """:func:`call` for the operators with packed arguments."""
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = getattr(load(), name)
+    rc = fn(*args)
+    if rc:
+        check(rc, name)
 
 
 class RouteLayerArgs(C.Structure):

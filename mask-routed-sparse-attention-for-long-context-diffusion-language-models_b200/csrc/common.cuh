@@ -234,6 +234,10 @@ class DeviceScope {
   int prev_ = -1, dev_ = -1;
 };
 
+// SMs of the current device (asked once per device: an attribute query costs
+// as much as a tenth of a launch).
+int sm_count();
+
 // Keeps, per host thread, the CUDA error behind the last MRSA_ERR_LAUNCH
 // (read through mrsa_last_error()).
 void note_cuda_error(cudaError_t e, const char* where);

@@ -2,6 +2,7 @@
 // fusion, plus the ABI's small host helpers.
 #include <math.h>
 
+#include <atomic>
 #include <cstdio>
 
 #include "common.cuh"
@@ -170,6 +171,16 @@ int convert_error_flags(int clear) {
   }
   return v;
 }
+int sm_count() {
+  static std::atomic<int> known[64];
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  if ((n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1) return 148;
+  known[dev].store(n, std::memory_order_relaxed);
+  return n;
+}
+
 thread_local char g_last_error[256] = "";
 
 void note_cuda_error(cudaError_t e, const char* where) {

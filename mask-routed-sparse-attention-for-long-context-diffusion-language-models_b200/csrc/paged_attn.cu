@@ -430,14 +430,6 @@ int row_tile_of(int64_t rows) {
   return rows <= 8 ? 8 : (rows <= 16 ? 16 : 32);
 }
 
-int sm_count() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1)
-    return 148;
-  return n;
-}
-
 // CTAs that fill the machine: two of the small ones per SM.
 int grid_of(int64_t rows) { return rows > kTokenRows ? sm_count() : 2 * sm_count(); }
 

@@ -508,14 +508,6 @@ PlanArgs plan_args(const mrsa_page_table* t, const int32_t* seqs, int64_t n, voi
   return a;
 }
 
-int sm_count() {
-  int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n < 1)
-    return 148;
-  return n;
-}
-
 template <typename K>
 int launch_move(K kernel, const MoveArgs& a, int64_t most_pages, bool after_plan, cudaStream_t s) {
   const int64_t vecs = a.page_bytes / 16, parts = (vecs + M_THREADS * M_UNROLL - 1) / (M_THREADS * M_UNROLL);

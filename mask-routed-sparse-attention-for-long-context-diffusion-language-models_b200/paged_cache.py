@@ -28,7 +28,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .rotary import DTYPES, LAYOUTS, check_heads, check_rotation, inner_contiguous
+from .rotary import DTYPES, LAYOUTS, check_heads, check_rotation, inner_contiguous, new_heads
 
 PAGE_SIZES = (16, 32, 64, 128, 256)
 MAX_SEQS = 1024    # sequences per call of the page operators
@@ -42,26 +42,25 @@ _STATUS = {BAD_SEQUENCE: "a sequence number is out of range or was given twice",
 
 
 def _ints(x: torch.Tensor, name: str, ndim: int, device=None) -> torch.Tensor:
-    if x.dtype != torch.int32 or x.ndim != ndim or x.device.type != "cuda":
+    if x.dtype is not torch.int32 or x.ndim != ndim or not x.is_cuda:
         raise ValueError(f"{name} must be an int32 CUDA tensor with {ndim} dimension{'s' if ndim > 1 else ''}")
     if device is not None and x.device != device:
         raise ValueError(f"{name} must be on the table's device")
-    return x.contiguous()
+    return x if x.is_contiguous() else x.contiguous()
 
 
 def _page_table(table, lengths, refcount, status, pages, page_size) -> bytes:
     """``mrsa_page_table``; the state tensors themselves are written, so they
     have to be contiguous."""
-    dev = table.device
-    if table.dtype != torch.int32 or table.ndim != 2 or dev.type != "cuda" or not table.is_contiguous():
+    dev, i32 = table.device, torch.int32
+    if table.dtype is not i32 or table.ndim != 2 or not table.is_cuda or not table.is_contiguous():
         raise ValueError("table must be a contiguous int32 CUDA tensor [sequences, max_pages]")
-    if lengths.dtype != torch.int32 or lengths.shape != table.shape[:1] or lengths.device != dev or \
-            not lengths.is_contiguous():
+    n, w = table.shape
+    if lengths.dtype is not i32 or lengths.shape != (n,) or lengths.device != dev or not lengths.is_contiguous():
         raise ValueError("lengths must be contiguous int32 [sequences] on the table's device")
     rp = sp = 0
     if refcount is not None:
-        if refcount.dtype != torch.int32 or refcount.ndim != 1 or refcount.device != dev or \
-                not refcount.is_contiguous():
+        if refcount.dtype is not i32 or refcount.ndim != 1 or refcount.device != dev or not refcount.is_contiguous():
             raise ValueError("refcount must be contiguous int32 [pages] on the table's device")
         if pages is None:
             pages = refcount.shape[0]
@@ -71,10 +70,9 @@ def _page_table(table, lengths, refcount, status, pages, page_size) -> bytes:
     if page_size not in PAGE_SIZES:
         raise ValueError(f"page_size must be one of {PAGE_SIZES}, got {page_size}")
     if status is not None:
-        if status.dtype != torch.int32 or status.numel() != 1 or status.device != dev:
+        if status.dtype is not i32 or status.numel() != 1 or status.device != dev:
             raise ValueError("status must be one int32 on the table's device")
         sp = status.data_ptr()
-    n, w = table.shape
     return _lib.PAGE_TABLE.pack(table.data_ptr(), lengths.data_ptr(), rp, sp, n, w, pages, page_size)
 
 
@@ -91,7 +89,7 @@ def _page_pool(pool, device) -> bytes:
 
 def _workspace(pt: bytes, n: int, device) -> tuple[torch.Tensor, int]:
     size = _lib.load().mrsa_page_workspace(pt, n)
-    return torch.empty(size, dtype=torch.uint8, device=device), size
+    return torch.empty_strided((size,), (1,), dtype=torch.uint8, device=device), size
 
 
 def _aligned(x: torch.Tensor) -> torch.Tensor:
@@ -112,7 +110,7 @@ def page_free(table, lengths, refcount, seqs, *, status=None) -> None:
     seqs = _ints(seqs, "seqs", 1, table.device)
     n = _count(seqs, "seqs")
     pt = _page_table(table, lengths, refcount, status, None, PAGE_SIZES[0])
-    _lib.call("mrsa_page_free", pt, seqs.data_ptr(), n, _lib.raw_stream(table.device))
+    _lib.call_packed("mrsa_page_free", pt, seqs.data_ptr(), n, _lib.raw_stream(table.device))
 
 
 def page_extend(table, lengths, refcount, seqs, tokens, *, page_size: int, status=None) -> None:
@@ -135,7 +133,7 @@ def page_extend(table, lengths, refcount, seqs, tokens, *, page_size: int, statu
     if n == 0:
         return
     ws, size = _workspace(pt, n, dev)
-    _lib.call("mrsa_page_extend", pt, seqs.data_ptr(), 0 if each is None else each.data_ptr(), more, n, ws.data_ptr(),
+    _lib.call_packed("mrsa_page_extend", pt, seqs.data_ptr(), 0 if each is None else each.data_ptr(), more, n, ws.data_ptr(),
               size, _lib.raw_stream(dev))
 
 
@@ -162,7 +160,7 @@ def page_fork(pool, table, lengths, refcount, src, dst, share=None, *, status=No
     if n == 0:
         return
     ws, size = _workspace(pt, n, dev)
-    _lib.call("mrsa_page_fork", pt, pp, src.data_ptr(), dst.data_ptr(), sp, n, ws.data_ptr(), size,
+    _lib.call_packed("mrsa_page_fork", pt, pp, src.data_ptr(), dst.data_ptr(), sp, n, ws.data_ptr(), size,
               _lib.raw_stream(dev))
 
 
@@ -185,7 +183,7 @@ def page_compact(pool, table, lengths, refcount, seqs, keep, *, status=None) -> 
         return
     keep = _aligned(keep.contiguous())
     ws, size = _workspace(pt, n, dev)
-    _lib.call("mrsa_page_compact", pt, pp, seqs.data_ptr(), keep.data_ptr(), n, ws.data_ptr(), size,
+    _lib.call_packed("mrsa_page_compact", pt, pp, seqs.data_ptr(), keep.data_ptr(), n, ws.data_ptr(), size,
               _lib.raw_stream(dev))
 
 
@@ -205,16 +203,19 @@ def page_copy(pool, src, dst, *, status=None) -> None:
     # the copy needs no table: the struct's is any valid pointer that is not read
     sp = 0 if status is None else _ints(status.reshape(1), "status", 1, dev).data_ptr()
     pt = _lib.PAGE_TABLE.pack(src.data_ptr(), src.data_ptr(), 0, sp, 1, 1, pool.shape[2], pool.shape[3])
-    _lib.call("mrsa_page_copy", pt, pp, src.data_ptr(), dst.data_ptr(), n, _lib.raw_stream(dev))
+    _lib.call_packed("mrsa_page_copy", pt, pp, src.data_ptr(), dst.data_ptr(), n, _lib.raw_stream(dev))
 
 
-def _check_pages(k_pages, v_pages):
+def _page_strides(k_pages, v_pages):
+    """Strides of a layer's pages, checked."""
     if k_pages.ndim != 4 or v_pages.shape != k_pages.shape:
         raise ValueError("k_pages and v_pages must share a [pages, page_size, kv_heads, D] shape")
-    if v_pages.dtype != k_pages.dtype or v_pages.device != k_pages.device or k_pages.device.type != "cuda":
+    if v_pages.dtype is not k_pages.dtype or v_pages.device != k_pages.device or not k_pages.is_cuda:
         raise ValueError("k_pages and v_pages must share type and CUDA device")
-    if k_pages.stride(3) != 1 or v_pages.stride(3) != 1:
+    ks, vs = k_pages.stride(), v_pages.stride()
+    if ks[3] != 1 or vs[3] != 1:
         raise ValueError("the last dimension of k_pages and v_pages must be contiguous")
+    return ks, vs
 
 
 def paged_append(k_pages, v_pages, table, lengths, seqs, k, v, *, q=None, position_ids=None, inv_freq=None,
@@ -232,15 +233,16 @@ def paged_append(k_pages, v_pages, table, lengths, seqs, k, v, *, q=None, positi
     not written, and ``status`` says so."""
     check_heads(k, "k")
     check_heads(v, "v", k)
-    if v.shape != k.shape:
-        raise ValueError("v must have k's shape")
-    _check_pages(k_pages, v_pages)
     b, l, hkv, d = k.shape
-    dev = k.device
-    if k.dtype not in DTYPES or k_pages.dtype != k.dtype or k_pages.device != dev:
+    if v.shape[2] != hkv:
+        raise ValueError("v must have k's shape")
+    kps, vps = _page_strides(k_pages, v_pages)
+    dev, dtype = k.device, DTYPES.get(k.dtype)
+    if dtype is None or k_pages.dtype is not k.dtype or k_pages.device != dev:
         raise ValueError("k, v and the pages must share a type (BF16, FP16 or FP32) and a device")
-    if k_pages.shape[2:] != (hkv, d):
-        raise ValueError(f"the pages hold heads of {tuple(k_pages.shape[2:])}, k has {(hkv, d)}")
+    pages, page_size, ph, pd = k_pages.shape
+    if ph != hkv or pd != d:
+        raise ValueError(f"the pages hold heads of {(ph, pd)}, k has {(hkv, d)}")
     seqs = _ints(seqs, "seqs", 1, table.device)
     if seqs.shape[0] != b or table.device != dev:
         raise ValueError("seqs must name one sequence per batch row, on the tensors' device")
@@ -251,7 +253,8 @@ def paged_append(k_pages, v_pages, table, lengths, seqs, k, v, *, q=None, positi
         inv_freq, pairs = check_rotation(inv_freq, position_ids, b, l, d, layout, dev)
         ip = inv_freq.data_ptr()
         if position_ids is not None:
-            position_ids = position_ids.contiguous()
+            if not position_ids.is_contiguous():
+                position_ids = position_ids.contiguous()
             pos = position_ids.data_ptr()
     st = 0
     if start is not None:
@@ -259,7 +262,6 @@ def paged_append(k_pages, v_pages, table, lengths, seqs, k, v, *, q=None, positi
         if start.shape[0] != b:
             raise ValueError("start must hold one position per sequence")
         st = start.data_ptr()
-    pages, page_size = k_pages.shape[:2]
     pt = _page_table(table, lengths, refcount, status, pages, page_size)
     k, v = inner_contiguous(k), inner_contiguous(v)
     qo, hq, qp, qop, qs = None, 0, 0, 0, (0, 0, 0)
@@ -267,15 +269,15 @@ def paged_append(k_pages, v_pages, table, lengths, seqs, k, v, *, q=None, positi
         check_heads(q, "q", k)
         q = inner_contiguous(q)
         hq = q.shape[2]
-        qo = torch.empty((b, l, hq, d), dtype=k.dtype, device=dev)
+        qo = new_heads(b, l, hq, d, k.dtype, dev)
         qp, qop, qs = q.data_ptr(), qo.data_ptr(), q.stride()
-    ks, vs, kps, vps = k.stride(), v.stride(), k_pages.stride(), v_pages.stride()
+    ks, vs = k.stride(), v.stride()
     ra = _lib.ROTARY_ARGS.pack(qp, qop, k.data_ptr(), 0, pos, ip, qs[0], qs[1], qs[2], ks[0], ks[1], ks[2],
-                               b, l, hq, hkv, d, pairs, float(attention_factor), DTYPES[k.dtype], LAYOUTS[layout], 0)
+                               b, l, hq, hkv, d, pairs, float(attention_factor), dtype, LAYOUTS[layout], 0)
     ap = _lib.APPEND_ARGS.pack(k_pages.data_ptr(), v_pages.data_ptr(), v.data_ptr(), seqs.data_ptr(), st,
                                kps[0], kps[1], kps[2], vps[0], vps[1], vps[2], vs[0], vs[1], vs[2],
                                0 if refcount is None else 1)
-    _lib.call("mrsa_paged_append", ra, pt, ap, _lib.raw_stream(dev))
+    _lib.call_packed("mrsa_paged_append", ra, pt, ap, _lib.raw_stream(dev))
     return qo
 
 
@@ -294,13 +296,15 @@ def paged_attention(q, k_pages, v_pages, table, lengths, seqs, *, causal: bool =
     zeros and -inf.  ``scale`` defaults to ``D ** -0.5``.  Forward only: it
     raises under autograd rather than return an output without a gradient."""
     check_heads(q, "q")
-    _check_pages(k_pages, v_pages)
+    ks, vs = _page_strides(k_pages, v_pages)
     b, l, hq, d = q.shape
-    dev = q.device
+    dev, qs = q.device, q.stride()
     pages, page_size, hkv, dk = k_pages.shape
-    if q.dtype not in (torch.bfloat16, torch.float16) or k_pages.dtype != q.dtype or k_pages.device != dev:
+    dtype = q.dtype
+    if (dtype is not torch.bfloat16 and dtype is not torch.float16) or k_pages.dtype is not dtype or \
+            k_pages.device != dev:
         raise ValueError("q and the pages must share a type (BF16 or FP16) and a device")
-    if d not in (64, 128) or dk != d or hkv < 1 or hq < hkv or hq % hkv:
+    if (d != 128 and d != 64) or dk != d or hkv < 1 or hq < hkv or hq % hkv:
         raise ValueError(f"heads must be of 64 or 128 dims, Hq a multiple of Hkv; got q {tuple(q.shape)}, "
                          f"pages {tuple(k_pages.shape)}")
     if torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad):
@@ -313,24 +317,26 @@ def paged_attention(q, k_pages, v_pages, table, lengths, seqs, *, causal: bool =
         raise ValueError("scale must be positive")
     vp = 0
     if key_valid is not None:
-        if key_valid.dtype != torch.bool or key_valid.shape != (b, table.shape[1] * page_size) or \
-                key_valid.device != dev:
-            raise ValueError(f"key_valid must be bool {(b, table.shape[1] * page_size)} on the tensors' device")
+        width = table.shape[1] * page_size
+        if key_valid.dtype is not torch.bool or key_valid.shape != (b, width) or key_valid.device != dev:
+            raise ValueError(f"key_valid must be bool {(b, width)} on the tensors' device")
         key_valid = _aligned(key_valid.contiguous())
         vp = key_valid.data_ptr()
-    if q.stride(3) != 1 or q.data_ptr() % 16 or any(s % 8 for s in q.stride()[:3]):
+    if qs[3] != 1 or (qs[0] | qs[1] | qs[2]) % 8 or q.data_ptr() % 16:
         q = _aligned(q.contiguous())
+        qs = q.stride()
     pt = _page_table(table, lengths, None, status, pages, page_size)
-    out = torch.empty((b, l, hq, d), dtype=q.dtype, device=dev)
-    lse = torch.empty((b, l, hq), dtype=torch.float32, device=dev) if return_lse else None
-    qs, ks, vs = q.stride(), k_pages.stride(), v_pages.stride()
+    out = new_heads(b, l, hq, d, dtype, dev)
+    lse, lp = None, 0
+    if return_lse:
+        lse = torch.empty_strided((b, l, hq), (l * hq, hq, 1), dtype=torch.float32, device=dev)
+        lp = lse.data_ptr()
     args = _lib.PAGED_ATTENTION_ARGS.pack(
-        q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(), vp,
-        seqs.data_ptr(), qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], b, l, hq, hkv, d, scale,
-        DTYPES[q.dtype], causal)
+        q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), lp, vp, seqs.data_ptr(),
+        qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], b, l, hq, hkv, d, scale, DTYPES[dtype], causal)
     size = _lib.load().mrsa_paged_attention_workspace(args)
-    ws = torch.empty(size, dtype=torch.uint8, device=dev)
-    _lib.call("mrsa_paged_attention", args, pt, ws.data_ptr(), size, _lib.raw_stream(dev))
+    ws = torch.empty_strided((size,), (1,), dtype=torch.uint8, device=dev)
+    _lib.call_packed("mrsa_paged_attention", args, pt, ws.data_ptr(), size, _lib.raw_stream(dev))
     return (out, lse) if return_lse else out
 
 
