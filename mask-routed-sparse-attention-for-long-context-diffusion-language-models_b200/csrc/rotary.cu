@@ -9,12 +9,16 @@
 // and sums are fp32; the result is rounded once to the tensors' type.
 //
 // Every byte is read and written once, so HBM bounds it (and, for a few
-// tokens, the launch).  A work item is two 16-byte vectors of one head, the
-// two halves of its pairs in the half layout, which a thread loads before it
-// takes its share of the CTA's angles: the loads' latency then covers the
-// trigonometry, which is done once per (token, pair) and not per head.  A turn
-// count is reduced in fp64 (positions past 1e5 would otherwise take sincosf's
-// slow path): the fp32 angle over 2 pi, minus its nearest whole number.
+// tokens, the launch).  A CTA takes a few tokens of one batch row (and a
+// part of a token's items, where it has more than threads); a thread keeps its place in a head (two 16-byte vectors that hold V whole pairs in
+// either layout) and goes from token to token, so what it does per token is
+// little more than the rotation.  Up to six of its tokens are under way at a
+// time as asynchronous copies into shared-memory slots of its own: as many in
+// registers would halve the warps that fit (16384 tokens of 28 + 4 heads: 78
+// us).  The tokens' angles (once per token and pair, not per head) and slots
+// are worked out meanwhile.  A turn count is reduced in fp64 (positions past
+// 1e5 would otherwise take sincosf's slow path): the fp32 angle over 2 pi,
+// minus its nearest whole number.
 #include "common.cuh"
 #include "pages.cuh"
 
@@ -24,9 +28,10 @@ using namespace mrsa;
 
 namespace {
 
-constexpr int R_THREADS = 256;
-constexpr int R_ITEMS = 2;          // items a thread has in flight
-constexpr int R_MAX_TOKENS = 16;    // tokens per CTA
+constexpr int R_THREADS = 256;      // per CTA, about: whole warps that share a token's items evenly
+constexpr int R_MAX_THREADS = 384;
+constexpr int R_AHEAD = 7;          // tokens a thread has in flight
+constexpr int R_MAX_RUN = 16;       // tokens per CTA
 constexpr int R_MAX_PAIRS = 128;
 
 struct Part {
@@ -45,9 +50,10 @@ struct RotaryArgs {
   const float* inv;
   float factor;
   int inverse, interleaved, pairs, head_dim;
-  int items_head, items_token, tokens_cta;
+  int items_head, items_token;
+  int run, runs;         // tokens per CTA, CTAs per batch row
+  int side;              // tokens that the CTA's threads work on side by side
   int len;               // tokens per sequence
-  int64_t tokens;        // batch * len
   PageSlots slots;       // where the paged parts' tokens go
   const int32_t* start;  // [batch] or NULL: lengths - len
   int any_paged;
@@ -74,132 +80,154 @@ __device__ __forceinline__ float2 turn_of(int64_t pos, float inv, float factor, 
   return make_float2(c * factor, (inverse ? -s : s) * factor);
 }
 
-// One item: the vectors at element offsets oa and ob of a head (ob < 0: only
-// the first).  kV elements each.
-struct Item {
-  const char* x;
-  char* y;
-  int oa, ob, pair;   // pair: the first pair's index when the item turns, else -1
-  int tok;
-};
+// The (cos, sin) of a slot's kPairs pairs.
+template <int kPairs>
+__device__ __forceinline__ void pairs_of(const float2* c, int slots, int slot, float2* w) {
+#pragma unroll
+  for (int e = 0; e < kPairs; e += 2) {
+    const float4 two = *reinterpret_cast<const float4*>(c + ((e >> 1) * slots + slot) * 2);
+    w[e] = make_float2(two.x, two.y);
+    w[e + 1] = make_float2(two.z, two.w);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void turn_pair(T& a, T& b, float2 w) {
+  const float u = to_f(a), v = to_f(b);
+  a = from_f<T>(u * w.x - v * w.y);
+  b = from_f<T>(v * w.x + u * w.y);
+}
 
 template <typename T, int V>
-__global__ void __launch_bounds__(R_THREADS) rotary_kernel(const __grid_constant__ RotaryArgs a) {
-  extern __shared__ float2 cs[];               // [tokens_cta][pairs]
-  __shared__ int64_t dst_page[R_MAX_TOKENS];   // page of each token's slot, < 0: not written
-  __shared__ int dst_slot[R_MAX_TOKENS];
-  const int tid = threadIdx.x;
-  const int64_t tok0 = static_cast<int64_t>(blockIdx.x) * a.tokens_cta;
-  const int nt = a.tokens - tok0 < a.tokens_cta ? static_cast<int>(a.tokens - tok0) : a.tokens_cta;
-  const int total = nt * a.items_token;
-  const int vecs = a.head_dim / V, rvecs = 2 * a.pairs / V;
+__device__ __forceinline__ void turn_neighbours(Vec<T, V>& x, const float2* c, int slots, int slot) {
+  if constexpr (V > 1) {
+    float2 w[V / 2 + 1];
+    pairs_of<V / 2>(c, slots, slot, w);
+#pragma unroll
+    for (int e = 0; e < V / 2; ++e) turn_pair(x.e[2 * e], x.e[2 * e + 1], w[e]);
+  }
+}
 
-  auto locate = [&](int it, Item& m, bool& paged, const Part*& p, int& head) {
-    m.tok = it / a.items_token;
-    int r = it - m.tok * a.items_token;
-    head = r / a.items_head;
-    const int j = r - head * a.items_head;
-    int w = 0;
-    if (head >= a.part[0].heads) { head -= a.part[0].heads; w = 1; if (head >= a.part[1].heads) { head -= a.part[1].heads; w = 2; } }
-    p = &a.part[w];
-    paged = p->paged != 0;
-    const int64_t t = tok0 + m.tok, b = t / a.len, l = t - b * a.len;
-    m.x = reinterpret_cast<const char*>(static_cast<const T*>(p->x) + b * p->xb + l * p->xt + head * p->xh);
-    m.y = reinterpret_cast<char*>(static_cast<T*>(p->y));
-    if (!paged) m.y = reinterpret_cast<char*>(static_cast<T*>(p->y) + b * p->yb + l * p->yt + head * p->yh);
-    // vector indexes: in the half layout the item's vectors are j and j + n / V
-    // while they turn, and two neighbours past 2n; else always two neighbours
-    int va, vb;
-    m.pair = -1;
-    if (p->turn && !a.interleaved && j < rvecs / 2) {
-      va = j; vb = j + rvecs / 2; m.pair = j * V;
-    } else {
-      va = 2 * j; vb = 2 * j + 1;
-      if (p->turn && a.interleaved && va < rvecs) m.pair = va * (V / 2);
-    }
-    m.oa = va * V;
-    m.ob = vb < vecs ? vb * V : -1;
-  };
-
-  for (int base = 0; base < total; base += R_THREADS * R_ITEMS) {
-    Item m[R_ITEMS];
-    const Part* part[R_ITEMS];
-    int head[R_ITEMS];
-    bool paged[R_ITEMS];
-    Vec<T, V> xa[R_ITEMS], xb[R_ITEMS];
-#pragma unroll
-    for (int k = 0; k < R_ITEMS; ++k) {
-      const int it = base + k * R_THREADS + tid;
-      if (it >= total) continue;
-      locate(it, m[k], paged[k], part[k], head[k]);
-      xa[k] = *reinterpret_cast<const Vec<T, V>*>(m[k].x + m[k].oa * sizeof(T));
-      if (m[k].ob >= 0) xb[k] = *reinterpret_cast<const Vec<T, V>*>(m[k].x + m[k].ob * sizeof(T));
-    }
-    if (base == 0) {
-      if (a.any_paged && tid < nt) {
-        const int64_t t = tok0 + tid, b = t / a.len, l = t - b * a.len;
-        const int64_t at = a.slots.position(b, a.start, a.len) + l;
-        dst_page[tid] = a.slots.page_of(b, at);
-        dst_slot[tid] = static_cast<int>(at & (a.slots.page_size - 1));
-      }
-      for (int i = tid; i < nt * a.pairs; i += R_THREADS) {
-        const int tok = i / a.pairs, p = i - tok * a.pairs;
-        const int64_t t = tok0 + tok;
-        int64_t pos;
-        if (a.pos != nullptr) {
-          pos = a.pos[t];
-        } else {
-          const int64_t b = t / a.len;
-          pos = a.slots.position(b, a.start, a.len) + (t - b * a.len);
-        }
-        cs[i] = turn_of(pos, a.inv[p], a.factor, a.inverse);
-      }
-      __syncthreads();
-    }
-#pragma unroll
-    for (int k = 0; k < R_ITEMS; ++k) {
-      const int it = base + k * R_THREADS + tid;
-      if (it >= total) continue;
-      if (m[k].pair >= 0) {
-        const float2* c = cs + m[k].tok * a.pairs + m[k].pair;
-        if (!a.interleaved) {
-#pragma unroll
-          for (int e = 0; e < V; ++e) {
-            const float u = to_f(xa[k].e[e]), v = to_f(xb[k].e[e]);
-            const float2 w = c[e];
-            xa[k].e[e] = from_f<T>(u * w.x - v * w.y);
-            xb[k].e[e] = from_f<T>(v * w.x + u * w.y);
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e + 1 < V; e += 2) {
-            const float u = to_f(xa[k].e[e]), v = to_f(xa[k].e[e + 1]);
-            const float2 w = c[e / 2];
-            xa[k].e[e] = from_f<T>(u * w.x - v * w.y);
-            xa[k].e[e + 1] = from_f<T>(v * w.x + u * w.y);
-          }
-          if (m[k].ob >= 0 && m[k].ob < 2 * a.pairs) {
-#pragma unroll
-            for (int e = 0; e + 1 < V; e += 2) {
-              const float u = to_f(xb[k].e[e]), v = to_f(xb[k].e[e + 1]);
-              const float2 w = c[V / 2 + e / 2];
-              xb[k].e[e] = from_f<T>(u * w.x - v * w.y);
-              xb[k].e[e + 1] = from_f<T>(v * w.x + u * w.y);
-            }
-          }
-        }
-      }
-      char* y = m[k].y;
-      if (paged[k]) {
-        const int64_t page = dst_page[m[k].tok];
-        if (page < 0) continue;
-        y += (page * part[k]->yb + dst_slot[m[k].tok] * part[k]->yt + head[k] * part[k]->yh) *
-             static_cast<int64_t>(sizeof(T));
-      }
-      *reinterpret_cast<Vec<T, V>*>(y + m[k].oa * sizeof(T)) = xa[k];
-      if (m[k].ob >= 0) *reinterpret_cast<Vec<T, V>*>(y + m[k].ob * sizeof(T)) = xb[k];
+// kWide: 16-byte vectors through asynchronous copies; else element by element.
+template <typename T, int V, bool kWide>
+__global__ void __launch_bounds__(R_MAX_THREADS) rotary_kernel(const __grid_constant__ RotaryArgs a) {
+  // wide: each thread's slots [R_AHEAD][2][thread], 16 bytes each; then (cos, sin)
+  // of a token's pairs, `per` of them (those of one vector) to a slot, pair
+  // slot * per + e at [token][e / 2][slot][e % 2]: neighbouring threads' reads of
+  // two pairs lie side by side
+  extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ int64_t dst_page[R_MAX_RUN];      // page of each token's slot, < 0: not written
+  __shared__ int dst_slot[R_MAX_RUN];
+  using Vec = ::Vec<T, V>;
+  constexpr int kIn = V > 1 ? V / 2 : 1;       // pairs of a vector in the interleaved layout; V in the half layout
+  const int tid = threadIdx.x, threads = blockDim.x;
+  Vec* ring = reinterpret_cast<Vec*>(smem) + tid;
+  float2* cs = reinterpret_cast<float2*>(smem + (kWide ? R_AHEAD * 2 * threads * 16 : 0));
+  const int64_t b = blockIdx.x / a.runs;
+  const int l0 = static_cast<int>(blockIdx.x - b * a.runs) * a.run, nt = a.len - l0 < a.run ? a.len - l0 : a.run;
+  const int vecs = a.head_dim / V;
+  const int per = a.interleaved ? kIn : V;
+  const int slots = (a.pairs + per - 1) / per, cs_tok = slots * ((per + 1) / 2) * 2;
+  const int tok0 = a.side > 1 ? tid / a.items_token : 0;
+  const int item = a.side > 1 ? tid - tok0 * a.items_token : static_cast<int>(blockIdx.y) * threads + tid;
+  const bool has = item < a.items_token && tok0 < a.side;
+  // ---- this thread's place: part, head, vectors
+  int head = has ? item / a.items_head : 0;
+  const int j = has ? item - head * a.items_head : 0;
+  int w = 0;
+  if (head >= a.part[0].heads) {
+    head -= a.part[0].heads;
+    w = 1;
+    if (head >= a.part[1].heads) {
+      head -= a.part[1].heads;
+      w = 2;
     }
   }
+  const Part& p = a.part[w];
+  // two vectors a stretch apart, so that neighbouring threads' accesses touch: in
+  // the half layout the two of the same pairs, then those past 2n; else the
+  // head's first and second half
+  const bool half = p.turn && !a.interleaved;
+  const int lead = half ? slots : 0;                   // items that turn as (j, j + slots)
+  const bool turn_ab = j < lead;
+  const int va = turn_ab ? j : lead + j, vb = turn_ab ? j + slots : lead + j + a.items_head - lead;
+  const bool has_b = vb < vecs;
+  const int dab = (vb - va) * V;
+  const bool turn_a = p.turn && a.interleaved && va < slots, turn_b = p.turn && a.interleaved && vb < slots;
+  const bool paged = p.paged;
+  const int64_t xt = p.xt, yt = p.yt, yb = p.yb;
+  const T* x = static_cast<const T*>(p.x) + b * p.xb + l0 * xt + head * p.xh + va * V;
+  T* y = static_cast<T*>(p.y) + head * p.yh + va * V;
+  if (!paged) y += b * yb + l0 * yt;
+  auto fetch = [&](int t, int slot) {
+    if constexpr (kWide) {
+      if (has && t < nt) {
+        cp_async16(&ring[slot * 2 * threads], x + t * xt);
+        if (has_b) cp_async16(&ring[(slot * 2 + 1) * threads], x + t * xt + dab);
+      }
+      cp_async_commit();
+    }
+  };
+  if constexpr (kWide) {
+#pragma unroll
+    for (int k = 0; k < R_AHEAD - 1; ++k) fetch(tok0 + k * a.side, k);
+  }
+  // ---- the tokens' slots and angles
+  if (a.any_paged && tid < nt) {
+    const int64_t at = a.slots.position(b, a.start, a.len) + l0 + tid;
+    dst_page[tid] = a.slots.page_of(b, at);
+    dst_slot[tid] = static_cast<int>(at & (a.slots.page_size - 1));
+  }
+  if (a.pairs > 0) {
+    const int q = tid % a.pairs, at = q / per, e = q - at * per, step = threads / a.pairs;
+    const float inv = a.inv[q];
+    float2* c = cs + ((e >> 1) * slots + at) * 2 + (e & 1);
+    if (tid < step * a.pairs)
+      for (int tok = tid / a.pairs; tok < nt; tok += step) {
+        const int64_t pos = a.pos != nullptr ? a.pos[b * a.len + l0 + tok]
+                                             : a.slots.position(b, a.start, a.len) + l0 + tok;
+        c[tok * cs_tok] = turn_of(pos, inv, a.factor, a.inverse);
+      }
+  }
+  __syncthreads();
+  int slot = 0;
+  for (int t = tok0; t < nt; t += a.side) {
+    Vec xa, xb;
+    if constexpr (kWide) {
+      fetch(t + (R_AHEAD - 1) * a.side, slot == 0 ? R_AHEAD - 1 : slot - 1);
+      cp_async_wait<R_AHEAD - 1>();     // this thread's own copies: no other thread reads them
+      asm volatile("" ::: "memory");
+      xa = ring[slot * 2 * threads];
+      xb = ring[(slot * 2 + 1) * threads];
+      asm volatile("" ::: "memory");
+      slot = slot == R_AHEAD - 1 ? 0 : slot + 1;
+      if (!has) continue;
+    } else {
+      if (!has) break;
+      xa = *reinterpret_cast<const Vec*>(x + t * xt);
+      if (has_b) xb = *reinterpret_cast<const Vec*>(x + t * xt + dab);
+    }
+    const float2* c = cs + t * cs_tok;
+    if (turn_ab) {
+      float2 w2[V + 1];
+      pairs_of<V>(c, slots, j, w2);
+#pragma unroll
+      for (int e = 0; e < V; ++e) turn_pair(xa.e[e], xb.e[e], w2[e]);
+    }
+    if (turn_a) turn_neighbours<T, V>(xa, c, slots, va);
+    if (turn_b) turn_neighbours<T, V>(xb, c, slots, vb);
+    T* dst = y;
+    if (!paged) {
+      dst += t * yt;
+    } else {
+      const int64_t page = dst_page[t];
+      if (page < 0) continue;
+      dst += page * yb + dst_slot[t] * yt;
+    }
+    *reinterpret_cast<Vec*>(dst) = xa;
+    if (has_b) *reinterpret_cast<Vec*>(dst + dab) = xb;
+  }
+  if constexpr (kWide) cp_async_wait<0>();
 }
 
 // Whether 16-byte accesses fit: bases, strides, and the vectors' edges.
@@ -217,35 +245,53 @@ bool wide_ok(const RotaryArgs& a, int esize) {
 }
 
 template <typename T>
-int rotary_launch(RotaryArgs& a, cudaStream_t s) {
+int rotary_launch(RotaryArgs& a, int64_t batch, cudaStream_t s) {
   const bool wide = wide_ok(a, sizeof(T));
   // without 16-byte alignment: single elements (pairs in the interleaved layout)
   const int v = wide ? 16 / static_cast<int>(sizeof(T)) : (a.interleaved ? 2 : 1);
   if (a.head_dim % v) return MRSA_ERR_SHAPE;
   a.items_head = (a.head_dim / v + 1) / 2;
   const int64_t items = static_cast<int64_t>(a.part[0].heads + a.part[1].heads + a.part[2].heads) * a.items_head;
-  if (items > (1 << 24)) return MRSA_ERR_SHAPE;
+  if (items > (1 << 23)) return MRSA_ERR_SHAPE;
   a.items_token = static_cast<int>(items);
-  int64_t per = (R_THREADS * R_ITEMS) / items;
-  if (per > R_MAX_TOKENS) per = R_MAX_TOKENS;
-  if (per < 1) per = 1;
-  a.tokens_cta = static_cast<int>(per);
-  const int64_t blocks = (a.tokens + per - 1) / per;
-  if (blocks > 0x7fffffffLL) return MRSA_ERR_SHAPE;
-  const size_t smem = static_cast<size_t>(per) * a.pairs * sizeof(float2);
-  const unsigned g = static_cast<unsigned>(blocks);
-  if (wide) rotary_kernel<T, 16 / static_cast<int>(sizeof(T))><<<g, R_THREADS, smem, s>>>(a);
-  else if (a.interleaved) rotary_kernel<T, 2><<<g, R_THREADS, smem, s>>>(a);
-  else rotary_kernel<T, 1><<<g, R_THREADS, smem, s>>>(a);
+  a.side = items < R_THREADS ? static_cast<int>(R_THREADS / items) : 1;
+  if (a.side > R_MAX_RUN) a.side = R_MAX_RUN;
+  // few tokens: as many CTAs as there are; many: enough of them to a CTA for
+  // its loads to run ahead
+  // a token's items in as few passes as fit, each of the same whole warps
+  const unsigned passes = static_cast<unsigned>((items + R_MAX_THREADS - 1) / R_MAX_THREADS);
+  const int threads = items < R_THREADS ? R_THREADS : static_cast<int>(((items + passes - 1) / passes + 31) / 32 * 32);
+  int64_t run = batch * a.len * passes / (static_cast<int64_t>(sm_count()) * 8);
+  run = run < a.side ? a.side : run;
+  run = run > R_MAX_RUN ? R_MAX_RUN : run;
+  run = run > a.len ? a.len : run;
+  a.run = static_cast<int>(run);
+  a.runs = static_cast<int>((a.len + run - 1) / run);
+  if (batch * a.runs > 0x7fffffffLL) return MRSA_ERR_SHAPE;
+  const int pv = a.interleaved ? (v > 1 ? v / 2 : 1) : v;            // pairs to a slot of the angles
+  const size_t angles = static_cast<size_t>(run) * ((a.pairs + pv - 1) / pv) * ((pv + 1) / 2) * 2 * sizeof(float2);
+  const dim3 g(static_cast<unsigned>(batch * a.runs), passes);
+  if (wide) {
+    const auto kernel = rotary_kernel<T, 16 / static_cast<int>(sizeof(T)), true>;
+    const size_t ring = static_cast<size_t>(R_AHEAD) * 2 * threads * 16;
+    constexpr size_t kMost = R_AHEAD * 2 * R_MAX_THREADS * 16 + R_MAX_RUN * R_MAX_PAIRS * sizeof(float2) * 2;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kMost)) != cudaSuccess)
+      return MRSA_ERR_LAUNCH;
+    kernel<<<g, threads, ring + angles, s>>>(a);
+  } else if (a.interleaved) {
+    rotary_kernel<T, 2, false><<<g, threads, angles, s>>>(a);
+  } else {
+    rotary_kernel<T, 1, false><<<g, threads, angles, s>>>(a);
+  }
   MRSA_CHECK_LAUNCH();
   return MRSA_OK;
 }
 
-int dispatch(RotaryArgs& a, int dtype, cudaStream_t s) {
+int dispatch(RotaryArgs& a, int64_t batch, int dtype, cudaStream_t s) {
   switch (dtype) {
-    case MRSA_BF16: return rotary_launch<__nv_bfloat16>(a, s);
-    case MRSA_F16: return rotary_launch<__half>(a, s);
-    case MRSA_F32: return rotary_launch<float>(a, s);
+    case MRSA_BF16: return rotary_launch<__nv_bfloat16>(a, batch, s);
+    case MRSA_F16: return rotary_launch<__half>(a, batch, s);
+    case MRSA_F32: return rotary_launch<float>(a, batch, s);
     default: return MRSA_ERR_ARG;
   }
 }
@@ -273,7 +319,6 @@ RotaryArgs base_args(const mrsa_rotary_args* r) {
   a.pairs = static_cast<int>(r->pairs);
   a.head_dim = static_cast<int>(r->head_dim);
   a.len = static_cast<int>(r->len);
-  a.tokens = r->batch * r->len;
   const int64_t D = r->head_dim;
   a.part[0] = {r->q, r->q_out, r->q_batch_stride, r->q_token_stride, r->q_head_stride,
                r->len * r->q_heads * D, r->q_heads * D, D, static_cast<int>(r->q_heads), r->pairs > 0, 0};
@@ -292,7 +337,7 @@ extern "C" int mrsa_rotary(const mrsa_rotary_args* r, mrsa_stream_t stream) {
   if (r->position_ids == nullptr) return MRSA_ERR_NULL;
   mrsa::DeviceScope device_scope(r->position_ids);
   RotaryArgs a = base_args(r);
-  return dispatch(a, r->dtype, static_cast<cudaStream_t>(stream));
+  return dispatch(a, r->batch, r->dtype, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int mrsa_paged_append(const mrsa_rotary_args* r, const mrsa_page_table* t, const mrsa_paged_append_args* p,
@@ -324,5 +369,5 @@ extern "C" int mrsa_paged_append(const mrsa_rotary_args* r, const mrsa_page_tabl
   a.slots.page_shift = mrsa::log2_int(t->page_size);
   a.start = p->start;
   a.any_paged = 1;
-  return dispatch(a, r->dtype, static_cast<cudaStream_t>(stream));
+  return dispatch(a, r->batch, r->dtype, static_cast<cudaStream_t>(stream));
 }
