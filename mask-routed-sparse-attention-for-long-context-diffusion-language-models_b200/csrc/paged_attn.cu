@@ -90,9 +90,7 @@ __global__ void __launch_bounds__(A_THREADS) paged_token_kernel(const __grid_con
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
 
-  paged::count_tiles<A_THREADS>(a, A_TILE, sm.prefix, sm.warp_sums);
-  if (blockIdx.x == 0)
-    for (int i = tid; i <= a.batch; i += A_THREADS) a.prefix[i] = sm.prefix[i];
+  paged::count_tiles<A_THREADS>(a, sm.prefix, sm.warp_sums);
   const int per = a.kv_heads * a.row_tiles;            // units per batch row
   const int64_t total = static_cast<int64_t>(sm.prefix[a.batch]) * per;
   const int64_t grid = paged::dealt(a, total);
@@ -335,73 +333,98 @@ __global__ void __launch_bounds__(A_THREADS) paged_token_kernel(const __grid_con
   }
 }
 
-// One block per (batch row, KV head, query row): nothing to do for a unit that
-// one CTA finished, zeros for one without keys, else its pieces joined, eight
-// warps on every eighth piece.
+// The pieces of each query row joined: nothing to do for a unit that one CTA
+// finished, zeros for one without keys.  kShare warps work on a row, each on
+// every kShare-th piece: all eight of the block when few rows have many pieces
+// (one long sequence), one when many rows have few.  All that comes from the
+// lengths alone is worked out before the wait for the parts.
 constexpr int J_WARPS = 8;
 
-template <int kD, bool kF16>
+template <int kD, bool kF16, int kShare>
 __global__ void __launch_bounds__(32 * J_WARPS) paged_join_kernel(const __grid_constant__ Args a) {
   constexpr int kV = kD / 32;
-  __shared__ float acc_s[J_WARPS][kD], m_s[J_WARPS], l_s[J_WARPS];
-  asm volatile("griddepcontrol.wait;\n" ::: "memory");
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int r = blockIdx.x % a.rows, bh = blockIdx.x / a.rows, h = bh % a.kv_heads, b = bh / a.kv_heads;
+  __shared__ float acc_s[kShare > 1 ? J_WARPS : 1][kD], m_s[J_WARPS], l_s[J_WARPS];
+  __shared__ int prefix[paged::kMaxBatch + 1], warp_sums[J_WARPS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = warp % kShare;
+  paged::count_tiles<32 * J_WARPS>(a, prefix, warp_sums);
   const int per = a.kv_heads * a.row_tiles;
-  const int p0 = a.prefix[b], tiles = a.prefix[b + 1] - p0;
-  const int64_t total = static_cast<int64_t>(a.prefix[a.batch]) * per;
-  const int rt = r / a.row_tile, rr = r - rt * a.row_tile;
-  const int i = r / a.group, g = r - i * a.group;
-  const int64_t at = (static_cast<int64_t>(b) * a.len + i) * a.q_heads + h * a.group + g;
-  if (tiles == 0) {
-    for (int d = threadIdx.x; d < kD; d += 32 * J_WARPS) store_out<kF16>(a.out + (at * kD + d) * 2, 0.f);
-    if (threadIdx.x == 0 && a.lse != nullptr) a.lse[at] = -INFINITY;
-    return;
-  }
-  const int64_t first = static_cast<int64_t>(p0) * per + static_cast<int64_t>(h * a.row_tiles + rt) * tiles;
-  const int64_t grid = paged::dealt(a, total);
-  const int c0 = paged::holder(first, total, grid), c1 = paged::holder(first + tiles - 1, total, grid);
-  if (c0 == c1) return;
-  float m = -INFINITY, l = 0.f, acc[kV];
-#pragma unroll
-  for (int e = 0; e < kV; ++e) acc[e] = 0.f;
-#pragma unroll 4
-  for (int c = c0 + warp; c <= c1; c += J_WARPS) {
-    const int64_t slot = paged::slot_of(c, c0, first, total, grid);
-    const float* ml = a.part_ml + (slot * a.row_tile + rr) * 2;
-    const float* o = a.part_o + (slot * a.row_tile + rr) * kD + lane * kV;
-    const float pm = ml[0], pl = ml[1];
-    float x[kV];
-#pragma unroll
-    for (int e = 0; e < kV; ++e) x[e] = o[e];
-    const float top = fmaxf(m, pm);
-    const float cm = m == -INFINITY ? 0.f : fast_exp2(m - top), cp = pm == -INFINITY ? 0.f : fast_exp2(pm - top);
-    m = top;
-    l = l * cm + pl * cp;
-#pragma unroll
-    for (int e = 0; e < kV; ++e) acc[e] = acc[e] * cm + x[e] * cp;
-  }
-#pragma unroll
-  for (int e = 0; e < kV; ++e) acc_s[warp][lane * kV + e] = acc[e];
-  if (lane == 0) {
-    m_s[warp] = m;
-    l_s[warp] = l;
-  }
-  __syncthreads();
-  for (int d = threadIdx.x; d < kD; d += 32 * J_WARPS) {
-    float top = m_s[0];
-#pragma unroll
-    for (int w = 1; w < J_WARPS; ++w) top = fmaxf(top, m_s[w]);
-    float sum = 0.f, v = 0.f;
-#pragma unroll
-    for (int w = 0; w < J_WARPS; ++w) {
-      const float c = m_s[w] == -INFINITY ? 0.f : fast_exp2(m_s[w] - top);
-      sum += c * l_s[w];
-      v += c * acc_s[w][d];
+  const int64_t total = static_cast<int64_t>(prefix[a.batch]) * per, grid = paged::dealt(a, total);
+  const int64_t rows = static_cast<int64_t>(a.batch) * a.kv_heads * a.rows;
+  bool waited = false;
+  for (int64_t row = blockIdx.x * (J_WARPS / kShare) + warp / kShare; row < rows;
+       row += static_cast<int64_t>(gridDim.x) * (J_WARPS / kShare)) {
+    const int64_t bh = row / a.rows;
+    const int r = static_cast<int>(row - bh * a.rows), b = static_cast<int>(bh / a.kv_heads);
+    const int h = static_cast<int>(bh) - b * a.kv_heads;
+    const int tiles = prefix[b + 1] - prefix[b];
+    const int rt = r / a.row_tile, rr = r - rt * a.row_tile;
+    const int i = r / a.group, g = r - i * a.group;
+    const int64_t at = (static_cast<int64_t>(b) * a.len + i) * a.q_heads + h * a.group + g;
+    const int64_t first = static_cast<int64_t>(prefix[b]) * per + static_cast<int64_t>(h * a.row_tiles + rt) * tiles;
+    int c0 = 0, c1 = -1;
+    if (tiles > 0) {
+      c0 = paged::holder(first, total, grid);
+      c1 = paged::holder(first + tiles - 1, total, grid);
+      if (c0 == c1) continue;
     }
-    store_out<kF16>(a.out + (at * kD + d) * 2, sum > 0.f ? v / sum : 0.f);
-    if (d == 0 && a.lse != nullptr) a.lse[at] = sum > 0.f ? (top + log2f(sum)) * kLn2 : -INFINITY;
+    if (!waited) {
+      waited = true;
+      asm volatile("griddepcontrol.wait;\n" ::: "memory");
+    }
+    float m = -INFINITY, l = 0.f, acc[kV];
+#pragma unroll
+    for (int e = 0; e < kV; ++e) acc[e] = 0.f;
+    const int64_t slot0 = paged::slot_of(c0, c0, first, total, grid);
+#pragma unroll 4
+    for (int c = c0 + sub; c <= c1; c += kShare) {
+      const int64_t slot = c == c0 ? slot0 : 2 * static_cast<int64_t>(c);
+      const float* ml = a.part_ml + (slot * a.row_tile + rr) * 2;
+      const float* o = a.part_o + (slot * a.row_tile + rr) * kD + lane * kV;
+      const float2 p = __ldcg(reinterpret_cast<const float2*>(ml));
+      float x[kV];
+      if constexpr (kV == 4) {
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(o));
+        x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+      } else {
+        const float2 v = __ldcg(reinterpret_cast<const float2*>(o));
+        x[0] = v.x; x[1] = v.y;
+      }
+      const float top = fmaxf(m, p.x);
+      const float cm = m == -INFINITY ? 0.f : fast_exp2(m - top), cp = p.x == -INFINITY ? 0.f : fast_exp2(p.x - top);
+      m = top;
+      l = l * cm + p.y * cp;
+#pragma unroll
+      for (int e = 0; e < kV; ++e) acc[e] = acc[e] * cm + x[e] * cp;
+    }
+    if constexpr (kShare > 1) {
+#pragma unroll
+      for (int e = 0; e < kV; ++e) acc_s[warp][lane * kV + e] = acc[e];
+      if (lane == 0) {
+        m_s[warp] = m;
+        l_s[warp] = l;
+      }
+      __syncthreads();          // kShare is the whole block: its warps take the same turns
+      if (sub == 0) {
+#pragma unroll
+        for (int w = 1; w < kShare; ++w) {
+          const float pm = m_s[w], top = fmaxf(m, pm);
+          const float cm = m == -INFINITY ? 0.f : fast_exp2(m - top), cp = pm == -INFINITY ? 0.f : fast_exp2(pm - top);
+          m = top;
+          l = l * cm + l_s[w] * cp;
+#pragma unroll
+          for (int e = 0; e < kV; ++e) acc[e] = acc[e] * cm + acc_s[w][lane * kV + e] * cp;
+        }
+      }
+      __syncthreads();
+    }
+    if (sub == 0) {
+#pragma unroll
+      for (int e = 0; e < kV; ++e) store_out<kF16>(a.out + (at * kD + lane * kV + e) * 2, l > 0.f ? acc[e] / l : 0.f);
+      if (lane == 0 && a.lse != nullptr) a.lse[at] = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+    }
   }
+  // a block that read no part waits too: what follows in the stream follows this grid's end
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
 }
 
 template <int kD, int kNT, bool kF16>
@@ -446,14 +469,16 @@ namespace mrsa {
 namespace paged {
 
 size_t workspace(int64_t grid, int64_t row_tile, int64_t head_dim) {
-  return static_cast<size_t>(2 * grid * row_tile * (head_dim + 2) + kMaxBatch + 64) * 4;
+  return static_cast<size_t>(2 * grid * row_tile * (head_dim + 2)) * 4;
 }
 
 int launch_join(const Args& a, int dtype, int head_dim, cudaStream_t s) {
-  const int64_t blocks = static_cast<int64_t>(a.batch) * a.kv_heads * a.rows;
-  if (blocks > 0x7fffffffLL) return MRSA_ERR_SHAPE;
+  const int64_t units = static_cast<int64_t>(a.batch) * a.kv_heads * a.row_tiles;
+  const int64_t rows = static_cast<int64_t>(a.batch) * a.kv_heads * a.rows;
+  const bool share = a.grid >= 8 * units;         // eight pieces and more to a unit
+  const int64_t blocks = share ? rows : (rows + J_WARPS - 1) / J_WARPS, most = 8 * static_cast<int64_t>(sm_count());
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks < most ? blocks : most));
   cfg.blockDim = dim3(32 * J_WARPS);
   cfg.stream = s;
   cudaLaunchAttribute attr;
@@ -461,12 +486,16 @@ int launch_join(const Args& a, int dtype, int head_dim, cudaStream_t s) {
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
+  void (*kernel)(const Args);
   const bool f16 = dtype == MRSA_F16;
-  const cudaError_t e =
-      head_dim == 128 ? (f16 ? cudaLaunchKernelEx(&cfg, paged_join_kernel<128, true>, a)
-                             : cudaLaunchKernelEx(&cfg, paged_join_kernel<128, false>, a))
-                      : (f16 ? cudaLaunchKernelEx(&cfg, paged_join_kernel<64, true>, a)
-                             : cudaLaunchKernelEx(&cfg, paged_join_kernel<64, false>, a));
+  if (head_dim == 128) {
+    if (f16) kernel = share ? paged_join_kernel<128, true, J_WARPS> : paged_join_kernel<128, true, 1>;
+    else kernel = share ? paged_join_kernel<128, false, J_WARPS> : paged_join_kernel<128, false, 1>;
+  } else {
+    if (f16) kernel = share ? paged_join_kernel<64, true, J_WARPS> : paged_join_kernel<64, true, 1>;
+    else kernel = share ? paged_join_kernel<64, false, J_WARPS> : paged_join_kernel<64, false, 1>;
+  }
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
   if (e != cudaSuccess) {
     note_cuda_error(e, __func__);
     (void)cudaGetLastError();
@@ -535,11 +564,11 @@ extern "C" int mrsa_paged_attention(const mrsa_paged_attention_args* p, const mr
   a.scale_log2 = p->scale * kLog2e;
   a.row_tile = row_tile_of(a.rows);
   a.row_tiles = (a.rows + a.row_tile - 1) / a.row_tile;
+  a.tile = A_TILE;          // of both kernels
   a.grid = grid_of(a.rows);
   const int64_t slots = 2 * static_cast<int64_t>(a.grid) * a.row_tile;
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = a.part_o + slots * p->head_dim;
-  a.prefix = reinterpret_cast<int32_t*>(a.part_ml + slots * 2);
   // more batch rows than a CTA keeps tile counts of: one stretch of them after another
   for (int64_t b0 = 0; b0 < p->batch; b0 += paged::kMaxBatch) {
     a.batch = static_cast<int>(p->batch - b0 < paged::kMaxBatch ? p->batch - b0 : paged::kMaxBatch);

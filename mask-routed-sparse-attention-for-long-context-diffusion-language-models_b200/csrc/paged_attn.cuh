@@ -35,11 +35,11 @@ struct Args {
   int64_t kp, ks, kh, vp, vs, vh;      // bytes: page, slot, head
   int max_seqs, max_pages, pages, page_size, page_shift;
   int batch, len, q_heads, kv_heads, group, rows, row_tile, row_tiles, causal;
+  int tile;                            // keys per tile
   int grid;                            // CTAs that the tiles are dealt to
   float scale_log2;                    // softmax scale times log2(e)
   float* part_o;                       // [2 * grid][row_tile][D]
   float* part_ml;                      // [2 * grid][row_tile][2]: maximum (log2), sum
-  int32_t* prefix;                     // [batch + 1] tiles per (head, row tile) before each batch row
 };
 
 // Cached tokens of batch row b that may be read.
@@ -101,15 +101,15 @@ __device__ __forceinline__ Piece piece_at(const Args& a, const int* prefix, int6
   return p;
 }
 
-// Tiles of `tile` keys before each batch row (per head and row tile), by all
+// Key tiles before each batch row (per head and row tile), by all
 // threads of the CTA.
 template <int kThreads>
-__device__ __forceinline__ void count_tiles(const Args& a, int tile, int* prefix, int* warp_sums) {
+__device__ __forceinline__ void count_tiles(const Args& a, int* prefix, int* warp_sums) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int run = 0;
   for (int b0 = 0; b0 < a.batch; b0 += kThreads) {
     const int b = b0 + static_cast<int>(threadIdx.x);
-    const int t = b < a.batch ? (cached_tokens(a, b) + tile - 1) / tile : 0;
+    const int t = b < a.batch ? (cached_tokens(a, b) + a.tile - 1) / a.tile : 0;
     int x = t;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {

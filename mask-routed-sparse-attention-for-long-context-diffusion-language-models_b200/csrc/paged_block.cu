@@ -15,8 +15,8 @@
 // and 1; warp 8: K tiles and key masks, warp 11: V tiles, both by TMA, one box
 // per page part and 64 dims, straight from the pages the table names; warps 9
 // and 10: MMA issue.  Rings and buffers run on from one unit of the stretch to
-// the next.  Masked keys leave the softmax; their V rows are zeroed in shared
-// memory first, since what a masked or unused slot holds may not be a number.
+// the next.  Masked keys leave the softmax, and warp 11 zeroes their V rows in
+// shared memory, since what a masked or unused slot holds may not be a number.
 // Every wait is bounded: a CTA that gives up unwinds and sets bit 7 of
 // mrsa_device_error_flags.
 #include <cuda.h>
@@ -49,8 +49,9 @@ struct __align__(1024) BlockSmem {
   unsigned char q[2][kD / 64][B_ROWS * 128];     // [row tile][64 dims][row], 128-byte swizzled
   unsigned char k[NKS][kD / 64][B_TILE * 128];
   unsigned char v[NVS][kD / 64][B_TILE * 128];   // the MN-major B operand of P.V
+  float limit[NMS][B_TILE];                      // +inf for a key that counts, else -inf
   unsigned long long kmask[NMS];                 // bit j: key j of the tile counts
-  uint64_t qfull[2], kfull[NKS], kfree[NKS], vfull[NVS], vfree[NVS], mfull[NMS];
+  uint64_t qfull[2], kfull[NKS], kfree[NKS], vfull[NVS], vfree[NVS], vclean[NVS], mfull[NMS];
   uint64_t sfull[4], pready[4], pfree[4], drain[2];
   uint32_t tmem_base;
   int abort_flag;
@@ -98,6 +99,7 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
     for (int s = 0; s < NVS; ++s) {
       tc::mbar_init(tc::smem_addr(&sm.vfull[s]), 1);
       tc::mbar_init(tc::smem_addr(&sm.vfree[s]), 2);
+      tc::mbar_init(tc::smem_addr(&sm.vclean[s]), 1);
     }
     for (int s = 0; s < NMS; ++s) tc::mbar_init(tc::smem_addr(&sm.mfull[s]), 1);
     for (int s = 0; s < 4; ++s) {
@@ -116,9 +118,7 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
     tc::tmem_alloc(tc::smem_addr(&sm.tmem_base), 512);
     tc::tmem_relinquish();
   }
-  paged::count_tiles<B_THREADS>(a, B_TILE, sm.prefix, sm.warp_sums);
-  if (blockIdx.x == 0)
-    for (int i = tid; i <= a.batch; i += B_THREADS) a.prefix[i] = sm.prefix[i];
+  paged::count_tiles<B_THREADS>(a, sm.prefix, sm.warp_sums);
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
@@ -139,6 +139,27 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
     static_assert(NKS == NVS, "K and V stages share their index");
     if (lane == 0) tc::prefetch_tensormap(map);
     const TilePages tp(a);
+    // V rows of keys that do not count, zeroed kLag tiles behind the copies (a
+    // P of zero does not cancel what is not a number); the MMA warps wait for
+    // it where a tile has such keys
+    constexpr int kLag = 2;
+    auto clean = [&](int tile) -> bool {
+      if (!tc::wait_bounded_warp(tc::smem_addr(&sm.mfull[tile % NMS]), (tile / NMS) & 1, abort_flag)) return false;
+      const unsigned long long km = sm.kmask[tile % NMS];
+      const int st = tile % NVS;
+      if (km != ~0ull) {
+        if (!tc::wait_bounded_warp(tc::smem_addr(&sm.vfull[st]), (tile / NVS) & 1, abort_flag)) return false;
+        for (unsigned long long rest = ~km; rest != 0; rest &= rest - 1) {
+          const int key = __ffsll(static_cast<long long>(rest)) - 1;
+          if (lane < kD / 8)
+            *reinterpret_cast<uint4*>(sm.v[st][lane >> 3] + key * 128 + (lane & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+        }
+        tc::fence_proxy_async();
+        __syncwarp();
+      }
+      if (lane == 0) tc::mbar_arrive(tc::smem_addr(&sm.vclean[st]));
+      return true;
+    };
     int e = 0;                                   // tiles of the stretch so far
     for (int64_t t_now = t_begin; ok && t_now < t_end;) {
       const Piece p = paged::piece_at(a, sm.prefix, t_now, t_end);
@@ -170,8 +191,11 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const int in = 32 * i + lane, key = t * B_TILE + in;
-            mk[i] = __ballot_sync(0xffffffffu, key < p.n && vb[i] != 0u && ((has >> (in / tp.part_keys)) & 1u));
+            const bool counts = key < p.n && vb[i] != 0u && ((has >> (in / tp.part_keys)) & 1u);
+            mk[i] = __ballot_sync(0xffffffffu, counts);
+            sm.limit[e % NMS][in] = counts ? INFINITY : -INFINITY;
           }
+          __syncwarp();
           if (lane == 0) {
             sm.kmask[e % NMS] = static_cast<unsigned long long>(mk[0]) | (static_cast<unsigned long long>(mk[1]) << 32);
             tc::mbar_arrive(tc::smem_addr(&sm.mfull[e % NMS]));
@@ -188,9 +212,12 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
                             p.h, page, bar);
         }
         __syncwarp();
+        if (!is_k && e >= kLag && !(ok = clean(e - kLag))) break;
       }
       t_now += p.tile1 - p.tile0;
     }
+    if (!is_k)
+      for (int tt = e < kLag ? 0 : e - kLag; ok && tt < e; ++tt) ok = clean(tt);
     // wait (bounded, even after an abort) for the copies in flight
     if (lane == 0)
       for (int tt = e - NKS < 0 ? 0 : e - NKS; tt < e; ++tt)
@@ -250,7 +277,9 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
         for (int i = 0; ok && i < nt; ++i, ++e, ++k) {
           const int sb = 2 * g + (k & 1), sv = e % NVS;
           if (!(ok = tc::wait_bounded_warp(tc::smem_addr(&sm.pready[sb]), (k >> 1) & 1, abort_flag))) break;
-          if (!(ok = tc::wait_bounded_warp(tc::smem_addr(&sm.vfull[sv]), (e / NVS) & 1, abort_flag))) break;
+          // (the softmax has read the mask, and its slot is not reused before this P.V)
+          uint64_t* vbar = sm.kmask[e % NMS] == ~0ull ? &sm.vfull[sv] : &sm.vclean[sv];
+          if (!(ok = tc::wait_bounded_warp(tc::smem_addr(vbar), (e / NVS) & 1, abort_flag))) break;
           tc::fence_after_sync();
           const uint64_t dv = tc::desc_adv(dv0, sv * kStage);
           const uint32_t dO = tbase + kOCol + 128 * g, aP = tbase + B_TILE * sb;
@@ -319,9 +348,16 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
           const int seen = last - j0;              // columns past it are out of this row's sight
           const bool full = km == ~0ull && seen >= B_TILE - 1;
           if (km != ~0ull) {
+            // one minimum per column instead of a test and a choice; of NaN and -inf it is -inf
+            const float4* lim = reinterpret_cast<const float4*>(sm.limit[e % NMS]);
 #pragma unroll
-            for (int c = 0; c < B_TILE; ++c)
-              if (!((km >> c) & 1ull)) x[c] = __float_as_uint(-INFINITY);
+            for (int c = 0; c < B_TILE; c += 4) {
+              const float4 w = lim[c / 4];
+              x[c] = __float_as_uint(fminf(__uint_as_float(x[c]), w.x));
+              x[c + 1] = __float_as_uint(fminf(__uint_as_float(x[c + 1]), w.y));
+              x[c + 2] = __float_as_uint(fminf(__uint_as_float(x[c + 2]), w.z));
+              x[c + 3] = __float_as_uint(fminf(__uint_as_float(x[c + 3]), w.w));
+            }
           }
           if (seen < B_TILE - 1) {
 #pragma unroll
@@ -371,20 +407,6 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
           tc::tmem_st16(t_s, &pk[0]);
           tc::tmem_st16(t_s + 16, &pk[16]);
           tc::tmem_wait_st();
-          if (km != ~0ull) {
-            // V rows of keys that do not count: zeroed (by both groups alike), seen by the tensor core
-            const int sv = e % NVS, key = r >> 1;
-            if (!(ok = tc::wait_bounded_warp(tc::smem_addr(&sm.vfull[sv]), (e / NVS) & 1, abort_flag))) break;
-            if (!((km >> key) & 1ull)) {
-#pragma unroll
-              for (int hf = 0; hf < kHalves; ++hf)
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                  *reinterpret_cast<uint4*>(sm.v[sv][hf] + key * 128 + (r & 1) * 64 + j * 16) = make_uint4(0u, 0u, 0u, 0u);
-            }
-            tc::fence_proxy_async();
-            __syncwarp();
-          }
           if (__any_sync(0xffffffffu, rescale)) {
             // O holds every earlier tile of the unit once the P.V before this one is done
             if (!(ok = tc::wait_bounded_warp(tc::smem_addr(&sm.pfree[2 * g + ((k - 1) & 1)]), ((k - 1) >> 1) & 1, abort_flag)))
