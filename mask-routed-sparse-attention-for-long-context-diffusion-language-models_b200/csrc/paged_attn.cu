@@ -74,7 +74,7 @@ struct TokenSmem {
   alignas(128) unsigned char ring[A_WARPS][A_STAGES][2][A_KEYS * kD * 2];
   uint32_t mask[A_WARPS][A_STAGES];        // keys of the stage that count
   float m[A_WARPS][8 * kNT], l[A_WARPS][8 * kNT];
-  int prefix[paged::kMaxBatch + 1];
+  paged::Batch batch;
   int warp_sums[A_WARPS];
 };
 
@@ -90,15 +90,15 @@ __global__ void __launch_bounds__(A_THREADS) paged_token_kernel(const __grid_con
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
 
-  paged::count_tiles<A_THREADS>(a, sm.prefix, sm.warp_sums);
+  paged::count_tiles<A_THREADS>(a, sm.batch, sm.warp_sums);
   const int per = a.kv_heads * a.row_tiles;            // units per batch row
-  const int64_t total = static_cast<int64_t>(sm.prefix[a.batch]) * per;
+  const int64_t total = static_cast<int64_t>(sm.batch.prefix[a.batch]) * per;
   const int64_t grid = paged::dealt(a, total);
   const int64_t t_begin = blockIdx.x < grid ? paged::stretch(blockIdx.x, total, grid) : 0;
   const int64_t t_end = blockIdx.x < grid ? paged::stretch(blockIdx.x + 1, total, grid) : 0;
 
   for (int64_t t_now = t_begin; t_now < t_end;) {
-    const paged::Piece pc = paged::piece_at(a, sm.prefix, t_now, t_end);
+    const paged::Piece pc = paged::piece_at(a, sm.batch, t_now, t_end);
     const int b = pc.b, h = pc.h, n = pc.n, r0 = pc.r0, nrows = pc.nrows, tile0 = pc.tile0, tile1 = pc.tile1;
 
     // ---- this thread's part of Q^T: column lane / 4 of each 8-row block
@@ -344,9 +344,11 @@ template <int kD, bool kF16, int kShare>
 __global__ void __launch_bounds__(32 * J_WARPS) paged_join_kernel(const __grid_constant__ Args a) {
   constexpr int kV = kD / 32;
   __shared__ float acc_s[kShare > 1 ? J_WARPS : 1][kD], m_s[J_WARPS], l_s[J_WARPS];
-  __shared__ int prefix[paged::kMaxBatch + 1], warp_sums[J_WARPS];
+  __shared__ paged::Batch batch;
+  __shared__ int warp_sums[J_WARPS];
+  const int* prefix = batch.prefix;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = warp % kShare;
-  paged::count_tiles<32 * J_WARPS>(a, prefix, warp_sums);
+  paged::count_tiles<32 * J_WARPS>(a, batch, warp_sums);
   const int per = a.kv_heads * a.row_tiles;
   const int64_t total = static_cast<int64_t>(prefix[a.batch]) * per, grid = paged::dealt(a, total);
   const int64_t rows = static_cast<int64_t>(a.batch) * a.kv_heads * a.rows;

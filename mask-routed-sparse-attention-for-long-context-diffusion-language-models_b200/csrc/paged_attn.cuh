@@ -18,7 +18,7 @@
 namespace mrsa {
 namespace paged {
 
-constexpr int kMaxBatch = 1024;   // batch rows per launch
+constexpr int kMaxBatch = 512;    // batch rows per launch
 
 struct Args {
   const char* q;
@@ -78,8 +78,15 @@ struct Piece {
   __device__ __forceinline__ bool whole() const { return tile0 == 0 && tile1 == tiles; }
 };
 
+// What a CTA keeps of the batch: each row's sequence and cached tokens, and the
+// key tiles before it (per head and row tile).
+struct Batch {
+  int prefix[kMaxBatch + 1], seq[kMaxBatch], len[kMaxBatch];
+};
+
 // The part that begins at tile `t` and ends with its unit or at `end`.
-__device__ __forceinline__ Piece piece_at(const Args& a, const int* prefix, int64_t t, int64_t end) {
+__device__ __forceinline__ Piece piece_at(const Args& a, const Batch& s, int64_t t, int64_t end) {
+  const int* prefix = s.prefix;
   const int per = a.kv_heads * a.row_tiles;            // units per batch row
   int lo = 0, hi = a.batch - 1;                        // the last batch row whose tiles begin at or before t
   while (lo < hi) {
@@ -90,26 +97,32 @@ __device__ __forceinline__ Piece piece_at(const Args& a, const int* prefix, int6
   p.b = lo;
   p.tiles = prefix[lo + 1] - prefix[lo];
   const int64_t in_row = t - static_cast<int64_t>(prefix[lo]) * per;
-  const int unit = static_cast<int>(in_row / p.tiles);
+  const int unit = in_row >> 32 ? static_cast<int>(in_row / p.tiles)
+                                : static_cast<int>(static_cast<uint32_t>(in_row) / static_cast<uint32_t>(p.tiles));
   p.tile0 = static_cast<int>(in_row - static_cast<int64_t>(unit) * p.tiles);
   p.tile1 = end - t < p.tiles - p.tile0 ? p.tile0 + static_cast<int>(end - t) : p.tiles;
   p.h = unit / a.row_tiles;
   p.r0 = (unit - p.h * a.row_tiles) * a.row_tile;
   p.nrows = a.rows - p.r0 < a.row_tile ? a.rows - p.r0 : a.row_tile;
-  p.seq = a.seqs[lo];
-  p.n = a.lengths[p.seq];
+  p.seq = s.seq[lo];
+  p.n = s.len[lo];
   return p;
 }
 
-// Key tiles before each batch row (per head and row tile), by all
-// threads of the CTA.
+// Fills `s`, by all threads of the CTA.
 template <int kThreads>
-__device__ __forceinline__ void count_tiles(const Args& a, int* prefix, int* warp_sums) {
+__device__ __forceinline__ void count_tiles(const Args& a, Batch& s, int* warp_sums) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int run = 0;
   for (int b0 = 0; b0 < a.batch; b0 += kThreads) {
     const int b = b0 + static_cast<int>(threadIdx.x);
-    const int t = b < a.batch ? (cached_tokens(a, b) + a.tile - 1) / a.tile : 0;
+    int t = 0;
+    if (b < a.batch) {
+      const int n = cached_tokens(a, b);
+      s.seq[b] = a.seqs[b];
+      s.len[b] = n;
+      t = (n + a.tile - 1) / a.tile;
+    }
     int x = t;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -124,10 +137,10 @@ __device__ __forceinline__ void count_tiles(const Args& a, int* prefix, int* war
       if (w < warp) before += warp_sums[w];
       run += warp_sums[w];
     }
-    if (b < a.batch) prefix[b] = before + x - t;
+    if (b < a.batch) s.prefix[b] = before + x - t;
     __syncthreads();
   }
-  if (threadIdx.x == 0) prefix[a.batch] = run;
+  if (threadIdx.x == 0) s.prefix[a.batch] = run;
   __syncthreads();
 }
 

@@ -55,7 +55,7 @@ struct __align__(1024) BlockSmem {
   uint64_t sfull[4], pready[4], pfree[4], drain[2];
   uint32_t tmem_base;
   int abort_flag;
-  int prefix[paged::kMaxBatch + 1];
+  paged::Batch batch;
   int warp_sums[B_THREADS / 32];
 };
 static_assert(sizeof(BlockSmem<128>) + 1024 <= 232448, "paged attention shared memory over budget");
@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
 
-  if (tid == 0) {
+  if (tid == 32) {
     for (int s = 0; s < NKS; ++s) {
       tc::mbar_init(tc::smem_addr(&sm.kfull[s]), 1);
       tc::mbar_init(tc::smem_addr(&sm.kfree[s]), 2);
@@ -114,16 +114,16 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
     sm.abort_flag = 0;
     tc::fence_mbar_init();
   }
-  if (warp == 0) {
+  if (warp == 2) {
     tc::tmem_alloc(tc::smem_addr(&sm.tmem_base), 512);
     tc::tmem_relinquish();
   }
-  paged::count_tiles<B_THREADS>(a, sm.prefix, sm.warp_sums);
+  paged::count_tiles<B_THREADS>(a, sm.batch, sm.warp_sums);
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tbase = sm.tmem_base;
-  const int64_t total = static_cast<int64_t>(sm.prefix[a.batch]) * a.kv_heads * a.row_tiles;
+  const int64_t total = static_cast<int64_t>(sm.batch.prefix[a.batch]) * a.kv_heads * a.row_tiles;
   const int64_t grid = paged::dealt(a, total);
   const int64_t t_begin = blockIdx.x < grid ? paged::stretch(blockIdx.x, total, grid) : 0;
   const int64_t t_end = blockIdx.x < grid ? paged::stretch(blockIdx.x + 1, total, grid) : 0;
@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
     };
     int e = 0;                                   // tiles of the stretch so far
     for (int64_t t_now = t_begin; ok && t_now < t_end;) {
-      const Piece p = paged::piece_at(a, sm.prefix, t_now, t_end);
+      const Piece p = paged::piece_at(a, sm.batch, t_now, t_end);
       const uint8_t* valid = a.valid != nullptr && is_k
                                  ? a.valid + static_cast<int64_t>(p.b) * a.max_pages * a.page_size : nullptr;
       // the next tile's page numbers and mask bytes are requested a tile ahead
@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
       return true;
     };
     for (int64_t t_now = t_begin; ok && t_now < t_end;) {
-      const Piece p = paged::piece_at(a, sm.prefix, t_now, t_end);
+      const Piece p = paged::piece_at(a, sm.batch, t_now, t_end);
       const int nt = p.tile1 - p.tile0;
       if (p.nrows <= g * B_ROWS) {
         // no rows for this group: the unit's stages released unused, in order
@@ -311,22 +311,31 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
     const uint32_t t_o = tbase + lane_off + kOCol + 128 * g;
     int e0 = 0, k = 0;            // tiles of the stretch before this unit; tiles of this group so far
     for (int64_t t_now = t_begin; ok && t_now < t_end;) {
-      const Piece p = paged::piece_at(a, sm.prefix, t_now, t_end);
+      const Piece p = paged::piece_at(a, sm.batch, t_now, t_end);
       const int nt = p.tile1 - p.tile0;
       if (p.nrows > g * B_ROWS) {
         // ---- this row of Q (the S products of the unit before are done: the last S was read)
         const int row = g * B_ROWS + r;
         const bool row_ok = row < p.nrows;
-        const int qi = (p.r0 + (row_ok ? row : 0)) / a.group, qg = (p.r0 + (row_ok ? row : 0)) - qi * a.group;
+        const int qi = (p.r0 + (row_ok ? row : 0)) / a.group;
+        // the warp's 32 rows, whole rows at a time (a thread per row would touch 32 lines with every load)
         {
-          const char* src = a.q + p.b * a.qb + qi * a.qt + (p.h * a.group + qg) * a.qh;
-          uint4 x[kD / 8];
+          constexpr int kPieces = kD / 8, kPer = 32 / kPieces;     // 16-byte pieces of a row, rows per load
+          const int j = lane % kPieces;
+          uint4 x[kPieces];
 #pragma unroll
-          for (int j = 0; j < kD / 8; ++j)
-            x[j] = row_ok ? *reinterpret_cast<const uint4*>(src + j * 16) : make_uint4(0u, 0u, 0u, 0u);
+          for (int i = 0; i < kPieces; ++i) {
+            const int in = (warp & 3) * 32 + i * kPer + lane / kPieces, qr = g * B_ROWS + in;
+            const int ti = (p.r0 + qr) / a.group, tg = (p.r0 + qr) - ti * a.group;
+            x[i] = qr < p.nrows
+                       ? *reinterpret_cast<const uint4*>(a.q + p.b * a.qb + ti * a.qt + (p.h * a.group + tg) * a.qh + j * 16)
+                       : make_uint4(0u, 0u, 0u, 0u);
+          }
 #pragma unroll
-          for (int j = 0; j < kD / 8; ++j)
-            *reinterpret_cast<uint4*>(sm.q[g][j / 8] + r * 128 + (((j & 7) ^ (r & 7)) * 16)) = x[j];
+          for (int i = 0; i < kPieces; ++i) {
+            const int in = (warp & 3) * 32 + i * kPer + lane / kPieces;
+            *reinterpret_cast<uint4*>(sm.q[g][j / 8] + in * 128 + (((j & 7) ^ (in & 7)) * 16)) = x[i];
+          }
         }
         tc::fence_proxy_async();
         __syncwarp();
@@ -433,44 +442,73 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
         tc::fence_after_sync();
         const bool whole = p.whole();
         const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
-        const int64_t orow = paged::out_row(a, p, row_ok ? row : 0);
-        const int64_t prow = static_cast<int64_t>(2 * blockIdx.x + (t_now == t_begin ? 0 : 1)) * a.row_tile + row;
+        // rows leave through shared memory (the warp's own rows of Q, which no product
+        // reads any more), so that the warp writes whole rows
+        const int64_t prow0 = static_cast<int64_t>(2 * blockIdx.x + (t_now == t_begin ? 0 : 1)) * a.row_tile + g * B_ROWS +
+                              (warp & 3) * 32;
+        const int nrow = p.nrows - g * B_ROWS - (warp & 3) * 32;      // rows of this warp that exist
+        // 16-byte piece j of the warp's row i, rows of kRowPieces pieces
+        auto stage = [&](int i, int j, int pieces) -> uint4* {
+          const int at = i * pieces + (j ^ (i & 7));
+          return reinterpret_cast<uint4*>(sm.q[g][at / 256 % kHalves] + (warp & 3) * 4096) + at % 256;
+        };
+        if (whole) {
+          constexpr int kRowPieces = kD / 8;
 #pragma unroll
-        for (int cc = 0; cc < kD; cc += 16) {
-          uint32_t o[16];
-          tc::tmem_ld16(t_o + cc, o);
-          tc::tmem_wait_ld();
-          if (row_ok) {
-            if (whole) {
-              uint32_t w[8];
+          for (int cc = 0; cc < kD; cc += 32) {
+            uint32_t o[32];
+            tc::tmem_ld16(t_o + cc, *reinterpret_cast<uint32_t(*)[16]>(&o[0]));
+            tc::tmem_ld16(t_o + cc + 16, *reinterpret_cast<uint32_t(*)[16]>(&o[16]));
+            tc::tmem_wait_ld();
 #pragma unroll
-              for (int j = 0; j < 8; ++j) {
+            for (int j = 0; j < 4; ++j) {
+              uint32_t w[4];
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
                 // a row that saw nothing has P = 0 throughout, and its O is 0
-                const float f0 = __uint_as_float(o[2 * j]) * inv, f1 = __uint_as_float(o[2 * j + 1]) * inv;
+                const float f0 = __uint_as_float(o[8 * j + 2 * q]) * inv, f1 = __uint_as_float(o[8 * j + 2 * q + 1]) * inv;
                 if constexpr (kF16) {
                   const __half2 hv = __floats2half2_rn(f0, f1);
-                  w[j] = *reinterpret_cast<const uint32_t*>(&hv);
+                  w[q] = *reinterpret_cast<const uint32_t*>(&hv);
                 } else {
-                  w[j] = pack_bf16x2(f0, f1);
+                  w[q] = pack_bf16x2(f0, f1);
                 }
               }
-              uint4* dst = reinterpret_cast<uint4*>(a.out + (orow * kD + cc) * 2);
-              dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
-              dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
-            } else {
-              uint4* dst = reinterpret_cast<uint4*>(a.part_o + prow * kD + cc);
-#pragma unroll
-              for (int j = 0; j < 4; ++j) dst[j] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+              *stage(lane, cc / 8 + j, kRowPieces) = make_uint4(w[0], w[1], w[2], w[3]);
             }
           }
           __syncwarp();
-        }
-        if (row_ok) {
-          if (whole) {
-            if (a.lse != nullptr) a.lse[orow] = l_run > 0.f ? (m_run + log2f(l_run)) * kLn2 : -INFINITY;
-          } else {
-            a.part_ml[prow * 2] = m_run;
-            a.part_ml[prow * 2 + 1] = l_run;
+#pragma unroll 4
+          for (int i = lane / kRowPieces; i < nrow && i < 32; i += 32 / kRowPieces)
+            *reinterpret_cast<uint4*>(a.out + paged::out_row(a, p, g * B_ROWS + (warp & 3) * 32 + i) * kD * 2 +
+                                      (lane % kRowPieces) * 16) = *stage(i, lane % kRowPieces, kRowPieces);
+          if (row_ok && a.lse != nullptr)
+            a.lse[paged::out_row(a, p, row)] = l_run > 0.f ? (m_run + log2f(l_run)) * kLn2 : -INFINITY;
+        } else {
+          // fp32: 64 (kD 128) or 32 (kD 64) columns at a time
+          constexpr int kCols = kD / 2, kRowPieces = kCols / 4;
+#pragma unroll
+          for (int cc = 0; cc < kD; cc += kCols) {
+#pragma unroll
+            for (int c = 0; c < kCols; c += 32) {
+              uint32_t o[32];
+              tc::tmem_ld16(t_o + cc + c, *reinterpret_cast<uint32_t(*)[16]>(&o[0]));
+              tc::tmem_ld16(t_o + cc + c + 16, *reinterpret_cast<uint32_t(*)[16]>(&o[16]));
+              tc::tmem_wait_ld();
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                *stage(lane, c / 4 + j, kRowPieces) = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+            }
+            __syncwarp();
+#pragma unroll 4
+            for (int i = lane / kRowPieces; i < nrow && i < 32; i += 32 / kRowPieces)
+              *reinterpret_cast<uint4*>(a.part_o + (prow0 + i) * kD + cc + (lane % kRowPieces) * 4) =
+                  *stage(i, lane % kRowPieces, kRowPieces);
+            __syncwarp();
+          }
+          if (row_ok) {
+            a.part_ml[(prow0 + lane) * 2] = m_run;
+            a.part_ml[(prow0 + lane) * 2 + 1] = l_run;
           }
         }
         tc::fence_before_sync();       // O was read before the next unit's first P is announced
@@ -484,7 +522,7 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
   tc::fence_before_sync();
   __syncthreads();
   if (tid == 0 && sm.abort_flag) atomicOr(&g_paged_error, 1);
-  if (warp == 0) {
+  if (warp == 2) {
     tc::fence_after_sync();
     tc::tmem_dealloc(tbase, 512);
   }
