@@ -194,6 +194,19 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
   return d;
 }
 
+// n / d for n < 2^31 by a multiplication (Granlund and Montgomery 1994).
+struct FastDiv {
+  uint32_t mul, shift;
+  void set(uint32_t d) {
+    shift = 0;
+    while ((uint64_t(1) << shift) < d) ++shift;
+    mul = static_cast<uint32_t>((((uint64_t(1) << shift) - d) << 32) / d + 1);
+  }
+  __device__ __forceinline__ int div(int n) const {
+    return static_cast<int>((__umulhi(static_cast<uint32_t>(n), mul) + static_cast<uint32_t>(n)) >> shift);
+  }
+};
+
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));

@@ -91,13 +91,11 @@ __global__ void __launch_bounds__(A_THREADS) paged_token_kernel(const __grid_con
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
 
   paged::count_tiles<A_THREADS>(a, sm.batch, sm.warp_sums);
-  const int per = a.kv_heads * a.row_tiles;            // units per batch row
-  const int64_t total = static_cast<int64_t>(sm.batch.prefix[a.batch]) * per;
-  const int64_t grid = paged::dealt(a, total);
-  const int64_t t_begin = blockIdx.x < grid ? paged::stretch(blockIdx.x, total, grid) : 0;
-  const int64_t t_end = blockIdx.x < grid ? paged::stretch(blockIdx.x + 1, total, grid) : 0;
+  const paged::Deal deal(a, sm.batch.prefix[a.batch] * a.kv_heads * a.row_tiles);
+  const int cta = static_cast<int>(blockIdx.x);
+  const int t_begin = cta < deal.ctas ? deal.begin(cta) : 0, t_end = cta < deal.ctas ? deal.begin(cta + 1) : 0;
 
-  for (int64_t t_now = t_begin; t_now < t_end;) {
+  for (int t_now = t_begin; t_now < t_end;) {
     const paged::Piece pc = paged::piece_at(a, sm.batch, t_now, t_end);
     const int b = pc.b, h = pc.h, n = pc.n, r0 = pc.r0, nrows = pc.nrows, tile0 = pc.tile0, tile1 = pc.tile1;
 
@@ -107,7 +105,7 @@ __global__ void __launch_bounds__(A_THREADS) paged_token_kernel(const __grid_con
     for (int nt = 0; nt < kNT; ++nt) {
       const int r = r0 + nt * 8 + (lane >> 2);
       const bool ok = r < a.rows;
-      const int i = ok ? r / a.group : 0, g = ok ? r - i * a.group : 0;
+      const int i = ok ? a.by_group.div(r) : 0, g = ok ? r - i * a.group : 0;
       const char* q = a.q + b * a.qb + i * a.qt + (h * a.group + g) * a.qh + (lane & 3) * 4;
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
@@ -122,7 +120,7 @@ __global__ void __launch_bounds__(A_THREADS) paged_token_kernel(const __grid_con
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int r = r0 + nt * 8 + (lane & 3) * 2 + e;
-        last[nt][e] = a.causal ? n - a.len + r / a.group : n - 1;
+        last[nt][e] = a.causal ? n - a.len + a.by_group.div(r) : n - 1;
       }
 
     float o[kSteps][kNT][4], m[kNT][2], l[kNT][2];
@@ -349,8 +347,8 @@ __global__ void __launch_bounds__(32 * J_WARPS) paged_join_kernel(const __grid_c
   const int* prefix = batch.prefix;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = warp % kShare;
   paged::count_tiles<32 * J_WARPS>(a, batch, warp_sums);
-  const int per = a.kv_heads * a.row_tiles;
-  const int64_t total = static_cast<int64_t>(prefix[a.batch]) * per, grid = paged::dealt(a, total);
+  const int per = a.kv_heads * a.row_tiles;            // units per batch row
+  const paged::Deal deal(a, prefix[a.batch] * per);
   const int64_t rows = static_cast<int64_t>(a.batch) * a.kv_heads * a.rows;
   bool waited = false;
   for (int64_t row = blockIdx.x * (J_WARPS / kShare) + warp / kShare; row < rows;
@@ -360,13 +358,13 @@ __global__ void __launch_bounds__(32 * J_WARPS) paged_join_kernel(const __grid_c
     const int h = static_cast<int>(bh) - b * a.kv_heads;
     const int tiles = prefix[b + 1] - prefix[b];
     const int rt = r / a.row_tile, rr = r - rt * a.row_tile;
-    const int i = r / a.group, g = r - i * a.group;
+    const int i = a.by_group.div(r), g = r - i * a.group;
     const int64_t at = (static_cast<int64_t>(b) * a.len + i) * a.q_heads + h * a.group + g;
-    const int64_t first = static_cast<int64_t>(prefix[b]) * per + static_cast<int64_t>(h * a.row_tiles + rt) * tiles;
+    const int first = prefix[b] * per + (h * a.row_tiles + rt) * tiles;
     int c0 = 0, c1 = -1;
     if (tiles > 0) {
-      c0 = paged::holder(first, total, grid);
-      c1 = paged::holder(first + tiles - 1, total, grid);
+      c0 = deal.holder(first);
+      c1 = deal.holder(first + tiles - 1);
       if (c0 == c1) continue;
     }
     if (!waited) {
@@ -376,7 +374,8 @@ __global__ void __launch_bounds__(32 * J_WARPS) paged_join_kernel(const __grid_c
     float m = -INFINITY, l = 0.f, acc[kV];
 #pragma unroll
     for (int e = 0; e < kV; ++e) acc[e] = 0.f;
-    const int64_t slot0 = paged::slot_of(c0, c0, first, total, grid);
+    // the unit's first piece is the last of its CTA's, unless it is also its first
+    const int64_t slot0 = 2 * static_cast<int64_t>(c0) + (deal.begin(c0) != first ? 1 : 0);
 #pragma unroll 4
     for (int c = c0 + sub; c <= c1; c += kShare) {
       const int64_t slot = c == c0 ? slot0 : 2 * static_cast<int64_t>(c);
@@ -571,9 +570,15 @@ extern "C" int mrsa_paged_attention(const mrsa_paged_attention_args* p, const mr
   const int64_t slots = 2 * static_cast<int64_t>(a.grid) * a.row_tile;
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = a.part_o + slots * p->head_dim;
-  // more batch rows than a CTA keeps tile counts of: one stretch of them after another
-  for (int64_t b0 = 0; b0 < p->batch; b0 += paged::kMaxBatch) {
-    a.batch = static_cast<int>(p->batch - b0 < paged::kMaxBatch ? p->batch - b0 : paged::kMaxBatch);
+  a.by_group.set(static_cast<uint32_t>(a.group));
+  // more batch rows than a CTA keeps lengths of, or than 31 bits count tiles of:
+  // some of them after the others
+  const int64_t row_most = t->max_pages * t->page_size / A_TILE + 1;
+  int64_t at_once = 0x7fffffffLL / (row_most * a.kv_heads * a.row_tiles);
+  if (at_once < 1) return MRSA_ERR_SHAPE;
+  if (at_once > paged::kMaxBatch) at_once = paged::kMaxBatch;
+  for (int64_t b0 = 0; b0 < p->batch; b0 += at_once) {
+    a.batch = static_cast<int>(p->batch - b0 < at_once ? p->batch - b0 : at_once);
     a.q = static_cast<const char*>(p->q) + b0 * a.qb;
     a.out = static_cast<char*>(p->out) + b0 * p->len * p->q_heads * p->head_dim * 2;
     a.lse = p->lse != nullptr ? p->lse + b0 * p->len * p->q_heads : nullptr;

@@ -35,6 +35,7 @@ struct Args {
   int64_t kp, ks, kh, vp, vs, vh;      // bytes: page, slot, head
   int max_seqs, max_pages, pages, page_size, page_shift;
   int batch, len, q_heads, kv_heads, group, rows, row_tile, row_tiles, causal;
+  FastDiv by_group;
   int tile;                            // keys per tile
   int grid;                            // CTAs that the tiles are dealt to
   float scale_log2;                    // softmax scale times log2(e)
@@ -57,18 +58,23 @@ __device__ __forceinline__ int cached_tokens(const Args& a, int b) {
   return n;
 }
 
-// CTAs that get tiles: no stretch is empty.
-__device__ __forceinline__ int64_t dealt(const Args& a, int64_t total) { return total < a.grid ? total : a.grid; }
-// First tile of CTA c's stretch, and the CTA whose stretch holds tile t.
-__device__ __forceinline__ int64_t stretch(int64_t c, int64_t total, int64_t grid) { return c * total / grid; }
-__device__ __forceinline__ int holder(int64_t t, int64_t total, int64_t grid) {
-  return static_cast<int>(((t + 1) * grid - 1) / total);
-}
-
-// Slot of the piece that CTA c holds of a unit starting at tile `first`.
-__device__ __forceinline__ int slot_of(int c, int c0, int64_t first, int64_t total, int64_t grid) {
-  return 2 * c + ((c == c0 && stretch(c, total, grid) != first) ? 1 : 0);
-}
+// The tiles in stretches that differ by one at most, none empty: the first
+// `extra` CTAs get base + 1.  (The host keeps a launch below 2^31 tiles: 64-bit
+// divisions here cost each launch a microsecond.)
+struct Deal {
+  int total, ctas, base, extra;
+  __device__ __forceinline__ Deal(const Args& a, int all) : total(all) {
+    ctas = all < a.grid ? (all > 0 ? all : 1) : a.grid;
+    base = all / ctas;
+    extra = all - base * ctas;
+  }
+  // First tile of CTA c's stretch; the CTA whose stretch holds tile t.
+  __device__ __forceinline__ int begin(int c) const { return c * base + (c < extra ? c : extra); }
+  __device__ __forceinline__ int holder(int t) const {
+    const int wide = extra * (base + 1);
+    return t < wide ? t / (base + 1) : extra + (t - wide) / base;
+  }
+};
 
 // A CTA's part of one unit.
 struct Piece {
@@ -85,22 +91,20 @@ struct Batch {
 };
 
 // The part that begins at tile `t` and ends with its unit or at `end`.
-__device__ __forceinline__ Piece piece_at(const Args& a, const Batch& s, int64_t t, int64_t end) {
+__device__ __forceinline__ Piece piece_at(const Args& a, const Batch& s, int t, int end) {
   const int* prefix = s.prefix;
   const int per = a.kv_heads * a.row_tiles;            // units per batch row
   int lo = 0, hi = a.batch - 1;                        // the last batch row whose tiles begin at or before t
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (static_cast<int64_t>(prefix[mid]) * per <= t) lo = mid; else hi = mid - 1;
+    if (prefix[mid] * per <= t) lo = mid; else hi = mid - 1;
   }
   Piece p;
   p.b = lo;
   p.tiles = prefix[lo + 1] - prefix[lo];
-  const int64_t in_row = t - static_cast<int64_t>(prefix[lo]) * per;
-  const int unit = in_row >> 32 ? static_cast<int>(in_row / p.tiles)
-                                : static_cast<int>(static_cast<uint32_t>(in_row) / static_cast<uint32_t>(p.tiles));
-  p.tile0 = static_cast<int>(in_row - static_cast<int64_t>(unit) * p.tiles);
-  p.tile1 = end - t < p.tiles - p.tile0 ? p.tile0 + static_cast<int>(end - t) : p.tiles;
+  const int in_row = t - prefix[lo] * per, unit = in_row / p.tiles;
+  p.tile0 = in_row - unit * p.tiles;
+  p.tile1 = end - t < p.tiles - p.tile0 ? p.tile0 + end - t : p.tiles;
   p.h = unit / a.row_tiles;
   p.r0 = (unit - p.h * a.row_tiles) * a.row_tile;
   p.nrows = a.rows - p.r0 < a.row_tile ? a.rows - p.r0 : a.row_tile;
@@ -146,7 +150,7 @@ __device__ __forceinline__ void count_tiles(const Args& a, Batch& s, int* warp_s
 
 // The output row of query row r of a piece.
 __device__ __forceinline__ int64_t out_row(const Args& a, const Piece& p, int r) {
-  const int i = (p.r0 + r) / a.group, g = (p.r0 + r) - i * a.group;
+  const int i = a.by_group.div(p.r0 + r), g = (p.r0 + r) - i * a.group;
   return (static_cast<int64_t>(p.b) * a.len + i) * a.q_heads + p.h * a.group + g;
 }
 

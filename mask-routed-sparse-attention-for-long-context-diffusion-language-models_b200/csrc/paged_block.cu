@@ -80,7 +80,7 @@ struct TilePages {
   }
 };
 
-template <int kD, bool kF16>
+template <int kD, bool kF16, bool kCausal>
 __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_constant__ CUtensorMap tm_k,
                                                                    const __grid_constant__ CUtensorMap tm_v,
                                                                    const __grid_constant__ Args a) {
@@ -123,10 +123,9 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tbase = sm.tmem_base;
-  const int64_t total = static_cast<int64_t>(sm.batch.prefix[a.batch]) * a.kv_heads * a.row_tiles;
-  const int64_t grid = paged::dealt(a, total);
-  const int64_t t_begin = blockIdx.x < grid ? paged::stretch(blockIdx.x, total, grid) : 0;
-  const int64_t t_end = blockIdx.x < grid ? paged::stretch(blockIdx.x + 1, total, grid) : 0;
+  const paged::Deal deal(a, sm.batch.prefix[a.batch] * a.kv_heads * a.row_tiles);
+  const int cta = static_cast<int>(blockIdx.x);
+  const int t_begin = cta < deal.ctas ? deal.begin(cta) : 0, t_end = cta < deal.ctas ? deal.begin(cta + 1) : 0;
   bool ok = true;
 
   if (warp == W_K || warp == W_V) {
@@ -161,7 +160,7 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
       return true;
     };
     int e = 0;                                   // tiles of the stretch so far
-    for (int64_t t_now = t_begin; ok && t_now < t_end;) {
+    for (int t_now = t_begin; ok && t_now < t_end;) {
       const Piece p = paged::piece_at(a, sm.batch, t_now, t_end);
       const uint8_t* valid = a.valid != nullptr && is_k
                                  ? a.valid + static_cast<int64_t>(p.b) * a.max_pages * a.page_size : nullptr;
@@ -255,7 +254,7 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
       __syncwarp();
       return true;
     };
-    for (int64_t t_now = t_begin; ok && t_now < t_end;) {
+    for (int t_now = t_begin; ok && t_now < t_end;) {
       const Piece p = paged::piece_at(a, sm.batch, t_now, t_end);
       const int nt = p.tile1 - p.tile0;
       if (p.nrows <= g * B_ROWS) {
@@ -310,37 +309,34 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t t_o = tbase + lane_off + kOCol + 128 * g;
     int e0 = 0, k = 0;            // tiles of the stretch before this unit; tiles of this group so far
-    for (int64_t t_now = t_begin; ok && t_now < t_end;) {
+    for (int t_now = t_begin; ok && t_now < t_end;) {
       const Piece p = paged::piece_at(a, sm.batch, t_now, t_end);
       const int nt = p.tile1 - p.tile0;
       if (p.nrows > g * B_ROWS) {
         // ---- this row of Q (the S products of the unit before are done: the last S was read)
         const int row = g * B_ROWS + r;
         const bool row_ok = row < p.nrows;
-        const int qi = (p.r0 + (row_ok ? row : 0)) / a.group;
-        // the warp's 32 rows, whole rows at a time (a thread per row would touch 32 lines with every load)
+        // the warp's 32 rows, whole rows at a time (a thread per row would touch 32
+        // lines with every load) and all at once; the loop is not unrolled, for a
+        // unit's start finds its instructions uncached
         {
-          constexpr int kPieces = kD / 8, kPer = 32 / kPieces;     // 16-byte pieces of a row, rows per load
+          constexpr int kPieces = kD / 8, kPer = 32 / kPieces;     // 16-byte pieces of a row, rows per step
           const int j = lane % kPieces;
-          uint4 x[kPieces];
-#pragma unroll
-          for (int i = 0; i < kPieces; ++i) {
-            const int in = (warp & 3) * 32 + i * kPer + lane / kPieces, qr = g * B_ROWS + in;
-            const int ti = (p.r0 + qr) / a.group, tg = (p.r0 + qr) - ti * a.group;
-            x[i] = qr < p.nrows
-                       ? *reinterpret_cast<const uint4*>(a.q + p.b * a.qb + ti * a.qt + (p.h * a.group + tg) * a.qh + j * 16)
-                       : make_uint4(0u, 0u, 0u, 0u);
+          const char* src = a.q + p.b * a.qb + (p.h * a.group) * a.qh + j * 16;
+#pragma unroll 1
+          for (int in = (warp & 3) * 32 + lane / kPieces, i = 0; i < kPieces; ++i, in += kPer) {
+            const int qr = g * B_ROWS + in, ti = a.by_group.div(p.r0 + qr), tg = p.r0 + qr - ti * a.group;
+            const bool on = qr < p.nrows;
+            cp_async16_zfill(sm.q[g][j / 8] + in * 128 + (((j & 7) ^ (in & 7)) * 16),
+                             on ? src + ti * a.qt + tg * a.qh : src, on);
           }
-#pragma unroll
-          for (int i = 0; i < kPieces; ++i) {
-            const int in = (warp & 3) * 32 + i * kPer + lane / kPieces;
-            *reinterpret_cast<uint4*>(sm.q[g][j / 8] + in * 128 + (((j & 7) ^ (in & 7)) * 16)) = x[i];
-          }
+          cp_async_commit();
+          cp_async_wait<0>();
         }
         tc::fence_proxy_async();
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(tc::smem_addr(&sm.qfull[g]));
-        const int last = a.causal ? p.n - a.len + qi : p.n - 1;   // the last key this row may see
+        const int last = p.n - a.len + a.by_group.div(p.r0 + (row_ok ? row : 0));   // causal: the last key this row may see
         float m_run = -INFINITY, l_run = 0.f;
         for (int i = 0; i < nt; ++i, ++k) {
           const int sb = 2 * g + (k & 1), e = e0 + i;
@@ -354,8 +350,6 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
           tc::tmem_wait_ld();
           if (!(ok = tc::wait_bounded_warp(tc::smem_addr(&sm.mfull[e % NMS]), (e / NMS) & 1, abort_flag))) break;
           const unsigned long long km = sm.kmask[e % NMS];
-          const int seen = last - j0;              // columns past it are out of this row's sight
-          const bool full = km == ~0ull && seen >= B_TILE - 1;
           if (km != ~0ull) {
             // one minimum per column instead of a test and a choice; of NaN and -inf it is -inf
             const float4* lim = reinterpret_cast<const float4*>(sm.limit[e % NMS]);
@@ -368,7 +362,8 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
               x[c + 3] = __float_as_uint(fminf(__uint_as_float(x[c + 3]), w.w));
             }
           }
-          if (seen < B_TILE - 1) {
+          const int seen = last - j0;              // columns past it are out of this row's sight
+          if (kCausal && seen < B_TILE - 1) {
 #pragma unroll
             for (int c = 0; c < B_TILE; ++c)
               if (c > seen) x[c] = __float_as_uint(-INFINITY);
@@ -393,8 +388,12 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
           const float2 sl2 = make_float2(a.scale_log2, a.scale_log2), nb2 = make_float2(nbase, nbase);
           float2 s2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
           uint32_t pk[32];
-          // a quarter of a full tile's exponentials on the FMA pipe (the choice is the row's own)
-          if (full) {
+          // A quarter of the exponentials on the FMA pipe.  It gives 2^-126 for -inf,
+          // which the zeroed V row of a masked key cancels and a sum of at least one
+          // does not see (a row that has seen nothing is known by its maximum); the
+          // V rows out of a causal row's sight are not zeroed, so its last tiles
+          // take the other way.
+          if (!kCausal || seen >= B_TILE - 1) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) {
               const float2 y = ffma2(make_float2(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1])), sl2, nb2);
@@ -441,6 +440,7 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
         if (!ok) break;
         tc::fence_after_sync();
         const bool whole = p.whole();
+        if (m_run == -INFINITY) l_run = 0.f;       // the row saw no key
         const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
         // rows leave through shared memory (the warp's own rows of Q, which no product
         // reads any more), so that the warp writes whole rows
@@ -454,7 +454,7 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
         };
         if (whole) {
           constexpr int kRowPieces = kD / 8;
-#pragma unroll
+#pragma unroll 1
           for (int cc = 0; cc < kD; cc += 32) {
             uint32_t o[32];
             tc::tmem_ld16(t_o + cc, *reinterpret_cast<uint32_t(*)[16]>(&o[0]));
@@ -465,7 +465,6 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
               uint32_t w[4];
 #pragma unroll
               for (int q = 0; q < 4; ++q) {
-                // a row that saw nothing has P = 0 throughout, and its O is 0
                 const float f0 = __uint_as_float(o[8 * j + 2 * q]) * inv, f1 = __uint_as_float(o[8 * j + 2 * q + 1]) * inv;
                 if constexpr (kF16) {
                   const __half2 hv = __floats2half2_rn(f0, f1);
@@ -487,9 +486,9 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
         } else {
           // fp32: 64 (kD 128) or 32 (kD 64) columns at a time
           constexpr int kCols = kD / 2, kRowPieces = kCols / 4;
-#pragma unroll
+#pragma unroll 1
           for (int cc = 0; cc < kD; cc += kCols) {
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < kCols; c += 32) {
               uint32_t o[32];
               tc::tmem_ld16(t_o + cc + c, *reinterpret_cast<uint32_t(*)[16]>(&o[0]));
@@ -562,9 +561,10 @@ int launch(const Args& a, cudaStream_t s) {
     return MRSA_ERR_LAUNCH;
   }
   const int smem = static_cast<int>(sizeof(BlockSmem<kD>) + 1024);
-  if (cudaFuncSetAttribute(paged_block_kernel<kD, kF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+  const auto kernel = a.causal ? paged_block_kernel<kD, kF16, true> : paged_block_kernel<kD, kF16, false>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return MRSA_ERR_LAUNCH;
-  paged_block_kernel<kD, kF16><<<static_cast<unsigned>(a.grid), B_THREADS, smem, s>>>(tk, tv, a);
+  kernel<<<static_cast<unsigned>(a.grid), B_THREADS, smem, s>>>(tk, tv, a);
   MRSA_CHECK_LAUNCH();
   return MRSA_OK;
 }
