@@ -138,21 +138,23 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
     static_assert(NKS == NVS, "K and V stages share their index");
     if (lane == 0) tc::prefetch_tensormap(map);
     const TilePages tp(a);
-    // V rows of keys that do not count, zeroed kLag tiles behind the copies (a
-    // P of zero does not cancel what is not a number); the MMA warps wait for
-    // it where a tile has such keys
-    constexpr int kLag = 2;
+    // V rows of keys that do not count, zeroed (a P of zero does not cancel what
+    // is not a number); the MMA warps wait for it where a tile has such keys.
+    // The V warp does it one tile behind its copies (masked, 37 x 32 tokens over
+    // 16384: 418 us; two behind 417; in the K warp 421 and up).
+    constexpr int kLag = 1;
     auto clean = [&](int tile) -> bool {
       if (!tc::wait_bounded_warp(tc::smem_addr(&sm.mfull[tile % NMS]), (tile / NMS) & 1, abort_flag)) return false;
       const unsigned long long km = sm.kmask[tile % NMS];
       const int st = tile % NVS;
       if (km != ~0ull) {
         if (!tc::wait_bounded_warp(tc::smem_addr(&sm.vfull[st]), (tile / NVS) & 1, abort_flag)) return false;
-        for (unsigned long long rest = ~km; rest != 0; rest &= rest - 1) {
-          const int key = __ffsll(static_cast<long long>(rest)) - 1;
-          if (lane < kD / 8)
-            *reinterpret_cast<uint4*>(sm.v[st][lane >> 3] + key * 128 + (lane & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
-        }
+        constexpr int kPer = 32 / (kD / 8);      // rows per step
+        const int j = lane % (kD / 8);
+#pragma unroll 4
+        for (int key = lane / (kD / 8); key < B_TILE; key += kPer)
+          if (!((km >> key) & 1ull))
+            *reinterpret_cast<uint4*>(sm.v[st][j >> 3] + key * 128 + (j & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
         tc::fence_proxy_async();
         __syncwarp();
       }
