@@ -7,6 +7,7 @@ or fails to load, every op raises.
 from __future__ import annotations
 
 import ctypes as C
+import importlib.util
 import os
 import struct
 
@@ -14,6 +15,7 @@ import torch
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libmrsa_b200.so")
+EXT_PATH = os.path.join(_HERE, "mrsa_b200_ext.so")
 
 ERR_NULL, ERR_SHAPE, ERR_ALIGN, ERR_LAUNCH, ERR_ARG, ERR_WORKSPACE = -1, -2, -3, -4, -5, -6
 BF16, F32, F16 = 0, 1, 2
@@ -145,14 +147,8 @@ def stream_of(t: torch.Tensor):
     return C.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
 
 
-def raw_stream(device: torch.device) -> int:
-    """Handle of the device's current stream."""
-    return torch._C._cuda_getCurrentRawStream(device.index)
-
-
-# The argument structs of the rotary and paged operators, packed as bytes: a
-# call then converts two or three pointers instead of thirty arguments (about
-# 1 us instead of 6 us, which counts where a step is a few microseconds long).
+# The argument structs of the rotary and paged operators, for callers of the C
+# entry points: a packed struct's bytes are passed as its pointer.
 ROTARY_ARGS = struct.Struct("@6P6q6qf3i")            # mrsa_rotary_args
 PAGE_TABLE = struct.Struct("@4P4q")                  # mrsa_page_table
 PAGE_POOL = struct.Struct("@P8q")                    # mrsa_page_pool
@@ -164,17 +160,25 @@ def call(name: str, *args):
     check(getattr(load(), name)(*args), name)
 
 
-_entries: dict = {}
+_ext = None
 
 
-def call_packed(name: str, *args):
-    """:func:`call` for the operators with packed arguments."""
-    fn = _entries.get(name)
-    if fn is None:
-        fn = _entries[name] = getattr(load(), name)
-    rc = fn(*args)
-    if rc:
-        check(rc, name)
+def ext():
+    """The binding of the rotary and paged operators (idempotent).  Raises if
+    it is absent."""
+    global _ext
+    if _ext is None:
+        load()
+        if not os.path.exists(EXT_PATH):
+            raise RuntimeError(
+                f"{EXT_PATH} is missing: build it with __graft_entry__.build() "
+                "(the MRSA ops have no CPU fallback)")
+        spec = importlib.util.spec_from_file_location("mrsa_b200_ext", EXT_PATH)
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        mod.set_check(check)
+        _ext = mod
+    return _ext
 
 
 class RouteLayerArgs(C.Structure):

@@ -1,4 +1,6 @@
-"""Build ``libmrsa_b200.so`` (all kernels + the C ABI) for sm_100a with nvcc.
+"""Build ``libmrsa_b200.so`` (all kernels + the C ABI) for sm_100a with nvcc,
+and ``mrsa_b200_ext.so`` (``csrc/binding.cpp``, the Python binding of the rotary
+and paged operators) with the host compiler.
 
 Objects go to ``_build/`` next to this file and the shared library is written
 in-tree, so it travels with the source tree to the GPU host.  Rebuilds only
@@ -12,12 +14,14 @@ import glob
 import os
 import shutil
 import subprocess
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libmrsa_b200.so")
+EXT = os.path.join(HERE, "mrsa_b200_ext.so")
 INCLUDE = os.path.join(ROOT, "include")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -47,8 +51,34 @@ def up_to_date() -> bool:
     return all(os.path.getmtime(p) <= t for p in _deps())
 
 
+def build_binding(force: bool = False) -> str:
+    """The Python binding, linked against torch and the kernel library."""
+    src = os.path.join(CSRC, "binding.cpp")
+    deps = [src, os.path.join(INCLUDE, "mrsa.h")]
+    if not force and os.path.exists(EXT) and all(os.path.getmtime(p) <= os.path.getmtime(EXT) for p in deps):
+        return EXT
+    import torch
+
+    base = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(_nvcc()))
+    tmp = EXT + ".tmp"
+    # g++ as nvcc takes it: torch and this module have to share one libstdc++
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-I" + os.path.join(base, "include"), "-I" + os.path.join(base, "include", "torch", "csrc", "api", "include"),
+           "-I" + os.path.join(cuda, "include"), "-I" + sysconfig.get_paths()["include"], src, "-o", tmp,
+           "-L" + os.path.join(base, "lib"), "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python",
+           "-L" + HERE, "-l:" + os.path.basename(LIB), "-Wl,-rpath,$ORIGIN"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"building {os.path.basename(EXT)} failed:\n{res.stderr}")
+    os.replace(tmp, EXT)
+    return EXT
+
+
 def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) -> str:
     if not force and up_to_date():
+        build_binding()
         return LIB
     nvcc = _nvcc()
     os.makedirs(BUILD, exist_ok=True)
@@ -72,6 +102,7 @@ def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) 
     if res.returncode != 0:
         raise RuntimeError(f"nvcc link failed:\n{res.stderr}")
     os.replace(tmp, LIB)
+    build_binding(force)
     return LIB
 
 
