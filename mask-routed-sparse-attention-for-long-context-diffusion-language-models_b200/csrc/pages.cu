@@ -1,9 +1,10 @@
 // Pages of a key-value cache: free, extend, fork, compact, copy.
 //
 // The bookkeeping of one call (reference counts, the search for free pages,
-// table rows) is one launch of one cluster of eight CTAs: its steps depend on
-// one another across the whole table, and the cluster's hardware barrier
-// separates them in a fraction of what another launch costs.  The pages' bytes
+// table rows) is one launch of one CTA, or for large tables of one cluster of
+// up to eight: its steps depend on one another across the whole table, and a
+// CTA's or a cluster's barrier separates them in a fraction of what another
+// launch costs.  The pages' bytes
 // are then moved by a second launch over all SMs, which reads from the
 // workspace what to copy.  The host never learns lengths or page numbers, so
 // the calls can be queued, or captured in a graph, without waiting for the GPU.
@@ -18,7 +19,7 @@ using namespace mrsa;
 
 namespace {
 
-constexpr int P_CLUSTER = 8;
+constexpr int P_CLUSTER = 8;          // CTAs at most
 constexpr int P_THREADS = 1024;
 constexpr int P_WARPS = P_THREADS / 32;
 constexpr int P_MAX = MRSA_PAGE_MAX_SEQS;
@@ -70,40 +71,41 @@ struct PlanArgs {
   Ws ws;
 };
 
-__device__ __forceinline__ void cluster_sync() {
-  __threadfence();
-  asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;\n" ::: "memory");
-}
 __device__ __forceinline__ int cluster_rank() {
   int r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r));
   return r;
 }
+__device__ __forceinline__ int cluster_size() {
+  int r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;\n" : "=r"(r));
+  return r;
+}
+// Every CTA's writes so far are seen by all of them.
+__device__ __forceinline__ void all_sync(int ctas) {
+  if (ctas == 1) __syncthreads();
+  else asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;\n" ::: "memory");
+}
 
 // Exclusive prefix sum of `v` over the CTA's threads; *total gets the sum.
-__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* warp_sums, int64_t* total) {
+// Each warp sums up the warps before it by itself: one barrier.  `turn`
+// alternates between two sets of partial sums.
+__device__ __forceinline__ int block_scan(int v, int (*partial)[P_WARPS], int& turn, int* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int64_t x = v;
+  int x = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
     if (lane >= o) x += y;
   }
-  __syncthreads();   // the previous call's readers are done
-  if (lane == 31) warp_sums[warp] = x;
+  int* sums = partial[turn];
+  turn ^= 1;
+  if (lane == 31) sums[warp] = x;
   __syncthreads();
-  if (warp == 0) {
-    int64_t s = warp_sums[lane];
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t y = __shfl_up_sync(0xffffffffu, s, o);
-      if (lane >= o) s += y;
-    }
-    warp_sums[lane] = s;
-  }
-  __syncthreads();
-  *total = warp_sums[P_WARPS - 1];
-  return x - v + (warp > 0 ? warp_sums[warp - 1] : 0);
+  int s = sums[lane];
+  const int before = __reduce_add_sync(0xffffffffu, lane < warp ? s : 0);
+  *total = __reduce_add_sync(0xffffffffu, s);
+  return before + x - v;
 }
 
 struct PlanSmem {
@@ -113,8 +115,7 @@ struct PlanSmem {
   int32_t used[P_MAX];                 // pages that seq holds in the end
   int32_t len[P_MAX];                  // its tokens in the end
   int32_t offset[P_MAX + 1];           // its first new page's place in the list
-  int64_t warp_sums[P_WARPS];
-  int warp_count[P_WARPS];
+  int partial[2][P_WARPS];
   int bad;
 };
 
@@ -122,11 +123,12 @@ struct PlanSmem {
 // cluster's threads in groups of 128, several groups to a sequence when there
 // are fewer sequences than groups.  f(i, j) runs for every page j in [0, count(i)).
 template <typename Count, typename F>
-__device__ __forceinline__ void for_pages(int n, int rank, Count count, F f) {
-  constexpr int kGroup = 128, kGroups = P_CLUSTER * P_THREADS / kGroup;
+__device__ __forceinline__ void for_pages(int n, int rank, int ctas, Count count, F f) {
+  constexpr int kGroup = 128;
+  const int groups = ctas * (P_THREADS / kGroup);
   const int gid = rank * (P_THREADS / kGroup) + threadIdx.x / kGroup, t = threadIdx.x % kGroup;
-  const int each = n < kGroups ? kGroups / n : 1;
-  for (int i = gid / each; i < n; i += kGroups) {
+  const int each = n < groups ? groups / n : 1;
+  for (int i = gid / each; i < n; i += groups) {
     const int c = count(i);
     for (int j = (gid % each) * kGroup + t; j < c; j += each * kGroup) f(i, j);
     if (each > 1) break;
@@ -134,10 +136,10 @@ __device__ __forceinline__ void for_pages(int n, int rank, Count count, F f) {
 }
 
 template <Op kOp>
-__global__ void __cluster_dims__(P_CLUSTER, 1, 1) __launch_bounds__(P_THREADS, 1) page_plan_kernel(
+__global__ void __launch_bounds__(P_THREADS, 1) page_plan_kernel(
     const __grid_constant__ PlanArgs a) {
   __shared__ PlanSmem sm;
-  const int tid = threadIdx.x, rank = cluster_rank(), lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, rank = cluster_rank(), ctas = cluster_size(), lane = tid & 31, warp = tid >> 5;
   const int n = a.n, ps = static_cast<int>(a.t.page_size), shift = a.shift;
   const int mp = static_cast<int>(a.t.max_pages), pages = static_cast<int>(a.t.pages);
   const int64_t most = static_cast<int64_t>(mp) * ps;
@@ -147,7 +149,7 @@ __global__ void __cluster_dims__(P_CLUSTER, 1, 1) __launch_bounds__(P_THREADS, 1
   // ---- the call's sequences, checked by every CTA alike
   if (tid == 0) sm.bad = 0;
   __syncthreads();
-  int64_t need = 0;
+  int need = 0, turn = 0;
   if (tid < n) {
     const int s = a.seqs[tid];
     int bad = (s < 0 || s >= a.t.max_seqs) ? MRSA_PAGE_BAD_SEQUENCE : 0;
@@ -198,7 +200,7 @@ __global__ void __cluster_dims__(P_CLUSTER, 1, 1) __launch_bounds__(P_THREADS, 1
     const bool clash = (i < j && sm.seq[i] == sm.seq[j]) || (kOp == kFork && sm.seq[i] == sm.src[j]);
     if (clash) atomicOr(&sm.bad, MRSA_PAGE_BAD_SEQUENCE);
   }
-  cluster_sync();   // every CTA has read lengths and sequence numbers before one of them writes
+  all_sync(ctas);   // every CTA has read lengths and sequence numbers before one of them writes
   if (sm.bad) {     // every CTA leaves here, or none does
     if (rank == 0 && tid == 0) {
       report(a.t.status, sm.bad);
@@ -214,7 +216,7 @@ __global__ void __cluster_dims__(P_CLUSTER, 1, 1) __launch_bounds__(P_THREADS, 1
 
   if (kOp == kFree || kOp == kFork) {
     // ---- the rows' pages given up
-    for_pages(n, rank, [&](int i) { return sm.old_used[i]; }, [&](int i, int j) {
+    for_pages(n, rank, ctas, [&](int i) { return sm.old_used[i]; }, [&](int i, int j) {
       int32_t* c = cell(sm.seq[i], j);
       give_up(*c);
       *c = -1;
@@ -223,7 +225,7 @@ __global__ void __cluster_dims__(P_CLUSTER, 1, 1) __launch_bounds__(P_THREADS, 1
       if (rank == 0 && tid < n) a.t.lengths[sm.seq[tid]] = 0;
       return;
     }
-    cluster_sync();
+    all_sync(ctas);
   }
 
   if (kOp == kCompact) {
@@ -232,7 +234,7 @@ __global__ void __cluster_dims__(P_CLUSTER, 1, 1) __launch_bounds__(P_THREADS, 1
     for (int i = 0; i < n; ++i) {
       const int64_t len = a.t.lengths[sm.seq[i]];
       const uint8_t* keep = a.keep + i * most;
-      for (int j = gw; j < sm.old_used[i]; j += P_CLUSTER * P_WARPS) {
+      for (int j = gw; j < sm.old_used[i]; j += ctas * P_WARPS) {
         int c = 0;
         for (int s0 = 0; s0 < ps; s0 += 32) {
           const int64_t p = static_cast<int64_t>(j) * ps + s0 + lane;
@@ -241,35 +243,34 @@ __global__ void __cluster_dims__(P_CLUSTER, 1, 1) __launch_bounds__(P_THREADS, 1
         if (lane == 0) a.ws.before[static_cast<int64_t>(i) * mp + j] = c;
       }
     }
-    cluster_sync();
-    for (int i = rank; i < n; i += P_CLUSTER) {
+    all_sync(ctas);
+    for (int i = rank; i < n; i += ctas) {
       const int64_t len = a.t.lengths[sm.seq[i]];
       const int used = sm.old_used[i];
       int32_t* b = a.ws.before + static_cast<int64_t>(i) * mp;
-      int64_t run = 0, full = 0;   // full: pages so far that keep every token, until one does not
+      int run = 0, full = 0;       // full: pages so far that keep every token, until one does not
       bool open = true;
       for (int j0 = 0; j0 < used; j0 += P_THREADS) {
         const int j = j0 + tid;
         const int c = j < used ? __ldcg(b + j) : 0;
         const int64_t here = len - static_cast<int64_t>(j) * ps;
         const bool whole = j < used && c == (here < ps ? here : ps);
-        int64_t total, none;
-        const int64_t before = run + block_scan(c, sm.warp_sums, &total);
-        if (j < used) b[j] = static_cast<int32_t>(before);
-        // pages of this stretch before its first that is not whole
-        const int64_t holes = block_scan(whole ? 0 : 1, sm.warp_sums, &none);
-        int64_t lead;
-        block_scan(whole && holes == 0 ? 1 : 0, sm.warp_sums, &lead);
+        int total, holes;
+        const int before = run + block_scan(c, sm.partial, turn, &total);
+        if (j < used) b[j] = before;
+        // whole pages of this stretch before its first that is not
+        const int hole = block_scan(whole ? 0 : 1, sm.partial, turn, &holes);
+        const int lead = __syncthreads_count(whole && hole == 0);
         if (open) full += lead;
-        open = open && none == 0;
+        open = open && holes == 0;
         run += total;
       }
       if (tid == 0) {
-        a.ws.left[i] = static_cast<int32_t>(run);
-        a.ws.stay[i] = static_cast<int32_t>(full < used ? full : used);
+        a.ws.left[i] = run;
+        a.ws.stay[i] = full < used ? full : used;
       }
     }
-    cluster_sync();
+    all_sync(ctas);
     if (tid < n) {
       const int left = __ldcg(a.ws.left + tid), stay = __ldcg(a.ws.stay + tid);
       sm.len[tid] = left;
@@ -280,26 +281,47 @@ __global__ void __cluster_dims__(P_CLUSTER, 1, 1) __launch_bounds__(P_THREADS, 1
   }
 
   // ---- each sequence's place among the new pages
-  int64_t total;
-  const int64_t mine = block_scan(tid < n ? need : 0, sm.warp_sums, &total);
-  const int64_t wanted = total < static_cast<int64_t>(pages) + 1 ? total : static_cast<int64_t>(pages) + 1;
-  if (tid < n) sm.offset[tid] = static_cast<int>(mine < wanted ? mine : wanted);
+  int total;
+  const int mine = block_scan(tid < n ? need : 0, sm.partial, turn, &total);
+  if (tid < n) sm.offset[tid] = mine;
 
-  // ---- the lowest free pages: each CTA counts its stretch of the pool, then lists them
-  const int per = ((pages + P_CLUSTER - 1) / P_CLUSTER + P_THREADS - 1) / P_THREADS * P_THREADS;
-  const int p0 = rank * per, p1 = p0 + per < pages ? p0 + per : pages;
+  // ---- the lowest free pages: each CTA lists those of its stretch of the pool, after
+  // counting them where there are several CTAs; four neighbouring pages to a thread
+  constexpr int kStep = P_THREADS * 4;
+  const int per = ((pages + ctas - 1) / ctas + kStep - 1) / kStep * kStep;
+  const int p0 = rank * per < pages ? rank * per : pages, p1 = p0 + per < pages ? p0 + per : pages;
+  auto zeros_at = [&](int p) -> unsigned {       // bit i: page p + i is free
+    unsigned z = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (p + i < p1 && __ldcg(a.t.refcount + p + i) == 0) z |= 1u << i;
+    return z;
+  };
   if (total > 0) {
-    int64_t zeros = 0;
-    for (int p = p0 + tid; p < p1; p += P_THREADS) zeros += __ldcg(a.t.refcount + p) == 0;
-    int64_t sum;
-    block_scan(zeros, sm.warp_sums, &sum);
-    if (tid == 0) a.ws.zeros[rank] = static_cast<int32_t>(sum);
-    cluster_sync();
-    int64_t place = 0, all = 0;
-    for (int r = 0; r < P_CLUSTER; ++r) {
-      const int z = __ldcg(a.ws.zeros + r);
-      if (r < rank) place += z;
-      all += z;
+    int place = 0;
+    if (ctas > 1) {
+      int zeros = 0;
+      for (int p = p0 + tid * 4; p < p1; p += kStep) zeros += __popc(zeros_at(p));
+      int sum;
+      block_scan(zeros, sm.partial, turn, &sum);
+      if (tid == 0) a.ws.zeros[rank] = sum;
+      all_sync(ctas);
+      for (int r = 0; r < rank; ++r) place += __ldcg(a.ws.zeros + r);
+    }
+    int all = place;
+    for (int q = p0; q < p1 && all < total; q += kStep) {
+      const int p = q + tid * 4;
+      const unsigned z = zeros_at(p);
+      int sum;
+      int at = all + block_scan(__popc(z), sm.partial, turn, &sum);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (((z >> i) & 1u) && at < total) a.ws.fresh[at++] = p + i;
+      all += sum;
+    }
+    if (ctas > 1) {
+      all = 0;
+      for (int r = 0; r < ctas; ++r) all += __ldcg(a.ws.zeros + r);
     }
     if (all < total) {   // every CTA sees the same counts
       if (rank == 0) {
@@ -311,15 +333,7 @@ __global__ void __cluster_dims__(P_CLUSTER, 1, 1) __launch_bounds__(P_THREADS, 1
       }
       return;
     }
-    for (int q = p0; q < p1 && place < total; q += P_THREADS) {
-      const int p = q + tid;
-      const bool is = p < p1 && __ldcg(a.t.refcount + p) == 0;
-      int64_t sum2;
-      const int64_t at = place + block_scan(is ? 1 : 0, sm.warp_sums, &sum2);
-      if (is && at < total) a.ws.fresh[at] = p;
-      place += sum2;
-    }
-    cluster_sync();
+    all_sync(ctas);
   }
 
   if (kOp == kCompact) {
@@ -329,7 +343,7 @@ __global__ void __cluster_dims__(P_CLUSTER, 1, 1) __launch_bounds__(P_THREADS, 1
       const int64_t len = a.t.lengths[sm.seq[i]];
       const uint8_t* keep = a.keep + i * most;
       const int64_t moved0 = static_cast<int64_t>(sm.first[i]) * ps;
-      for (int j = sm.first[i] + gw; j < sm.old_used[i]; j += P_CLUSTER * P_WARPS) {
+      for (int j = sm.first[i] + gw; j < sm.old_used[i]; j += ctas * P_WARPS) {
         int page = *cell(sm.seq[i], j);
         if (page < 0 || page >= pages) {
           if (lane == 0) report(a.t.status, MRSA_PAGE_OUTSIDE);
@@ -347,12 +361,12 @@ __global__ void __cluster_dims__(P_CLUSTER, 1, 1) __launch_bounds__(P_THREADS, 1
         }
       }
     }
-    for_pages(n, rank, [&](int i) { return sm.used[i] - sm.first[i]; }, [&](int i, int j) {
+    for_pages(n, rank, ctas, [&](int i) { return sm.used[i] - sm.first[i]; }, [&](int i, int j) {
       const int rest = sm.len[i] - (sm.first[i] + j) * ps;
       a.ws.from[sm.offset[i] + j] = rest < ps ? rest : ps;
     });
-    cluster_sync();
-    for_pages(n, rank, [&](int i) { return sm.old_used[i]; }, [&](int i, int j) {
+    all_sync(ctas);
+    for_pages(n, rank, ctas, [&](int i) { return sm.old_used[i]; }, [&](int i, int j) {
       if (j < sm.first[i]) return;
       int32_t* c = cell(sm.seq[i], j);
       give_up(*c);
@@ -361,7 +375,7 @@ __global__ void __cluster_dims__(P_CLUSTER, 1, 1) __launch_bounds__(P_THREADS, 1
   }
 
   // ---- the rows' new cells
-  for_pages(n, rank, [&](int i) { return sm.used[i]; }, [&](int i, int j) {
+  for_pages(n, rank, ctas, [&](int i) { return sm.used[i]; }, [&](int i, int j) {
     int page;
     if (kOp == kFork && j < sm.first[i]) {
       page = *cell(sm.src[i], j);
@@ -435,40 +449,44 @@ __global__ void __launch_bounds__(M_THREADS) page_copy_kernel(const __grid_const
   }
 }
 
-// Kept tokens: the same units, with each token's slot looked up.
+// Kept tokens: one unit is M_THREADS vectors of one new page in M_PLANES
+// planes, a thread's slot looked up once for all of them.
+constexpr int M_PLANES = 8;
+
 __global__ void __launch_bounds__(M_THREADS) page_gather_kernel(const __grid_constant__ MoveArgs a) {
   asm volatile("griddepcontrol.wait;\n" ::: "memory");
   const int count = *a.head;
   const int ps = 1 << a.shift;
   const int vecs = static_cast<int>(a.page_bytes / 16);
   const int hv = static_cast<int>(a.pool.row_bytes / 16), tv = hv * static_cast<int>(a.pool.heads);
-  const int parts = (vecs + M_THREADS * M_UNROLL - 1) / (M_THREADS * M_UNROLL);
-  const int64_t planes = a.pool.layers * 2, units = static_cast<int64_t>(count) * planes * parts;
+  const int parts = (vecs + M_THREADS - 1) / M_THREADS;
+  const int planes = static_cast<int>(a.pool.layers) * 2, sets = (planes + M_PLANES - 1) / M_PLANES;
+  const int64_t units = static_cast<int64_t>(count) * sets * parts;
   for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
-    const int part = static_cast<int>(u % parts);
     const int64_t r = u / parts;
-    const int plane = static_cast<int>(r % planes);
-    const int i = static_cast<int>(r / planes);
-    const int tokens = a.src[i], to = a.dst[i];
-    char* base = static_cast<char*>(a.pool.data) + (plane >> 1) * a.pool.layer_stride + (plane & 1) * a.pool.kv_stride;
-    uint4 v[M_UNROLL];
-    int64_t at[M_UNROLL];
+    const int i = static_cast<int>(r / sets), plane0 = static_cast<int>(r - static_cast<int64_t>(i) * sets) * M_PLANES;
+    const int e = static_cast<int>(u - r * parts) * M_THREADS + threadIdx.x;
+    const int t = e / tv, w = e - t * tv, h = w / hv, c = w - h * hv;
+    if (e >= vecs || t >= a.src[i]) continue;
+    const int old = a.rows[static_cast<int64_t>(i) * ps + t];
+    const int64_t in = h * a.pool.head_stride + c * 16;
+    const int64_t from = (old >> a.shift) * a.pool.page_stride + (old & (ps - 1)) * a.pool.token_stride + in;
+    const int64_t to = a.dst[i] * a.pool.page_stride + t * a.pool.token_stride + in;
+    uint4 v[M_PLANES];
 #pragma unroll
-    for (int k = 0; k < M_UNROLL; ++k) {
-      const int e = part * M_THREADS * M_UNROLL + k * M_THREADS + threadIdx.x;
-      const int t = e / tv, w = e - t * tv, h = w / hv, c = w - h * hv;
-      at[k] = -1;
-      if (e < vecs && t < tokens) {
-        const int old = a.rows[static_cast<int64_t>(i) * ps + t];
-        const int64_t in = h * a.pool.head_stride + c * 16;
-        at[k] = to * a.pool.page_stride + t * a.pool.token_stride + in;
-        v[k] = *reinterpret_cast<const uint4*>(base + (old >> a.shift) * a.pool.page_stride +
-                                               (old & (ps - 1)) * a.pool.token_stride + in);
-      }
+    for (int k = 0; k < M_PLANES; ++k) {
+      const int plane = plane0 + k;
+      if (plane < planes)
+        v[k] = *reinterpret_cast<const uint4*>(static_cast<char*>(a.pool.data) + (plane >> 1) * a.pool.layer_stride +
+                                               (plane & 1) * a.pool.kv_stride + from);
     }
 #pragma unroll
-    for (int k = 0; k < M_UNROLL; ++k)
-      if (at[k] >= 0) *reinterpret_cast<uint4*>(base + at[k]) = v[k];
+    for (int k = 0; k < M_PLANES; ++k) {
+      const int plane = plane0 + k;
+      if (plane < planes)
+        *reinterpret_cast<uint4*>(static_cast<char*>(a.pool.data) + (plane >> 1) * a.pool.layer_stride +
+                                  (plane & 1) * a.pool.kv_stride + to) = v[k];
+    }
   }
 }
 
@@ -492,7 +510,7 @@ int check_call(const mrsa_page_table* t, const void* seqs, int64_t n, const void
   if (t == nullptr) return MRSA_ERR_NULL;
   if (int rc = check_page_table(t)) return rc;
   if (!t->refcount || (n > 0 && !seqs)) return MRSA_ERR_NULL;
-  if (n < 0 || n > P_MAX) return MRSA_ERR_SHAPE;
+  if (n < 0 || n > P_MAX || n * t->max_pages > 0x7fffffffLL) return MRSA_ERR_SHAPE;
   if (needs_ws && n > 0 && (!ws || ws_bytes < mrsa_page_workspace(t, n))) return MRSA_ERR_WORKSPACE;
   if (needs_ws && (reinterpret_cast<uintptr_t>(ws) & 15)) return MRSA_ERR_ALIGN;
   return MRSA_OK;
@@ -508,10 +526,40 @@ PlanArgs plan_args(const mrsa_page_table* t, const int32_t* seqs, int64_t n, voi
   return a;
 }
 
+// One CTA where that keeps it busy for a few steps; more for larger tables,
+// pools and (compact) keep masks: a barrier of a cluster costs more than that
+// of a CTA (four forks and their blocks in a pool of 43 pages: 20.5 us with eight
+// CTAs).
+template <Op kOp>
+int launch_plan(const PlanArgs& a, cudaStream_t s) {
+  int64_t work = static_cast<int64_t>(a.n) * a.t.max_pages;
+  if (kOp == kCompact) work = work * a.t.page_size / 2;
+  if (kOp != kFree && work < a.t.pages) work = a.t.pages;
+  unsigned ctas = 1;
+  while (ctas < P_CLUSTER && work > static_cast<int64_t>(ctas) * 4 * P_THREADS) ctas *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(P_THREADS);
+  cfg.stream = s;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = ctas;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, page_plan_kernel<kOp>, a);
+  if (e != cudaSuccess) {
+    mrsa::note_cuda_error(e, __func__);
+    (void)cudaGetLastError();
+    return MRSA_ERR_LAUNCH;
+  }
+  return MRSA_OK;
+}
+
 template <typename K>
 int launch_move(K kernel, const MoveArgs& a, int64_t most_pages, bool after_plan, cudaStream_t s) {
-  const int64_t vecs = a.page_bytes / 16, parts = (vecs + M_THREADS * M_UNROLL - 1) / (M_THREADS * M_UNROLL);
-  int64_t units = most_pages * a.pool.layers * 2 * parts;
+  // both kernels' units are of at least M_THREADS * M_UNROLL vectors
+  int64_t units = (most_pages * a.pool.layers * 2 * (a.page_bytes / 16) + M_THREADS * M_UNROLL - 1) / (M_THREADS * M_UNROLL);
   const int64_t fill = static_cast<int64_t>(sm_count()) * 8;
   if (units > fill) units = fill;
   cudaLaunchConfig_t cfg = {};
@@ -543,9 +591,7 @@ extern "C" int mrsa_page_free(const mrsa_page_table* t, const int32_t* seqs, int
   if (int rc = check_call(t, seqs, n, nullptr, 0, false)) return rc;
   if (n == 0) return MRSA_OK;
   mrsa::DeviceScope device_scope(t->table);
-  page_plan_kernel<kFree><<<P_CLUSTER, P_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(plan_args(t, seqs, n, nullptr));
-  MRSA_CHECK_LAUNCH();
-  return MRSA_OK;
+  return launch_plan<kFree>(plan_args(t, seqs, n, nullptr), static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int mrsa_page_extend(const mrsa_page_table* t, const int32_t* seqs, const int32_t* tokens, int64_t all,
@@ -557,9 +603,7 @@ extern "C" int mrsa_page_extend(const mrsa_page_table* t, const int32_t* seqs, c
   PlanArgs a = plan_args(t, seqs, n, workspace);
   a.extra = tokens;
   a.all = all;
-  page_plan_kernel<kExtend><<<P_CLUSTER, P_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(a);
-  MRSA_CHECK_LAUNCH();
-  return MRSA_OK;
+  return launch_plan<kExtend>(a, static_cast<cudaStream_t>(stream));
 }
 
 namespace {
@@ -591,8 +635,7 @@ extern "C" int mrsa_page_fork(const mrsa_page_table* t, const mrsa_page_pool* po
   PlanArgs a = plan_args(t, dst, n, workspace);
   a.src = src;
   a.extra = share;
-  page_plan_kernel<kFork><<<P_CLUSTER, P_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(a);
-  MRSA_CHECK_LAUNCH();
+  if (int rc = launch_plan<kFork>(a, static_cast<cudaStream_t>(stream))) return rc;
   MoveArgs m = move_args(t, pool);
   m.head = a.ws.head;
   m.dst = a.ws.fresh;
@@ -611,8 +654,7 @@ extern "C" int mrsa_page_compact(const mrsa_page_table* t, const mrsa_page_pool*
   mrsa::DeviceScope device_scope(t->table);
   PlanArgs a = plan_args(t, seqs, n, workspace);
   a.keep = keep;
-  page_plan_kernel<kCompact><<<P_CLUSTER, P_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(a);
-  MRSA_CHECK_LAUNCH();
+  if (int rc = launch_plan<kCompact>(a, static_cast<cudaStream_t>(stream))) return rc;
   MoveArgs m = move_args(t, pool);
   m.head = a.ws.head;
   m.dst = a.ws.fresh;
