@@ -6,8 +6,8 @@
 // over a sequence's cached tokens (masked tokens and, when causal, tokens past
 // the query's own position have weight zero; a row that sees nothing gets
 // zeros and -inf).  With R query rows per KV head a key's 4 D bytes (K and V)
-// meet 4 D R products and sums: R flops per byte, so up to some 40 rows the
-// cache's bytes bound it.
+// meet 4 D R products and sums: R flops per byte, so for few rows the cache's
+// bytes bound it.
 //
 // Four warps per CTA, each on 16 keys of a 64-key tile, as if alone: its own
 // ring of cp.async stages, its own running maximum, sum and output, no barrier
@@ -33,7 +33,11 @@ constexpr int A_WARPS = 4, A_THREADS = 32 * A_WARPS;
 constexpr int A_KEYS = 16;                  // keys per warp and tile
 constexpr int A_TILE = A_KEYS * A_WARPS;    // keys per tile
 constexpr int A_STAGES = 3;
-constexpr int kTokenRows = 32;              // more query rows per KV head go to the tensor cores (paged_block.cu)
+// More query rows per KV head go to the tensor cores (paged_block.cu).  131072
+// cached tokens of 28 / 4 heads: 14 rows 56 us here and 69 there, 21 rows 99
+// (in row tiles of 32) and 70; sixteen sequences of up to 16384: 64 and 80, 117
+// and 81.
+constexpr int kTokenRows = 16;
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
@@ -90,13 +94,20 @@ __global__ void __launch_bounds__(A_THREADS) paged_token_kernel(const __grid_con
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
 
-  paged::count_tiles<A_THREADS>(a, sm.batch, sm.warp_sums);
-  const paged::Deal deal(a, sm.batch.prefix[a.batch] * a.kv_heads * a.row_tiles);
   const int cta = static_cast<int>(blockIdx.x);
-  const int t_begin = cta < deal.ctas ? deal.begin(cta) : 0, t_end = cta < deal.ctas ? deal.begin(cta + 1) : 0;
+  int t_begin = 0, t_end = 1;
+  paged::Piece pc;
+  if (a.undivided) {
+    pc = paged::unit_at(a, cta);
+  } else {
+    paged::count_tiles<A_THREADS>(a, sm.batch, sm.warp_sums);
+    const paged::Deal deal(a, sm.batch.prefix[a.batch] * a.kv_heads * a.row_tiles);
+    t_begin = cta < deal.ctas ? deal.begin(cta) : 0;
+    t_end = cta < deal.ctas ? deal.begin(cta + 1) : 0;
+  }
 
   for (int t_now = t_begin; t_now < t_end;) {
-    const paged::Piece pc = paged::piece_at(a, sm.batch, t_now, t_end);
+    if (!a.undivided) pc = paged::piece_at(a, sm.batch, t_now, t_end);
     const int b = pc.b, h = pc.h, n = pc.n, r0 = pc.r0, nrows = pc.nrows, tile0 = pc.tile0, tile1 = pc.tile1;
 
     // ---- this thread's part of Q^T: column lane / 4 of each 8-row block
@@ -327,7 +338,7 @@ __global__ void __launch_bounds__(A_THREADS) paged_token_kernel(const __grid_con
       }
     }
     __syncthreads();
-    t_now += tile1 - tile0;
+    t_now += a.undivided ? 1 : tile1 - tile0;
   }
 }
 
@@ -434,24 +445,20 @@ int launch_token(const Args& a, cudaStream_t s) {
   const int smem = static_cast<int>(sizeof(TokenSmem<kD, kNT>));
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return MRSA_ERR_LAUNCH;
-  kernel<<<static_cast<unsigned>(a.grid), A_THREADS, smem, s>>>(a);
+  const unsigned ctas = static_cast<unsigned>(a.undivided ? a.batch * a.kv_heads * a.row_tiles : a.grid);
+  kernel<<<ctas, A_THREADS, smem, s>>>(a);
   MRSA_CHECK_LAUNCH();
   return MRSA_OK;
 }
 
 template <int kD, bool kF16>
 int launch_token_rows(const Args& a, cudaStream_t s) {
-  switch (a.row_tile) {
-    case 8: return launch_token<kD, 1, kF16>(a, s);
-    case 16: return launch_token<kD, 2, kF16>(a, s);
-    default: return launch_token<kD, 4, kF16>(a, s);
-  }
+  return a.row_tile == 8 ? launch_token<kD, 1, kF16>(a, s) : launch_token<kD, 2, kF16>(a, s);
 }
 
 // Query rows per KV head that a unit holds.
 int row_tile_of(int64_t rows) {
-  if (rows > kTokenRows) return paged::kBlockRows;
-  return rows <= 8 ? 8 : (rows <= 16 ? 16 : 32);
+  return rows > kTokenRows ? paged::kBlockRows : (rows <= 8 ? 8 : 16);
 }
 
 // CTAs that fill the machine: two of the small ones per SM.
@@ -584,12 +591,20 @@ extern "C" int mrsa_paged_attention(const mrsa_paged_attention_args* p, const mr
     a.lse = p->lse != nullptr ? p->lse + b0 * p->len * p->q_heads : nullptr;
     a.valid = p->key_valid != nullptr ? p->key_valid + b0 * t->max_pages * t->page_size : nullptr;
     a.seqs = p->seqs + b0;
+    // A CTA takes 0.7 us for a tile, dealing and joining cost 2 us and a launch:
+    // units are left whole where a table row holds few tiles, or where there are
+    // so many units that they fill the machine by themselves (one token of 28 / 4
+    // heads: one sequence of 128 tokens 6.0 against 6.8 us, of 500 10.4 against
+    // 6.8; 64 of up to 1024 24 against 29 us, 16 of them 16.5 against 13.7).
+    const int64_t units = static_cast<int64_t>(a.batch) * a.kv_heads * a.row_tiles;
+    const int64_t most = units / 16 > 2 ? units / 16 : 2;
+    a.undivided = a.rows <= kTokenRows && t->max_pages * t->page_size <= most * A_TILE && units <= 0x7fffffffLL;
     int rc;
     if (a.rows > kTokenRows) rc = paged::launch_block(a, p->dtype, static_cast<int>(p->head_dim), s);
     else if (p->dtype == MRSA_F16) rc = p->head_dim == 128 ? launch_token_rows<128, true>(a, s) : launch_token_rows<64, true>(a, s);
     else rc = p->head_dim == 128 ? launch_token_rows<128, false>(a, s) : launch_token_rows<64, false>(a, s);
     if (rc) return rc;
-    if ((rc = paged::launch_join(a, p->dtype, static_cast<int>(p->head_dim), s))) return rc;
+    if (!a.undivided && (rc = paged::launch_join(a, p->dtype, static_cast<int>(p->head_dim), s))) return rc;
   }
   return MRSA_OK;
 }

@@ -38,6 +38,7 @@ struct Args {
   FastDiv by_group;
   int tile;                            // keys per tile
   int grid;                            // CTAs that the tiles are dealt to
+  int undivided;                       // CTA u has the whole of unit u: nothing to deal or to join
   float scale_log2;                    // softmax scale times log2(e)
   float* part_o;                       // [2 * grid][row_tile][D]
   float* part_ml;                      // [2 * grid][row_tile][2]: maximum (log2), sum
@@ -110,6 +111,21 @@ __device__ __forceinline__ Piece piece_at(const Args& a, const Batch& s, int t, 
   p.nrows = a.rows - p.r0 < a.row_tile ? a.rows - p.r0 : a.row_tile;
   p.seq = s.seq[lo];
   p.n = s.len[lo];
+  return p;
+}
+
+// The whole of unit u.
+__device__ __forceinline__ Piece unit_at(const Args& a, int u) {
+  const int per = a.kv_heads * a.row_tiles, b = u / per, unit = u - b * per;
+  Piece p;
+  p.b = b;
+  p.n = cached_tokens(a, b);
+  p.seq = p.n > 0 ? a.seqs[b] : 0;
+  p.tile0 = 0;
+  p.tile1 = p.tiles = (p.n + a.tile - 1) / a.tile;
+  p.h = unit / a.row_tiles;
+  p.r0 = (unit - p.h * a.row_tiles) * a.row_tile;
+  p.nrows = a.rows - p.r0 < a.row_tile ? a.rows - p.r0 : a.row_tile;
   return p;
 }
 
