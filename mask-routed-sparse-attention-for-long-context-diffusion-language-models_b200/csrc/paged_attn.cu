@@ -591,14 +591,19 @@ extern "C" int mrsa_paged_attention(const mrsa_paged_attention_args* p, const mr
     a.lse = p->lse != nullptr ? p->lse + b0 * p->len * p->q_heads : nullptr;
     a.valid = p->key_valid != nullptr ? p->key_valid + b0 * t->max_pages * t->page_size : nullptr;
     a.seqs = p->seqs + b0;
-    // A CTA takes 0.7 us for a tile, dealing and joining cost 2 us and a launch:
-    // units are left whole where a table row holds few tiles, or where there are
-    // so many units that they fill the machine by themselves (one token of 28 / 4
-    // heads: one sequence of 128 tokens 6.0 against 6.8 us, of 500 10.4 against
-    // 6.8; 64 of up to 1024 24 against 29 us, 16 of them 16.5 against 13.7).
+    // Whole units or equal stretches: for rows of T tiles, a unit per CTA takes T
+    // tiles per wave, stretches units * T / grid, and for each unit that they cut
+    // or begin about `cut` tiles' time (parts written and joined, another launch,
+    // the pipeline drained).  Lengths are not known here, so only rows of up to 32
+    // tiles, where the longest of a ragged batch cannot hold the others up for
+    // long.  Measured, us, whole and cut: one token, one sequence of 128 6.0 and
+    // 6.8, of 512 10.4 and 6.8; sixteen of up to 512 10.7 and 12.5, of up to 1024
+    // 16.5 and 13.7; 64 of up to 1024 24 and 29.  32 tokens, one sequence of 256
+    // 12.5 and 15.6, of 1024 25 and 16; 16 of up to 1024 25 and 33; 48 45 and 64.
     const int64_t units = static_cast<int64_t>(a.batch) * a.kv_heads * a.row_tiles;
-    const int64_t most = units / 16 > 2 ? units / 16 : 2;
-    a.undivided = a.rows <= kTokenRows && t->max_pages * t->page_size <= most * A_TILE && units <= 0x7fffffffLL;
+    const int64_t T = t->max_pages * t->page_size / A_TILE + 1, cut = a.rows > kTokenRows ? 8 : 6;
+    a.undivided = T <= 33 && units <= 0x7fffffffLL &&
+                  T * ((units + a.grid - 1) / a.grid) * a.grid <= units * T + cut * (a.grid + units);
     int rc;
     if (a.rows > kTokenRows) rc = paged::launch_block(a, p->dtype, static_cast<int>(p->head_dim), s);
     else if (p->dtype == MRSA_F16) rc = p->head_dim == 128 ? launch_token_rows<128, true>(a, s) : launch_token_rows<64, true>(a, s);

@@ -118,14 +118,28 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
     tc::tmem_alloc(tc::smem_addr(&sm.tmem_base), 512);
     tc::tmem_relinquish();
   }
-  paged::count_tiles<B_THREADS>(a, sm.batch, sm.warp_sums);
+  const int cta = static_cast<int>(blockIdx.x);
+  Piece unit = {};
+  if (a.undivided) unit = paged::unit_at(a, cta);
+  else paged::count_tiles<B_THREADS>(a, sm.batch, sm.warp_sums);
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tbase = sm.tmem_base;
-  const paged::Deal deal(a, sm.batch.prefix[a.batch] * a.kv_heads * a.row_tiles);
-  const int cta = static_cast<int>(blockIdx.x);
-  const int t_begin = cta < deal.ctas ? deal.begin(cta) : 0, t_end = cta < deal.ctas ? deal.begin(cta + 1) : 0;
+  int t_begin = 0, t_end = unit.tiles;
+  if (!a.undivided) {
+    const paged::Deal deal(a, sm.batch.prefix[a.batch] * a.kv_heads * a.row_tiles);
+    t_begin = cta < deal.ctas ? deal.begin(cta) : 0;
+    t_end = cta < deal.ctas ? deal.begin(cta + 1) : 0;
+  } else if (unit.tiles == 0) {
+    // no keys: zeros, and -inf
+    for (int i = tid; i < unit.nrows * (kD / 8); i += B_THREADS)
+      *reinterpret_cast<uint4*>(a.out + paged::out_row(a, unit, i / (kD / 8)) * kD * 2 + (i % (kD / 8)) * 16) =
+          make_uint4(0u, 0u, 0u, 0u);
+    if (a.lse != nullptr)
+      for (int i = tid; i < unit.nrows; i += B_THREADS) a.lse[paged::out_row(a, unit, i)] = -INFINITY;
+  }
+  auto part_at = [&](int t) { return a.undivided ? unit : paged::piece_at(a, sm.batch, t, t_end); };
   bool ok = true;
 
   if (warp == W_K || warp == W_V) {
@@ -163,7 +177,7 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
     };
     int e = 0;                                   // tiles of the stretch so far
     for (int t_now = t_begin; ok && t_now < t_end;) {
-      const Piece p = paged::piece_at(a, sm.batch, t_now, t_end);
+      const Piece p = part_at(t_now);
       const uint8_t* valid = a.valid != nullptr && is_k
                                  ? a.valid + static_cast<int64_t>(p.b) * a.max_pages * a.page_size : nullptr;
       // the next tile's page numbers and mask bytes are requested a tile ahead
@@ -257,7 +271,7 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
       return true;
     };
     for (int t_now = t_begin; ok && t_now < t_end;) {
-      const Piece p = paged::piece_at(a, sm.batch, t_now, t_end);
+      const Piece p = part_at(t_now);
       const int nt = p.tile1 - p.tile0;
       if (p.nrows <= g * B_ROWS) {
         // no rows for this group: the unit's stages released unused, in order
@@ -312,7 +326,7 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
     const uint32_t t_o = tbase + lane_off + kOCol + 128 * g;
     int e0 = 0, k = 0;            // tiles of the stretch before this unit; tiles of this group so far
     for (int t_now = t_begin; ok && t_now < t_end;) {
-      const Piece p = paged::piece_at(a, sm.batch, t_now, t_end);
+      const Piece p = part_at(t_now);
       const int nt = p.tile1 - p.tile0;
       if (p.nrows > g * B_ROWS) {
         // ---- this row of Q (the S products of the unit before are done: the last S was read)
@@ -566,7 +580,8 @@ int launch(const Args& a, cudaStream_t s) {
   const auto kernel = a.causal ? paged_block_kernel<kD, kF16, true> : paged_block_kernel<kD, kF16, false>;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return MRSA_ERR_LAUNCH;
-  kernel<<<static_cast<unsigned>(a.grid), B_THREADS, smem, s>>>(tk, tv, a);
+  const unsigned ctas = static_cast<unsigned>(a.undivided ? a.batch * a.kv_heads * a.row_tiles : a.grid);
+  kernel<<<ctas, B_THREADS, smem, s>>>(tk, tv, a);
   MRSA_CHECK_LAUNCH();
   return MRSA_OK;
 }
