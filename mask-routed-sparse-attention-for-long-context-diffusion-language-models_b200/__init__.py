@@ -16,6 +16,7 @@ from .local_attention import (bidir_local_attention, cached_local_attention, fle
                               window_attention, window_attention_backward)
 from .paged_cache import (PagedKVCache, page_compact, page_copy, page_extend, page_fork, page_free, paged_append,
                           paged_attention)
+from .paged_decode import PagedDream
 from .rope_fp32 import rope_rotary_pos_emb, single_tensor_rope_autograd, yarn_inv_freq, yarn_rope_qk
 from .rotary import rotary_embedding, rotary_inv_freq
 from .route_weights import route_weights, route_weights_backward, route_weights_torch
@@ -38,7 +39,7 @@ __all__ = [
     "selected_token_attention_tilelang", "load_library", "chunk_pool_backward", "route_weights_backward",
     "route_scores_backward", "fuse_outputs_backward", "window_attention_backward",
     "rotary_embedding", "rotary_inv_freq", "PagedKVCache", "page_compact", "page_copy", "page_extend", "page_fork",
-    "page_free", "paged_append", "paged_attention",
+    "page_free", "paged_append", "paged_attention", "PagedDream",
 ]
 
 
