@@ -12,6 +12,7 @@
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "../../include/mrsa.h"
@@ -116,23 +117,16 @@ void set_k(mrsa_rotary_args& a, const Tensor& k) {
   a.k_heads = k.size(2);
 }
 
-// rotary(q, k, position_ids, inv_freq, attention_factor, layout, inverse)
-PyObject* rotary(PyObject*, PyObject* const* o, Py_ssize_t n) {
-  HANDLE_TH_ERRORS
-  TORCH_CHECK_TYPE(n == 7, "rotary takes 7 arguments");
-  Tensor q = tensor(o[0], "q"), k = tensor(o[1], "k"), pos = tensor(o[2], "position_ids"), inv = tensor(o[3], "inv_freq");
-  const double factor = PyFloat_AsDouble(o[4]);
-  if (PyErr_Occurred()) return nullptr;
+// (q', k') of checked arguments; k may be undefined.
+std::pair<Tensor, Tensor> rotate(Tensor q, Tensor k, Tensor pos, Tensor inv, double factor, bool interleaved, bool inverse) {
   mrsa_rotary_args a = {};
-  a.interleaved = layout_of(o[5]);
-  a.inverse = PyObject_IsTrue(o[6]);
   check_heads(q, "q");
   a.dtype = type_of(q);
   TORCH_CHECK_VALUE(a.dtype >= 0, "q must be BF16, FP16 or FP32, got ", q.scalar_type());
   if (k.defined()) check_like(k, "k", q);
   TORCH_CHECK_VALUE(pos.defined() && inv.defined(), "position_ids must be int64 (B, L) and inv_freq fp32 [n]");
   a.pairs = check_rotation(inv, pos, q);
-  TORCH_CHECK_VALUE(!a.interleaved || q.size(3) % 2 == 0, "the interleaved layout needs an even head dim");
+  TORCH_CHECK_VALUE(!interleaved || q.size(3) % 2 == 0, "the interleaved layout needs an even head dim");
   q = inner_contiguous(q);
   Tensor qo = heads_like(q), ko;
   set_q(a, q, qo);
@@ -148,7 +142,53 @@ PyObject* rotary(PyObject*, PyObject* const* o, Py_ssize_t n) {
   a.len = q.size(1);
   a.head_dim = q.size(3);
   a.attention_factor = static_cast<float>(factor);
-  if (!finish(mrsa_rotary(&a, stream_of(q)), "mrsa_rotary")) return nullptr;
+  a.interleaved = interleaved;
+  a.inverse = inverse;
+  const int rc = mrsa_rotary(&a, stream_of(q));
+  TORCH_CHECK_VALUE(rc != MRSA_ERR_SHAPE && rc != MRSA_ERR_ARG && rc != MRSA_ERR_NULL && rc != MRSA_ERR_ALIGN,
+                    "mrsa_rotary: ", mrsa_strerror(rc));
+  TORCH_CHECK(rc == 0, "mrsa_rotary: ", mrsa_strerror(rc), " [", mrsa_last_error(), "]");
+  return {std::move(qo), std::move(ko)};
+}
+
+// The gradient of a rotation is the rotation by minus the angle.
+struct Rotary : torch::autograd::Function<Rotary> {
+  using List = torch::autograd::variable_list;
+  static List forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& pos,
+                      const Tensor& inv, double factor, bool interleaved) {
+    ctx->save_for_backward({pos, inv});
+    ctx->saved_data["factor"] = factor;
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["pair"] = k.defined();
+    auto [qo, ko] = rotate(q, k, pos, inv, factor, interleaved, false);
+    return k.defined() ? List{qo, ko} : List{qo};
+  }
+  static List backward(torch::autograd::AutogradContext* ctx, const List& g) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!c10::GradMode::is_enabled(), "rotary_embedding: the gradient of its gradient is not recorded");
+    const auto saved = ctx->get_saved_variables();
+    auto [dq, dk] = rotate(g[0], ctx->saved_data["pair"].toBool() ? g[1] : Tensor(), saved[0], saved[1],
+                           ctx->saved_data["factor"].toDouble(), ctx->saved_data["interleaved"].toBool(), true);
+    return {dq, dk, Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+// rotary(q, k, position_ids, inv_freq, attention_factor, layout)
+PyObject* rotary(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(n == 6, "rotary takes 6 arguments");
+  const Tensor &q = tensor(o[0], "q"), &k = tensor(o[1], "k"), &pos = tensor(o[2], "position_ids"),
+               &inv = tensor(o[3], "inv_freq");
+  const double factor = PyFloat_AsDouble(o[4]);
+  if (PyErr_Occurred()) return nullptr;
+  const bool interleaved = layout_of(o[5]) == 1;
+  Tensor qo, ko;
+  if (c10::GradMode::is_enabled() && ((q.defined() && q.requires_grad()) || (k.defined() && k.requires_grad()))) {
+    auto r = Rotary::apply(q, k, pos, inv, factor, interleaved);
+    qo = std::move(r[0]);
+    if (r.size() > 1) ko = std::move(r[1]);
+  } else {
+    std::tie(qo, ko) = rotate(q, k, pos, inv, factor, interleaved, false);
+  }
   PyObject* r = PyTuple_New(2);
   PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(std::move(qo)));
   if (ko.defined()) {

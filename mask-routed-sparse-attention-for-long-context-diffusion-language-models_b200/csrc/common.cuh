@@ -5,6 +5,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/mrsa.h"
 
 namespace mrsa {
@@ -250,6 +252,19 @@ class DeviceScope {
 // SMs of the current device (asked once per device: an attribute query costs
 // as much as a tenth of a launch).
 int sm_count();
+
+// Lets `kernel` have `bytes` of dynamic shared memory, asking the driver once
+// per kernel and device.
+template <typename K>
+bool allow_smem(K* kernel, int bytes, std::atomic<uint64_t>& devices) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+  const uint64_t bit = uint64_t(1) << dev;
+  if (devices.load(std::memory_order_relaxed) & bit) return true;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
+  devices.fetch_or(bit, std::memory_order_relaxed);
+  return true;
+}
 
 // Keeps, per host thread, the CUDA error behind the last MRSA_ERR_LAUNCH
 // (read through mrsa_last_error()).

@@ -443,8 +443,8 @@ template <int kD, int kNT, bool kF16>
 int launch_token(const Args& a, cudaStream_t s) {
   const auto kernel = paged_token_kernel<kD, kNT, kF16>;
   const int smem = static_cast<int>(sizeof(TokenSmem<kD, kNT>));
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-    return MRSA_ERR_LAUNCH;
+  static std::atomic<uint64_t> allowed;
+  if (!allow_smem(kernel, smem, allowed)) return MRSA_ERR_LAUNCH;
   const unsigned ctas = static_cast<unsigned>(a.undivided ? a.batch * a.kv_heads * a.row_tiles : a.grid);
   kernel<<<ctas, A_THREADS, smem, s>>>(a);
   MRSA_CHECK_LAUNCH();

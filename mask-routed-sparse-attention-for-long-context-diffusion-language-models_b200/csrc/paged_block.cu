@@ -569,7 +569,7 @@ bool page_map(CUtensorMap* m, const void* base, int64_t page, int64_t slot, int6
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int kD, bool kF16>
+template <int kD, bool kF16, bool kCausal>
 int launch(const Args& a, cudaStream_t s) {
   CUtensorMap tk, tv;
   if (!page_map(&tk, a.k, a.kp, a.ks, a.kh, a, kD, kF16) || !page_map(&tv, a.v, a.vp, a.vs, a.vh, a, kD, kF16)) {
@@ -577,9 +577,9 @@ int launch(const Args& a, cudaStream_t s) {
     return MRSA_ERR_LAUNCH;
   }
   const int smem = static_cast<int>(sizeof(BlockSmem<kD>) + 1024);
-  const auto kernel = a.causal ? paged_block_kernel<kD, kF16, true> : paged_block_kernel<kD, kF16, false>;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-    return MRSA_ERR_LAUNCH;
+  const auto kernel = paged_block_kernel<kD, kF16, kCausal>;
+  static std::atomic<uint64_t> allowed;
+  if (!allow_smem(kernel, smem, allowed)) return MRSA_ERR_LAUNCH;
   const unsigned ctas = static_cast<unsigned>(a.undivided ? a.batch * a.kv_heads * a.row_tiles : a.grid);
   kernel<<<ctas, B_THREADS, smem, s>>>(tk, tv, a);
   MRSA_CHECK_LAUNCH();
@@ -591,9 +591,14 @@ int launch(const Args& a, cudaStream_t s) {
 namespace mrsa {
 namespace paged {
 
+template <int kD, bool kF16>
+int launch_causal(const Args& a, cudaStream_t s) {
+  return a.causal ? launch<kD, kF16, true>(a, s) : launch<kD, kF16, false>(a, s);
+}
+
 int launch_block(const Args& a, int dtype, int head_dim, cudaStream_t s) {
-  if (dtype == MRSA_F16) return head_dim == 128 ? launch<128, true>(a, s) : launch<64, true>(a, s);
-  return head_dim == 128 ? launch<128, false>(a, s) : launch<64, false>(a, s);
+  if (dtype == MRSA_F16) return head_dim == 128 ? launch_causal<128, true>(a, s) : launch_causal<64, true>(a, s);
+  return head_dim == 128 ? launch_causal<128, false>(a, s) : launch_causal<64, false>(a, s);
 }
 
 }  // namespace paged

@@ -275,8 +275,8 @@ int rotary_launch(RotaryArgs& a, int64_t batch, cudaStream_t s) {
     const auto kernel = rotary_kernel<T, 16 / static_cast<int>(sizeof(T)), true>;
     const size_t ring = static_cast<size_t>(R_AHEAD) * 2 * threads * 16;
     constexpr size_t kMost = R_AHEAD * 2 * R_MAX_THREADS * 16 + R_MAX_RUN * R_MAX_PAIRS * sizeof(float2) * 2;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kMost)) != cudaSuccess)
-      return MRSA_ERR_LAUNCH;
+    static std::atomic<uint64_t> allowed;
+    if (!allow_smem(kernel, static_cast<int>(kMost), allowed)) return MRSA_ERR_LAUNCH;
     kernel<<<g, threads, ring + angles, s>>>(a);
   } else if (a.interleaved) {
     rotary_kernel<T, 2, false><<<g, threads, angles, s>>>(a);

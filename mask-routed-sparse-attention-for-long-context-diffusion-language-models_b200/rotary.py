@@ -9,7 +9,6 @@ bf16, fp16 or fp32, views of a fused projection as they are, and its gradient.
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .rope_fp32 import yarn_inv_freq
@@ -41,22 +40,6 @@ def rotary_inv_freq(dim: int, base: float = 1.0e6, *, scaling: str = "none", fac
     return inv.to(dtype=torch.float32, device=device), 1.0
 
 
-class _Rotary(torch.autograd.Function):
-    """The gradient of a rotation is the rotation by minus the angle."""
-
-    @staticmethod
-    def forward(ctx, q, k, position_ids, inv_freq, factor, layout):
-        ctx.save_for_backward(position_ids, inv_freq)
-        ctx.rest = factor, layout
-        return _lib.ext().rotary(q, k, position_ids, inv_freq, factor, layout, False)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, gq, gk):
-        dq, dk = _lib.ext().rotary(gq, gk, *ctx.saved_tensors, *ctx.rest, True)
-        return dq, dk, None, None, None, None
-
-
 def rotary_embedding(q: torch.Tensor, k: torch.Tensor | None, position_ids: torch.Tensor, inv_freq: torch.Tensor,
                      attention_factor: float = 1.0, *, layout: str = "half"):
     """Rotary positions of ``q [B, L, Hq, D]`` and ``k [B, L, Hk, D]`` (or
@@ -68,6 +51,4 @@ def rotary_embedding(q: torch.Tensor, k: torch.Tensor | None, position_ids: torc
     inv_freq`` and cos and sin are times ``attention_factor``, as in
     :func:`yarn_rope_qk`; fp32 arithmetic, one rounding.  Any batch, token and
     head strides.  Records the gradient of q and k where one is wanted."""
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        return _Rotary.apply(q, k, position_ids, inv_freq, attention_factor, layout)
-    return _lib.ext().rotary(q, k, position_ids, inv_freq, attention_factor, layout, False)
+    return _lib.ext().rotary(q, k, position_ids, inv_freq, attention_factor, layout)
