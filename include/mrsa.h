@@ -539,7 +539,7 @@ typedef struct {
   float* lse;                 /* [batch, len, q_heads] natural log, or NULL */
   const uint8_t* key_valid;   /* [batch, max_pages * page_size], 0: token masked; NULL: none is */
   const int32_t* seqs;        /* [batch] */
-  int64_t q_batch_stride, q_token_stride, q_head_stride;   /* in elements, multiples of 8 */
+  int64_t q_batch_stride, q_token_stride, q_head_stride;   /* in elements, positive multiples of 8 */
   int64_t k_page_stride, k_slot_stride, k_head_stride;
   int64_t v_page_stride, v_slot_stride, v_head_stride;
   int64_t batch, len, q_heads, kv_heads, head_dim;         /* head_dim 64 or 128 */

@@ -510,7 +510,7 @@ PyObject* attend(PyObject*, PyObject* const* o, Py_ssize_t n) {
     valid = aligned(valid);
     a.key_valid = in<uint8_t>(valid);
   }
-  if (q.stride(3) != 1 || ((q.stride(0) | q.stride(1) | q.stride(2)) & 7) ||
+  if (q.stride(3) != 1 || q.stride(0) <= 0 || q.stride(1) <= 0 || q.stride(2) <= 0 || ((q.stride(0) | q.stride(1) | q.stride(2)) & 7) ||
       (reinterpret_cast<uintptr_t>(q.const_data_ptr()) & 15))
     q = aligned(q);
   Tensor out = heads_like(q), lse;

@@ -368,7 +368,7 @@ __global__ void __launch_bounds__(32 * J_WARPS) paged_join_kernel(const __grid_c
     const int r = static_cast<int>(row - bh * a.rows), b = static_cast<int>(bh / a.kv_heads);
     const int h = static_cast<int>(bh) - b * a.kv_heads;
     const int tiles = prefix[b + 1] - prefix[b];
-    const int rt = r / a.row_tile, rr = r - rt * a.row_tile;
+    const int rt = r / a.row_step, rr = r - rt * a.row_step;
     const int i = a.by_group.div(r), g = r - i * a.group;
     const int64_t at = (static_cast<int64_t>(b) * a.len + i) * a.q_heads + h * a.group + g;
     const int first = prefix[b] * per + (h * a.row_tiles + rt) * tiles;
@@ -456,13 +456,14 @@ int launch_token_rows(const Args& a, cudaStream_t s) {
   return a.row_tile == 8 ? launch_token<kD, 1, kF16>(a, s) : launch_token<kD, 2, kF16>(a, s);
 }
 
-// Query rows per KV head that a unit holds.
-int row_tile_of(int64_t rows) {
-  return rows > kTokenRows ? paged::kBlockRows : (rows <= 8 ? 8 : 16);
+bool to_tensor_cores(int64_t rows, int64_t group) { return rows > kTokenRows && group <= paged::kBlockGroup; }
+
+int row_tile_of(int64_t rows, int64_t group) {
+  return to_tensor_cores(rows, group) ? paged::kBlockRows : (rows <= 8 ? 8 : 16);
 }
 
 // CTAs that fill the machine: two of the small ones per SM.
-int grid_of(int64_t rows) { return rows > kTokenRows ? sm_count() : 2 * sm_count(); }
+int grid_of(int64_t rows, int64_t group) { return to_tensor_cores(rows, group) ? sm_count() : 2 * sm_count(); }
 
 bool sizes_ok(const mrsa_paged_attention_args* p) {
   return p->batch >= 0 && p->len >= 0 && p->kv_heads >= 1 && p->q_heads >= p->kv_heads &&
@@ -476,11 +477,11 @@ bool sizes_ok(const mrsa_paged_attention_args* p) {
 namespace mrsa {
 namespace paged {
 
-size_t workspace(int64_t grid, int64_t row_tile, int64_t head_dim) {
+static size_t workspace(int64_t grid, int64_t row_tile, int64_t head_dim) {
   return static_cast<size_t>(2 * grid * row_tile * (head_dim + 2)) * 4;
 }
 
-int launch_join(const Args& a, int dtype, int head_dim, cudaStream_t s) {
+static int launch_join(const Args& a, int dtype, int head_dim, cudaStream_t s) {
   const int64_t units = static_cast<int64_t>(a.batch) * a.kv_heads * a.row_tiles;
   const int64_t rows = static_cast<int64_t>(a.batch) * a.kv_heads * a.rows;
   const bool share = a.grid >= 8 * units;         // eight pieces and more to a unit
@@ -517,8 +518,8 @@ int launch_join(const Args& a, int dtype, int head_dim, cudaStream_t s) {
 
 extern "C" size_t mrsa_paged_attention_workspace(const mrsa_paged_attention_args* p) {
   if (p == nullptr || !sizes_ok(p)) return 0;
-  const int64_t rows = p->len * (p->q_heads / p->kv_heads);
-  return paged::workspace(grid_of(rows), row_tile_of(rows), p->head_dim);
+  const int64_t group = p->q_heads / p->kv_heads, rows = p->len * group;
+  return paged::workspace(grid_of(rows, group), row_tile_of(rows, group), p->head_dim);
 }
 
 extern "C" int mrsa_paged_attention(const mrsa_paged_attention_args* p, const mrsa_page_table* t, void* workspace,
@@ -570,10 +571,13 @@ extern "C" int mrsa_paged_attention(const mrsa_paged_attention_args* p, const mr
   a.rows = a.len * a.group;
   a.causal = p->causal != 0;
   a.scale_log2 = p->scale * kLog2e;
-  a.row_tile = row_tile_of(a.rows);
-  a.row_tiles = (a.rows + a.row_tile - 1) / a.row_tile;
+  const bool block = to_tensor_cores(a.rows, a.group);
+  a.row_tile = row_tile_of(a.rows, a.group);
+  a.group_rows = block ? paged::kBlockGroup / a.group * a.group : a.row_tile;
+  a.row_step = block ? 2 * a.group_rows : a.row_tile;
+  a.row_tiles = (a.rows + a.row_step - 1) / a.row_step;
   a.tile = A_TILE;          // of both kernels
-  a.grid = grid_of(a.rows);
+  a.grid = grid_of(a.rows, a.group);
   const int64_t slots = 2 * static_cast<int64_t>(a.grid) * a.row_tile;
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = a.part_o + slots * p->head_dim;
@@ -601,15 +605,18 @@ extern "C" int mrsa_paged_attention(const mrsa_paged_attention_args* p, const mr
     // 16.5 and 13.7; 64 of up to 1024 24 and 29.  32 tokens, one sequence of 256
     // 12.5 and 15.6, of 1024 25 and 16; 16 of up to 1024 25 and 33; 48 45 and 64.
     const int64_t units = static_cast<int64_t>(a.batch) * a.kv_heads * a.row_tiles;
-    const int64_t T = t->max_pages * t->page_size / A_TILE + 1, cut = a.rows > kTokenRows ? 8 : 6;
+    const int64_t T = t->max_pages * t->page_size / A_TILE + 1, cut = block ? 8 : 6;
     a.undivided = T <= 33 && units <= 0x7fffffffLL &&
                   T * ((units + a.grid - 1) / a.grid) * a.grid <= units * T + cut * (a.grid + units);
     int rc;
-    if (a.rows > kTokenRows) rc = paged::launch_block(a, p->dtype, static_cast<int>(p->head_dim), s);
+    if (block) rc = paged::launch_block(a, p->dtype, static_cast<int>(p->head_dim), s);
     else if (p->dtype == MRSA_F16) rc = p->head_dim == 128 ? launch_token_rows<128, true>(a, s) : launch_token_rows<64, true>(a, s);
     else rc = p->head_dim == 128 ? launch_token_rows<128, false>(a, s) : launch_token_rows<64, false>(a, s);
     if (rc) return rc;
-    if (!a.undivided && (rc = paged::launch_join(a, p->dtype, static_cast<int>(p->head_dim), s))) return rc;
+    if (!a.undivided &&
+        (rc = block ? paged::launch_block_join(a, p->dtype, static_cast<int>(p->head_dim), s)
+                    : paged::launch_join(a, p->dtype, static_cast<int>(p->head_dim), s)))
+      return rc;
   }
   return MRSA_OK;
 }

@@ -1,7 +1,7 @@
 // How the work of attention over pages is cut: shared by the kernels that do
 // it and the one that joins their parts.
 //
-// A unit is one batch row, one KV head and one tile of its query rows (row r =
+// A unit is one batch row, one KV head and `row_step` of its query rows (row r =
 // token r / G of the call, head r % G of the group); it walks the sequence's
 // cached tokens in tiles of `tile` keys.  All units' key tiles, end to end,
 // are dealt to the CTAs in equal stretches, so ragged lengths and one long
@@ -34,13 +34,16 @@ struct Args {
   int64_t qb, qt, qh;                  // bytes
   int64_t kp, ks, kh, vp, vs, vh;      // bytes: page, slot, head
   int max_seqs, max_pages, pages, page_size, page_shift;
-  int batch, len, q_heads, kv_heads, group, rows, row_tile, row_tiles, causal;
+  int batch, len, q_heads, kv_heads, group, rows, causal;
+  int row_step, row_tiles;             // query rows of a unit; units that hold a head's rows
+  int row_tile;                        // rows of a part in the workspace
+  int group_rows;                      // rows per MMA tile of 128 (paged_block.cu)
   FastDiv by_group;
   int tile;                            // keys per tile
   int grid;                            // CTAs that the tiles are dealt to
   int undivided;                       // CTA u has the whole of unit u: nothing to deal or to join
   float scale_log2;                    // softmax scale times log2(e)
-  float* part_o;                       // [2 * grid][row_tile][D]
+  float* part_o;                       // [2 * grid][row_tile][D]; paged_block.cu: [2 * grid][D / 4][row_tile][4]
   float* part_ml;                      // [2 * grid][row_tile][2]: maximum (log2), sum
 };
 
@@ -107,8 +110,8 @@ __device__ __forceinline__ Piece piece_at(const Args& a, const Batch& s, int t, 
   p.tile0 = in_row - unit * p.tiles;
   p.tile1 = end - t < p.tiles - p.tile0 ? p.tile0 + end - t : p.tiles;
   p.h = unit / a.row_tiles;
-  p.r0 = (unit - p.h * a.row_tiles) * a.row_tile;
-  p.nrows = a.rows - p.r0 < a.row_tile ? a.rows - p.r0 : a.row_tile;
+  p.r0 = (unit - p.h * a.row_tiles) * a.row_step;
+  p.nrows = a.rows - p.r0 < a.row_step ? a.rows - p.r0 : a.row_step;
   p.seq = s.seq[lo];
   p.n = s.len[lo];
   return p;
@@ -124,8 +127,8 @@ __device__ __forceinline__ Piece unit_at(const Args& a, int u) {
   p.tile0 = 0;
   p.tile1 = p.tiles = (p.n + a.tile - 1) / a.tile;
   p.h = unit / a.row_tiles;
-  p.r0 = (unit - p.h * a.row_tiles) * a.row_tile;
-  p.nrows = a.rows - p.r0 < a.row_tile ? a.rows - p.r0 : a.row_tile;
+  p.r0 = (unit - p.h * a.row_tiles) * a.row_step;
+  p.nrows = a.rows - p.r0 < a.row_step ? a.rows - p.r0 : a.row_step;
   return p;
 }
 
@@ -170,12 +173,12 @@ __device__ __forceinline__ int64_t out_row(const Args& a, const Piece& p, int r)
   return (static_cast<int64_t>(p.b) * a.len + i) * a.q_heads + p.h * a.group + g;
 }
 
-// paged_block.cu: the units of a.row_tile = kBlockRows rows on a.grid CTAs, one per SM.
-constexpr int kBlockRows = 256;
+// paged_block.cu: units of two MMA tiles of 128 rows, each of the rows of whole
+// tokens, on a.grid CTAs, one per SM; and the join of their parts.
+constexpr int kBlockRows = 256, kBlockGroup = 128;
 int launch_block(const Args& a, int dtype, int head_dim, cudaStream_t s);
+int launch_block_join(const Args& a, int dtype, int head_dim, cudaStream_t s);
 
-size_t workspace(int64_t grid, int64_t row_tile, int64_t head_dim);
-int launch_join(const Args& a, int dtype, int head_dim, cudaStream_t s);
 
 }  // namespace paged
 }  // namespace mrsa

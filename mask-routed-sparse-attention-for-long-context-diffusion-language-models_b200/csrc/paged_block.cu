@@ -37,7 +37,7 @@ using paged::Args;
 using paged::Piece;
 
 constexpr int B_TILE = 64;         // keys per tile
-constexpr int B_ROWS = 128;        // rows per MMA tile; two per CTA
+constexpr int B_ROWS = paged::kBlockGroup;   // rows per MMA tile; two per CTA
 constexpr int NKS = 4, NVS = 4;    // K and V stages
 constexpr int NMS = 8;             // key-mask slots
 constexpr int B_THREADS = 384;
@@ -46,9 +46,11 @@ constexpr uint32_t kOCol = 256;    // S buffer i at [64 i, 64 i + 64), O of grou
 
 template <int kD>
 struct __align__(1024) BlockSmem {
-  unsigned char q[2][kD / 64][B_ROWS * 128];     // [row tile][64 dims][row], 128-byte swizzled
+  unsigned char q[2][kD / 64][B_ROWS * 128];     // [row tile][64 dims][row], 128-byte swizzled; rows past
+                                                 // a.group_rows hold anything: a row's products are its own
   unsigned char k[NKS][kD / 64][B_TILE * 128];
   unsigned char v[NVS][kD / 64][B_TILE * 128];   // the MN-major B operand of P.V
+  uint4 stage[8][128];                           // [softmax warp]: 32 output rows of 64 bytes
   float limit[NMS][B_TILE];                      // +inf for a key that counts, else -inf
   unsigned long long kmask[NMS];                 // bit j: key j of the tile counts
   uint64_t qfull[2], kfull[NKS], kfree[NKS], vfull[NVS], vfree[NVS], vclean[NVS], mfull[NMS];
@@ -81,7 +83,8 @@ struct TilePages {
 };
 
 template <int kD, bool kF16, bool kCausal>
-__global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_constant__ CUtensorMap tm_k,
+__global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_constant__ CUtensorMap tm_q,
+                                                                   const __grid_constant__ CUtensorMap tm_k,
                                                                    const __grid_constant__ CUtensorMap tm_v,
                                                                    const __grid_constant__ Args a) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
@@ -108,7 +111,7 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
       tc::mbar_init(tc::smem_addr(&sm.pfree[s]), 1);
     }
     for (int s = 0; s < 2; ++s) {
-      tc::mbar_init(tc::smem_addr(&sm.qfull[s]), 4);
+      tc::mbar_init(tc::smem_addr(&sm.qfull[s]), 1);
       tc::mbar_init(tc::smem_addr(&sm.drain[s]), 1);
     }
     sm.abort_flag = 0;
@@ -273,7 +276,7 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
     for (int t_now = t_begin; ok && t_now < t_end;) {
       const Piece p = part_at(t_now);
       const int nt = p.tile1 - p.tile0;
-      if (p.nrows <= g * B_ROWS) {
+      if (p.nrows <= g * a.group_rows) {
         // no rows for this group: the unit's stages released unused, in order
         for (int i = 0; ok && i < nt; ++i, ++e) {
           ok = tc::wait_bounded_warp(tc::smem_addr(&sm.kfull[e % NKS]), (e / NKS) & 1, abort_flag) &&
@@ -285,7 +288,18 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
           __syncwarp();
         }
       } else {
-        ok = tc::wait_bounded_warp(tc::smem_addr(&sm.qfull[g]), units & 1, abort_flag);
+        // Q: the tokens of this tile, G rows each.  Every product with the Q before is
+        // done: the softmax has had its last S.
+        const uint32_t qb = tc::smem_addr(&sm.qfull[g]);
+        if (tc::elect_one()) {
+          tc::mbar_arrive_expect_tx(qb, a.group_rows * kD * 2);
+#pragma unroll
+          for (int hf = 0; hf < kHalves; ++hf)
+            tc::tma_load_5d(tc::smem_addr(sm.q[g][hf]), &tm_q, 0, hf, p.h * a.group,
+                            a.by_group.div(p.r0 + g * a.group_rows), p.b, qb);
+        }
+        __syncwarp();
+        ok = tc::wait_bounded_warp(qb, units & 1, abort_flag);
         ++units;
         if (ok) ok = issue_s(e, k);
         if (ok && nt > 1) ok = issue_s(e + 1, k + 1);
@@ -320,7 +334,7 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
     }
     __syncwarp();
   } else {
-    // ============================ Q, softmax and epilogue (warps 0-7) ========
+    // ============================ softmax and epilogue (warps 0-7) ===========
     const int g = warp >> 2, r = (warp & 3) * 32 + lane;      // row tile; row = TMEM lane
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t t_o = tbase + lane_off + kOCol + 128 * g;
@@ -328,31 +342,12 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
     for (int t_now = t_begin; ok && t_now < t_end;) {
       const Piece p = part_at(t_now);
       const int nt = p.tile1 - p.tile0;
-      if (p.nrows > g * B_ROWS) {
-        // ---- this row of Q (the S products of the unit before are done: the last S was read)
-        const int row = g * B_ROWS + r;
-        const bool row_ok = row < p.nrows;
-        // the warp's 32 rows, whole rows at a time (a thread per row would touch 32
-        // lines with every load) and all at once; the loop is not unrolled, for a
-        // unit's start finds its instructions uncached
-        {
-          constexpr int kPieces = kD / 8, kPer = 32 / kPieces;     // 16-byte pieces of a row, rows per step
-          const int j = lane % kPieces;
-          const char* src = a.q + p.b * a.qb + (p.h * a.group) * a.qh + j * 16;
-#pragma unroll 1
-          for (int in = (warp & 3) * 32 + lane / kPieces, i = 0; i < kPieces; ++i, in += kPer) {
-            const int qr = g * B_ROWS + in, ti = a.by_group.div(p.r0 + qr), tg = p.r0 + qr - ti * a.group;
-            const bool on = qr < p.nrows;
-            cp_async16_zfill(sm.q[g][j / 8] + in * 128 + (((j & 7) ^ (in & 7)) * 16),
-                             on ? src + ti * a.qt + tg * a.qh : src, on);
-          }
-          cp_async_commit();
-          cp_async_wait<0>();
-        }
-        tc::fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(tc::smem_addr(&sm.qfull[g]));
-        const int last = p.n - a.len + a.by_group.div(p.r0 + (row_ok ? row : 0));   // causal: the last key this row may see
+      const int rows_here = p.nrows - g * a.group_rows;        // of this row tile, where positive
+      if (rows_here > 0) {
+        const int row = g * a.group_rows + r;
+        const bool row_ok = r < a.group_rows && r < rows_here;
+        // causal: the last key this row may see
+        const int last = p.n - a.len + a.by_group.div(p.r0 + (row_ok ? row : 0));
         float m_run = -INFINITY, l_run = 0.f;
         for (int i = 0; i < nt; ++i, ++k) {
           const int sb = 2 * g + (k & 1), e = e0 + i;
@@ -458,18 +453,11 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
         const bool whole = p.whole();
         if (m_run == -INFINITY) l_run = 0.f;       // the row saw no key
         const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
-        // rows leave through shared memory (the warp's own rows of Q, which no product
-        // reads any more), so that the warp writes whole rows
-        const int64_t prow0 = static_cast<int64_t>(2 * blockIdx.x + (t_now == t_begin ? 0 : 1)) * a.row_tile + g * B_ROWS +
-                              (warp & 3) * 32;
-        const int nrow = p.nrows - g * B_ROWS - (warp & 3) * 32;      // rows of this warp that exist
-        // 16-byte piece j of the warp's row i, rows of kRowPieces pieces
-        auto stage = [&](int i, int j, int pieces) -> uint4* {
-          const int at = i * pieces + (j ^ (i & 7));
-          return reinterpret_cast<uint4*>(sm.q[g][at / 256 % kHalves] + (warp & 3) * 4096) + at % 256;
-        };
         if (whole) {
-          constexpr int kRowPieces = kD / 8;
+          // rows leave through shared memory, 32 columns at a time, so that the warp writes
+          // 64 bytes of each: 16-byte piece j of its row i at i * 4 + (j ^ (i & 3)) there
+          uint4* stage = sm.stage[warp];
+          const int nrow = (rows_here < a.group_rows ? rows_here : a.group_rows) - (warp & 3) * 32;   // this warp's
 #pragma unroll 1
           for (int cc = 0; cc < kD; cc += 32) {
             uint32_t o[32];
@@ -489,42 +477,38 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
                   w[q] = pack_bf16x2(f0, f1);
                 }
               }
-              *stage(lane, cc / 8 + j, kRowPieces) = make_uint4(w[0], w[1], w[2], w[3]);
+              stage[lane * 4 + (j ^ (lane & 3))] = make_uint4(w[0], w[1], w[2], w[3]);
             }
+            __syncwarp();
+#pragma unroll
+            for (int i = lane / 4; i < 32; i += 8)
+              if (i < nrow)
+                *reinterpret_cast<uint4*>(a.out + paged::out_row(a, p, g * a.group_rows + (warp & 3) * 32 + i) * kD * 2 +
+                                          cc * 2 + (lane % 4) * 16) = stage[i * 4 + ((lane ^ i) & 3)];
+            __syncwarp();
           }
-          __syncwarp();
-#pragma unroll 4
-          for (int i = lane / kRowPieces; i < nrow && i < 32; i += 32 / kRowPieces)
-            *reinterpret_cast<uint4*>(a.out + paged::out_row(a, p, g * B_ROWS + (warp & 3) * 32 + i) * kD * 2 +
-                                      (lane % kRowPieces) * 16) = *stage(i, lane % kRowPieces, kRowPieces);
           if (row_ok && a.lse != nullptr)
             a.lse[paged::out_row(a, p, row)] = l_run > 0.f ? (m_run + log2f(l_run)) * kLn2 : -INFINITY;
         } else {
-          // fp32: 64 (kD 128) or 32 (kD 64) columns at a time
-          constexpr int kCols = kD / 2, kRowPieces = kCols / 4;
+          // four columns of all rows side by side: the warp's stores are whole lines
+          const int64_t slot = 2 * blockIdx.x + (t_now == t_begin ? 0 : 1);
+          float* dst = a.part_o + (slot * (kD / 4) * a.row_tile + g * B_ROWS + r) * 4;
 #pragma unroll 1
-          for (int cc = 0; cc < kD; cc += kCols) {
-#pragma unroll 1
-            for (int c = 0; c < kCols; c += 32) {
-              uint32_t o[32];
-              tc::tmem_ld16(t_o + cc + c, *reinterpret_cast<uint32_t(*)[16]>(&o[0]));
-              tc::tmem_ld16(t_o + cc + c + 16, *reinterpret_cast<uint32_t(*)[16]>(&o[16]));
-              tc::tmem_wait_ld();
+          for (int cc = 0; cc < kD; cc += 32) {
+            uint32_t o[32];
+            tc::tmem_ld16(t_o + cc, *reinterpret_cast<uint32_t(*)[16]>(&o[0]));
+            tc::tmem_ld16(t_o + cc + 16, *reinterpret_cast<uint32_t(*)[16]>(&o[16]));
+            tc::tmem_wait_ld();
+            if (row_ok) {
 #pragma unroll
               for (int j = 0; j < 8; ++j)
-                *stage(lane, c / 4 + j, kRowPieces) = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+                *reinterpret_cast<uint4*>(dst + static_cast<int64_t>(cc / 4 + j) * a.row_tile * 4) =
+                    make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
             }
             __syncwarp();
-#pragma unroll 4
-            for (int i = lane / kRowPieces; i < nrow && i < 32; i += 32 / kRowPieces)
-              *reinterpret_cast<uint4*>(a.part_o + (prow0 + i) * kD + cc + (lane % kRowPieces) * 4) =
-                  *stage(i, lane % kRowPieces, kRowPieces);
-            __syncwarp();
           }
-          if (row_ok) {
-            a.part_ml[(prow0 + lane) * 2] = m_run;
-            a.part_ml[(prow0 + lane) * 2 + 1] = l_run;
-          }
+          if (row_ok)
+            *reinterpret_cast<float2*>(a.part_ml + (slot * a.row_tile + g * B_ROWS + r) * 2) = make_float2(m_run, l_run);
         }
         tc::fence_before_sync();       // O was read before the next unit's first P is announced
         __syncwarp();
@@ -543,13 +527,125 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
   }
 }
 
+// The parts of each unit joined: a lane per row, columns of four as the parts lie
+// in the workspace.  kShare: a block per 32 rows and 16 columns of a unit, its
+// warps on every eighth part (few units have many parts: one long sequence);
+// else a block per 32 rows, its warps on every eighth column of four.  Nothing to do for a unit that one CTA finished; zeros for one without keys.
+// All that comes from the lengths alone is worked out before the wait.
+template <int kD, bool kF16, bool kShare>
+__global__ void __launch_bounds__(256) paged_block_join_kernel(const __grid_constant__ Args a) {
+  constexpr int kCols = kShare ? 4 : kD / 32;  // columns of four per warp
+  constexpr int kSets = kShare ? kD / 16 : 1;  // blocks that share 32 rows
+  constexpr int kBlocks = paged::kBlockRows / 32 * kSets;
+  __shared__ float4 acc_s[kShare ? 8 : 1][kCols][32];
+  __shared__ float2 ml_s[kShare ? 8 : 1][32];
+  __shared__ paged::Batch batch;
+  __shared__ int warp_sums[8];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  paged::count_tiles<256>(a, batch, warp_sums);
+  const int per = a.kv_heads * a.row_tiles;            // units per batch row
+  const paged::Deal deal(a, batch.prefix[a.batch] * per);
+  const int64_t work = static_cast<int64_t>(a.batch) * per * kBlocks;
+  bool waited = false;
+  for (int64_t w = blockIdx.x; w < work; w += gridDim.x) {
+    const int part = static_cast<int>(w % kBlocks), rb = part / kSets, set = part % kSets;
+    const int u = static_cast<int>(w / kBlocks), b = u / per, unit = u - b * per;
+    auto column = [&](int j) { return kShare ? set * kCols + j : warp + 8 * j; };
+    Piece p;
+    p.b = b;
+    p.h = unit / a.row_tiles;
+    p.r0 = (unit - p.h * a.row_tiles) * a.row_step;
+    p.nrows = a.rows - p.r0 < a.row_step ? a.rows - p.r0 : a.row_step;
+    const int g = rb / (B_ROWS / 32), r = (rb % (B_ROWS / 32)) * 32 + lane;
+    const bool row_ok = r < a.group_rows && g * a.group_rows + r < p.nrows;
+    if (!__any_sync(0xffffffffu, row_ok)) continue;
+    const int tiles = batch.prefix[b + 1] - batch.prefix[b], first = batch.prefix[b] * per + unit * tiles;
+    int c0 = 0, c1 = -1;
+    if (tiles > 0) {
+      c0 = deal.holder(first);
+      c1 = deal.holder(first + tiles - 1);
+      if (c0 == c1) continue;
+    }
+    if (!waited) {
+      waited = true;
+      asm volatile("griddepcontrol.wait;\n" ::: "memory");
+    }
+    float m = -INFINITY, l = 0.f;
+    float4 acc[kCols];
+#pragma unroll
+    for (int j = 0; j < kCols; ++j) acc[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+    // the unit's first piece is the last of its CTA's, unless it is also its first
+    const int64_t slot0 = 2 * static_cast<int64_t>(c0) + (deal.begin(c0) != first ? 1 : 0);
+#pragma unroll 4
+    for (int c = kShare ? c0 + warp : c0; c <= c1; c += kShare ? 8 : 1) {
+      const int64_t slot = c == c0 ? slot0 : 2 * static_cast<int64_t>(c);
+      const int64_t row = g * B_ROWS + (row_ok ? r : 0);
+      const float2 ml = __ldcg(reinterpret_cast<const float2*>(a.part_ml + (slot * a.row_tile + row) * 2));
+      float4 x[kCols];
+#pragma unroll
+      for (int j = 0; j < kCols; ++j)
+        x[j] = __ldcg(reinterpret_cast<const float4*>(a.part_o + ((slot * (kD / 4) + column(j)) * a.row_tile + row) * 4));
+      const float top = fmaxf(m, ml.x);
+      const float cm = m == -INFINITY ? 0.f : fast_exp2(m - top), cp = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - top);
+      m = top;
+      l = l * cm + ml.y * cp;
+#pragma unroll
+      for (int j = 0; j < kCols; ++j) {
+        acc[j].x = acc[j].x * cm + x[j].x * cp;
+        acc[j].y = acc[j].y * cm + x[j].y * cp;
+        acc[j].z = acc[j].z * cm + x[j].z * cp;
+        acc[j].w = acc[j].w * cm + x[j].w * cp;
+      }
+    }
+    if constexpr (kShare) {
+      __syncthreads();             // the block's turn before is done (its warps take the same turns)
+#pragma unroll
+      for (int j = 0; j < kCols; ++j) acc_s[warp][j][lane] = acc[j];
+      ml_s[warp][lane] = make_float2(m, l);
+      __syncthreads();
+      if (warp != 0) continue;
+#pragma unroll
+      for (int k = 1; k < 8; ++k) {
+        const float2 ml = ml_s[k][lane];
+        const float top = fmaxf(m, ml.x);
+        const float cm = m == -INFINITY ? 0.f : fast_exp2(m - top), cp = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - top);
+        m = top;
+        l = l * cm + ml.y * cp;
+#pragma unroll
+        for (int j = 0; j < kCols; ++j) {
+          const float4 x = acc_s[k][j][lane];
+          acc[j].x = acc[j].x * cm + x.x * cp;
+          acc[j].y = acc[j].y * cm + x.y * cp;
+          acc[j].z = acc[j].z * cm + x.z * cp;
+          acc[j].w = acc[j].w * cm + x.w * cp;
+        }
+      }
+    }
+    if (!row_ok) continue;
+    const int64_t at = paged::out_row(a, p, g * a.group_rows + r);
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+#pragma unroll
+    for (int j = 0; j < kCols; ++j) {
+      uint2 v;
+      if constexpr (kF16) {
+        const __half2 lo = __floats2half2_rn(acc[j].x * inv, acc[j].y * inv), hi = __floats2half2_rn(acc[j].z * inv, acc[j].w * inv);
+        v = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+      } else {
+        v = make_uint2(pack_bf16x2(acc[j].x * inv, acc[j].y * inv), pack_bf16x2(acc[j].z * inv, acc[j].w * inv));
+      }
+      *reinterpret_cast<uint2*>(a.out + at * kD * 2 + column(j) * 8) = v;
+    }
+    if (warp == 0 && set == 0 && a.lse != nullptr) a.lse[at] = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+  }
+  // a block that read no part waits too: what follows in the stream follows this grid's end
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+}
+
 PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
 std::once_flag g_encode_once;
 
-// Pages as (dim of 64, slot, 64 dims, head, page); one box: 64 dims of the
-// slots of one page that a tile covers.
-bool page_map(CUtensorMap* m, const void* base, int64_t page, int64_t slot, int64_t head, const Args& a, int head_dim,
-              bool f16) {
+bool make_map(CUtensorMap* m, const void* base, const cuuint64_t (&dims)[5], const cuuint64_t (&strides)[4],
+              const cuuint32_t (&box)[5], bool f16) {
   std::call_once(g_encode_once, [] {
     void* fn = nullptr;
     cudaDriverEntryPointQueryResult q;
@@ -558,22 +654,42 @@ bool page_map(CUtensorMap* m, const void* base, int64_t page, int64_t slot, int6
       g_encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
   });
   if (g_encode == nullptr) return false;
-  const cuuint64_t dims[5] = {64, static_cast<cuuint64_t>(a.page_size), static_cast<cuuint64_t>(head_dim / 64),
-                              static_cast<cuuint64_t>(a.kv_heads), static_cast<cuuint64_t>(a.pages)};
-  const cuuint64_t strides[4] = {static_cast<cuuint64_t>(slot), 128, static_cast<cuuint64_t>(head),
-                                 static_cast<cuuint64_t>(page)};
-  const cuuint32_t box[5] = {64, static_cast<cuuint32_t>(a.page_size < B_TILE ? a.page_size : B_TILE), 1, 1, 1};
   const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
   return g_encode(m, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(base),
                   dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Pages as (64 dims, slot, half, head, page); one box: 64 dims of the slots of
+// one page that a tile covers.
+bool page_map(CUtensorMap* m, const void* base, int64_t page, int64_t slot, int64_t head, const Args& a, int head_dim,
+              bool f16) {
+  const cuuint64_t dims[5] = {64, static_cast<cuuint64_t>(a.page_size), static_cast<cuuint64_t>(head_dim / 64),
+                              static_cast<cuuint64_t>(a.kv_heads), static_cast<cuuint64_t>(a.pages)};
+  const cuuint64_t strides[4] = {static_cast<cuuint64_t>(slot), 128, static_cast<cuuint64_t>(head),
+                                 static_cast<cuuint64_t>(page)};
+  const cuuint32_t box[5] = {64, static_cast<cuuint32_t>(a.page_size < B_TILE ? a.page_size : B_TILE), 1, 1, 1};
+  return make_map(m, base, dims, strides, box, f16);
+}
+
+// Q as (64 dims, half, head, token, batch row); one box: 64 dims of a group's
+// heads in the tokens of an MMA tile, rows (token, head) back to back.
+bool q_map(CUtensorMap* m, const Args& a, int head_dim, bool f16) {
+  const cuuint64_t dims[5] = {64, static_cast<cuuint64_t>(head_dim / 64), static_cast<cuuint64_t>(a.q_heads),
+                              static_cast<cuuint64_t>(a.len), static_cast<cuuint64_t>(a.batch)};
+  // the stride of a dimension of one is never used, and may be anything in the caller's tensor
+  const cuuint64_t strides[4] = {128, static_cast<cuuint64_t>(a.q_heads > 1 ? a.qh : 1024),
+                                 static_cast<cuuint64_t>(a.len > 1 ? a.qt : 1024),
+                                 static_cast<cuuint64_t>(a.batch > 1 ? a.qb : 1024)};
+  const cuuint32_t box[5] = {64, 1, static_cast<cuuint32_t>(a.group), static_cast<cuuint32_t>(a.group_rows / a.group), 1};
+  return make_map(m, a.q, dims, strides, box, f16);
+}
+
 template <int kD, bool kF16, bool kCausal>
 int launch(const Args& a, cudaStream_t s) {
-  CUtensorMap tk, tv;
-  if (!page_map(&tk, a.k, a.kp, a.ks, a.kh, a, kD, kF16) || !page_map(&tv, a.v, a.vp, a.vs, a.vh, a, kD, kF16)) {
-    note_cuda_error(cudaErrorInvalidValue, "page tensor map");
+  CUtensorMap tq, tk, tv;
+  if (!q_map(&tq, a, kD, kF16) || !page_map(&tk, a.k, a.kp, a.ks, a.kh, a, kD, kF16) || !page_map(&tv, a.v, a.vp, a.vs, a.vh, a, kD, kF16)) {
+    note_cuda_error(cudaErrorInvalidValue, "tensor map of q or the pages");
     return MRSA_ERR_LAUNCH;
   }
   const int smem = static_cast<int>(sizeof(BlockSmem<kD>) + 1024);
@@ -581,7 +697,7 @@ int launch(const Args& a, cudaStream_t s) {
   static std::atomic<uint64_t> allowed;
   if (!allow_smem(kernel, smem, allowed)) return MRSA_ERR_LAUNCH;
   const unsigned ctas = static_cast<unsigned>(a.undivided ? a.batch * a.kv_heads * a.row_tiles : a.grid);
-  kernel<<<ctas, B_THREADS, smem, s>>>(tk, tv, a);
+  kernel<<<ctas, B_THREADS, smem, s>>>(tq, tk, tv, a);
   MRSA_CHECK_LAUNCH();
   return MRSA_OK;
 }
@@ -599,6 +715,37 @@ int launch_causal(const Args& a, cudaStream_t s) {
 int launch_block(const Args& a, int dtype, int head_dim, cudaStream_t s) {
   if (dtype == MRSA_F16) return head_dim == 128 ? launch_causal<128, true>(a, s) : launch_causal<64, true>(a, s);
   return head_dim == 128 ? launch_causal<128, false>(a, s) : launch_causal<64, false>(a, s);
+}
+
+template <int kD, bool kF16>
+void (*join_of(bool share))(const Args) {
+  return share ? paged_block_join_kernel<kD, kF16, true> : paged_block_join_kernel<kD, kF16, false>;
+}
+
+int launch_block_join(const Args& a, int dtype, int head_dim, cudaStream_t s) {
+  const int64_t units = static_cast<int64_t>(a.batch) * a.kv_heads * a.row_tiles;
+  const bool share = a.grid >= 8 * units;         // eight parts and more to a unit
+  const int64_t blocks = units * (kBlockRows / 32) * (share ? head_dim / 16 : 1);
+  const int64_t most = 8 * static_cast<int64_t>(sm_count());
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks < most ? blocks : most));
+  cfg.blockDim = dim3(256);
+  cfg.stream = s;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  void (*kernel)(const Args);
+  if (head_dim == 128) kernel = dtype == MRSA_F16 ? join_of<128, true>(share) : join_of<128, false>(share);
+  else kernel = dtype == MRSA_F16 ? join_of<64, true>(share) : join_of<64, false>(share);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
+  if (e != cudaSuccess) {
+    note_cuda_error(e, __func__);
+    (void)cudaGetLastError();
+    return MRSA_ERR_LAUNCH;
+  }
+  return MRSA_OK;
 }
 
 }  // namespace paged
