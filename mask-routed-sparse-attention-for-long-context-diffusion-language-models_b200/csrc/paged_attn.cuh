@@ -40,6 +40,7 @@ struct Args {
   int group_rows;                      // rows per MMA tile of 128 (paged_block.cu)
   FastDiv by_group;
   int tile;                            // keys per tile
+  int cut;                             // what a unit costs beside its tiles, in tiles
   int grid;                            // CTAs that the tiles are dealt to
   int undivided;                       // CTA u has the whole of unit u: nothing to deal or to join
   float scale_log2;                    // softmax scale times log2(e)
@@ -62,8 +63,8 @@ __device__ __forceinline__ int cached_tokens(const Args& a, int b) {
   return n;
 }
 
-// The tiles in stretches that differ by one at most, none empty: the first
-// `extra` CTAs get base + 1.  (The host keeps a launch below 2^31 tiles: 64-bit
+// The whole cost in stretches that differ by one at most, none empty: the first
+// `extra` CTAs get base + 1.  (The host keeps a launch below 2^31: 64-bit
 // divisions here cost each launch a microsecond.)
 struct Deal {
   int total, ctas, base, extra;
@@ -72,7 +73,7 @@ struct Deal {
     base = all / ctas;
     extra = all - base * ctas;
   }
-  // First tile of CTA c's stretch; the CTA whose stretch holds tile t.
+  // Where CTA c's stretch begins; the CTA whose stretch holds step t.
   __device__ __forceinline__ int begin(int c) const { return c * base + (c < extra ? c : extra); }
   __device__ __forceinline__ int holder(int t) const {
     const int wide = extra * (base + 1);
@@ -84,12 +85,13 @@ struct Deal {
 struct Piece {
   int b, h, r0, nrows;          // batch row, KV head, first query row, query rows
   int seq, n;                   // the sequence's row of the table, its cached tokens
-  int tile0, tile1, tiles;      // this part's key tiles, and all of the unit's
+  int tile0, tile1, tiles;      // this part's key tiles (none where tile1 <= tile0), and all of the unit's
+  int span;                     // how much of the stretch it takes
   __device__ __forceinline__ bool whole() const { return tile0 == 0 && tile1 == tiles; }
 };
 
 // What a CTA keeps of the batch: each row's sequence and cached tokens, and the
-// key tiles before it (per head and row tile).
+// cost of the rows before it (tiles and cuts, per head and row tile).
 struct Batch {
   int prefix[kMaxBatch + 1], seq[kMaxBatch], len[kMaxBatch];
 };
@@ -105,10 +107,12 @@ __device__ __forceinline__ Piece piece_at(const Args& a, const Batch& s, int t, 
   }
   Piece p;
   p.b = lo;
-  p.tiles = prefix[lo + 1] - prefix[lo];
-  const int in_row = t - prefix[lo] * per, unit = in_row / p.tiles;
-  p.tile0 = in_row - unit * p.tiles;
-  p.tile1 = end - t < p.tiles - p.tile0 ? p.tile0 + end - t : p.tiles;
+  const int cost = prefix[lo + 1] - prefix[lo], in_row = t - prefix[lo] * per, unit = in_row / cost;
+  const int at = in_row - unit * cost;                 // the unit's first `cut` steps are no tiles
+  p.tiles = cost - a.cut;
+  p.span = end - t < cost - at ? end - t : cost - at;
+  p.tile0 = at > a.cut ? at - a.cut : 0;
+  p.tile1 = at + p.span - a.cut;
   p.h = unit / a.row_tiles;
   p.r0 = (unit - p.h * a.row_tiles) * a.row_step;
   p.nrows = a.rows - p.r0 < a.row_step ? a.rows - p.r0 : a.row_step;
@@ -125,7 +129,7 @@ __device__ __forceinline__ Piece unit_at(const Args& a, int u) {
   p.n = cached_tokens(a, b);
   p.seq = p.n > 0 ? a.seqs[b] : 0;
   p.tile0 = 0;
-  p.tile1 = p.tiles = (p.n + a.tile - 1) / a.tile;
+  p.tile1 = p.tiles = p.span = (p.n + a.tile - 1) / a.tile;
   p.h = unit / a.row_tiles;
   p.r0 = (unit - p.h * a.row_tiles) * a.row_step;
   p.nrows = a.rows - p.r0 < a.row_step ? a.rows - p.r0 : a.row_step;
@@ -144,7 +148,7 @@ __device__ __forceinline__ void count_tiles(const Args& a, Batch& s, int* warp_s
       const int n = cached_tokens(a, b);
       s.seq[b] = a.seqs[b];
       s.len[b] = n;
-      t = (n + a.tile - 1) / a.tile;
+      t = n > 0 ? (n + a.tile - 1) / a.tile + a.cut : 0;
     }
     int x = t;
 #pragma unroll

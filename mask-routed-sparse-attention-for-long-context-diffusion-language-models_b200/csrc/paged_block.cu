@@ -232,7 +232,7 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
         __syncwarp();
         if (!is_k && e >= kLag && !(ok = clean(e - kLag))) break;
       }
-      t_now += p.tile1 - p.tile0;
+      t_now += p.span;
     }
     if (!is_k)
       for (int tt = e < kLag ? 0 : e - kLag; ok && tt < e; ++tt) ok = clean(tt);
@@ -275,8 +275,10 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
     };
     for (int t_now = t_begin; ok && t_now < t_end;) {
       const Piece p = part_at(t_now);
-      const int nt = p.tile1 - p.tile0;
-      if (p.nrows <= g * a.group_rows) {
+      const int nt = p.tile1 > p.tile0 ? p.tile1 - p.tile0 : 0;
+      if (nt == 0) {
+        // the stretch ends before the unit's first tile
+      } else if (p.nrows <= g * a.group_rows) {
         // no rows for this group: the unit's stages released unused, in order
         for (int i = 0; ok && i < nt; ++i, ++e) {
           ok = tc::wait_bounded_warp(tc::smem_addr(&sm.kfull[e % NKS]), (e / NKS) & 1, abort_flag) &&
@@ -326,7 +328,7 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
           if (i + 2 < nt) ok = issue_s(e + 2, k + 2);
         }
       }
-      t_now += nt;
+      t_now += p.span;
     }
     if (tc::elect_one()) {
       tc::mma_commit(tc::smem_addr(&sm.drain[g]));
@@ -341,9 +343,9 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
     int e0 = 0, k = 0;            // tiles of the stretch before this unit; tiles of this group so far
     for (int t_now = t_begin; ok && t_now < t_end;) {
       const Piece p = part_at(t_now);
-      const int nt = p.tile1 - p.tile0;
+      const int nt = p.tile1 > p.tile0 ? p.tile1 - p.tile0 : 0;
       const int rows_here = p.nrows - g * a.group_rows;        // of this row tile, where positive
-      if (rows_here > 0) {
+      if (nt > 0 && rows_here > 0) {
         const int row = g * a.group_rows + r;
         const bool row_ok = r < a.group_rows && r < rows_here;
         // causal: the last key this row may see
@@ -514,7 +516,7 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
         __syncwarp();
       }
       e0 += nt;
-      t_now += nt;
+      t_now += p.span;
     }
   }
 
@@ -559,11 +561,11 @@ __global__ void __launch_bounds__(256) paged_block_join_kernel(const __grid_cons
     const int g = rb / (B_ROWS / 32), r = (rb % (B_ROWS / 32)) * 32 + lane;
     const bool row_ok = r < a.group_rows && g * a.group_rows + r < p.nrows;
     if (!__any_sync(0xffffffffu, row_ok)) continue;
-    const int tiles = batch.prefix[b + 1] - batch.prefix[b], first = batch.prefix[b] * per + unit * tiles;
+    const int cost = batch.prefix[b + 1] - batch.prefix[b], first = batch.prefix[b] * per + unit * cost;
     int c0 = 0, c1 = -1;
-    if (tiles > 0) {
-      c0 = deal.holder(first);
-      c1 = deal.holder(first + tiles - 1);
+    if (cost > 0) {
+      c0 = deal.holder(first + a.cut);
+      c1 = deal.holder(first + cost - 1);
       if (c0 == c1) continue;
     }
     if (!waited) {
@@ -575,7 +577,7 @@ __global__ void __launch_bounds__(256) paged_block_join_kernel(const __grid_cons
 #pragma unroll
     for (int j = 0; j < kCols; ++j) acc[j] = make_float4(0.f, 0.f, 0.f, 0.f);
     // the unit's first piece is the last of its CTA's, unless it is also its first
-    const int64_t slot0 = 2 * static_cast<int64_t>(c0) + (deal.begin(c0) != first ? 1 : 0);
+    const int64_t slot0 = 2 * static_cast<int64_t>(c0) + (deal.begin(c0) < first ? 1 : 0);
 #pragma unroll 4
     for (int c = kShare ? c0 + warp : c0; c <= c1; c += kShare ? 8 : 1) {
       const int64_t slot = c == c0 ? slot0 : 2 * static_cast<int64_t>(c);
