@@ -266,6 +266,40 @@ bool allow_smem(K* kernel, int bytes, std::atomic<uint64_t>& devices) {
   return true;
 }
 
+void note_cuda_error(cudaError_t e, const char* where);
+
+// Programmatic dependent launch, for chains of short kernels: a kernel launched
+// with launch_chained may be put in place while the one before it in the stream
+// still runs (once every CTA of that has called chain_next, or ended), and
+// touches no memory (nor allocates tensor memory that the one before may still
+// ask for) before chain_wait, which returns when all before it is done and seen.
+// Every thread of such a kernel calls chain_wait, so that the end of a grid
+// implies the end of those before it, and calls chain_next after it, so that a
+// kernel put in place early finds everything but the one before it done.
+__device__ __forceinline__ void chain_next() { asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory"); }
+__device__ __forceinline__ void chain_wait() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
+
+template <typename... P, typename... A>
+int launch_chained(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t s, const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+  if (e != cudaSuccess) {
+    note_cuda_error(e, __func__);
+    (void)cudaGetLastError();
+    return MRSA_ERR_LAUNCH;
+  }
+  return MRSA_OK;
+}
+
 // Keeps, per host thread, the CUDA error behind the last MRSA_ERR_LAUNCH
 // (read through mrsa_last_error()).
 void note_cuda_error(cudaError_t e, const char* where);

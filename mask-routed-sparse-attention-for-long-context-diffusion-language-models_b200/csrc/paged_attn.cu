@@ -92,7 +92,8 @@ __global__ void __launch_bounds__(A_THREADS) paged_token_kernel(const __grid_con
   constexpr int kRowBytes = kD * 2;
   static_assert(A_STAGES * 2 * A_KEYS * kRowBytes >= kRows * kD * 4, "a warp's output rows must fit its ring");
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+  chain_wait();
+  chain_next();
 
   const int cta = static_cast<int>(blockIdx.x);
   int t_begin = 0, t_end = 1;
@@ -384,7 +385,7 @@ __global__ void __launch_bounds__(32 * J_WARPS) paged_join_kernel(const __grid_c
     }
     if (!waited) {
       waited = true;
-      asm volatile("griddepcontrol.wait;\n" ::: "memory");
+      chain_wait();
     }
     float m = -INFINITY, l = 0.f, acc[kV];
 #pragma unroll
@@ -440,7 +441,7 @@ __global__ void __launch_bounds__(32 * J_WARPS) paged_join_kernel(const __grid_c
     }
   }
   // a block that read no part waits too: what follows in the stream follows this grid's end
-  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  chain_wait();
 }
 
 template <int kD, int kNT, bool kF16>
@@ -450,9 +451,7 @@ int launch_token(const Args& a, cudaStream_t s) {
   static std::atomic<uint64_t> allowed;
   if (!allow_smem(kernel, smem, allowed)) return MRSA_ERR_LAUNCH;
   const unsigned ctas = static_cast<unsigned>(a.undivided ? a.batch * a.kv_heads * a.row_tiles : a.grid);
-  kernel<<<ctas, A_THREADS, smem, s>>>(a);
-  MRSA_CHECK_LAUNCH();
-  return MRSA_OK;
+  return launch_chained(kernel, dim3(ctas), A_THREADS, smem, s, a);
 }
 
 template <int kD, bool kF16>
@@ -490,15 +489,6 @@ static int launch_join(const Args& a, int dtype, int head_dim, cudaStream_t s) {
   const int64_t rows = static_cast<int64_t>(a.batch) * a.kv_heads * a.rows;
   const bool share = a.grid >= 8 * units;         // eight pieces and more to a unit
   const int64_t blocks = share ? rows : (rows + J_WARPS - 1) / J_WARPS, most = 8 * static_cast<int64_t>(sm_count());
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(blocks < most ? blocks : most));
-  cfg.blockDim = dim3(32 * J_WARPS);
-  cfg.stream = s;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
   void (*kernel)(const Args);
   const bool f16 = dtype == MRSA_F16;
   if (head_dim == 128) {
@@ -508,13 +498,7 @@ static int launch_join(const Args& a, int dtype, int head_dim, cudaStream_t s) {
     if (f16) kernel = share ? paged_join_kernel<64, true, J_WARPS> : paged_join_kernel<64, true, 1>;
     else kernel = share ? paged_join_kernel<64, false, J_WARPS> : paged_join_kernel<64, false, 1>;
   }
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
-  if (e != cudaSuccess) {
-    note_cuda_error(e, __func__);
-    (void)cudaGetLastError();
-    return MRSA_ERR_LAUNCH;
-  }
-  return MRSA_OK;
+  return launch_chained(kernel, dim3(static_cast<unsigned>(blocks < most ? blocks : most)), 32 * J_WARPS, 0, s, a);
 }
 
 }  // namespace paged

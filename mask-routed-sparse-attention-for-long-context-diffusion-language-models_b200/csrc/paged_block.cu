@@ -92,7 +92,6 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
   constexpr int kHalves = kD / 64, kQHalf = B_ROWS * 128, kKHalf = B_TILE * 128, kStage = kHalves * kKHalf;
   volatile int* abort_flag = &sm.abort_flag;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
 
   if (tid == 32) {
     for (int s = 0; s < NKS; ++s) {
@@ -117,6 +116,8 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
     sm.abort_flag = 0;
     tc::fence_mbar_init();
   }
+  chain_wait();
+  chain_next();
   if (warp == 2) {
     tc::tmem_alloc(tc::smem_addr(&sm.tmem_base), 512);
     tc::tmem_relinquish();
@@ -570,7 +571,7 @@ __global__ void __launch_bounds__(256) paged_block_join_kernel(const __grid_cons
     }
     if (!waited) {
       waited = true;
-      asm volatile("griddepcontrol.wait;\n" ::: "memory");
+      chain_wait();
     }
     float m = -INFINITY, l = 0.f;
     float4 acc[kCols];
@@ -640,7 +641,7 @@ __global__ void __launch_bounds__(256) paged_block_join_kernel(const __grid_cons
     if (warp == 0 && set == 0 && a.lse != nullptr) a.lse[at] = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
   }
   // a block that read no part waits too: what follows in the stream follows this grid's end
-  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  chain_wait();
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
@@ -699,9 +700,7 @@ int launch(const Args& a, cudaStream_t s) {
   static std::atomic<uint64_t> allowed;
   if (!allow_smem(kernel, smem, allowed)) return MRSA_ERR_LAUNCH;
   const unsigned ctas = static_cast<unsigned>(a.undivided ? a.batch * a.kv_heads * a.row_tiles : a.grid);
-  kernel<<<ctas, B_THREADS, smem, s>>>(tq, tk, tv, a);
-  MRSA_CHECK_LAUNCH();
-  return MRSA_OK;
+  return launch_chained(kernel, dim3(ctas), B_THREADS, smem, s, tq, tk, tv, a);
 }
 
 }  // namespace
@@ -729,25 +728,10 @@ int launch_block_join(const Args& a, int dtype, int head_dim, cudaStream_t s) {
   const bool share = a.grid >= 8 * units;         // eight parts and more to a unit
   const int64_t blocks = units * (kBlockRows / 32) * (share ? head_dim / 16 : 1);
   const int64_t most = 8 * static_cast<int64_t>(sm_count());
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(blocks < most ? blocks : most));
-  cfg.blockDim = dim3(256);
-  cfg.stream = s;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
   void (*kernel)(const Args);
   if (head_dim == 128) kernel = dtype == MRSA_F16 ? join_of<128, true>(share) : join_of<128, false>(share);
   else kernel = dtype == MRSA_F16 ? join_of<64, true>(share) : join_of<64, false>(share);
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
-  if (e != cudaSuccess) {
-    note_cuda_error(e, __func__);
-    (void)cudaGetLastError();
-    return MRSA_ERR_LAUNCH;
-  }
-  return MRSA_OK;
+  return launch_chained(kernel, dim3(static_cast<unsigned>(blocks < most ? blocks : most)), 256, 0, s, a);
 }
 
 }  // namespace paged

@@ -143,8 +143,9 @@ __global__ void __launch_bounds__(P_THREADS, 1) page_plan_kernel(
   const int n = a.n, ps = static_cast<int>(a.t.page_size), shift = a.shift;
   const int mp = static_cast<int>(a.t.max_pages), pages = static_cast<int>(a.t.pages);
   const int64_t most = static_cast<int64_t>(mp) * ps;
-  // The copies may be put in place now; they wait for this grid's end.
-  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
+  // The copies (or the next call) may be put in place now; they wait for this grid's end.
+  chain_wait();
+  chain_next();
 
   // ---- the call's sequences, checked by every CTA alike
   if (tid == 0) sm.bad = 0;
@@ -420,7 +421,8 @@ constexpr int M_UNROLL = 4;
 // Whole pages: one unit is M_THREADS * M_UNROLL vectors of one page of one
 // plane, read whole before it is written.
 __global__ void __launch_bounds__(M_THREADS) page_copy_kernel(const __grid_constant__ MoveArgs a) {
-  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  chain_wait();
+  chain_next();
   const int count = a.head != nullptr ? *a.head : a.count;
   const int vecs = static_cast<int>(a.page_bytes / 16);
   const int parts = (vecs + M_THREADS * M_UNROLL - 1) / (M_THREADS * M_UNROLL);
@@ -454,7 +456,8 @@ __global__ void __launch_bounds__(M_THREADS) page_copy_kernel(const __grid_const
 constexpr int M_PLANES = 8;
 
 __global__ void __launch_bounds__(M_THREADS) page_gather_kernel(const __grid_constant__ MoveArgs a) {
-  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  chain_wait();
+  chain_next();
   const int count = *a.head;
   const int ps = 1 << a.shift;
   const int vecs = static_cast<int>(a.page_bytes / 16);
@@ -537,16 +540,19 @@ int launch_plan(const PlanArgs& a, cudaStream_t s) {
   if (kOp != kFree && work < a.t.pages) work = a.t.pages;
   unsigned ctas = 1;
   while (ctas < P_CLUSTER && work > static_cast<int64_t>(ctas) * 4 * P_THREADS) ctas *= 2;
+  if (ctas == 1) return launch_chained(page_plan_kernel<kOp>, dim3(1), P_THREADS, 0, s, a);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(P_THREADS);
   cfg.stream = s;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = ctas;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ctas;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, page_plan_kernel<kOp>, a);
   if (e != cudaSuccess) {
     mrsa::note_cuda_error(e, __func__);
@@ -557,27 +563,12 @@ int launch_plan(const PlanArgs& a, cudaStream_t s) {
 }
 
 template <typename K>
-int launch_move(K kernel, const MoveArgs& a, int64_t most_pages, bool after_plan, cudaStream_t s) {
+int launch_move(K kernel, const MoveArgs& a, int64_t most_pages, cudaStream_t s) {
   // both kernels' units are of at least M_THREADS * M_UNROLL vectors
   int64_t units = (most_pages * a.pool.layers * 2 * (a.page_bytes / 16) + M_THREADS * M_UNROLL - 1) / (M_THREADS * M_UNROLL);
   const int64_t fill = static_cast<int64_t>(sm_count()) * 8;
   if (units > fill) units = fill;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(units < 1 ? 1 : units));
-  cfg.blockDim = dim3(M_THREADS);
-  cfg.stream = s;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = after_plan ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
-  if (e != cudaSuccess) {
-    mrsa::note_cuda_error(e, __func__);
-    (void)cudaGetLastError();
-    return MRSA_ERR_LAUNCH;
-  }
-  return MRSA_OK;
+  return launch_chained(kernel, dim3(static_cast<unsigned>(units < 1 ? 1 : units)), M_THREADS, 0, s, a);
 }
 
 }  // namespace
@@ -640,7 +631,7 @@ extern "C" int mrsa_page_fork(const mrsa_page_table* t, const mrsa_page_pool* po
   m.head = a.ws.head;
   m.dst = a.ws.fresh;
   m.src = a.ws.from;
-  return launch_move(page_copy_kernel, m, most_new(t, n), true, static_cast<cudaStream_t>(stream));
+  return launch_move(page_copy_kernel, m, most_new(t, n), static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int mrsa_page_compact(const mrsa_page_table* t, const mrsa_page_pool* pool, const int32_t* seqs,
@@ -660,7 +651,7 @@ extern "C" int mrsa_page_compact(const mrsa_page_table* t, const mrsa_page_pool*
   m.dst = a.ws.fresh;
   m.src = a.ws.from;
   m.rows = a.ws.rows;
-  return launch_move(page_gather_kernel, m, most_new(t, n), true, static_cast<cudaStream_t>(stream));
+  return launch_move(page_gather_kernel, m, most_new(t, n), static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int mrsa_page_copy(const mrsa_page_table* t, const mrsa_page_pool* pool, const int32_t* src,
@@ -676,5 +667,5 @@ extern "C" int mrsa_page_copy(const mrsa_page_table* t, const mrsa_page_pool* po
   m.count = static_cast<int>(n);
   m.dst = dst;
   m.src = src;
-  return launch_move(page_copy_kernel, m, n, false, static_cast<cudaStream_t>(stream));
+  return launch_move(page_copy_kernel, m, n, static_cast<cudaStream_t>(stream));
 }

@@ -125,6 +125,8 @@ __global__ void __launch_bounds__(R_MAX_THREADS) rotary_kernel(const __grid_cons
   float2* cs = reinterpret_cast<float2*>(smem + (kWide ? R_AHEAD * 2 * threads * 16 : 0));
   const int64_t b = blockIdx.x / a.runs;
   const int l0 = static_cast<int>(blockIdx.x - b * a.runs) * a.run, nt = a.len - l0 < a.run ? a.len - l0 : a.run;
+  chain_wait();
+  chain_next();
   const int vecs = a.head_dim / V;
   const int per = a.interleaved ? kIn : V;
   const int slots = (a.pairs + per - 1) / per, cs_tok = slots * ((per + 1) / 2) * 2;
@@ -277,14 +279,10 @@ int rotary_launch(RotaryArgs& a, int64_t batch, cudaStream_t s) {
     constexpr size_t kMost = R_AHEAD * 2 * R_MAX_THREADS * 16 + R_MAX_RUN * R_MAX_PAIRS * sizeof(float2) * 2;
     static std::atomic<uint64_t> allowed;
     if (!allow_smem(kernel, static_cast<int>(kMost), allowed)) return MRSA_ERR_LAUNCH;
-    kernel<<<g, threads, ring + angles, s>>>(a);
-  } else if (a.interleaved) {
-    rotary_kernel<T, 2, false><<<g, threads, angles, s>>>(a);
-  } else {
-    rotary_kernel<T, 1, false><<<g, threads, angles, s>>>(a);
+    return launch_chained(kernel, g, threads, ring + angles, s, a);
   }
-  MRSA_CHECK_LAUNCH();
-  return MRSA_OK;
+  if (a.interleaved) return launch_chained(rotary_kernel<T, 2, false>, g, threads, angles, s, a);
+  return launch_chained(rotary_kernel<T, 1, false>, g, threads, angles, s, a);
 }
 
 int dispatch(RotaryArgs& a, int64_t batch, int dtype, cudaStream_t s) {
