@@ -461,12 +461,19 @@ int launch_token_rows(const Args& a, cudaStream_t s) {
 
 bool to_tensor_cores(int64_t rows, int64_t group) { return rows > kTokenRows && group <= paged::kBlockGroup; }
 
+// At most one MMA tile of whole tokens: a CTA takes two units of one tile side by side.
+bool to_halves(int64_t rows, int64_t group) { return rows <= paged::kBlockGroup / group * group; }
+
 int row_tile_of(int64_t rows, int64_t group) {
-  return to_tensor_cores(rows, group) ? paged::kBlockRows : (rows <= 8 ? 8 : 16);
+  if (to_tensor_cores(rows, group)) return (to_halves(rows, group) ? 1 : 2) * paged::kBlockGroup;
+  return rows <= 8 ? 8 : 16;
 }
 
-// CTAs that fill the machine: two of the small ones per SM.
-int grid_of(int64_t rows, int64_t group) { return to_tensor_cores(rows, group) ? sm_count() : 2 * sm_count(); }
+// What the tiles are dealt to: CTAs that fill the machine, two of the small ones
+// per SM, or halves of the large ones.
+int grid_of(int64_t rows, int64_t group) {
+  return to_tensor_cores(rows, group) && !to_halves(rows, group) ? sm_count() : 2 * sm_count();
+}
 
 bool sizes_ok(const mrsa_paged_attention_args* p) {
   return p->batch >= 0 && p->len >= 0 && p->kv_heads >= 1 && p->q_heads >= p->kv_heads &&
@@ -562,7 +569,9 @@ extern "C" int mrsa_paged_attention(const mrsa_paged_attention_args* p, const mr
   const bool block = to_tensor_cores(a.rows, a.group);
   a.row_tile = row_tile_of(a.rows, a.group);
   a.group_rows = block ? paged::kBlockGroup / a.group * a.group : a.row_tile;
-  a.row_step = block ? 2 * a.group_rows : a.row_tile;
+  a.split = block && to_halves(a.rows, a.group);
+  a.row_step = block && !a.split ? 2 * a.group_rows : a.row_tile;
+  if (a.split) a.row_step = a.group_rows;
   a.row_tiles = (a.rows + a.row_step - 1) / a.row_step;
   a.tile = A_TILE;          // of both kernels
   // Measured for 0, 2, 4 and 6 (block: 0, 2, 4, 7): one token of 64 sequences of up

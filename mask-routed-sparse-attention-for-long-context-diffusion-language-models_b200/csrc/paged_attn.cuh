@@ -38,10 +38,11 @@ struct Args {
   int row_step, row_tiles;             // query rows of a unit; units that hold a head's rows
   int row_tile;                        // rows of a part in the workspace
   int group_rows;                      // rows per MMA tile of 128 (paged_block.cu)
+  int split;                           // units of one MMA tile, two stretches to a CTA (paged_block.cu)
   FastDiv by_group;
   int tile;                            // keys per tile
   int cut;                             // what a unit costs beside its tiles, in tiles
-  int grid;                            // CTAs that the tiles are dealt to
+  int grid;                            // CTAs (split: halves of CTAs) that the tiles are dealt to
   int undivided;                       // CTA u has the whole of unit u: nothing to deal or to join
   float scale_log2;                    // softmax scale times log2(e)
   float* part_o;                       // [2 * grid][row_tile][D]; paged_block.cu: [2 * grid][D / 4][row_tile][4]
@@ -177,9 +178,10 @@ __device__ __forceinline__ int64_t out_row(const Args& a, const Piece& p, int r)
   return (static_cast<int64_t>(p.b) * a.len + i) * a.q_heads + p.h * a.group + g;
 }
 
-// paged_block.cu: units of two MMA tiles of 128 rows, each of the rows of whole
-// tokens, on a.grid CTAs, one per SM; and the join of their parts.
-constexpr int kBlockRows = 256, kBlockGroup = 128;
+// paged_block.cu: units of MMA tiles of up to 128 rows, those of whole tokens: of
+// two tiles, a CTA's for the same keys, or of one (`split`), a CTA working on two
+// stretches at a time; and the join of their parts.
+constexpr int kBlockGroup = 128;
 int launch_block(const Args& a, int dtype, int head_dim, cudaStream_t s);
 int launch_block_join(const Args& a, int dtype, int head_dim, cudaStream_t s);
 

@@ -5,7 +5,9 @@
 // 7-head group are 224, near the machine's ridge, so the products have to run
 // at tensor-core rate and each K and V tile has to serve all rows that fit.
 // One CTA holds 256 rows of one KV head as two MMA tiles of 128 and walks its
-// stretch of the key tiles (paged_attn.cuh) in tiles of 64:
+// stretch of the key tiles (paged_attn.cuh) in tiles of 64; where a head's rows
+// fit one MMA tile, its two halves work on stretches of their own (kSplit; 112
+// rows over 131072 tokens 67 us with one half idle, 62 so):
 //   S[128 x 64]  = Q . K_t^T              (UMMA M=128, N=64,  TMEM)
 //   P            = exp2(S scale log2e - m)  (one thread per row, lazy maximum)
 //   O[128 x D]  += P . V_t                (UMMA M=128, N=D, A = P in TMEM)
@@ -81,7 +83,7 @@ struct TilePages {
   }
 };
 
-template <int kD, bool kF16, bool kCausal>
+template <int kD, bool kF16, bool kCausal, bool kSplit>
 __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_constant__ CUtensorMap tm_q,
                                                                    const __grid_constant__ CUtensorMap tm_k,
                                                                    const __grid_constant__ CUtensorMap tm_v,
@@ -89,17 +91,25 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   auto& sm = *reinterpret_cast<BlockSmem<kD>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   constexpr int kHalves = kD / 64, kQHalf = B_ROWS * 128, kKHalf = B_TILE * 128, kStage = kHalves * kKHalf;
+  // Stage, its phase, mask slot and phase of tile e of a stretch: shared by both
+  // halves of the CTA, or (kSplit) half of them each
+  auto stage_of = [](int g, int e) { return kSplit ? 2 * g + (e & 1) : e % NKS; };
+  auto phase_of = [](int e) { return static_cast<uint32_t>(kSplit ? (e >> 1) & 1 : (e / NKS) & 1); };
+  auto slot_of = [](int g, int e) { return kSplit ? 4 * g + (e & 3) : e % NMS; };
+  auto slot_phase = [](int e) { return static_cast<uint32_t>(kSplit ? (e >> 2) & 1 : (e / NMS) & 1); };
+  constexpr int kStages = kSplit ? NKS / 2 : NKS;      // of one stretch
+  static_assert(NKS == 4 && NVS == 4 && NMS == 8, "stage_of and the others");
   volatile int* abort_flag = &sm.abort_flag;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (tid == 32) {
     for (int s = 0; s < NKS; ++s) {
       tc::mbar_init(tc::smem_addr(&sm.kfull[s]), 1);
-      tc::mbar_init(tc::smem_addr(&sm.kfree[s]), 2);
+      tc::mbar_init(tc::smem_addr(&sm.kfree[s]), kSplit ? 1 : 2);
     }
     for (int s = 0; s < NVS; ++s) {
       tc::mbar_init(tc::smem_addr(&sm.vfull[s]), 1);
-      tc::mbar_init(tc::smem_addr(&sm.vfree[s]), 2);
+      tc::mbar_init(tc::smem_addr(&sm.vfree[s]), kSplit ? 1 : 2);
       tc::mbar_init(tc::smem_addr(&sm.vclean[s]), 1);
     }
     for (int s = 0; s < NMS; ++s) tc::mbar_init(tc::smem_addr(&sm.mfull[s]), 1);
@@ -121,10 +131,13 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
     tc::tmem_alloc(tc::smem_addr(&sm.tmem_base), 512);
     tc::tmem_relinquish();
   }
-  const int cta = static_cast<int>(blockIdx.x);
+  // the half of the CTA that this warp works for (the loaders of a shared stretch: either)
+  const int g = warp < 8 ? warp >> 2 : (warp == W_MMA + 1 || warp == W_V ? 1 : 0);
+  const int worker = kSplit ? 2 * static_cast<int>(blockIdx.x) + g : static_cast<int>(blockIdx.x);
+  const int units_all = a.batch * a.kv_heads * a.row_tiles;
   Piece unit = {};
-  if (a.undivided) unit = paged::unit_at(a, cta);
-  else paged::count_tiles<B_THREADS>(a, sm.batch, sm.warp_sums);
+  if (!a.undivided) paged::count_tiles<B_THREADS>(a, sm.batch, sm.warp_sums);
+  else if (worker < units_all) unit = paged::unit_at(a, worker);
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
@@ -132,40 +145,60 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
   int t_begin = 0, t_end = unit.tiles;
   if (!a.undivided) {
     const paged::Deal deal(a, sm.batch.prefix[a.batch] * a.kv_heads * a.row_tiles);
-    t_begin = cta < deal.ctas ? deal.begin(cta) : 0;
-    t_end = cta < deal.ctas ? deal.begin(cta + 1) : 0;
-  } else if (unit.tiles == 0) {
+    t_begin = worker < deal.ctas ? deal.begin(worker) : 0;
+    t_end = worker < deal.ctas ? deal.begin(worker + 1) : 0;
+  } else if (unit.tiles == 0 && worker < units_all && warp < 8) {
     // no keys: zeros, and -inf
-    for (int i = tid; i < unit.nrows * (kD / 8); i += B_THREADS)
+    const int from = kSplit ? tid & 127 : tid, step = kSplit ? 128 : 256;
+    for (int i = from; i < unit.nrows * (kD / 8); i += step)
       *reinterpret_cast<uint4*>(a.out + paged::out_row(a, unit, i / (kD / 8)) * kD * 2 + (i % (kD / 8)) * 16) =
           make_uint4(0u, 0u, 0u, 0u);
     if (a.lse != nullptr)
-      for (int i = tid; i < unit.nrows; i += B_THREADS) a.lse[paged::out_row(a, unit, i)] = -INFINITY;
+      for (int i = from; i < unit.nrows; i += step) a.lse[paged::out_row(a, unit, i)] = -INFINITY;
   }
   auto part_at = [&](int t) { return a.undivided ? unit : paged::piece_at(a, sm.batch, t, t_end); };
   bool ok = true;
 
   if (warp == W_K || warp == W_V) {
     // ============================ K tiles and key masks; V tiles =============
-    const bool is_k = warp == W_K;
-    const CUtensorMap* map = is_k ? &tm_k : &tm_v;
-    uint64_t* full = is_k ? sm.kfull : sm.vfull;
-    uint64_t* freed = is_k ? sm.kfree : sm.vfree;
-    unsigned char* ring = is_k ? sm.k[0][0] : sm.v[0][0];
-    static_assert(NKS == NVS, "K and V stages share their index");
-    if (lane == 0) tc::prefetch_tensormap(map);
+    // A shared stretch: the K warp and the V warp.  Split: one warp per half, which
+    // copies K a tile ahead of V.
+    const bool do_k = kSplit || warp == W_K, do_v = kSplit || warp == W_V;
+    if (lane == 0) {
+      if (do_k) tc::prefetch_tensormap(&tm_k);
+      if (do_v) tc::prefetch_tensormap(&tm_v);
+    }
     const TilePages tp(a);
+    int copied_k = 0, copied_v = 0;              // tiles whose copies were issued
+    // tile e's copies into its stage; the pages of its parts are known
+    auto copy_tile = [&](const CUtensorMap* map, unsigned char* ring, uint64_t* full, uint64_t* freed, const Piece& p, int t,
+                         int e, int page, unsigned has, int& copied) -> bool {
+      const int st = stage_of(g, e);
+      if (e >= kStages && !tc::wait_bounded_warp(tc::smem_addr(&freed[st]), phase_of(e - kStages), abort_flag)) return false;
+      const uint32_t bar = tc::smem_addr(&full[st]);
+      if (lane == 0) tc::mbar_arrive_expect_tx(bar, __popc(has) * tp.part_keys * kD * 2);
+      __syncwarp();
+      if (page >= 0) {
+        const int slot = (t * B_TILE + lane * tp.part_keys) & (a.page_size - 1);
+#pragma unroll
+        for (int hf = 0; hf < kHalves; ++hf)
+          tc::tma_load_5d(tc::smem_addr(ring + st * kStage + hf * kKHalf + lane * tp.part_keys * 128), map, 0, slot, hf,
+                          p.h, page, bar);
+      }
+      __syncwarp();
+      copied = e + 1;
+      return true;
+    };
     // V rows of keys that do not count, zeroed (a P of zero does not cancel what
     // is not a number); the MMA warps wait for it where a tile has such keys.
     // The V warp does it one tile behind its copies (masked, 37 x 32 tokens over
     // 16384: 418 us; two behind 417; in the K warp 421 and up).
-    constexpr int kLag = 1;
-    auto clean = [&](int tile) -> bool {
-      if (!tc::wait_bounded_warp(tc::smem_addr(&sm.mfull[tile % NMS]), (tile / NMS) & 1, abort_flag)) return false;
-      const unsigned long long km = sm.kmask[tile % NMS];
-      const int st = tile % NVS;
+    auto clean = [&](int e) -> bool {
+      const int sl = slot_of(g, e), st = stage_of(g, e);
+      if (!tc::wait_bounded_warp(tc::smem_addr(&sm.mfull[sl]), slot_phase(e), abort_flag)) return false;
+      const unsigned long long km = sm.kmask[sl];
       if (km != ~0ull) {
-        if (!tc::wait_bounded_warp(tc::smem_addr(&sm.vfull[st]), (tile / NVS) & 1, abort_flag)) return false;
+        if (!tc::wait_bounded_warp(tc::smem_addr(&sm.vfull[st]), phase_of(e), abort_flag)) return false;
         constexpr int kPer = 32 / (kD / 8);      // rows per step
         const int j = lane % (kD / 8);
 #pragma unroll 4
@@ -179,9 +212,18 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
       return true;
     };
     int e = 0;                                   // tiles of the stretch so far
+    // split: the V copy of the tile before, which follows this tile's K
+    Piece v_piece = {};
+    int v_tile = 0, v_page = -1;
+    unsigned v_has = 0;
+    auto copy_v = [&]() -> bool {                // of tile e - 1, then the tile before it cleaned
+      return copy_tile(&tm_v, sm.v[0][0], sm.vfull, sm.vfree, v_piece, v_tile, e - 1, v_page, v_has,
+                       copied_v) &&
+             (e < 2 || clean(e - 2));
+    };
     for (int t_now = t_begin; ok && t_now < t_end;) {
       const Piece p = part_at(t_now);
-      const uint8_t* valid = a.valid != nullptr && is_k
+      const uint8_t* valid = a.valid != nullptr && do_k
                                  ? a.valid + static_cast<int64_t>(p.b) * a.max_pages * a.page_size : nullptr;
       // the next tile's page numbers and mask bytes are requested a tile ahead
       auto valid_bytes = [&](int tile, uint32_t (&vb)[2]) {
@@ -195,53 +237,55 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
       uint32_t vb_next[2];
       valid_bytes(p.tile0, vb_next);
       for (int t = p.tile0; t < p.tile1; ++t, ++e) {
-        const int st = e % NKS;
         const int page = page_next;
         const uint32_t vb[2] = {vb_next[0], vb_next[1]};
         page_next = tp.look_up(a, p, t + 1, lane);
         valid_bytes(t + 1, vb_next);
-        // the stage was released by both groups for tile e - NKS; the mask slot
-        // was last read by the softmax of tile e - NMS, before that release
-        if (e >= NKS && !(ok = tc::wait_bounded_warp(tc::smem_addr(&freed[st]), ((e / NKS) - 1) & 1, abort_flag))) break;
         const unsigned has = __ballot_sync(0xffffffffu, page >= 0);
-        if (is_k) {
+        if (do_k) {
+          // the mask slot was last read by the softmax and the P.V of the tile that had it
+          // before, which come before the release of this tile's K stage
+          const int st = stage_of(g, e);
+          if (e >= kStages && !(ok = tc::wait_bounded_warp(tc::smem_addr(&sm.kfree[st]), phase_of(e - kStages), abort_flag)))
+            break;
           uint32_t mk[2];
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const int in = 32 * i + lane, key = t * B_TILE + in;
             mk[i] = __ballot_sync(0xffffffffu, key < p.n && vb[i] != 0u && ((has >> (in / tp.part_keys)) & 1u));
           }
-          __syncwarp();
           if (lane == 0) {
-            sm.kmask[e % NMS] = static_cast<unsigned long long>(mk[0]) | (static_cast<unsigned long long>(mk[1]) << 32);
-            tc::mbar_arrive(tc::smem_addr(&sm.mfull[e % NMS]));
+            const int sl = slot_of(g, e);
+            sm.kmask[sl] = static_cast<unsigned long long>(mk[0]) | (static_cast<unsigned long long>(mk[1]) << 32);
+            tc::mbar_arrive(tc::smem_addr(&sm.mfull[sl]));
           }
+          if (!(ok = copy_tile(&tm_k, sm.k[0][0], sm.kfull, sm.kfree, p, t, e, page, has, copied_k))) break;
         }
-        const uint32_t bar = tc::smem_addr(&full[st]);
-        if (lane == 0) tc::mbar_arrive_expect_tx(bar, __popc(has) * tp.part_keys * kD * 2);
-        __syncwarp();
-        if (page >= 0) {
-          const int slot = (t * B_TILE + lane * tp.part_keys) & (a.page_size - 1);
-#pragma unroll
-          for (int hf = 0; hf < kHalves; ++hf)
-            tc::tma_load_5d(tc::smem_addr(ring + st * kStage + hf * kKHalf + lane * tp.part_keys * 128), map, 0, slot, hf,
-                            p.h, page, bar);
+        if (kSplit) {
+          if (e > 0 && !(ok = copy_v())) break;
+          v_piece = p;
+          v_tile = t;
+          v_page = page;
+          v_has = has;
+        } else if (do_v) {
+          ok = copy_tile(&tm_v, sm.v[0][0], sm.vfull, sm.vfree, p, t, e, page, has, copied_v) && (e == 0 || clean(e - 1));
+          if (!ok) break;
         }
-        __syncwarp();
-        if (!is_k && e >= kLag && !(ok = clean(e - kLag))) break;
       }
       t_now += p.span;
     }
-    if (!is_k)
-      for (int tt = e < kLag ? 0 : e - kLag; ok && tt < e; ++tt) ok = clean(tt);
+    if (kSplit && ok && e > 0) ok = copy_v();
+    if (do_v && ok && e > 0) ok = clean(e - 1);
     // wait (bounded, even after an abort) for the copies in flight
-    if (lane == 0)
-      for (int tt = e - NKS < 0 ? 0 : e - NKS; tt < e; ++tt)
-        tc::mbar_wait(tc::smem_addr(&full[tt % NKS]), (tt / NKS) & 1);
+    if (lane == 0) {
+      for (int tt = copied_k > kStages ? copied_k - kStages : 0; tt < copied_k; ++tt)
+        tc::mbar_wait(tc::smem_addr(&sm.kfull[stage_of(g, tt)]), phase_of(tt));
+      for (int tt = copied_v > kStages ? copied_v - kStages : 0; tt < copied_v; ++tt)
+        tc::mbar_wait(tc::smem_addr(&sm.vfull[stage_of(g, tt)]), phase_of(tt));
+    }
     __syncwarp();
   } else if (warp >= W_MMA) {
     // ============================ MMA issue (one warp per row tile) ==========
-    const int g = warp - W_MMA;
     // kind::f16: the bf16 format bits cleared for fp16 operands
     constexpr uint32_t kType = kF16 ? ~((1u << 7) | (1u << 10)) : ~0u;
     constexpr uint32_t id_s = tc::idesc_bf16_f32(128, B_TILE, 0, 0) & kType;
@@ -249,13 +293,14 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
     const uint64_t dq = tc::smem_desc_sw128(tc::smem_addr(sm.q[g][0]), 16, 1024);
     const uint64_t dk0 = tc::smem_desc_sw128(tc::smem_addr(sm.k[0][0]), 16, 1024);
     const uint64_t dv0 = tc::smem_desc_sw128(tc::smem_addr(sm.v[0][0]), kKHalf, 1024);
+    const int row0 = kSplit ? 0 : g * a.group_rows;
     int e = 0, k = 0, units = 0;                  // tiles of the stretch, tiles and units of this group, so far
     // S of the stretch's tile ee, the group's tile kk, into buffer 2g + (kk & 1),
     // once the P that was there has been read
     auto issue_s = [&](int ee, int kk) -> bool {
-      const int sb = 2 * g + (kk & 1), st = ee % NKS;
+      const int sb = 2 * g + (kk & 1), st = stage_of(g, ee);
       if (kk >= 2 && !tc::wait_bounded_warp(tc::smem_addr(&sm.pfree[sb]), ((kk - 2) >> 1) & 1, abort_flag)) return false;
-      if (!tc::wait_bounded_warp(tc::smem_addr(&sm.kfull[st]), (ee / NKS) & 1, abort_flag)) return false;
+      if (!tc::wait_bounded_warp(tc::smem_addr(&sm.kfull[st]), phase_of(ee), abort_flag)) return false;
       tc::fence_after_sync();
       const uint64_t db = tc::desc_adv(dk0, st * kStage);
       const uint32_t dS = tbase + B_TILE * sb;
@@ -276,7 +321,7 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
       const int nt = p.tile1 > p.tile0 ? p.tile1 - p.tile0 : 0;
       if (nt == 0) {
         // the stretch ends before the unit's first tile
-      } else if (p.nrows <= g * a.group_rows) {
+      } else if (!kSplit && p.nrows <= g * a.group_rows) {
         // no rows for this group: the unit's stages released unused, in order
         for (int i = 0; ok && i < nt; ++i, ++e) {
           ok = tc::wait_bounded_warp(tc::smem_addr(&sm.kfull[e % NKS]), (e / NKS) & 1, abort_flag) &&
@@ -296,7 +341,7 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
 #pragma unroll
           for (int hf = 0; hf < kHalves; ++hf)
             tc::tma_load_5d(tc::smem_addr(sm.q[g][hf]), &tm_q, 0, hf, p.h * a.group,
-                            a.by_group.div(p.r0 + g * a.group_rows), p.b, qb);
+                            a.by_group.div(p.r0 + row0), p.b, qb);
         }
         __syncwarp();
         ok = tc::wait_bounded_warp(qb, units & 1, abort_flag);
@@ -304,11 +349,11 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
         if (ok) ok = issue_s(e, k);
         if (ok && nt > 1) ok = issue_s(e + 1, k + 1);
         for (int i = 0; ok && i < nt; ++i, ++e, ++k) {
-          const int sb = 2 * g + (k & 1), sv = e % NVS;
+          const int sb = 2 * g + (k & 1), sv = stage_of(g, e);
           if (!(ok = tc::wait_bounded_warp(tc::smem_addr(&sm.pready[sb]), (k >> 1) & 1, abort_flag))) break;
           // (the softmax has read the mask, and its slot is not reused before this P.V)
-          uint64_t* vbar = sm.kmask[e % NMS] == ~0ull ? &sm.vfull[sv] : &sm.vclean[sv];
-          if (!(ok = tc::wait_bounded_warp(tc::smem_addr(vbar), (e / NVS) & 1, abort_flag))) break;
+          uint64_t* vbar = sm.kmask[slot_of(g, e)] == ~0ull ? &sm.vfull[sv] : &sm.vclean[sv];
+          if (!(ok = tc::wait_bounded_warp(tc::smem_addr(vbar), phase_of(e), abort_flag))) break;
           tc::fence_after_sync();
           const uint64_t dv = tc::desc_adv(dv0, sv * kStage);
           const uint32_t dO = tbase + kOCol + 128 * g, aP = tbase + B_TILE * sb;
@@ -335,16 +380,17 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
     __syncwarp();
   } else {
     // ============================ softmax and epilogue (warps 0-7) ===========
-    const int g = warp >> 2, r = (warp & 3) * 32 + lane;      // row tile; row = TMEM lane
+    const int r = (warp & 3) * 32 + lane;                    // row = TMEM lane
+    const int row0 = kSplit ? 0 : g * a.group_rows;          // of this half, in the unit
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t t_o = tbase + lane_off + kOCol + 128 * g;
     int e0 = 0, k = 0;            // tiles of the stretch before this unit; tiles of this group so far
     for (int t_now = t_begin; ok && t_now < t_end;) {
       const Piece p = part_at(t_now);
       const int nt = p.tile1 > p.tile0 ? p.tile1 - p.tile0 : 0;
-      const int rows_here = p.nrows - g * a.group_rows;        // of this row tile, where positive
+      const int rows_here = p.nrows - row0;                    // of this row tile, where positive
       if (nt > 0 && rows_here > 0) {
-        const int row = g * a.group_rows + r;
+        const int row = row0 + r;
         const bool row_ok = r < a.group_rows && r < rows_here;
         // causal: the last key this row may see
         const int last = p.n - a.len + a.by_group.div(p.r0 + (row_ok ? row : 0));
@@ -359,8 +405,8 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
 #pragma unroll
           for (int c = 0; c < 64; c += 16) tc::tmem_ld16(t_s + c, *reinterpret_cast<uint32_t(*)[16]>(&x[c]));
           tc::tmem_wait_ld();
-          if (!(ok = tc::wait_bounded_warp(tc::smem_addr(&sm.mfull[e % NMS]), (e / NMS) & 1, abort_flag))) break;
-          const unsigned long long km = sm.kmask[e % NMS];
+          if (!(ok = tc::wait_bounded_warp(tc::smem_addr(&sm.mfull[slot_of(g, e)]), slot_phase(e), abort_flag))) break;
+          const unsigned long long km = sm.kmask[slot_of(g, e)];
           if (km != ~0ull) {
             // (a minimum with +-inf from shared memory in place of the choice: 415 us for
             // 377 at 37 x 32 tokens over 16384, masked)
@@ -481,7 +527,7 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
 #pragma unroll
             for (int i = lane / 4; i < 32; i += 8)
               if (i < nrow)
-                *reinterpret_cast<uint4*>(a.out + paged::out_row(a, p, g * a.group_rows + (warp & 3) * 32 + i) * kD * 2 +
+                *reinterpret_cast<uint4*>(a.out + paged::out_row(a, p, row0 + (warp & 3) * 32 + i) * kD * 2 +
                                           cc * 2 + (lane % 4) * 16) = stage[i * 4 + ((lane ^ i) & 3)];
             __syncwarp();
           }
@@ -489,8 +535,9 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
             a.lse[paged::out_row(a, p, row)] = l_run > 0.f ? (m_run + log2f(l_run)) * kLn2 : -INFINITY;
         } else {
           // four columns of all rows side by side: the warp's stores are whole lines
-          const int64_t slot = 2 * blockIdx.x + (t_now == t_begin ? 0 : 1);
-          float* dst = a.part_o + (slot * (kD / 4) * a.row_tile + g * B_ROWS + r) * 4;
+          const int64_t slot = 2 * worker + (t_now == t_begin ? 0 : 1);
+          const int prow = (kSplit ? 0 : g * B_ROWS) + r;
+          float* dst = a.part_o + (slot * (kD / 4) * a.row_tile + prow) * 4;
 #pragma unroll 1
           for (int cc = 0; cc < kD; cc += 32) {
             uint32_t o[32];
@@ -506,7 +553,7 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
             __syncwarp();
           }
           if (row_ok)
-            *reinterpret_cast<float2*>(a.part_ml + (slot * a.row_tile + g * B_ROWS + r) * 2) = make_float2(m_run, l_run);
+            *reinterpret_cast<float2*>(a.part_ml + (slot * a.row_tile + prow) * 2) = make_float2(m_run, l_run);
         }
         tc::fence_before_sync();       // O was read before the next unit's first P is announced
         __syncwarp();
@@ -534,7 +581,6 @@ template <int kD, bool kF16, bool kShare>
 __global__ void __launch_bounds__(256) paged_block_join_kernel(const __grid_constant__ Args a) {
   constexpr int kCols = kShare ? 4 : kD / 32;  // columns of four per warp
   constexpr int kSets = kShare ? kD / 16 : 1;  // blocks that share 32 rows
-  constexpr int kBlocks = paged::kBlockRows / 32 * kSets;
   __shared__ float4 acc_s[kShare ? 8 : 1][kCols][32];
   __shared__ float2 ml_s[kShare ? 8 : 1][32];
   __shared__ paged::Batch batch;
@@ -543,11 +589,12 @@ __global__ void __launch_bounds__(256) paged_block_join_kernel(const __grid_cons
   paged::count_tiles<256>(a, batch, warp_sums);
   const int per = a.kv_heads * a.row_tiles;            // units per batch row
   const paged::Deal deal(a, batch.prefix[a.batch] * per);
-  const int64_t work = static_cast<int64_t>(a.batch) * per * kBlocks;
+  const int blocks = a.row_tile / 32 * kSets;
+  const int64_t work = static_cast<int64_t>(a.batch) * per * blocks;
   bool waited = false;
   for (int64_t w = blockIdx.x; w < work; w += gridDim.x) {
-    const int part = static_cast<int>(w % kBlocks), rb = part / kSets, set = part % kSets;
-    const int u = static_cast<int>(w / kBlocks), b = u / per, unit = u - b * per;
+    const int part = static_cast<int>(w % blocks), rb = part / kSets, set = part % kSets;
+    const int u = static_cast<int>(w / blocks), b = u / per, unit = u - b * per;
     auto column = [&](int j) { return kShare ? set * kCols + j : warp + 8 * j; };
     Piece p;
     p.b = b;
@@ -683,7 +730,7 @@ bool q_map(CUtensorMap* m, const Args& a, int head_dim, bool f16) {
   return make_map(m, a.q, dims, strides, box, f16);
 }
 
-template <int kD, bool kF16, bool kCausal>
+template <int kD, bool kF16, bool kCausal, bool kSplit>
 int launch(const Args& a, cudaStream_t s) {
   CUtensorMap tq, tk, tv;
   if (!q_map(&tq, a, kD, kF16) || !page_map(&tk, a.k, a.kp, a.ks, a.kh, a, kD, kF16) || !page_map(&tv, a.v, a.vp, a.vs, a.vh, a, kD, kF16)) {
@@ -691,10 +738,11 @@ int launch(const Args& a, cudaStream_t s) {
     return MRSA_ERR_LAUNCH;
   }
   const int smem = static_cast<int>(sizeof(BlockSmem<kD>) + 1024);
-  const auto kernel = paged_block_kernel<kD, kF16, kCausal>;
+  const auto kernel = paged_block_kernel<kD, kF16, kCausal, kSplit>;
   static std::atomic<uint64_t> allowed;
   if (!allow_smem(kernel, smem, allowed)) return MRSA_ERR_LAUNCH;
-  const unsigned ctas = static_cast<unsigned>(a.undivided ? a.batch * a.kv_heads * a.row_tiles : a.grid);
+  const unsigned workers = static_cast<unsigned>(a.undivided ? a.batch * a.kv_heads * a.row_tiles : a.grid);
+  const unsigned ctas = kSplit ? (workers + 1) / 2 : workers;
   return launch_chained(kernel, dim3(ctas), B_THREADS, smem, s, tq, tk, tv, a);
 }
 
@@ -705,7 +753,8 @@ namespace paged {
 
 template <int kD, bool kF16>
 int launch_causal(const Args& a, cudaStream_t s) {
-  return a.causal ? launch<kD, kF16, true>(a, s) : launch<kD, kF16, false>(a, s);
+  if (a.split) return a.causal ? launch<kD, kF16, true, true>(a, s) : launch<kD, kF16, false, true>(a, s);
+  return a.causal ? launch<kD, kF16, true, false>(a, s) : launch<kD, kF16, false, false>(a, s);
 }
 
 int launch_block(const Args& a, int dtype, int head_dim, cudaStream_t s) {
@@ -721,7 +770,7 @@ void (*join_of(bool share))(const Args) {
 int launch_block_join(const Args& a, int dtype, int head_dim, cudaStream_t s) {
   const int64_t units = static_cast<int64_t>(a.batch) * a.kv_heads * a.row_tiles;
   const bool share = a.grid >= 8 * units;         // eight parts and more to a unit
-  const int64_t blocks = units * (kBlockRows / 32) * (share ? head_dim / 16 : 1);
+  const int64_t blocks = units * (a.row_tile / 32) * (share ? head_dim / 16 : 1);
   const int64_t most = 8 * static_cast<int64_t>(sm_count());
   void (*kernel)(const Args);
   if (head_dim == 128) kernel = dtype == MRSA_F16 ? join_of<128, true>(share) : join_of<128, false>(share);
