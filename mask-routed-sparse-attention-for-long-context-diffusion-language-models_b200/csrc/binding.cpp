@@ -120,11 +120,9 @@ void set_k(mrsa_rotary_args& a, const Tensor& k) {
 // (q', k') of checked arguments; k may be undefined.
 std::pair<Tensor, Tensor> rotate(Tensor q, Tensor k, Tensor pos, Tensor inv, double factor, bool interleaved, bool inverse) {
   mrsa_rotary_args a = {};
-  check_heads(q, "q");
   a.dtype = type_of(q);
   TORCH_CHECK_VALUE(a.dtype >= 0, "q must be BF16, FP16 or FP32, got ", q.scalar_type());
   if (k.defined()) check_like(k, "k", q);
-  TORCH_CHECK_VALUE(pos.defined() && inv.defined(), "position_ids must be int64 (B, L) and inv_freq fp32 [n]");
   a.pairs = check_rotation(inv, pos, q);
   TORCH_CHECK_VALUE(!interleaved || q.size(3) % 2 == 0, "the interleaved layout needs an even head dim");
   q = inner_contiguous(q);
@@ -154,14 +152,14 @@ std::pair<Tensor, Tensor> rotate(Tensor q, Tensor k, Tensor pos, Tensor inv, dou
 // The gradient of a rotation is the rotation by minus the angle.
 struct Rotary : torch::autograd::Function<Rotary> {
   using List = torch::autograd::variable_list;
-  static List forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& pos,
-                      const Tensor& inv, double factor, bool interleaved) {
+  static List forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const std::optional<Tensor>& k,
+                      const Tensor& pos, const Tensor& inv, double factor, bool interleaved) {
     ctx->save_for_backward({pos, inv});
     ctx->saved_data["factor"] = factor;
     ctx->saved_data["interleaved"] = interleaved;
-    ctx->saved_data["pair"] = k.defined();
-    auto [qo, ko] = rotate(q, k, pos, inv, factor, interleaved, false);
-    return k.defined() ? List{qo, ko} : List{qo};
+    ctx->saved_data["pair"] = k.has_value();
+    auto [qo, ko] = rotate(q, k ? *k : Tensor(), pos, inv, factor, interleaved, false);
+    return k ? List{qo, ko} : List{qo};
   }
   static List backward(torch::autograd::AutogradContext* ctx, const List& g) {
     TORCH_CHECK_NOT_IMPLEMENTED(!c10::GradMode::is_enabled(), "rotary_embedding: the gradient of its gradient is not recorded");
@@ -181,9 +179,12 @@ PyObject* rotary(PyObject*, PyObject* const* o, Py_ssize_t n) {
   const double factor = PyFloat_AsDouble(o[4]);
   if (PyErr_Occurred()) return nullptr;
   const bool interleaved = layout_of(o[5]) == 1;
+  check_heads(q, "q");
+  TORCH_CHECK_VALUE(pos.defined() && inv.defined(), "position_ids must be int64 (B, L) and inv_freq fp32 [n]");
   Tensor qo, ko;
-  if (c10::GradMode::is_enabled() && ((q.defined() && q.requires_grad()) || (k.defined() && k.requires_grad()))) {
-    auto r = Rotary::apply(q, k, pos, inv, factor, interleaved);
+  if (c10::GradMode::is_enabled() && (q.requires_grad() || (k.defined() && k.requires_grad()))) {
+    const std::optional<Tensor> pair = k.defined() ? std::optional<Tensor>(k) : std::nullopt;
+    auto r = Rotary::apply(q, pair, pos, inv, factor, interleaved);
     qo = std::move(r[0]);
     if (r.size() > 1) ko = std::move(r[1]);
   } else {

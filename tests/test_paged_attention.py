@@ -251,3 +251,59 @@ def test_argument_codes(mrsa):
     assert rc() == L.ERR_WORKSPACE and rc(b=0) == 0 and rc(l=0) == 0
     bad = L.PAGE_TABLE.pack(P, P, 0, 0, 4, 8, 100, 48)
     assert lib.mrsa_paged_attention(args(), bad, None, 0, None) == L.ERR_SHAPE
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("l,hq,hkv,d", [(1, 130, 1, 64), (2, 129, 1, 128), (1, 96, 1, 128), (1, 128, 1, 64), (64, 2, 1, 64),
+                                        (128, 1, 1, 128), (129, 1, 1, 128), (43, 6, 2, 64)])
+def test_groups_and_rows_at_the_tiles_edges(mrsa, cuda_device, l, hq, hkv, d):
+    """Rows that fill an MMA tile, or miss it by one; more heads to a KV head than it has rows."""
+    cache, g = filled(mrsa, cuda_device, [200, 0, 1, 3000, 130], hkv, d, 64, torch.bfloat16, seed=l + hq)
+    seqs = torch.tensor([4, 3, 2, 1, 0], dtype=torch.int32, device=cuda_device)
+    q = queries(cuda_device, g, 5, l, hq, d, torch.bfloat16)
+    compare(mrsa, cache, seqs, q)
+    compare(mrsa, cache, seqs, q, causal=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("l", [1, 32])
+def test_strides(mrsa, cuda_device, l):
+    """Every second head of the pages, a broadcast query, odd alignment, heads outside."""
+    dev = cuda_device
+    cache, g = filled(mrsa, dev, [150, 77], 4, 128, 32, torch.bfloat16)
+    whole = cache.pool
+    cache.pool = whole[:, :, :, :, ::2]
+    seqs = cache.seqs(1, 0)
+    compare(mrsa, cache, seqs, queries(dev, g, 1, l, 14, 128, torch.bfloat16).expand(2, l, 14, 128))
+    flat = torch.randn(2 * l * 14 * 128 + 3, device=dev, generator=g).bfloat16()
+    compare(mrsa, cache, seqs, flat[3:].view(2, l, 14, 128))
+    compare(mrsa, cache, seqs, torch.randn(2, 14, l, 128, device=dev, generator=g).bfloat16().transpose(1, 2))
+    with pytest.raises(ValueError, match="aligned"):
+        cache.pool = torch.empty(2 * 9 * 32 * 2 * 128 + 1, device=dev, dtype=torch.bfloat16)[1:].view(1, 2, 9, 32, 2, 128)
+        cache.attend(0, seqs, torch.zeros(2, l, 14, 128, device=dev, dtype=torch.bfloat16))
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits(mrsa, cuda_device):
+    """A pool of 4.7 GB a plane: the last pages and the first hold one sequence's tokens."""
+    dev = cuda_device
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GB")
+    g = torch.Generator(device=dev).manual_seed(1)
+    pages = 36000
+    cache = mrsa.PagedKVCache(1, pages, 8, 128, sequences=3, max_len=640, device=dev)
+    assert cache.pool[0, 0].numel() * 2 > 1 << 32
+    cache.refcount.fill_(1)                                   # only the ends are free
+    cache.refcount[[3, 35990, 35999, 35991, 0, 35995, 35996, 35997, 5, 35998]] = 0
+    cache.extend(cache.seqs(0), 300)
+    assert cache.table[0, :5].tolist() == [0, 3, 5, 35990, 35991]
+    k, v = torch.randn(2, 1, 300, 8, 128, device=dev, generator=g).bfloat16()
+    cache.append(0, cache.seqs(0), k, v)
+    cache.fork(cache.seqs(0), cache.seqs(1))
+    keep = torch.ones(1, 640, dtype=torch.bool, device=dev)
+    keep[0, 70:75] = False
+    cache.compact(cache.seqs(1), keep)
+    cache.check()
+    assert cache.table[1, :5].tolist() == [0, 35996, 35997, 35998, 35999]
+    for l, hq in ((1, 8), (32, 56)):
+        compare(mrsa, cache, cache.seqs(1, 0), queries(dev, g, 2, l, hq, 128, torch.bfloat16))

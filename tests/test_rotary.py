@@ -201,3 +201,24 @@ def test_rotary_argument_codes(mrsa):
     with pytest.raises(ValueError, match="CUDA"):
         mrsa.rotary_embedding(q, None, torch.zeros(1, 4, dtype=torch.long), torch.ones(32))
     assert C.sizeof(C.c_void_p) == 8 and L.ROTARY_ARGS.size == 160
+
+
+@pytest.mark.gpu
+def test_rotary_gradient_of_one_tensor(mrsa, cuda_device):
+    dev = cuda_device
+    pos = positions(1, 7, dev)
+    inv, _ = mrsa.rotary_inv_freq(64, device=dev)
+    q = torch.randn(1, 7, 3, 64, device=dev, requires_grad=True)
+    k = torch.randn(1, 7, 1, 64, device=dev)
+    g = torch.randn(1, 7, 3, 64, device=dev)
+    y, none = mrsa.rotary_embedding(q, None, pos, inv)
+    assert none is None
+    check(torch.autograd.grad(y, q, g)[0], g, pos, inv, 1.0, "half", -1.0)
+    y, yk = mrsa.rotary_embedding(q.detach(), k.requires_grad_(), pos, inv)
+    gk = torch.randn_like(yk)
+    check(torch.autograd.grad(yk, k, gk)[0], gk, pos, inv, 1.0, "half", -1.0)
+    with torch.no_grad():
+        assert not mrsa.rotary_embedding(q, None, pos, inv)[0].requires_grad
+    y, _ = mrsa.rotary_embedding(q, None, pos, inv)
+    with pytest.raises(NotImplementedError):
+        torch.autograd.grad(y, q, g, create_graph=True)
