@@ -2,8 +2,8 @@
 // output tensors and workspace, and the C entry points of mrsa.h.
 //
 // A decode step is a chain of launches of a few microseconds each.  Checked and
-// packed in Python, one such call took 11 to 15 us of host time, four times
-// its kernels; here it is three to five.  One function per operator, with
+// packed in Python, one such call took 11 to 15 us of host time, more than
+// its kernels; here it is about six.  One function per operator, with
 // positional arguments; the public functions with their defaults and
 // documentation are in rotary.py and paged_cache.py.
 #include <Python.h>

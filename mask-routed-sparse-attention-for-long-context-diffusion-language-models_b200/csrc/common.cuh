@@ -279,18 +279,23 @@ void note_cuda_error(cudaError_t e, const char* where);
 __device__ __forceinline__ void chain_next() { asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory"); }
 __device__ __forceinline__ void chain_wait() { asm volatile("griddepcontrol.wait;\n" ::: "memory"); }
 
+// launch_clusters is the same in clusters of `cluster` CTAs.
 template <typename... P, typename... A>
-int launch_chained(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t s, const A&... args) {
+int launch_clusters(void (*kernel)(P...), dim3 grid, unsigned cluster, int threads, size_t smem, cudaStream_t s,
+                    const A&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(static_cast<unsigned>(threads));
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, P(args)...);
   if (e != cudaSuccess) {
     note_cuda_error(e, __func__);
@@ -298,6 +303,10 @@ int launch_chained(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cu
     return MRSA_ERR_LAUNCH;
   }
   return MRSA_OK;
+}
+template <typename... P, typename... A>
+int launch_chained(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t s, const A&... args) {
+  return launch_clusters(kernel, grid, 1, threads, smem, s, args...);
 }
 
 // Keeps, per host thread, the CUDA error behind the last MRSA_ERR_LAUNCH

@@ -19,6 +19,11 @@
 // operand layout by transposing 8 x 8 blocks in registers.  P enters as a high
 // and a low 16-bit part (16 bits of it count): the second product costs
 // nothing where bytes bound, and the output is then as exact as its rounding.
+//
+// A unit (a sequence's rows of one KV head) has one CTA, or is cut into
+// stretches whose parts a second kernel joins, or, when units are few and short,
+// has a cluster of CTAs that join over each other's shared memory (the rule and
+// what each measured: mrsa_paged_attention).
 #include "paged_attn.cuh"
 
 #include <cuda_fp16.h>
@@ -78,9 +83,25 @@ struct TokenSmem {
   alignas(128) unsigned char ring[A_WARPS][A_STAGES][2][A_KEYS * kD * 2];
   uint32_t mask[A_WARPS][A_STAGES];        // keys of the stage that count
   float m[A_WARPS][8 * kNT], l[A_WARPS][8 * kNT];
+  float cta_m[8 * kNT], cta_l[8 * kNT];    // of the CTA, for its cluster
   paged::Batch batch;
   int warp_sums[A_WARPS];
 };
+
+// CTAs to a unit where a cluster shares it (the portable most).
+constexpr int A_CLUSTER = 8;
+
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;\n" ::: "memory");
+}
+// A float in the shared memory of the cluster's CTA `rank`, at this CTA's address p.
+__device__ __forceinline__ float of_rank(const float* p, int rank) {
+  uint32_t at;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(v) : "r"(at) : "memory");
+  return v;
+}
 
 template <int kD, int kNT, bool kF16>
 __global__ void __launch_bounds__(A_THREADS) paged_token_kernel(const __grid_constant__ Args a) {
@@ -99,7 +120,12 @@ __global__ void __launch_bounds__(A_THREADS) paged_token_kernel(const __grid_con
   int t_begin = 0, t_end = 1;
   paged::Piece pc;
   if (a.undivided) {
-    pc = paged::unit_at(a, cta);
+    pc = paged::unit_at(a, a.cluster ? cta / A_CLUSTER : cta);
+    if (a.cluster) {                   // this CTA's share of the unit's tiles
+      const int rank = cta % A_CLUSTER;
+      pc.tile0 = rank * pc.tiles / A_CLUSTER;
+      pc.tile1 = (rank + 1) * pc.tiles / A_CLUSTER;
+    }
   } else {
     paged::count_tiles<A_THREADS>(a, sm.batch, sm.warp_sums);
     const paged::Deal deal(a, sm.batch.prefix[a.batch] * a.kv_heads * a.row_tiles);
@@ -329,7 +355,13 @@ __global__ void __launch_bounds__(A_THREADS) paged_token_kernel(const __grid_con
         sum += c * sm.l[w][r];
         acc += c * reinterpret_cast<const float*>(sm.ring[w][0][0])[r * kD + d];
       }
-      if (whole) {
+      if (a.cluster) {
+        reinterpret_cast<float*>(sm.ring[0][0][0])[e] = acc;     // read by this thread alone before
+        if (d == 0) {
+          sm.cta_m[r] = top;
+          sm.cta_l[r] = sum;
+        }
+      } else if (whole) {
         const int64_t at = paged::out_row(a, pc, r);
         store_out<kF16>(a.out + (at * kD + d) * 2, sum > 0.f ? acc / sum : 0.f);
         if (d == 0 && a.lse != nullptr) a.lse[at] = sum > 0.f ? (top + log2f(sum)) * kLn2 : -INFINITY;
@@ -341,6 +373,32 @@ __global__ void __launch_bounds__(A_THREADS) paged_token_kernel(const __grid_con
           ml[1] = sum;
         }
       }
+    }
+    if (a.cluster) {
+      // the cluster's parts joined, each CTA an eighth of the outputs
+      cluster_barrier();
+      const int rank = cta % A_CLUSTER, all = nrows * kD, share = (all + A_CLUSTER - 1) / A_CLUSTER;
+      for (int e = rank * share + tid; e < all && e < (rank + 1) * share; e += A_THREADS) {
+        const int r = e / kD, d = e - r * kD;
+        float pm[A_CLUSTER], top = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < A_CLUSTER; ++c) {
+          pm[c] = of_rank(&sm.cta_m[r], c);
+          top = fmaxf(top, pm[c]);
+        }
+        float sum = 0.f, acc = 0.f;
+#pragma unroll
+        for (int c = 0; c < A_CLUSTER; ++c) {
+          const float w = pm[c] == -INFINITY ? 0.f : fast_exp2(pm[c] - top);
+          sum += w * of_rank(&sm.cta_l[r], c);
+          acc += w * of_rank(reinterpret_cast<const float*>(sm.ring[0][0][0]) + e, c);
+        }
+        const int64_t at = paged::out_row(a, pc, r);
+        store_out<kF16>(a.out + (at * kD + d) * 2, sum > 0.f ? acc / sum : 0.f);
+        if (d == 0 && a.lse != nullptr) a.lse[at] = sum > 0.f ? (top + log2f(sum)) * kLn2 : -INFINITY;
+      }
+      cluster_barrier();               // no CTA leaves while another reads its memory
+      return;
     }
     __syncthreads();
     t_now += a.undivided ? 1 : pc.span;
@@ -450,8 +508,9 @@ int launch_token(const Args& a, cudaStream_t s) {
   const int smem = static_cast<int>(sizeof(TokenSmem<kD, kNT>));
   static std::atomic<uint64_t> allowed;
   if (!allow_smem(kernel, smem, allowed)) return MRSA_ERR_LAUNCH;
-  const unsigned ctas = static_cast<unsigned>(a.undivided ? a.batch * a.kv_heads * a.row_tiles : a.grid);
-  return launch_chained(kernel, dim3(ctas), A_THREADS, smem, s, a);
+  const unsigned units = static_cast<unsigned>(a.batch * a.kv_heads * a.row_tiles);
+  const unsigned cluster = a.cluster ? A_CLUSTER : 1;
+  return launch_clusters(kernel, dim3(a.undivided ? units * cluster : a.grid), cluster, A_THREADS, smem, s, a);
 }
 
 template <int kD, bool kF16>
@@ -603,12 +662,21 @@ extern "C" int mrsa_paged_attention(const mrsa_paged_attention_args* p, const mr
     // tiles, where the longest of a ragged batch cannot hold the others up for
     // long.  Measured, us, whole and cut: one token, one sequence of 128 6.0 and
     // 6.8, of 512 10.4 and 6.8; sixteen of up to 512 10.7 and 12.5, of up to 1024
-    // 16.5 and 13.7; 64 of up to 1024 24 and 29.  32 tokens, one sequence of 256
-    // 12.5 and 15.6, of 1024 25 and 16; 16 of up to 1024 25 and 33; 48 45 and 64.
+    // 16.5 and 12.1; 64 of up to 1024 24 and 29.  32 tokens, one sequence of 256
+    // 11.7 and 10.9, of 1024 24 and 13; 16 of up to 1024 24 and 29; 48 45 and 51.
     const int64_t units = static_cast<int64_t>(a.batch) * a.kv_heads * a.row_tiles;
     const int64_t T = t->max_pages * t->page_size / A_TILE + 1, cut = block ? 8 : 6;
     a.undivided = T <= 33 && units <= 0x7fffffffLL &&
                   T * ((units + a.grid - 1) / a.grid) * a.grid <= units * T + cut * (a.grid + units);
+    // A cluster of eight CTAs to a unit, which join it over shared memory: no second
+    // launch, and no parts in memory.  For one token while the clusters' CTAs have
+    // an SM each, and for more than two tiles, of which each has some; past 32 its
+    // CTAs are too few against stretches over two CTAs per SM.  Measured, us, in a
+    // cluster and as below: one sequence of 256 5.8 and 7.4, of 1000 6.6 and 7.4, of
+    // 2000 8.1 and 8.2, of 4000 11.2 and 9.4; four of 128 6.4 and 6.0, of up to 500
+    // 6.8 and 8.1, of up to 2000 9.3 and 9.7; nine of up to 500 12.6 and 9.1.
+    a.cluster = !block && units * A_CLUSTER <= sm_count() && T > 3 && T <= 33;
+    if (a.cluster) a.undivided = 1;
     int rc;
     if (block) rc = paged::launch_block(a, p->dtype, static_cast<int>(p->head_dim), s);
     else if (p->dtype == MRSA_F16) rc = p->head_dim == 128 ? launch_token_rows<128, true>(a, s) : launch_token_rows<64, true>(a, s);

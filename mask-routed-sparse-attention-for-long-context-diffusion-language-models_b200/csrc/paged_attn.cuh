@@ -44,6 +44,7 @@ struct Args {
   int cut;                             // what a unit costs beside its tiles, in tiles
   int grid;                            // CTAs (split: halves of CTAs) that the tiles are dealt to
   int undivided;                       // CTA u has the whole of unit u: nothing to deal or to join
+  int cluster;                         // paged_attn.cu: the CTAs of a cluster share a unit, and join it
   float scale_log2;                    // softmax scale times log2(e)
   float* part_o;                       // [2 * grid][row_tile][D]; paged_block.cu: [2 * grid][D / 4][row_tile][4]
   float* part_ml;                      // [2 * grid][row_tile][2]: maximum (log2), sum

@@ -540,26 +540,7 @@ int launch_plan(const PlanArgs& a, cudaStream_t s) {
   if (kOp != kFree && work < a.t.pages) work = a.t.pages;
   unsigned ctas = 1;
   while (ctas < P_CLUSTER && work > static_cast<int64_t>(ctas) * 4 * P_THREADS) ctas *= 2;
-  if (ctas == 1) return launch_chained(page_plan_kernel<kOp>, dim3(1), P_THREADS, 0, s, a);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ctas);
-  cfg.blockDim = dim3(P_THREADS);
-  cfg.stream = s;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = ctas;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, page_plan_kernel<kOp>, a);
-  if (e != cudaSuccess) {
-    mrsa::note_cuda_error(e, __func__);
-    (void)cudaGetLastError();
-    return MRSA_ERR_LAUNCH;
-  }
-  return MRSA_OK;
+  return launch_clusters(page_plan_kernel<kOp>, dim3(ctas), ctas, P_THREADS, 0, s, a);
 }
 
 template <typename K>

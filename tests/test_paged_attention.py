@@ -307,3 +307,23 @@ def test_offsets_past_32_bits(mrsa, cuda_device):
     assert cache.table[1, :5].tolist() == [0, 35996, 35997, 35998, 35999]
     for l, hq in ((1, 8), (32, 56)):
         compare(mrsa, cache, cache.seqs(1, 0), queries(dev, g, 2, l, hq, 128, torch.bfloat16))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("hq,hkv,d,page", [(28, 4, 128, 64), (5, 1, 64, 16), (32, 2, 128, 32)])
+@pytest.mark.parametrize("lens", [[200], [511], [0, 130, 2048], [1, 64, 1985, 0]])
+def test_few_short_sequences(mrsa, cuda_device, dtype, hq, hkv, d, page, lens):
+    """One token of few sequences: several CTAs share a unit, some of them without a tile, or all masked."""
+    cache, g = filled(mrsa, cuda_device, lens, hkv, d, page, dtype, seed=len(lens))
+    seqs = torch.arange(len(lens), device=cuda_device, dtype=torch.int32).flip(0)
+    q = queries(cuda_device, g, len(lens), 1, hq, d, dtype)
+    first, lse = compare(mrsa, cache, seqs, q, causal=True)
+    for _ in range(3):                        # the join has an order of its own: the same bits each time
+        again, lse2 = cache.attend(0, seqs, q, causal=True, return_lse=True)
+        assert torch.equal(first, again) and torch.equal(lse, lse2)
+    width = cache.table.shape[1] * page
+    valid = torch.rand(len(lens), width, device=cuda_device, generator=g) < 0.4
+    valid[0] = False                          # a row that sees nothing
+    valid[-1, :130] = False                   # leading shares that see nothing
+    compare(mrsa, cache, seqs, q, valid=valid)
