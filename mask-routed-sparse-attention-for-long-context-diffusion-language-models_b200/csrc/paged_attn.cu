@@ -39,9 +39,9 @@ constexpr int A_KEYS = 16;                  // keys per warp and tile
 constexpr int A_TILE = A_KEYS * A_WARPS;    // keys per tile
 constexpr int A_STAGES = 3;
 // More query rows per KV head go to the tensor cores (paged_block.cu).  131072
-// cached tokens of 28 / 4 heads: 14 rows 56 us here and 69 there, 21 rows 99
-// (in row tiles of 32) and 70; sixteen sequences of up to 16384: 64 and 80, 117
-// and 81.
+// cached tokens of 28 / 4 heads: 14 rows 54 us here and 59 there, 21 rows 90
+// (in two row tiles) and 60; sixteen sequences of up to 16384: 73 and 73, 115
+// and 75; of up to 1000: 15.3 and 16.1, 19.3 and 17.0.
 constexpr int kTokenRows = 16;
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
