@@ -5,9 +5,11 @@
 //
 // over a sequence's cached tokens (masked tokens and, when causal, tokens past
 // the query's own position have weight zero; a row that sees nothing gets
-// zeros and -inf).  With R query rows per KV head a key's 4 D bytes (K and V)
-// meet 4 D R products and sums: R flops per byte, so for few rows the cache's
-// bytes bound it.
+// zeros and -inf).  A row that has seen a key has a sum of at least one, so a
+// sum of zero, and not a NaN, is what says that it saw nothing: a score that is
+// NaN or +inf makes the sum, the output and the LSE NaN.  With R query rows per
+// KV head a key's 4 D bytes (K and V) meet 4 D R products and sums: R flops per
+// byte, so for few rows the cache's bytes bound it.
 //
 // Four warps per CTA, each on 16 keys of a 64-key tile, as if alone: its own
 // ring of cp.async stages, its own running maximum, sum and output, no barrier
@@ -294,8 +296,9 @@ __global__ void __launch_bounds__(A_THREADS) paged_token_kernel(const __grid_con
         float p[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float ref = m[nt][e & 1];
-          p[e] = ref == -INFINITY ? 0.f : fast_exp2(x[e] - ref);
+          // (before a row's first score: 0 for a key that does not count, NaN for one that is NaN)
+          const float ref = m[nt][e & 1] == -INFINITY ? 0.f : m[nt][e & 1];
+          p[e] = fast_exp2(x[e] - ref);
           l[nt][e & 1] += p[e];
         }
         uint32_t lo0, lo1;
@@ -363,8 +366,8 @@ __global__ void __launch_bounds__(A_THREADS) paged_token_kernel(const __grid_con
         }
       } else if (whole) {
         const int64_t at = paged::out_row(a, pc, r);
-        store_out<kF16>(a.out + (at * kD + d) * 2, sum > 0.f ? acc / sum : 0.f);
-        if (d == 0 && a.lse != nullptr) a.lse[at] = sum > 0.f ? (top + log2f(sum)) * kLn2 : -INFINITY;
+        store_out<kF16>(a.out + (at * kD + d) * 2, sum == 0.f ? 0.f : acc / sum);
+        if (d == 0 && a.lse != nullptr) a.lse[at] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
       } else {
         a.part_o[(static_cast<int64_t>(slot) * a.row_tile + r) * kD + d] = acc;
         if (d == 0) {
@@ -394,8 +397,8 @@ __global__ void __launch_bounds__(A_THREADS) paged_token_kernel(const __grid_con
           acc += w * of_rank(reinterpret_cast<const float*>(sm.ring[0][0][0]) + e, c);
         }
         const int64_t at = paged::out_row(a, pc, r);
-        store_out<kF16>(a.out + (at * kD + d) * 2, sum > 0.f ? acc / sum : 0.f);
-        if (d == 0 && a.lse != nullptr) a.lse[at] = sum > 0.f ? (top + log2f(sum)) * kLn2 : -INFINITY;
+        store_out<kF16>(a.out + (at * kD + d) * 2, sum == 0.f ? 0.f : acc / sum);
+        if (d == 0 && a.lse != nullptr) a.lse[at] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * kLn2;
       }
       cluster_barrier();               // no CTA leaves while another reads its memory
       return;
@@ -494,8 +497,8 @@ __global__ void __launch_bounds__(32 * J_WARPS) paged_join_kernel(const __grid_c
     }
     if (sub == 0) {
 #pragma unroll
-      for (int e = 0; e < kV; ++e) store_out<kF16>(a.out + (at * kD + lane * kV + e) * 2, l > 0.f ? acc[e] / l : 0.f);
-      if (lane == 0 && a.lse != nullptr) a.lse[at] = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+      for (int e = 0; e < kV; ++e) store_out<kF16>(a.out + (at * kD + lane * kV + e) * 2, l == 0.f ? 0.f : acc[e] / l);
+      if (lane == 0 && a.lse != nullptr) a.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
     }
   }
   // a block that read no part waits too: what follows in the stream follows this grid's end
