@@ -554,9 +554,10 @@ size_t mrsa_paged_attention_workspace(const mrsa_paged_attention_args* a);
 /* Attention of len query tokens per sequence over its cached tokens, read
  * from their pages; the query tokens' own keys are in the cache already.
  * Masked tokens, and slots past a sequence's length, may hold anything (NaN
- * included).  A query that sees no token gets zeros and an lse of -inf.  A
- * bad sequence or page number is reported in the status word and reads as no
- * tokens. */
+ * included).  A query that sees no token gets zeros and an lse of -inf; one
+ * that sees a NaN or a score of +inf gets NaN in both.  With causal, a value
+ * that is not finite may reach queries before its token.  A bad sequence or
+ * page number is reported in the status word and reads as no tokens. */
 int mrsa_paged_attention(const mrsa_paged_attention_args* a, const mrsa_page_table* t, void* workspace,
                          size_t ws_bytes, mrsa_stream_t stream);
 

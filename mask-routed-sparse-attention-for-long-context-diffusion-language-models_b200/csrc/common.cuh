@@ -173,8 +173,10 @@ __device__ __forceinline__ float2 fmul2(float2 a, float2 b) {
 // |f| <= 1/2), 2^f by a degree-4 polynomial whose coefficients were fitted
 // for the attention kernels by Remez exchange on [-1/2, 1/2] (relative error 2.7e-6
 // evaluated in fp32, below fp16 P's rounding), and 2^n added to the exponent
-// field.  y is clamped to >= -126, so -inf gives 2^-126 rather than 0: only
-// for tiles without masked columns, where every row's sum is >= 1.
+// field.  y is clamped to >= -126, so -inf gives 2^-126 rather than 0, NaN the
+// same, and +inf no infinity.  A caller with masked columns has to cancel that
+// 2^-126 (zeroed V rows, a sum known to be >= 1), and every caller to find a
+// row's NaN and +inf by other means.
 __device__ __forceinline__ float2 exp2_poly2(float2 y) {
   constexpr float kShift = 12582912.0f;   // 1.5 * 2^23
   y.x = fmaxf(y.x, -126.0f);
@@ -193,6 +195,12 @@ __device__ __forceinline__ float2 exp2_poly2(float2 y) {
 __device__ __forceinline__ float fmax3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;\n" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// the same, NaN where one of them is
+__device__ __forceinline__ float fmax3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;\n" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
 

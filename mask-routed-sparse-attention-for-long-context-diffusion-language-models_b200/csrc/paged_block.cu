@@ -428,8 +428,8 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
           for (int c = 0; c < B_TILE; c += 8)
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-              m4[j] = fmax3(m4[j], __uint_as_float(x[c + 2 * j]), __uint_as_float(x[c + 2 * j + 1]));
-          const float tmax = fmax3(m4[0], m4[1], fmaxf(m4[2], m4[3])) * a.scale_log2;
+              m4[j] = fmax3_nan(m4[j], __uint_as_float(x[c + 2 * j]), __uint_as_float(x[c + 2 * j + 1]));
+          const float tmax = fmax3_nan(m4[0], m4[1], fmax3_nan(m4[2], m4[3], m4[3])) * a.scale_log2;
           // the reference moves, and O is scaled, only for a maximum 2^8 above it
           float corr = 1.f;
           bool rescale = false;
@@ -466,7 +466,10 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
             }
           }
           __syncwarp();
-          l_run += (s2[0].x + s2[1].x) + (s2[0].y + s2[1].y);
+          // a score that is NaN or +inf (which the polynomial does not keep) makes the row's
+          // sum NaN here, and that its output and its LSE
+          const float l_tile = (s2[0].x + s2[1].x) + (s2[0].y + s2[1].y);
+          l_run += tmax < INFINITY ? l_tile : __int_as_float(0x7fffffff);
           tc::tmem_st16(t_s, &pk[0]);
           tc::tmem_st16(t_s + 16, &pk[16]);
           tc::tmem_wait_st();
@@ -495,8 +498,8 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
         if (!ok) break;
         tc::fence_after_sync();
         const bool whole = p.whole();
-        if (m_run == -INFINITY) l_run = 0.f;       // the row saw no key
-        const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
+        if (m_run == -INFINITY && l_run == l_run) l_run = 0.f;       // the row saw no key
+        const float inv = l_run == 0.f ? 0.f : 1.f / l_run;          // 0: zeros, whatever O holds
         if (whole) {
           // rows leave through shared memory, 32 columns at a time, so that the warp writes
           // 64 bytes of each: 16-byte piece j of its row i at i * 4 + (j ^ (i & 3)) there
@@ -513,7 +516,8 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
               uint32_t w[4];
 #pragma unroll
               for (int q = 0; q < 4; ++q) {
-                const float f0 = __uint_as_float(o[8 * j + 2 * q]) * inv, f1 = __uint_as_float(o[8 * j + 2 * q + 1]) * inv;
+                const float f0 = inv == 0.f ? 0.f : __uint_as_float(o[8 * j + 2 * q]) * inv;
+                const float f1 = inv == 0.f ? 0.f : __uint_as_float(o[8 * j + 2 * q + 1]) * inv;
                 if constexpr (kF16) {
                   const __half2 hv = __floats2half2_rn(f0, f1);
                   w[q] = *reinterpret_cast<const uint32_t*>(&hv);
@@ -532,7 +536,7 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
             __syncwarp();
           }
           if (row_ok && a.lse != nullptr)
-            a.lse[paged::out_row(a, p, row)] = l_run > 0.f ? (m_run + log2f(l_run)) * kLn2 : -INFINITY;
+            a.lse[paged::out_row(a, p, row)] = l_run == 0.f ? -INFINITY : (m_run + log2f(l_run)) * kLn2;
         } else {
           // four columns of all rows side by side: the warp's stores are whole lines
           const int64_t slot = 2 * worker + (t_now == t_begin ? 0 : 1);
@@ -668,9 +672,10 @@ __global__ void __launch_bounds__(256) paged_block_join_kernel(const __grid_cons
     }
     if (!row_ok) continue;
     const int64_t at = paged::out_row(a, p, g * a.group_rows + r);
-    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
     for (int j = 0; j < kCols; ++j) {
+      if (inv == 0.f) acc[j] = make_float4(0.f, 0.f, 0.f, 0.f);
       uint2 v;
       if constexpr (kF16) {
         const __half2 lo = __floats2half2_rn(acc[j].x * inv, acc[j].y * inv), hi = __floats2half2_rn(acc[j].z * inv, acc[j].w * inv);
@@ -680,7 +685,7 @@ __global__ void __launch_bounds__(256) paged_block_join_kernel(const __grid_cons
       }
       *reinterpret_cast<uint2*>(a.out + at * kD * 2 + column(j) * 8) = v;
     }
-    if (warp == 0 && set == 0 && a.lse != nullptr) a.lse[at] = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+    if (warp == 0 && set == 0 && a.lse != nullptr) a.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
   }
   // a block that read no part waits too: what follows in the stream follows this grid's end
   chain_wait();

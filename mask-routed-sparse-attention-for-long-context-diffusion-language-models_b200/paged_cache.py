@@ -109,7 +109,10 @@ def paged_attention(q, k_pages, v_pages, table, lengths, seqs, *, causal: bool =
     masks cached tokens; what masked tokens and unused slots hold does not
     matter.  Returns ``o [B, L, Hq, D]``, with ``return_lse`` also the
     natural-log LSE ``[B, L, Hq]`` in fp32; a query that sees no token gets
-    zeros and -inf.  ``scale`` defaults to ``D ** -0.5``.  Forward only: it
+    zeros and -inf, one that sees a NaN or a score of +inf gets NaN in both.
+    A weight of zero does not cancel a cached value that is not finite: with
+    ``causal`` it may reach the queries before its token too.  ``scale``
+    defaults to ``D ** -0.5``.  Forward only: it
     raises under autograd rather than return an output without a gradient."""
     return _lib.ext().attend(q, k_pages, v_pages, table, lengths, seqs, causal, key_valid, scale, return_lse, status)
 

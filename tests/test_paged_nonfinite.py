@@ -106,3 +106,25 @@ def spoil(mrsa, dev, l, form, dtype):
 @pytest.mark.parametrize("l", [1, 2])
 def test_few_rows_keep_what_is_not_finite(mrsa, cuda_device, l, form, dtype):
     spoil(mrsa, cuda_device, l, form, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("form", sorted(FORMS))
+@pytest.mark.parametrize("l", [4, 16, 32, 45])
+def test_many_rows_keep_what_is_not_finite(mrsa, cuda_device, l, form, dtype):
+    spoil(mrsa, cuda_device, l, form, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("form", ["whole", "cut"])
+@pytest.mark.parametrize("l", [2, 32])
+def test_rows_before_the_cache_get_zeros(mrsa, cuda_device, l, form):
+    """Causal queries that see nothing, of a sequence whose every value is NaN."""
+    cache, g = filled(mrsa, cuda_device, [1], 4, 128, 64, torch.bfloat16)
+    wide(cache, FORMS[form][1])
+    cache.pool[0, 1] = math.nan
+    o, lse = cache.attend(0, cache.seqs(0), queries(cuda_device, g, 1, l, 28, 128, torch.bfloat16), causal=True,
+                          return_lse=True)
+    cache.check()
+    assert not o[0, :-1].any() and (lse[0, :-1] == -math.inf).all() and o[0, -1].isnan().all()
