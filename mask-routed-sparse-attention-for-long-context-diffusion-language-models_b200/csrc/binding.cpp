@@ -390,6 +390,13 @@ PyObject* page_copy(PyObject*, PyObject* const* o, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// An operator without a backward pass raises rather than lose a gradient.
+void forward_only(const char* op, std::initializer_list<const Tensor*> inputs) {
+  if (!c10::GradMode::is_enabled()) return;
+  for (const Tensor* x : inputs)
+    TORCH_CHECK_NOT_IMPLEMENTED(!x->defined() || !x->requires_grad(), op, " is forward-only");
+}
+
 // A layer's pages.
 void check_pages(const Tensor& k, const Tensor& v) {
   TORCH_CHECK_VALUE(k.defined() && v.defined() && k.dim() == 4 && v.sizes() == k.sizes(),
@@ -426,6 +433,7 @@ PyObject* append(PyObject*, PyObject* const* o, Py_ssize_t n) {
   TORCH_CHECK_VALUE(table.device() == k.device(), "the table must be on the tensors' device");
   const Tensor seqs = ints(tensor(o[4], "seqs"), "seqs", 1, table);
   TORCH_CHECK_VALUE(seqs.size(0) == k.size(0), "seqs must name one sequence per batch row");
+  forward_only("paged_append", {&q, &k, &v, &kp, &vp});
   if (inv.defined()) {
     a.pairs = check_rotation(inv, pos, k);
     a.inv_freq = in<float>(inv);
@@ -489,9 +497,7 @@ PyObject* attend(PyObject*, PyObject* const* o, Py_ssize_t n) {
                     "q and the pages must share a type (BF16 or FP16) and a device");
   TORCH_CHECK_VALUE((d == 64 || d == 128) && kp.size(3) == d && hkv >= 1 && hq >= hkv && hq % hkv == 0,
                     "heads must be of 64 or 128 dims, Hq a multiple of Hkv; got q ", q.sizes(), ", pages ", kp.sizes());
-  if (c10::GradMode::is_enabled() && (q.requires_grad() || kp.requires_grad() || vp.requires_grad())) {
-    TORCH_CHECK_NOT_IMPLEMENTED(false, "paged_attention is forward-only");
-  }
+  forward_only("paged_attention", {&q, &kp, &vp});
   const mrsa_page_table t = page_table(table, lengths, Tensor(), tensor(o[10], "status"), kp.size(0), kp.size(1));
   TORCH_CHECK_VALUE(table.device() == q.device(), "the table must be on the tensors' device");
   const Tensor seqs = ints(tensor(o[5], "seqs"), "seqs", 1, table);
