@@ -45,6 +45,12 @@ bool finish(int rc, const char* name) {
 
 void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
 
+// No operator here has a forward-mode derivative: a tangent is an error, not lost.
+void no_tangent(const char* op, std::initializer_list<const Tensor*> inputs) {
+  for (const Tensor* x : inputs)
+    TORCH_CHECK_NOT_IMPLEMENTED(!x->defined() || !x->_fw_grad(/*level=*/0).defined(), op, " has no forward-mode derivative");
+}
+
 Tensor inner_contiguous(const Tensor& x) { return x.stride(-1) == 1 || x.size(-1) == 1 ? x : x.contiguous(); }
 
 Tensor aligned(const Tensor& x) {
@@ -181,6 +187,7 @@ PyObject* rotary(PyObject*, PyObject* const* o, Py_ssize_t n) {
   const bool interleaved = layout_of(o[5]) == 1;
   check_heads(q, "q");
   TORCH_CHECK_VALUE(pos.defined() && inv.defined(), "position_ids must be int64 (B, L) and inv_freq fp32 [n]");
+  no_tangent("rotary_embedding", {&q, &k, &inv});
   Tensor qo, ko;
   if (c10::GradMode::is_enabled() && (q.requires_grad() || (k.defined() && k.requires_grad()))) {
     const std::optional<Tensor> pair = k.defined() ? std::optional<Tensor>(k) : std::nullopt;
@@ -434,6 +441,7 @@ PyObject* append(PyObject*, PyObject* const* o, Py_ssize_t n) {
   const Tensor seqs = ints(tensor(o[4], "seqs"), "seqs", 1, table);
   TORCH_CHECK_VALUE(seqs.size(0) == k.size(0), "seqs must name one sequence per batch row");
   forward_only("paged_append", {&q, &k, &v, &kp, &vp});
+  no_tangent("paged_append", {&q, &k, &v, &kp, &vp, &inv});
   if (inv.defined()) {
     a.pairs = check_rotation(inv, pos, k);
     a.inv_freq = in<float>(inv);
@@ -498,6 +506,7 @@ PyObject* attend(PyObject*, PyObject* const* o, Py_ssize_t n) {
   TORCH_CHECK_VALUE((d == 64 || d == 128) && kp.size(3) == d && hkv >= 1 && hq >= hkv && hq % hkv == 0,
                     "heads must be of 64 or 128 dims, Hq a multiple of Hkv; got q ", q.sizes(), ", pages ", kp.sizes());
   forward_only("paged_attention", {&q, &kp, &vp});
+  no_tangent("paged_attention", {&q, &kp, &vp});
   const mrsa_page_table t = page_table(table, lengths, Tensor(), tensor(o[10], "status"), kp.size(0), kp.size(1));
   TORCH_CHECK_VALUE(table.device() == q.device(), "the table must be on the tensors' device");
   const Tensor seqs = ints(tensor(o[5], "seqs"), "seqs", 1, table);

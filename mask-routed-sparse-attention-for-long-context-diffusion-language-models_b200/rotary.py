@@ -50,5 +50,6 @@ def rotary_embedding(q: torch.Tensor, k: torch.Tensor | None, position_ids: torc
     the other dims pass through.  The angle is the fp32 product ``position *
     inv_freq`` and cos and sin are times ``attention_factor``, as in
     :func:`yarn_rope_qk`; fp32 arithmetic, one rounding.  Any batch, token and
-    head strides.  Records the gradient of q and k where one is wanted."""
+    head strides.  Records the gradient of q and k where one is wanted;
+    forward-mode tangents are refused."""
     return _lib.ext().rotary(q, k, position_ids, inv_freq, attention_factor, layout)

@@ -33,3 +33,24 @@ def test_append_refuses_a_gradient(mrsa, cuda_device, name):
         append(mrsa, cache, a)
     cache.check()
     assert cache.pool.any()
+
+
+@pytest.mark.gpu
+def test_tangents_are_refused(mrsa, cuda_device):
+    from torch.autograd import forward_ad
+
+    cache, a = append_args(mrsa, cuda_device)
+    pos = torch.arange(3, device=cuda_device)[None]
+    state = cache.table, cache.lengths, cache.seqs(0)
+    calls = {
+        "rotary": (("q", "k", "inv_freq"), lambda a: mrsa.rotary_embedding(a["q"], a["k"], pos, a["inv_freq"])),
+        "append": (("q", "k", "v", "k_pages", "v_pages", "inv_freq"), lambda a: append(mrsa, cache, a)),
+        "attend": (("q", "k_pages", "v_pages"), lambda a: mrsa.paged_attention(a["q"], a["k_pages"], a["v_pages"], *state)),
+    }
+    with forward_ad.dual_level():
+        for names, call in calls.values():
+            for name in names:
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    call(a | {name: forward_ad.make_dual(a[name], torch.ones_like(a[name]))})
+            with torch.no_grad():
+                call(a)
