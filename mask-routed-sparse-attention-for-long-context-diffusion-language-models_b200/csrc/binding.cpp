@@ -51,6 +51,12 @@ void no_tangent(const char* op, std::initializer_list<const Tensor*> inputs) {
     TORCH_CHECK_NOT_IMPLEMENTED(!x->defined() || !x->_fw_grad(/*level=*/0).defined(), op, " has no forward-mode derivative");
 }
 
+// The frequencies are constants of a model: no gradient of theirs is recorded.
+void fixed_frequencies(const Tensor& inv) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!c10::GradMode::is_enabled() || !inv.defined() || !inv.requires_grad(),
+                              "the gradient of inv_freq is not recorded");
+}
+
 Tensor inner_contiguous(const Tensor& x) { return x.stride(-1) == 1 || x.size(-1) == 1 ? x : x.contiguous(); }
 
 Tensor aligned(const Tensor& x) {
@@ -188,6 +194,7 @@ PyObject* rotary(PyObject*, PyObject* const* o, Py_ssize_t n) {
   check_heads(q, "q");
   TORCH_CHECK_VALUE(pos.defined() && inv.defined(), "position_ids must be int64 (B, L) and inv_freq fp32 [n]");
   no_tangent("rotary_embedding", {&q, &k, &inv});
+  fixed_frequencies(inv);
   Tensor qo, ko;
   if (c10::GradMode::is_enabled() && (q.requires_grad() || (k.defined() && k.requires_grad()))) {
     const std::optional<Tensor> pair = k.defined() ? std::optional<Tensor>(k) : std::nullopt;
@@ -442,6 +449,7 @@ PyObject* append(PyObject*, PyObject* const* o, Py_ssize_t n) {
   TORCH_CHECK_VALUE(seqs.size(0) == k.size(0), "seqs must name one sequence per batch row");
   forward_only("paged_append", {&q, &k, &v, &kp, &vp});
   no_tangent("paged_append", {&q, &k, &v, &kp, &vp, &inv});
+  fixed_frequencies(inv);
   if (inv.defined()) {
     a.pairs = check_rotation(inv, pos, k);
     a.inv_freq = in<float>(inv);

@@ -51,5 +51,5 @@ def rotary_embedding(q: torch.Tensor, k: torch.Tensor | None, position_ids: torc
     inv_freq`` and cos and sin are times ``attention_factor``, as in
     :func:`yarn_rope_qk`; fp32 arithmetic, one rounding.  Any batch, token and
     head strides.  Records the gradient of q and k where one is wanted;
-    forward-mode tangents are refused."""
+    a gradient of ``inv_freq`` and forward-mode tangents are refused."""
     return _lib.ext().rotary(q, k, position_ids, inv_freq, attention_factor, layout)

@@ -54,3 +54,19 @@ def test_tangents_are_refused(mrsa, cuda_device):
                     call(a | {name: forward_ad.make_dual(a[name], torch.ones_like(a[name]))})
             with torch.no_grad():
                 call(a)
+
+
+@pytest.mark.gpu
+def test_gradient_of_frequencies_is_refused(mrsa, cuda_device):
+    cache, a = append_args(mrsa, cuda_device)
+    pos = torch.arange(3, device=cuda_device)[None]
+    inv = a["inv_freq"].requires_grad_()
+    for wants in (False, True):
+        q = a["q"].detach().requires_grad_(wants)
+        with pytest.raises(NotImplementedError, match="inv_freq"):
+            mrsa.rotary_embedding(q, a["k"], pos, inv)
+    with pytest.raises(NotImplementedError, match="inv_freq"):
+        append(mrsa, cache, a)
+    with torch.no_grad():
+        y, _ = mrsa.rotary_embedding(a["q"], a["k"], pos, inv)
+        assert torch.equal(append(mrsa, cache, a), y)
