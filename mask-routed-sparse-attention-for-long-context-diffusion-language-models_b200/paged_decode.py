@@ -13,11 +13,16 @@ A denoising loop::
     seq, cands = dec.cache.seqs(0), dec.cache.seqs(1, 2, 3, 4)
     dec.prefill(seq, prompt)                                   # [1, L] token ids
     dec.fork(seq, cands)                                       # the prompt's pages, held in common
+    at = dec.cache.lengths[1:5].clone()                        # where the blocks begin
     dec.cache.extend(cands, 32)                                # room for a block each
     for _ in range(steps):
-        logits = dec.step(cands, block)                        # [4, 32] ids: rewrites the block's keys and values
+        logits = dec.step(cands, block, start=at)              # [4, 32] ids: rewrites the block's keys and values
         block = choose(logits, block)
     dec.cache.free(losers)
+
+With ``start`` given, a block whose ``extend`` was refused (no free pages, too
+long) has no place and is not written; without it the last tokens that the
+sequence does have would be.
 """
 
 from __future__ import annotations
@@ -68,7 +73,11 @@ class PagedDream:
 
     def prefill(self, seqs, ids, **kw):
         """The tokens ``ids [B, S]`` appended to the sequences: room for them,
-        then :meth:`step`."""
+        then :meth:`step` from where they ended before.  Without that room
+        nothing is written, and :meth:`PagedKVCache.check` says why."""
+        lengths = self.cache.lengths
+        rows = seqs.clamp(0, lengths.shape[0] - 1)        # a number out of range is reported, not followed
+        kw.setdefault("start", lengths.index_select(0, rows))
         self.cache.extend(seqs, ids.shape[1])
         return self.step(seqs, ids, **kw)
 

@@ -134,3 +134,35 @@ def test_tokens_one_by_one_and_a_thinned_prompt(decoder, cuda_device):
         close(dec.prefill(thin, new[:, i:i + 1], position_ids=pos)[0], few.step(new[0, i:i + 1], pos[0]))
     cache.check()
     assert cache.lengths[cache.seqs(3, 1).long()].tolist() == [304, left + 4]
+
+
+@pytest.mark.parametrize("pages,max_len,causal,error", [(4, 640, False, RuntimeError), (4, 640, True, RuntimeError),
+                                                        (9, 256, False, ValueError)])
+def test_prefill_without_room_keeps_what_is_cached(mrsa, cuda_device, pages, max_len, causal, error):
+    from mrsa_b200.dream_forward import DreamConfig, DreamForward
+    from mrsa_b200.paged_decode import PagedDream
+
+    dev = cuda_device
+    cfg = DreamConfig(layers=2, hidden=896, ffn=1024, q_heads=14, kv_heads=2, vocab=512)
+    dec = PagedDream(DreamForward(cfg, seed=3, device=dev), pages=pages, sequences=2, max_len=max_len)
+    cache = dec.cache
+    ids = torch.randint(0, 512, (1, 300), device=dev, generator=torch.Generator(device=dev).manual_seed(4))
+    dec.prefill(cache.seqs(1), ids[:, :200], causal=causal)
+    cache.check()
+    state = [t.clone() for t in (cache.pool.view(torch.int16), cache.table, cache.lengths, cache.refcount)]
+    dec.prefill(cache.seqs(1), ids[:, 200:], causal=causal)        # 300 tokens need five pages
+    with pytest.raises(error):
+        cache.check()
+    for was, now in zip(state, (cache.pool.view(torch.int16), cache.table, cache.lengths, cache.refcount)):
+        assert torch.equal(was, now)
+    dec.prefill(cache.seqs(5), ids[:, :7])                         # no such sequence
+    with pytest.raises(ValueError, match="out of range"):
+        cache.check()
+    # what fits still continues the same tokens
+    a = dec.prefill(cache.seqs(1), ids[:, 200:250], causal=causal)
+    cache.check()
+    cache.free(cache.seqs(1))
+    dec.prefill(cache.seqs(0), ids[:, :200], causal=causal)
+    b = dec.prefill(cache.seqs(0), ids[:, 200:250], causal=causal)
+    cache.check()
+    assert torch.equal(a, b)
