@@ -170,9 +170,9 @@ __global__ void __launch_bounds__(P_THREADS, 1) page_plan_kernel(
       sm.first[tid] = used;
       sm.used[tid] = 0;
       sm.len[tid] = 0;
-      if (kOp == kExtend) {
+      if (kOp == kExtend && !bad) {
         const int64_t more = a.extra != nullptr ? a.extra[tid] : a.all;
-        if (more < 0 || len + more > most) bad |= MRSA_PAGE_TOO_LONG;
+        if (more < 0 || more > most - len) bad = MRSA_PAGE_TOO_LONG;   // (len + more may pass 64 bits)
         else {
           sm.len[tid] = static_cast<int>(len + more);
           sm.used[tid] = static_cast<int>((len + more + ps - 1) >> shift);

@@ -370,3 +370,26 @@ def test_page_argument_codes(mrsa):
     with pytest.raises(ValueError, match="CUDA"):
         mrsa.page_free(torch.zeros(1, 1, dtype=torch.int32), torch.zeros(1, dtype=torch.int32),
                        torch.zeros(1, dtype=torch.int32), torch.zeros(1, dtype=torch.int32))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [2 ** 63 - 1, 2 ** 63 - 41, 2 ** 62, 2 ** 32, 2 ** 31 - 40])
+def test_growth_past_any_whole_number_is_too_long(mrsa, cuda_device, tokens):
+    """Sums with the lengths that pass 64 or 32 bits."""
+    cache = mrsa.PagedKVCache(1, 12, 1, 64, sequences=3, max_len=128, page_size=16, device=cuda_device)
+    cache.extend(cache.seqs(0, 1), 40)
+    before = [cache.table.tolist(), cache.lengths.tolist(), cache.refcount.tolist()]
+    for seqs in ((0,), (1, 0, 2), (2,)):
+        cache.extend(cache.seqs(*seqs), tokens)
+        with pytest.raises(ValueError, match="outgrow"):
+            cache.check()
+        assert [cache.table.tolist(), cache.lengths.tolist(), cache.refcount.tolist()] == before
+    most = torch.tensor([2 ** 31 - 1], dtype=torch.int32, device=cuda_device)
+    cache.extend(cache.seqs(0), most)
+    with pytest.raises(ValueError, match="outgrow"):
+        cache.check()
+    with pytest.raises(OverflowError):
+        cache.extend(cache.seqs(0), 2 ** 63)
+    cache.extend(cache.seqs(0), 88)
+    cache.check()
+    assert cache.lengths.tolist() == [128, 40, 0]
