@@ -493,7 +493,8 @@ typedef struct {
 
 /* q and k turned as in mrsa_rotary (position_ids NULL: the cache positions;
  * pairs 0: not turned), q to q_out, k and v into their sequences' pages.  A
- * token that has no page is reported in the status word and not written. */
+ * token that has no page is reported in the status word and not written, and
+ * so is a batch row some of whose tokens an earlier batch row writes too. */
 int mrsa_paged_append(const mrsa_rotary_args* r, const mrsa_page_table* t, const mrsa_paged_append_args* p,
                       mrsa_stream_t stream);
 

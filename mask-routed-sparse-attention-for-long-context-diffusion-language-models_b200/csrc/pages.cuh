@@ -45,6 +45,13 @@ struct PageSlots {
     const int row = seqs[b];
     return (row < 0 || row >= max_seqs) ? -1 : static_cast<int64_t>(lengths[row]) - len;
   }
+  // Whether two batch rows' tokens overlap.
+  __device__ __forceinline__ bool same_tokens(int64_t b0, int64_t b1, const int32_t* start, int len) const {
+    if (seqs[b0] != seqs[b1]) return false;
+    if (start == nullptr) return true;
+    const int64_t apart = static_cast<int64_t>(start[b0]) - start[b1];
+    return apart < len && -apart < len;
+  }
   // Page that holds position `at` of batch row b and may be written; -1, with
   // a report, where there is none.
   __device__ __forceinline__ int64_t page_of(int64_t b, int64_t at) const {

@@ -191,7 +191,15 @@ __global__ void __launch_bounds__(R_MAX_THREADS) rotary_kernel(const __grid_cons
         c[tok * cs_tok] = turn_of(pos, inv, a.factor, a.inverse);
       }
   }
-  __syncthreads();
+  bool twice = false;      // an earlier batch row writes tokens of this row's: its own are not written
+  if (a.any_paged) {
+    int clash = 0;
+    for (int64_t other = tid; other < b; other += threads) clash |= a.slots.same_tokens(other, b, a.start, a.len);
+    twice = __syncthreads_or(clash);
+    if (twice && tid == 0) report(a.slots.status, MRSA_PAGE_BAD_SEQUENCE);
+  } else {
+    __syncthreads();
+  }
   int slot = 0;
   for (int t = tok0; t < nt; t += a.side) {
     Vec xa, xb;
@@ -223,7 +231,7 @@ __global__ void __launch_bounds__(R_MAX_THREADS) rotary_kernel(const __grid_cons
       dst += t * yt;
     } else {
       const int64_t page = dst_page[t];
-      if (page < 0) continue;
+      if (page < 0 || twice) continue;
       dst += page * yb + dst_slot[t] * yt;
     }
     *reinterpret_cast<Vec*>(dst) = xa;

@@ -92,7 +92,8 @@ def paged_append(k_pages, v_pages, table, lengths, seqs, k, v, *, q=None, positi
     :func:`rotary_embedding`, at ``position_ids`` (None: the cache
     positions).  Returns q, turned, or None without one.  A token outside its
     sequence, or (with ``refcount``) on a page that several sequences hold, is
-    not written, and ``status`` says so.  Forward only: it raises under
+    not written, nor is a row of the batch that names tokens which an earlier
+    row of it writes; ``status`` says so.  Forward only: it raises under
     autograd rather than return a q without its gradient."""
     return _lib.ext().append(k_pages, v_pages, table, lengths, seqs, k, v, q, position_ids, inv_freq, attention_factor,
                              layout, start, refcount, status)

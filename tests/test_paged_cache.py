@@ -393,3 +393,50 @@ def test_growth_past_any_whole_number_is_too_long(mrsa, cuda_device, tokens):
     cache.extend(cache.seqs(0), 88)
     cache.check()
     assert cache.lengths.tolist() == [128, 40, 0]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d,dtype", [(64, torch.bfloat16), (80, torch.float16), (10, torch.float32)])
+def test_append_of_the_same_tokens_twice(mrsa, cuda_device, d, dtype):
+    """The first row of a batch that writes a token is carried out, a later one is not and is reported."""
+    dev = cuda_device
+    rows, l = 300, 3
+    cache = mrsa.PagedKVCache(1, rows, 2, d, sequences=rows, max_len=16, page_size=16, dtype=dtype, device=dev)
+    cache.extend(torch.arange(rows, dtype=torch.int32, device=dev), 12)
+    g = torch.Generator(device=dev).manual_seed(1)
+    x = torch.randn(rows, l, 6, d, device=dev, generator=g).to(dtype)
+    q, k, v = x.split([2, 2, 2], 2)
+
+    def call(seqs, start=None):
+        cache.pool.zero_()
+        n = len(seqs)
+        y = cache.append(0, cache.seqs(*seqs), k[:n], v[:n], q=q[:n], start=None if start is None else cache.seqs(*start))
+        assert torch.equal(y, q[:n])                       # no frequencies: q as it is
+        want = torch.zeros_like(cache.pool)
+        done = []
+        for i, s in enumerate(seqs):
+            at = start[i] if start is not None else 12 - l
+            if any(s == s2 and abs(at - at2) < l for s2, at2 in done):
+                done.append((s, at))
+                continue
+            done.append((s, at))
+            page = cache.table[s, 0]
+            want[0, 0, page, at:at + l], want[0, 1, page, at:at + l] = k[i], v[i]
+        assert torch.equal(cache.pool, want)
+
+    def twice():
+        with pytest.raises(ValueError, match="twice"):
+            cache.check()
+
+    call([4, 2, 4]), twice()
+    call([7, 7]), twice()
+    order = list(range(rows))
+    call(order), cache.check()
+    order[299] = 0
+    call(order), twice()
+    order[150] = 149
+    call(order), twice()
+    call([5, 5, 6], [0, 3, 0]), cache.check()              # neighbouring ranges of one sequence
+    call([5, 5, 6], [0, 2, 2]), twice()
+    call([5, 6, 5], [4, 2, 2]), twice()
+    call([5, 5, 5, 5], [0, 9, 3, 6]), cache.check()
