@@ -455,7 +455,8 @@ enum {
   MRSA_PAGE_NO_PAGES = 2,      /* the pool has not enough free pages */
   MRSA_PAGE_TOO_LONG = 4,      /* a sequence would outgrow its table row, or its length was negative */
   MRSA_PAGE_OUTSIDE = 8,       /* a token outside its sequence, or a page number out of range */
-  MRSA_PAGE_SHARED = 16        /* a write to a page that several sequences hold */
+  MRSA_PAGE_SHARED = 16,       /* a write to a page that several sequences hold */
+  MRSA_PAGE_CLASH = 32         /* a page copied to twice, or copied to and from, in one call */
 };
 #define MRSA_PAGE_MAX_SEQS 1024   /* sequences per call of the page operators */
 
@@ -528,9 +529,16 @@ int mrsa_page_compact(const mrsa_page_table* t, const mrsa_page_pool* pool, cons
                       int64_t n, void* workspace, size_t ws_bytes, mrsa_stream_t stream);
 
 /* Page src[i] copied to page dst[i] in every plane (i < n); a page number out
- * of range is reported and skipped.  dst are distinct and none is a src. */
+ * of range is reported and skipped, a page copied to itself stays.  dst are
+ * distinct and none is a src. */
 int mrsa_page_copy(const mrsa_page_table* t, const mrsa_page_pool* pool, const int32_t* src, const int32_t* dst,
                    int64_t n, mrsa_stream_t stream);
+
+/* The same where that is not known of dst: if it does not hold, that is
+ * reported (MRSA_PAGE_CLASH) and nothing is copied. */
+size_t mrsa_page_copy_workspace(const mrsa_page_table* t);
+int mrsa_page_copy_checked(const mrsa_page_table* t, const mrsa_page_pool* pool, const int32_t* src,
+                           const int32_t* dst, int64_t n, void* workspace, size_t ws_bytes, mrsa_stream_t stream);
 
 typedef struct {
   const void* q;              /* [batch, len, q_heads, head_dim] */

@@ -88,6 +88,8 @@ _SIGS = {
     "mrsa_page_fork": [_vp, _vp, _vp, _vp, _vp, _i64, _vp, _sz, _vp],
     "mrsa_page_compact": [_vp, _vp, _vp, _vp, _i64, _vp, _sz, _vp],
     "mrsa_page_copy": [_vp, _vp, _vp, _vp, _i64, _vp],
+    "mrsa_page_copy_workspace": [_vp],
+    "mrsa_page_copy_checked": [_vp, _vp, _vp, _vp, _i64, _vp, _sz, _vp],
     "mrsa_paged_attention_workspace": [_vp],
     "mrsa_paged_attention": [_vp, _vp, _vp, _sz, _vp],
     "mrsa_device_error_flags": [_int],
@@ -100,6 +102,7 @@ _RESTYPE = {"mrsa_strerror": C.c_char_p, "mrsa_last_error": C.c_char_p, "mrsa_ro
             "mrsa_route_topk_workspace_size": _sz, "mrsa_selected_token_attention_smem": _sz,
             "mrsa_selected_attention_backward_workspace": _sz, "mrsa_route_scores_backward_workspace": _sz,
             "mrsa_local_attention_backward_workspace": _sz, "mrsa_page_workspace": _sz,
+            "mrsa_page_copy_workspace": _sz,
             "mrsa_paged_attention_workspace": _sz}
 
 EXPORTED = tuple(_SIGS)

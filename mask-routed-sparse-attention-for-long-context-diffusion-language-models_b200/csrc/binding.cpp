@@ -396,8 +396,10 @@ PyObject* page_copy(PyObject*, PyObject* const* o, Py_ssize_t n) {
     // a copy reads no table: one row of one page stands for it
     const mrsa_page_table t = page_table(src.slice(0, 0, 1).view({1, 1}), src.slice(0, 0, 1), Tensor(),
                                          tensor(o[3], "status"), pool.size(2), pool.size(3));
-    if (!finish(mrsa_page_copy(&t, &p, in<int32_t>(src), in<int32_t>(dst), src.size(0), stream_of(pool)),
-                "mrsa_page_copy"))
+    const size_t size = src.size(0) > 1 ? mrsa_page_copy_workspace(&t) : 0;
+    const Tensor ws = bytes_on(pool, size);
+    if (!finish(mrsa_page_copy_checked(&t, &p, in<int32_t>(src), in<int32_t>(dst), src.size(0), ws.mutable_data_ptr(),
+                                       size, stream_of(pool)), "mrsa_page_copy"))
       return nullptr;
   }
   Py_RETURN_NONE;

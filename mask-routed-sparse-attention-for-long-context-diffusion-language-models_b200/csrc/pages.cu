@@ -437,6 +437,7 @@ __global__ void __launch_bounds__(M_THREADS) page_copy_kernel(const __grid_const
       if (threadIdx.x == 0) report(a.status, MRSA_PAGE_OUTSIDE);
       continue;
     }
+    if (from == to) continue;
     char* base = static_cast<char*>(a.pool.data) + (plane >> 1) * a.pool.layer_stride + (plane & 1) * a.pool.kv_stride;
     const uint4* x = reinterpret_cast<const uint4*>(base + from * a.pool.page_stride);
     uint4* y = reinterpret_cast<uint4*>(base + to * a.pool.page_stride);
@@ -448,6 +449,37 @@ __global__ void __launch_bounds__(M_THREADS) page_copy_kernel(const __grid_const
 #pragma unroll
     for (int k = 0; k < M_UNROLL; ++k)
       if (v0 + k * M_THREADS < vecs) y[v0 + k * M_THREADS] = v[k];
+  }
+}
+
+// Whether a call's copies are independent: no page is copied to twice, or copied
+// to and from (a page copied to itself is copied to).  `mark` [pages] holds, for the
+// pages that the call names, 1 where one is a source, plus 2 for each copy to it.
+// One CTA: its barriers separate the steps.
+__global__ void __launch_bounds__(P_THREADS, 1) page_copy_check_kernel(const __grid_constant__ MoveArgs a, int32_t* head,
+                                                                       int32_t* mark) {
+  chain_wait();
+  chain_next();
+  auto inside = [&](int i) {     // a copy of a page out of range is not carried out
+    const int from = a.src[i], to = a.dst[i];
+    return from >= 0 && from < a.pages && to >= 0 && to < a.pages;
+  };
+  for (int i = threadIdx.x; i < a.count; i += P_THREADS)
+    if (inside(i)) mark[a.src[i]] = mark[a.dst[i]] = 0;
+  __syncthreads();
+  int clash = 0;
+  for (int i = threadIdx.x; i < a.count; i += P_THREADS)
+    if (inside(i)) {
+      if (a.src[i] != a.dst[i]) atomicOr(mark + a.src[i], 1);
+      clash |= atomicAdd(mark + a.dst[i], 2) >= 2;
+    }
+  __syncthreads();
+  for (int i = threadIdx.x; i < a.count; i += P_THREADS)
+    if (inside(i) && a.src[i] != a.dst[i]) clash |= __ldcg(mark + a.dst[i]) & 1;
+  clash = __syncthreads_or(clash);
+  if (threadIdx.x == 0) {
+    *head = clash ? 0 : a.count;
+    if (clash) report(a.status, MRSA_PAGE_CLASH);
   }
 }
 
@@ -635,18 +667,52 @@ extern "C" int mrsa_page_compact(const mrsa_page_table* t, const mrsa_page_pool*
   return launch_move(page_gather_kernel, m, most_new(t, n), static_cast<cudaStream_t>(stream));
 }
 
-extern "C" int mrsa_page_copy(const mrsa_page_table* t, const mrsa_page_pool* pool, const int32_t* src,
-                              const int32_t* dst, int64_t n, mrsa_stream_t stream) {
+namespace {
+
+int check_copy(const mrsa_page_table* t, const mrsa_page_pool* pool, const int32_t* src, const int32_t* dst, int64_t n) {
   if (t == nullptr || pool == nullptr) return MRSA_ERR_NULL;
   if (int rc = check_page_table(t)) return rc;
   if (int rc = check_pool(t, pool)) return rc;
   if (n < 0 || n > t->pages) return MRSA_ERR_SHAPE;
-  if (n == 0) return MRSA_OK;
-  if (!src || !dst) return MRSA_ERR_NULL;
-  mrsa::DeviceScope device_scope(t->table);
+  return n > 0 && (!src || !dst) ? MRSA_ERR_NULL : MRSA_OK;
+}
+
+MoveArgs copy_args(const mrsa_page_table* t, const mrsa_page_pool* pool, const int32_t* src, const int32_t* dst,
+                   int64_t n) {
   MoveArgs m = move_args(t, pool);
   m.count = static_cast<int>(n);
   m.dst = dst;
   m.src = src;
+  return m;
+}
+
+}  // namespace
+
+extern "C" int mrsa_page_copy(const mrsa_page_table* t, const mrsa_page_pool* pool, const int32_t* src,
+                              const int32_t* dst, int64_t n, mrsa_stream_t stream) {
+  if (int rc = check_copy(t, pool, src, dst, n)) return rc;
+  if (n == 0) return MRSA_OK;
+  mrsa::DeviceScope device_scope(t->table);
+  return launch_move(page_copy_kernel, copy_args(t, pool, src, dst, n), n, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" size_t mrsa_page_copy_workspace(const mrsa_page_table* t) {
+  return t == nullptr || t->pages < 1 ? 0 : static_cast<size_t>(64 + t->pages) * 4;
+}
+
+extern "C" int mrsa_page_copy_checked(const mrsa_page_table* t, const mrsa_page_pool* pool, const int32_t* src,
+                                      const int32_t* dst, int64_t n, void* workspace, size_t ws_bytes,
+                                      mrsa_stream_t stream) {
+  if (int rc = check_copy(t, pool, src, dst, n)) return rc;
+  if (n < 2) return mrsa_page_copy(t, pool, src, dst, n, stream);       // one copy cannot clash
+  if (!workspace || ws_bytes < mrsa_page_copy_workspace(t)) return MRSA_ERR_WORKSPACE;
+  if (reinterpret_cast<uintptr_t>(workspace) & 15) return MRSA_ERR_ALIGN;
+  mrsa::DeviceScope device_scope(t->table);
+  MoveArgs m = copy_args(t, pool, src, dst, n);
+  int32_t* head = static_cast<int32_t*>(workspace);
+  if (int rc = launch_chained(page_copy_check_kernel, dim3(1), P_THREADS, 0, static_cast<cudaStream_t>(stream), m, head,
+                              head + 64))
+    return rc;
+  m.head = head;
   return launch_move(page_copy_kernel, m, n, static_cast<cudaStream_t>(stream));
 }

@@ -31,12 +31,13 @@ from . import _lib
 
 PAGE_SIZES = (16, 32, 64, 128, 256)
 
-BAD_SEQUENCE, NO_PAGES, TOO_LONG, OUTSIDE, SHARED = 1, 2, 4, 8, 16
+BAD_SEQUENCE, NO_PAGES, TOO_LONG, OUTSIDE, SHARED, CLASH = 1, 2, 4, 8, 16, 32
 _STATUS = {BAD_SEQUENCE: "a sequence number is out of range or was given twice",
            NO_PAGES: "the pool has not enough free pages",
            TOO_LONG: "a sequence would outgrow its row of the table",
            OUTSIDE: "a token or a page number lies outside its sequence or the pool",
-           SHARED: "a write to a page that several sequences hold"}
+           SHARED: "a write to a page that several sequences hold",
+           CLASH: "a page is copied to twice, or copied to and from, in one call"}
 
 
 def page_free(table, lengths, refcount, seqs, *, status=None) -> None:
@@ -76,7 +77,9 @@ def page_compact(pool, table, lengths, refcount, seqs, keep, *, status=None) -> 
 
 def page_copy(pool, src, dst, *, status=None) -> None:
     """Page ``src[i]`` copied to page ``dst[i]`` (int32 ``[n]``) in every
-    layer; a page number out of range is skipped and ``status`` says so."""
+    layer; a page number out of range is skipped and ``status`` says so.  If a
+    page is copied to twice, or both copied from and to (a page copied to
+    itself stays as it is), nothing is copied and ``status`` says so."""
     _lib.ext().copy(pool, src, dst, status)
 
 

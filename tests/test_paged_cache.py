@@ -440,3 +440,55 @@ def test_append_of_the_same_tokens_twice(mrsa, cuda_device, d, dtype):
     call([5, 5, 6], [0, 2, 2]), twice()
     call([5, 6, 5], [4, 2, 2]), twice()
     call([5, 5, 5, 5], [0, 9, 3, 6]), cache.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("layout", ["tokens", "heads"])
+def test_copies_that_depend_on_each_other(mrsa, cuda_device, layout):
+    """All copies of a call are carried out, or none where two of them clash."""
+    dev = cuda_device
+    pages = 5000
+    pool = torch.randint(-99, 99, (2, 2, pages, 16, 2, 16), device=dev).bfloat16()
+    if layout == "heads":
+        pool = pool.transpose(3, 4).contiguous().transpose(3, 4)
+    status = torch.zeros(1, dtype=torch.int32, device=dev)
+
+    def copy(src, dst, says):
+        want = pool.clone()
+        if not says & 32:
+            ok = [(s, d) for s, d in zip(src, dst) if 0 <= s < pages and 0 <= d < pages]
+            want[:, :, [d for _, d in ok]] = pool[:, :, [s for s, _ in ok]]
+        status.zero_()
+        t = [torch.tensor(x, dtype=torch.int32, device=dev) for x in (src, dst)]
+        mrsa.page_copy(pool, *t, status=status)
+        assert status.item() == says and torch.equal(pool, want)
+
+    copy([1, 2], [3, 3], 32)                       # a target twice
+    copy([1, 3], [3, 4], 32)                       # a target that is a source
+    copy([1, 3], [3, 1], 32)                       # an exchange
+    copy([1, 3, 9], [3, 5000, 9], 8)               # out of range, and a page onto itself: neither clashes
+    copy([3, 4], [3, 3], 32)                       # a page that stays, and a copy to it
+    copy([3, 3], [3, 4], 0)
+    copy([7], [7], 0)
+    copy([4, 4, 4], [5, 6, 7], 0)
+    half = random.Random(1).sample(range(pages), pages)
+    copy(half[:2500], half[2500:], 0)
+    copy(half[:2500], half[2500:-1] + [half[2499]], 0)      # the last one onto itself
+    copy(half[:2500], half[2500:-1] + [half[2498]], 32)
+    copy(half[:2500], half[2500:-1] + [half[2500]], 32)
+
+
+def test_checked_copy_argument_codes(mrsa):
+    lib, L = mrsa._lib.load(), mrsa._lib
+    P = 4096
+    table = L.PAGE_TABLE.pack(P, P, P, 0, 4, 8, 100, 64)
+    pool = L.PAGE_POOL.pack(P, 1, 2 << 20, 1 << 20, 64 * 512, 512, 256, 2, 256)
+    size = lib.mrsa_page_copy_workspace(table)
+    assert size >= 400 and lib.mrsa_page_copy_workspace(None) == 0
+    assert lib.mrsa_page_copy_checked(None, pool, P, P, 2, P, size, None) == L.ERR_NULL
+    assert lib.mrsa_page_copy_checked(table, pool, P, None, 2, P, size, None) == L.ERR_NULL
+    assert lib.mrsa_page_copy_checked(table, pool, P, P, 101, P, size, None) == L.ERR_SHAPE
+    assert lib.mrsa_page_copy_checked(table, pool, P, P, 2, P, size - 1, None) == L.ERR_WORKSPACE
+    assert lib.mrsa_page_copy_checked(table, pool, P, P, 2, None, size, None) == L.ERR_WORKSPACE
+    assert lib.mrsa_page_copy_checked(table, pool, P, P, 2, P + 4, size, None) == L.ERR_ALIGN
+    assert lib.mrsa_page_copy_checked(table, pool, P, P, 0, None, 0, None) == 0
