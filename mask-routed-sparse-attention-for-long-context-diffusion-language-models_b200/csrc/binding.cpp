@@ -9,6 +9,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -257,9 +258,15 @@ mrsa_page_table page_table(const Tensor& table, const Tensor& lengths, const Ten
   return t;
 }
 
+// Memory that is written must not stand for several elements (an expanded tensor).
+void check_written(const Tensor& x, const char* name) {
+  TORCH_CHECK_VALUE(at::has_internal_overlap(x) != at::MemOverlap::Yes, name, " is written: its elements must not share memory");
+}
+
 mrsa_page_pool page_pool(const Tensor& pool, const Tensor& like) {
   TORCH_CHECK_VALUE(pool.defined() && pool.dim() == 6 && pool.size(1) == 2 && pool.device() == like.device(),
                     "pool must be [layers, 2, pages, page_size, kv_heads, D] on the table's device");
+  check_written(pool, "pool");
   const auto s = pool.strides();
   const int64_t ps = pool.size(3), heads = pool.size(4), d = pool.size(5), e = pool.element_size();
   TORCH_CHECK_VALUE(s[5] == 1 && ((s[3] == heads * d && s[4] == d) || (s[3] == d && s[4] == ps * d)),
@@ -440,6 +447,10 @@ PyObject* append(PyObject*, PyObject* const* o, Py_ssize_t n) {
   check_like(v, "v", k);
   TORCH_CHECK_VALUE(v.size(2) == k.size(2), "v must have k's shape");
   check_pages(kp, vp);
+  check_written(kp, "k_pages");
+  check_written(vp, "v_pages");
+  TORCH_CHECK_VALUE(kp.const_data_ptr() != vp.const_data_ptr() || kp.numel() == 0,
+                    "k_pages and v_pages are written: they must not be the same memory");
   a.dtype = type_of(k);
   TORCH_CHECK_VALUE(a.dtype >= 0 && kp.scalar_type() == k.scalar_type() && kp.device() == k.device(),
                     "k, v and the pages must share a type (BF16, FP16 or FP32) and a device");

@@ -492,3 +492,30 @@ def test_checked_copy_argument_codes(mrsa):
     assert lib.mrsa_page_copy_checked(table, pool, P, P, 2, None, size, None) == L.ERR_WORKSPACE
     assert lib.mrsa_page_copy_checked(table, pool, P, P, 2, P + 4, size, None) == L.ERR_ALIGN
     assert lib.mrsa_page_copy_checked(table, pool, P, P, 0, None, 0, None) == 0
+
+
+@pytest.mark.gpu
+def test_pages_that_share_memory_are_refused(mrsa, cuda_device):
+    dev = cuda_device
+    cache = mrsa.PagedKVCache(2, 6, 2, 64, sequences=4, max_len=64, page_size=16, device=dev)
+    s, pool = cache.seqs(0), cache.pool
+    state = cache.table, cache.lengths
+    cache.extend(s, 1)
+    k = torch.zeros(1, 1, 2, 64, dtype=torch.bfloat16, device=dev)
+    for dim, one in ((0, pool[:1]), (1, pool[:, :1]), (2, pool[:, :, :1]), (3, pool[:, :, :, :1])):
+        same = one.expand(*[-1 if i != dim else pool.shape[dim] for i in range(6)])
+        for bad in (lambda: mrsa.page_copy(same, s, cache.seqs(1)),
+                    lambda: mrsa.page_fork(same, *state, cache.refcount, s, cache.seqs(1)),
+                    lambda: mrsa.page_compact(same, *state, cache.refcount, s, torch.ones(1, 64, dtype=torch.bool, device=dev))):
+            with pytest.raises(ValueError, match="share memory"):
+                bad()
+    kp, vp = pool[0]
+    for pages in ((kp[:1].expand(6, -1, -1, -1), vp), (kp, vp[:, :1].expand(-1, 16, -1, -1)),
+                  (kp, vp[:, :, :1].expand(-1, -1, 2, -1))):
+        with pytest.raises(ValueError, match="share memory"):
+            mrsa.paged_append(*pages, *state, s, k, k)
+    with pytest.raises(ValueError, match="same memory"):
+        mrsa.paged_append(kp, kp, *state, s, k, k)
+    mrsa.paged_append(kp[:, :, ::2], vp[:, :, 1::2], *state, s, k[:, :, :1], k[:, :, :1])     # every second head: apart
+    mrsa.paged_append(kp, vp, *state, s, k.expand(1, 1, 2, 64), k[:, :, :1].expand(1, 1, 2, 64))
+    cache.check()
