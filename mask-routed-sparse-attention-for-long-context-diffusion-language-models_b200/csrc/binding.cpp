@@ -44,6 +44,12 @@ bool finish(int rc, const char* name) {
   return false;
 }
 
+bool truth(PyObject* o) {
+  const int r = PyObject_IsTrue(o);
+  if (r < 0) throw python_error();
+  return r != 0;
+}
+
 void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
 
 // No operator here has a forward-mode derivative: a tangent is an error, not lost.
@@ -532,7 +538,7 @@ PyObject* attend(PyObject*, PyObject* const* o, Py_ssize_t n) {
   TORCH_CHECK_VALUE(table.device() == q.device(), "the table must be on the tensors' device");
   const Tensor seqs = ints(tensor(o[5], "seqs"), "seqs", 1, table);
   TORCH_CHECK_VALUE(seqs.size(0) == b, "seqs must name one sequence per batch row");
-  a.causal = PyObject_IsTrue(o[6]);
+  a.causal = truth(o[6]);
   double scale = d == 64 ? 0.125 : 0.08838834764831845;
   if (o[8] != Py_None) {
     scale = PyFloat_AsDouble(o[8]);
@@ -551,7 +557,7 @@ PyObject* attend(PyObject*, PyObject* const* o, Py_ssize_t n) {
       (reinterpret_cast<uintptr_t>(q.const_data_ptr()) & 15))
     q = aligned(q);
   Tensor out = heads_like(q), lse;
-  if (PyObject_IsTrue(o[9])) {
+  if (truth(o[9])) {
     lse = at::empty({b, l, hq}, q.options().dtype(at::kFloat));
     a.lse = lse.mutable_data_ptr<float>();
   }

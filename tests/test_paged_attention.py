@@ -327,3 +327,14 @@ def test_few_short_sequences(mrsa, cuda_device, dtype, hq, hkv, d, page, lens):
     valid[0] = False                          # a row that sees nothing
     valid[-1, :130] = False                   # leading shares that see nothing
     compare(mrsa, cache, seqs, q, valid=valid)
+
+
+@pytest.mark.gpu
+def test_flags_that_are_no_truth_value(mrsa, cuda_device):
+    cache = mrsa.PagedKVCache(1, 6, 2, 64, sequences=4, max_len=64, page_size=16, device=cuda_device)
+    q = torch.zeros(1, 1, 4, 64, dtype=torch.bfloat16, device=cuda_device)
+    two = torch.ones(2, dtype=torch.bool)
+    for kw in (dict(causal=two), dict(return_lse=two)):
+        with pytest.raises(RuntimeError, match="ambiguous"):
+            cache.attend(0, cache.seqs(0), q, **kw)
+    assert cache.attend(0, cache.seqs(0), q, causal=1, return_lse=0).shape == q.shape
