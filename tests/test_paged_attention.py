@@ -338,3 +338,113 @@ def test_flags_that_are_no_truth_value(mrsa, cuda_device):
         with pytest.raises(RuntimeError, match="ambiguous"):
             cache.attend(0, cache.seqs(0), q, **kw)
     assert cache.attend(0, cache.seqs(0), q, causal=1, return_lse=0).shape == q.shape
+
+
+def tight(got, lse, q, want, mass, wlse, weight, few):
+    """Bounds for what the kernels promise, derived before any run.  The scores' fp32 sums move a probability by
+    1e-5 of itself, in the product and in the sum that divides it; few rows: P in two 16-bit parts leaves 2^-17 of it
+    (fp16: and, below its subnormals, 2^-25 of the maximum, with a sum of at least one), so 3e-5 of sum p |v| beside
+    the output's own rounding, element by element.  Many rows: P is rounded once, independently per key, so the
+    errors add in squares, those of one batch row's thousands of outputs to an rms of c of the root of o^2 + sum p^2 v^2.
+    A rounding is off by u / m times a number uniform in [-1, 1], with a mantissa m whose logarithm is uniform in [1, 2):
+    c = u / sqrt(3) sqrt(E[m^-2]) = 0.7355 u / sqrt(3); a factor of 1.2 for chance."""
+    u = UNIT[q.dtype]
+    err = (got.double() - want).abs()
+    if few:
+        bound = u * want.abs() + 3e-5 * mass + (2.0 ** -25 * (weight[1] + 1) if q.dtype == torch.float16 else 0.0)
+        assert (err <= bound).all(), (err / bound.clamp_min(1e-30)).max().item()
+    else:
+        each = (1, 2, 3)
+        rms = 0.7355 * u / math.sqrt(3) * (want.pow(2) + weight[0]).mean(each).sqrt() + 3e-5 * mass.mean(each)
+        off = err.pow(2).mean(each).sqrt()
+        assert (off <= 1.2 * rms).all(), (off / rms).tolist()
+    seen = wlse > -math.inf
+    assert ((lse.double() - wlse)[seen].abs() <= 3e-5 + 1e-6 * wlse[seen].abs()).all()
+
+
+def weights(cache, seqs, q, valid=None):
+    """Sums over the keys of (p v)^2 and of |v|, in 64 bits, [B, L, Hq, D]."""
+    b, l, hq, d = q.shape
+    page, hkv = cache.page_size, cache.pool.shape[4]
+    squares = torch.zeros(b, l, hq, d, dtype=torch.float64, device=q.device)
+    plain = squares.clone()
+    for i, s in enumerate(seqs.tolist()):
+        at = torch.arange(cache.lengths[s].item(), device=q.device)
+        use = at if valid is None else at[valid[i, :at.numel()]]
+        if use.numel():
+            k, v = cache.pool[0, :, cache.table[s][use // page].long(), use % page].double()
+            p = (torch.einsum("lhgd,nhd->lhgn", q[i].double().view(l, hkv, -1, d), k) * d ** -0.5).softmax(-1)
+            squares[i] = torch.einsum("lhgn,nhd->lhgd", p * p, v * v).reshape(l, hq, d)
+            plain[i] = v.abs().sum(0).repeat_interleave(hq // hkv, 0)
+    return squares, plain
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lens", [[17, 64, 190, 700, 1, 333], [500], [9000, 100]])
+@pytest.mark.parametrize("l,hq,hkv,d", [(1, 28, 4, 128), (2, 14, 2, 64), (1, 16, 1, 128), (4, 28, 4, 128), (32, 14, 2, 128),
+                                        (40, 16, 2, 64)])
+def test_no_more_than_the_stated_rounding(mrsa, cuda_device, l, hq, hkv, d, lens, dtype):
+    cache, g = filled(mrsa, cuda_device, lens, hkv, d, 64, dtype, seed=l)
+    seqs = torch.arange(len(lens), dtype=torch.int32, device=cuda_device)
+    q = queries(cuda_device, g, len(lens), l, hq, d, dtype)
+    valid = torch.rand(len(lens), cache.table.shape[1] * 64, device=cuda_device, generator=g) < 0.7
+    for mask in (None, valid):
+        got, lse = cache.attend(0, seqs, q, key_valid=mask, return_lse=True)
+        cache.check()
+        tight(got, lse, q, *reference(cache, seqs, q, False, mask, d ** -0.5), weights(cache, seqs, q, mask),
+              l * (hq // hkv) <= 16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("l,page", [(1, 64), (2, 16), (4, 128), (32, 64), (45, 32)])
+def test_every_tile_has_its_own_values(mrsa, cuda_device, l, page, dtype):
+    """Each query looks at one 64-key tile of a long sequence, whose keys and values are that tile's alone: a tile
+    read, weighed or joined in another's place is off by all of the output."""
+    dev = cuda_device
+    lens = [40000, 6401]
+    cache, g = filled(mrsa, dev, lens, 2, 128, page, dtype, seed=l)
+    tiles = [-(-n // 64) for n in lens]
+    code = torch.randint(0, 2, (sum(tiles), 2, 128), device=dev, generator=g).to(dtype) * 2 - 1
+    value = torch.randn(sum(tiles), 2, 128, device=dev, generator=g).to(dtype)
+    for s, n in enumerate(lens):
+        at = torch.arange(n, device=dev)
+        tile = at // 64 + sum(tiles[:s])
+        where = cache.table[s][at // page].long()
+        cache.pool[0, 0, where, at % page], cache.pool[0, 1, where, at % page] = code[tile], value[tile]
+    seqs = torch.tensor([0, 1], dtype=torch.int32, device=dev)
+    for turn in range(4 if l > 2 else 12):
+        q = torch.empty(2, l, 14, 128, dtype=dtype, device=dev)
+        want = torch.empty_like(q, dtype=torch.float64)
+        for s in range(2):
+            pick = sum(tiles[:s]) + torch.randint(0, tiles[s], (l, 2, 7), device=dev, generator=g)
+            pick[0, :, 0], pick[0, :, 1] = sum(tiles[:s]), sum(tiles[:s + 1]) - 1        # the first and the last
+            heads = torch.arange(2, device=dev)[None, :, None]
+            q[s] = (2 * code[pick, heads]).view(l, 14, 128)
+            want[s] = value[pick, heads].double().view(l, 14, 128)
+        got, lse = compare(mrsa, cache, seqs, q)
+        # the tile that is looked at has a score of 22.6, the others' are normal around 0 with a deviation of 2
+        assert ((got.double() - want).abs() <= 3 * UNIT[dtype] * want.abs() + 1e-3).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("width", [4, 40])
+@pytest.mark.parametrize("l", [1, 2, 4, 32])
+def test_pages_out_of_range_read_as_masked(mrsa, cuda_device, l, width):
+    cache, g = filled(mrsa, cuda_device, [100, 200], 4, 128, 64, torch.bfloat16)
+    cache.table = torch.cat((cache.table, cache.table.new_full((2, width - 4), -1)), 1).contiguous()
+    q = queries(cuda_device, g, 1, l, 28, 128, torch.bfloat16)
+    seqs, page = cache.seqs(1), cache.table[1, 2].clone()
+    valid = torch.ones(1, width * 64, dtype=torch.bool, device=cuda_device)
+    valid[0, 128:192] = False
+    want, mass, wlse = reference(cache, seqs, q, False, valid, 128 ** -0.5)
+    for bad in (-1, 10 ** 6):
+        cache.table[1, 2] = bad
+        o, lse = cache.attend(0, seqs, q, return_lse=True)
+        with pytest.raises(ValueError, match="lies outside"):
+            cache.check()
+        cache.table[1, 2] = page
+        u = UNIT[torch.bfloat16]
+        assert ((o.double() - want).abs() <= u * want.abs() + (u + 1e-5) * mass).all()
+        assert ((lse.double() - wlse).abs() <= 3e-5 + 1e-6 * wlse.abs()).all()
