@@ -194,7 +194,9 @@ __global__ void __launch_bounds__(R_MAX_THREADS) rotary_kernel(const __grid_cons
   bool twice = false;      // an earlier batch row writes tokens of this row's: its own are not written
   if (a.any_paged) {
     int clash = 0;
-    for (int64_t other = tid; other < b; other += threads) clash |= a.slots.same_tokens(other, b, a.start, a.len);
+    // (from the last thread: the first ones look up the slots meanwhile)
+    for (int64_t other = threads - 1 - tid; other < b; other += threads)
+      clash |= a.slots.same_tokens(other, b, a.start, a.len);
     twice = __syncthreads_or(clash);
     if (twice && tid == 0) report(a.slots.status, MRSA_PAGE_BAD_SEQUENCE);
   } else {
