@@ -3,7 +3,7 @@
 //
 // A decode step is a chain of launches of a few microseconds each.  Checked and
 // packed in Python, one such call took 11 to 15 us of host time, more than
-// its kernels; here it is about six.  One function per operator, with
+// its kernels; here it is five to ten.  One function per operator, with
 // positional arguments; the public functions with their defaults and
 // documentation are in rotary.py and paged_cache.py.
 #include <Python.h>

@@ -13,7 +13,9 @@
 //   O[128 x D]  += P . V_t                (UMMA M=128, N=D, A = P in TMEM)
 // P is rounded once to the type of V (8 or 11 bits; the sum of the
 // probabilities is of the unrounded ones), written over its own S and read
-// from there.  Warps 0-3 and 4-7: softmax, Q tile and epilogue of row tiles 0
+// from there: its rounding adds to the output's own, 1.4 times that error in
+// all.  A high and a low part, as for few rows, would be a second P.V, half as
+// much again of the 1024 cycles that a tile's products take.  Warps 0-3 and 4-7: softmax, Q tile and epilogue of row tiles 0
 // and 1; warp 8: K tiles and key masks, warp 11: V tiles, both by TMA, one box
 // per page part and 64 dims, straight from the pages the table names; warps 9
 // and 10: MMA issue.  Rings and buffers run on from one unit of the stretch to
@@ -409,7 +411,7 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
           const unsigned long long km = sm.kmask[slot_of(g, e)];
           if (km != ~0ull) {
             // (a minimum with +-inf from shared memory in place of the choice: 415 us for
-            // 377 at 37 x 32 tokens over 16384, masked)
+            // 385 at 37 x 32 tokens over 16384, masked)
             const uint32_t lo = static_cast<uint32_t>(km), hi = static_cast<uint32_t>(km >> 32);
 #pragma unroll
             for (int c = 0; c < 32; ++c) {

@@ -4,9 +4,8 @@
 // table rows) is one launch of one CTA, or for large tables of one cluster of
 // up to eight: its steps depend on one another across the whole table, and a
 // CTA's or a cluster's barrier separates them in a fraction of what another
-// launch costs.  The pages' bytes
-// are then moved by a second launch over all SMs, which reads from the
-// workspace what to copy.  The host never learns lengths or page numbers, so
+// launch costs.  The pages' bytes are then moved by a second launch over all
+// SMs, which reads from the workspace what to copy.  The host never learns lengths or page numbers, so
 // the calls can be queued, or captured in a graph, without waiting for the GPU.
 //
 // New pages are the lowest free ones in the order of the call's sequences and

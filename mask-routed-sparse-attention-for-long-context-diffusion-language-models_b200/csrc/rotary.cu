@@ -10,12 +10,13 @@
 //
 // Every byte is read and written once, so HBM bounds it (and, for a few
 // tokens, the launch).  A CTA takes a few tokens of one batch row (and a
-// part of a token's items, where it has more than threads); a thread keeps its place in a head (two 16-byte vectors that hold V whole pairs in
-// either layout) and goes from token to token, so what it does per token is
-// little more than the rotation.  Up to six of its tokens are under way at a
-// time as asynchronous copies into shared-memory slots of its own: as many in
-// registers would halve the warps that fit (16384 tokens of 28 + 4 heads: 78
-// us).  The tokens' angles (once per token and pair, not per head) and slots
+// part of a token's items, where it has more than threads); a thread keeps its
+// place in a head (two 16-byte vectors that hold V whole pairs in either
+// layout) and goes from token to token, so what it does per token is little
+// more than the rotation.  While it turns one, six more of its tokens are under
+// way as asynchronous copies into shared-memory slots of its own, seven in all:
+// as many in registers would halve the warps that fit (16384 tokens of 28 + 4
+// heads: 78 us for 45).  The tokens' angles (once per token and pair, not per head) and slots
 // are worked out meanwhile.  A turn count is reduced in fp64 (positions past
 // 1e5 would otherwise take sincosf's slow path): the fp32 angle over 2 pi,
 // minus its nearest whole number.
@@ -30,7 +31,7 @@ namespace {
 
 constexpr int R_THREADS = 256;      // per CTA, about: whole warps that share a token's items evenly
 constexpr int R_MAX_THREADS = 384;
-constexpr int R_AHEAD = 7;          // tokens a thread has in flight
+constexpr int R_AHEAD = 7;          // a thread's slots: the token that it turns, and six in flight
 constexpr int R_MAX_RUN = 16;       // tokens per CTA
 constexpr int R_MAX_PAIRS = 128;
 

@@ -6,7 +6,8 @@ numbers.  Candidates of one prompt hold its pages in common
 (:func:`page_compact`), and :func:`paged_append` rotates a step's q and k and
 puts k and v into their pages in one launch.  Every operator works on the
 device's own table: nothing waits for the GPU, and a call that cannot be
-carried out says so in a status word (:meth:`PagedKVCache.check` reads it).
+carried out says so in a status word (:meth:`PagedKVCache.check` reads it) and
+leaves the table as it was (a fork without pages leaves its targets empty).
 
 The operators take plain tensors, so that a server can keep its own
 bookkeeping next to them:
@@ -105,7 +106,8 @@ def paged_append(k_pages, v_pages, table, lengths, seqs, k, v, *, q=None, positi
 def paged_attention(q, k_pages, v_pages, table, lengths, seqs, *, causal: bool = False, key_valid=None,
                     scale: float | None = None, return_lse: bool = False, status=None):
     """Attention of ``q [B, L, Hq, D]`` (bf16 or fp16, D 64 or 128) over the
-    cached tokens of the sequences ``seqs`` ``[B]`` in one layer's pages.
+    cached tokens of the sequences ``seqs`` ``[B]`` in one layer's pages, which
+    hold the same type (fp32 pages can be appended to, but not attended to).
 
     The queries are a sequence's newest L tokens, whose keys and values the
     cache already holds: every query sees the whole sequence, as a block that
