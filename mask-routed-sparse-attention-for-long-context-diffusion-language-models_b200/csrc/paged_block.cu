@@ -378,6 +378,8 @@ __global__ void __launch_bounds__(B_THREADS, 1) paged_block_kernel(const __grid_
     if (tc::elect_one()) {
       tc::mma_commit(tc::smem_addr(&sm.drain[g]));
       tc::mbar_wait(tc::smem_addr(&sm.drain[g]), 0);
+      // the last Q tile, which is still in flight where the CTA gave up before it came
+      if (units > 0) tc::mbar_wait(tc::smem_addr(&sm.qfull[g]), (units - 1) & 1);
     }
     __syncwarp();
   } else {
