@@ -401,8 +401,8 @@ int mrsa_wait_selftest(int* result, int rounds, mrsa_stream_t stream);
  * bit 3 = mrsa_convert_bf16_to_f16 saturated a value; bit 4 = a CTA of the
  * selected-attention backward gave up on a wait (its gradients are then
  * incomplete); bit 5 = a GEMM CTA did; bit 6 = a CTA of the local-window
- * backward did; bit 7 = a CTA of mrsa_paged_attention did.  Synchronises the
- * current device; with clear != 0 also resets the mask.  Negative on a CUDA error.  Replaces the
+ * backward did; bit 7 = a CTA of mrsa_paged_attention did; bit 8 = one of
+ * mrsa_gemm_int8 did.  Synchronises the current device; with clear != 0 also resets the mask.  Negative on a CUDA error.  Replaces the
  * reference's host-side kernel-fallback reporting (dream_dllm_hils/attention.py:932-940). */
 int mrsa_device_error_flags(int clear);
 
@@ -569,6 +569,74 @@ size_t mrsa_paged_attention_workspace(const mrsa_paged_attention_args* a);
  * page number is reported in the status word and reads as no tokens. */
 int mrsa_paged_attention(const mrsa_paged_attention_args* a, const mrsa_page_table* t, void* workspace,
                          size_t ws_bytes, mrsa_stream_t stream);
+
+/* ------------------------------------------- norms, and layers in 8 bits */
+#define MRSA_NORM_MIN_EPS 1e-12f
+
+typedef struct {
+  const void* x;              /* [rows, dim] */
+  const void* residual;       /* [rows, dim] or NULL: h = x, and nothing is written to h */
+  const void* weight;         /* [dim] */
+  void* y;                    /* [rows, dim], contiguous, or NULL */
+  void* h;                    /* [rows, dim], contiguous: x + residual, rounded */
+  int8_t* q;                  /* [rows, dim], or NULL; one of y and q is given */
+  float* scale;               /* [rows], with q */
+  float* rstd;                /* [rows] for the gradient, or NULL; with y */
+  int64_t rows, dim;
+  int64_t x_stride, residual_stride, q_stride;   /* elements from row to row */
+  float eps;                  /* at least MRSA_NORM_MIN_EPS */
+  int32_t dtype;              /* of x, residual, weight, y and h: MRSA_BF16, MRSA_F16 or MRSA_F32 */
+} mrsa_norm_args;
+
+/* Norm with the residual's addition: h = x + residual, rounded to the type; v =
+ * h * weight / sqrt(mean(h^2) + eps) in fp32; y = v, rounded once, or v in 8 bits:
+ * scale = max|v| / 127 and q = the whole number nearest v / scale (either
+ * neighbour where fp32 does not tell).  A row of zeros has scale 0; a row with a
+ * NaN or an infinity has scale NaN and q 0. */
+int mrsa_add_rms_norm(const mrsa_norm_args* a, mrsa_stream_t stream);
+
+/* Rows of x in 8 bits, as there: scale = max|x| / 127, q = nearest(x / scale). */
+int mrsa_quantize_int8(const void* x, int64_t x_stride, int8_t* q, int64_t q_stride, float* scale, int64_t rows,
+                       int64_t dim, int dtype, mrsa_stream_t stream);
+
+typedef struct {
+  const void* grad_y;         /* [rows, dim] */
+  const void* grad_h;         /* [rows, dim] or NULL (zeros) */
+  const void* h;              /* [rows, dim] as the forward wrote it (x without a residual) */
+  const void* weight;         /* [dim] */
+  const float* rstd;          /* [rows] from the forward */
+  void* dx;                   /* [rows, dim], contiguous: the gradient of x and of the residual */
+  void* dweight;              /* [dim], or NULL: not wanted, and no workspace needed */
+  int64_t rows, dim;          /* rows >= 1 */
+  int64_t grad_y_stride, grad_h_stride, h_stride;
+  int32_t dtype;
+} mrsa_norm_backward_args;
+
+/* Gradient of mrsa_add_rms_norm (y form), every run the same bits. */
+int mrsa_add_rms_norm_backward(const mrsa_norm_backward_args* a, void* workspace, size_t ws_bytes,
+                               mrsa_stream_t stream);
+size_t mrsa_add_rms_norm_backward_workspace(int64_t rows, int64_t dim);
+
+#define MRSA_INT8_MAX_K 131071   /* 128 * 128 * K < 2^31 */
+
+typedef struct {
+  const int8_t* a;            /* [m, k], 16-byte aligned; rows a_stride bytes apart, a multiple of 16 */
+  const int8_t* b;            /* [n, k], 16-byte aligned; rows b_stride bytes apart, a multiple of 16 */
+  const float* a_scale;       /* [m] */
+  const float* b_scale;       /* [n] */
+  const void* bias;           /* [n] or NULL */
+  void* c;                    /* [m, n], contiguous (MRSA_GEMM_SWIGLU: [m, n / 2]) */
+  int64_t m, n, k, a_stride, b_stride;
+  int32_t dtype;              /* of c: MRSA_BF16, MRSA_F16 or MRSA_F32 */
+  int32_t bias_dtype;         /* the same choice */
+  int32_t epilogue;           /* MRSA_GEMM_PLAIN or MRSA_GEMM_SWIGLU (n % 256 == 0, no bias) */
+} mrsa_gemm_int8_args;
+
+/* C = A . B^T of signed 8-bit integers, summed exactly in 32 bits, then in fp32
+ * sum * a_scale[row] * b_scale[channel] + bias[channel], rounded once;
+ * MRSA_GEMM_SWIGLU: B's rows as in mrsa_gemm_bf16, C = silu(gate) * up.  Sets bit
+ * 8 of mrsa_device_error_flags if a CTA gave up on a bounded wait. */
+int mrsa_gemm_int8(const mrsa_gemm_int8_args* a, mrsa_stream_t stream);
 
 /* ---------------------------------------------------------------- layers */
 typedef struct {

@@ -92,6 +92,11 @@ _SIGS = {
     "mrsa_page_copy_checked": [_vp, _vp, _vp, _vp, _i64, _vp, _sz, _vp],
     "mrsa_paged_attention_workspace": [_vp],
     "mrsa_paged_attention": [_vp, _vp, _vp, _sz, _vp],
+    "mrsa_add_rms_norm": [_vp, _vp],
+    "mrsa_quantize_int8": [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _int, _vp],
+    "mrsa_add_rms_norm_backward": [_vp, _vp, _sz, _vp],
+    "mrsa_add_rms_norm_backward_workspace": [_i64, _i64],
+    "mrsa_gemm_int8": [_vp, _vp],
     "mrsa_device_error_flags": [_int],
     "mrsa_wait_selftest": [_vp, _int, _vp],
     "mrsa_route_layer_workspace_size": [_vp],
@@ -103,7 +108,7 @@ _RESTYPE = {"mrsa_strerror": C.c_char_p, "mrsa_last_error": C.c_char_p, "mrsa_ro
             "mrsa_selected_attention_backward_workspace": _sz, "mrsa_route_scores_backward_workspace": _sz,
             "mrsa_local_attention_backward_workspace": _sz, "mrsa_page_workspace": _sz,
             "mrsa_page_copy_workspace": _sz,
-            "mrsa_paged_attention_workspace": _sz}
+            "mrsa_paged_attention_workspace": _sz, "mrsa_add_rms_norm_backward_workspace": _sz}
 
 EXPORTED = tuple(_SIGS)
 
@@ -150,13 +155,16 @@ def stream_of(t: torch.Tensor):
     return C.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
 
 
-# The argument structs of the rotary and paged operators, for callers of the C
+# The argument structs of the operators that take one, for callers of the C
 # entry points: a packed struct's bytes are passed as its pointer.
 ROTARY_ARGS = struct.Struct("@6P6q6qf3i")            # mrsa_rotary_args
 PAGE_TABLE = struct.Struct("@4P4q")                  # mrsa_page_table
 PAGE_POOL = struct.Struct("@P8q")                    # mrsa_page_pool
 PAGED_ATTENTION_ARGS = struct.Struct("@7P14qf2i4x")  # mrsa_paged_attention_args
 APPEND_ARGS = struct.Struct("@5P9qi4x")              # mrsa_paged_append_args
+NORM_ARGS = struct.Struct("@8P5qfi")                 # mrsa_norm_args
+NORM_BACKWARD_ARGS = struct.Struct("@7P5qi4x")       # mrsa_norm_backward_args
+GEMM_INT8_ARGS = struct.Struct("@6P5q3i4x")          # mrsa_gemm_int8_args
 
 
 def call(name: str, *args):
@@ -167,7 +175,7 @@ _ext = None
 
 
 def ext():
-    """The binding of the rotary and paged operators (idempotent).  Raises if
+    """The binding of the rotary, paged, norm and 8-bit operators (idempotent).  Raises if
     it is absent."""
     global _ext
     if _ext is None:

@@ -1,17 +1,18 @@
-// Python binding of the rotary and paged operators: checks of arguments,
-// output tensors and workspace, and the C entry points of mrsa.h.
+// Python binding of the rotary, paged, norm and 8-bit operators: checks of
+// arguments, output tensors and workspace, and the C entry points of mrsa.h.
 //
 // A decode step is a chain of launches of a few microseconds each.  Checked and
 // packed in Python, one such call took 11 to 15 us of host time, more than
 // its kernels; here it is five to ten.  One function per operator, with
 // positional arguments; the public functions with their defaults and
-// documentation are in rotary.py and paged_cache.py.
+// documentation are in rotary.py, paged_cache.py, dense.py and int8.py.
 #include <Python.h>
 
 #include <ATen/ATen.h>
 #include <ATen/MemoryOverlap.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -592,6 +593,277 @@ PyObject* attend(PyObject*, PyObject* const* o, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---------------------------------------------------------------- norms and 8 bits
+int float_type(const Tensor& t, const char* name) {
+  const int type = type_of(t);
+  TORCH_CHECK_VALUE(type >= 0, name, " must be BF16, FP16 or FP32, got ", t.scalar_type());
+  return type;
+}
+
+// [..., D] as [rows, D], the last dimension contiguous.
+Tensor as_rows(const Tensor& x, const char* name) {
+  TORCH_CHECK_VALUE(x.defined() && x.is_cuda(), name, " must be a CUDA tensor");
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1, name, " must be (..., D) with D at least 1, got ", x.sizes());
+  const Tensor y = x.dim() == 2 ? x : x.reshape({x.numel() / x.size(-1), x.size(-1)});
+  return inner_contiguous(y);
+}
+
+int64_t pitch_of(int64_t n) { return (n + 15) / 16 * 16; }
+
+// 8-bit rows like x's, 16 bytes times a whole number apart, and their scales.
+std::pair<Tensor, Tensor> whole_like(const Tensor& x) {
+  const int64_t k = x.size(-1);
+  std::vector<int64_t> strides(x.dim(), 1);
+  for (int64_t i = x.dim() - 2, step = pitch_of(k); i >= 0; --i) {
+    strides[i] = step;
+    step *= x.size(i);
+  }
+  return {at::empty_strided(x.sizes(), strides, x.options().dtype(at::kChar)),
+          at::empty(x.sizes().slice(0, x.dim() - 1), x.options().dtype(at::kFloat))};
+}
+
+// The checked arguments of a norm: x, residual (or none) and weight as the C entry takes them.
+struct Norm {
+  Tensor x, residual, weight;
+  mrsa_norm_args a = {};
+  Norm(const Tensor& x_in, const Tensor& r_in, const Tensor& w_in, double eps) {
+    x = as_rows(x_in, "x");
+    a.dtype = float_type(x, "x");
+    a.rows = x.size(0);
+    a.dim = x.size(1);
+    TORCH_CHECK_VALUE(w_in.defined() && w_in.dim() == 1 && w_in.size(0) == a.dim && w_in.scalar_type() == x.scalar_type() &&
+                          w_in.device() == x.device(),
+                      "weight must be (", a.dim, ") of x's type and device");
+    weight = w_in.contiguous();
+    if (r_in.defined()) {
+      TORCH_CHECK_VALUE(r_in.sizes() == x_in.sizes() && r_in.scalar_type() == x.scalar_type() && r_in.device() == x.device(),
+                        "residual must share x's shape, type and device");
+      residual = as_rows(r_in, "residual");
+      a.residual = residual.const_data_ptr();
+      a.residual_stride = residual.stride(0);
+    }
+    TORCH_CHECK_VALUE(eps >= MRSA_NORM_MIN_EPS && eps <= 3.4028234663852886e38, "eps must be at least 1e-12, got ", eps);
+    a.eps = static_cast<float>(eps);
+    a.x = x.const_data_ptr();
+    a.weight = weight.const_data_ptr();
+    a.x_stride = x.stride(0);
+  }
+};
+
+void checked(int rc, const char* name) {
+  TORCH_CHECK_VALUE(rc != MRSA_ERR_SHAPE && rc != MRSA_ERR_ARG && rc != MRSA_ERR_NULL && rc != MRSA_ERR_ALIGN, name, ": ",
+                    mrsa_strerror(rc));
+  TORCH_CHECK(rc == 0, name, ": ", mrsa_strerror(rc), " [", mrsa_last_error(), "]");
+}
+
+// y, with a residual h, and with `keep` 1 / rms of each row.
+struct Normed {
+  Tensor y, h, rstd;
+};
+Normed add_norm(const Tensor& x, const Tensor& residual, const Tensor& weight, double eps, bool keep) {
+  Norm n(x, residual, weight, eps);
+  Normed r;
+  r.y = heads_like(x);
+  n.a.y = r.y.mutable_data_ptr();
+  if (residual.defined()) {
+    r.h = heads_like(x);
+    n.a.h = r.h.mutable_data_ptr();
+  }
+  if (keep) {
+    r.rstd = at::empty({n.a.rows}, x.options().dtype(at::kFloat));
+    n.a.rstd = r.rstd.mutable_data_ptr<float>();
+  }
+  if (n.a.rows > 0) checked(mrsa_add_rms_norm(&n.a, stream_of(x)), "mrsa_add_rms_norm");
+  return r;
+}
+
+struct AddRmsNorm : torch::autograd::Function<AddRmsNorm> {
+  using List = torch::autograd::variable_list;
+  static List forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& residual,
+                      const Tensor& weight, double eps) {
+    ctx->set_materialize_grads(false);
+    const Normed r = add_norm(x, residual ? *residual : Tensor(), weight, eps, true);
+    ctx->saved_data["add"] = residual.has_value();
+    ctx->save_for_backward({residual ? r.h : x, weight, r.rstd});
+    return residual ? List{r.y, r.h} : List{r.y};
+  }
+  static List backward(torch::autograd::AutogradContext* ctx, const List& g) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!c10::GradMode::is_enabled(), "add_rms_norm: the gradient of its gradient is not recorded");
+    const bool add = ctx->saved_data["add"].toBool();
+    const Tensor gh = add ? g[1] : Tensor();
+    if (!g[0].defined()) return {gh, add ? gh : Tensor(), Tensor(), Tensor()};
+    const auto saved = ctx->get_saved_variables();
+    const Tensor gy = as_rows(g[0], "the gradient"), h = as_rows(saved[0], "h"), weight = saved[1].contiguous();
+    mrsa_norm_backward_args a = {};
+    a.rows = h.size(0);
+    a.dim = h.size(1);
+    Tensor dx = heads_like(saved[0]), dw, ws, gh2;
+    const bool want_w = ctx->needs_input_grad(add ? 2 : 1);
+    if (a.rows == 0) return {dx, add ? dx : Tensor(), want_w ? at::zeros_like(weight) : Tensor(), Tensor()};
+    size_t size = 0;
+    if (want_w) {
+      dw = at::empty_like(weight);
+      size = mrsa_add_rms_norm_backward_workspace(a.rows, a.dim);
+      ws = bytes_on(h, size);
+      a.dweight = dw.mutable_data_ptr();
+    }
+    if (gh.defined()) {
+      gh2 = as_rows(gh, "the gradient");
+      a.grad_h = gh2.const_data_ptr();
+      a.grad_h_stride = gh2.stride(0);
+    }
+    a.grad_y = gy.const_data_ptr();
+    a.grad_y_stride = gy.stride(0);
+    a.h = h.const_data_ptr();
+    a.h_stride = h.stride(0);
+    a.weight = weight.const_data_ptr();
+    a.rstd = saved[2].const_data_ptr<float>();
+    a.dx = dx.mutable_data_ptr();
+    a.dtype = type_of(h);
+    checked(mrsa_add_rms_norm_backward(&a, want_w ? ws.mutable_data_ptr() : nullptr, size, stream_of(h)),
+            "mrsa_add_rms_norm_backward");
+    return {dx, add ? dx : Tensor(), dw, Tensor()};
+  }
+};
+
+PyObject* tuple_of(std::initializer_list<Tensor> all) {
+  PyObject* r = PyTuple_New(static_cast<Py_ssize_t>(all.size()));
+  Py_ssize_t i = 0;
+  for (const Tensor& t : all) PyTuple_SET_ITEM(r, i++, THPVariable_Wrap(t));
+  return r;
+}
+
+// add_rms_norm(x, residual, weight, eps) -> (y, h)
+PyObject* add_rms_norm(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(n == 4, "add_rms_norm takes 4 arguments");
+  const Tensor &x = tensor(o[0], "x"), &residual = tensor(o[1], "residual"), &weight = tensor(o[2], "weight");
+  const double eps = PyFloat_AsDouble(o[3]);
+  if (PyErr_Occurred()) return nullptr;
+  no_tangent("add_rms_norm", {&x, &residual, &weight});
+  TORCH_CHECK_VALUE(x.defined() && weight.defined(), "x and weight must be tensors");
+  if (c10::GradMode::is_enabled() &&
+      (x.requires_grad() || weight.requires_grad() || (residual.defined() && residual.requires_grad()))) {
+    const std::optional<Tensor> add = residual.defined() ? std::optional<Tensor>(residual) : std::nullopt;
+    const auto r = AddRmsNorm::apply(x, add, weight, eps);
+    return tuple_of({r[0], r.size() > 1 ? r[1] : x});
+  }
+  const Normed r = add_norm(x, residual, weight, eps, false);
+  return tuple_of({r.y, r.h.defined() ? r.h : x});
+  END_HANDLE_TH_ERRORS
+}
+
+// add_rms_norm_int8(x, residual, weight, eps) -> (q, scale, h)
+PyObject* add_rms_norm_int8(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(n == 4, "add_rms_norm_int8 takes 4 arguments");
+  const Tensor &x = tensor(o[0], "x"), &residual = tensor(o[1], "residual"), &weight = tensor(o[2], "weight");
+  const double eps = PyFloat_AsDouble(o[3]);
+  if (PyErr_Occurred()) return nullptr;
+  forward_only("add_rms_norm_int8", {&x, &residual, &weight});
+  no_tangent("add_rms_norm_int8", {&x, &residual, &weight});
+  Norm c(x, residual, weight, eps);
+  auto [q, scale] = whole_like(x);
+  Tensor h = x;
+  if (residual.defined()) {
+    h = heads_like(x);
+    c.a.h = h.mutable_data_ptr();
+  }
+  c.a.q = q.mutable_data_ptr<int8_t>();
+  c.a.q_stride = pitch_of(c.a.dim);
+  c.a.scale = scale.mutable_data_ptr<float>();
+  if (c.a.rows > 0 && !finish(mrsa_add_rms_norm(&c.a, stream_of(x)), "mrsa_add_rms_norm")) return nullptr;
+  return tuple_of({q, scale, h});
+  END_HANDLE_TH_ERRORS
+}
+
+// quantize_int8(x) -> (q, scale)
+PyObject* quantize_int8(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(n == 1, "quantize_int8 takes 1 argument");
+  const Tensor& x = tensor(o[0], "x");
+  forward_only("quantize_int8", {&x});
+  no_tangent("quantize_int8", {&x});
+  const Tensor rows = as_rows(x, "x");
+  const int type = float_type(x, "x");
+  auto [q, scale] = whole_like(x);
+  if (!finish(mrsa_quantize_int8(rows.const_data_ptr(), rows.stride(0), q.mutable_data_ptr<int8_t>(), pitch_of(rows.size(1)),
+                                 scale.mutable_data_ptr<float>(), rows.size(0), rows.size(1), type, stream_of(x)),
+              "mrsa_quantize_int8"))
+    return nullptr;
+  return tuple_of({q, scale});
+  END_HANDLE_TH_ERRORS
+}
+
+// 8-bit rows as the products read them: 16-byte boundaries, copied to such rows where they are not.
+Tensor whole_rows(const Tensor& x, const char* name) {
+  TORCH_CHECK_VALUE(x.defined() && x.scalar_type() == at::kChar, name, " must be INT8");
+  Tensor y = as_rows(x, name);
+  const int64_t k = y.size(1);
+  const bool fit = reinterpret_cast<uintptr_t>(y.const_data_ptr()) % 16 == 0 &&
+                   (y.size(0) <= 1 || (y.stride(0) % 16 == 0 && y.stride(0) >= k));
+  if (fit) return y;
+  Tensor z = at::empty_strided({y.size(0), k}, {pitch_of(k), 1}, y.options());
+  z.copy_(y);
+  return z;
+}
+int64_t row_pitch(const Tensor& x) { return x.size(0) > 1 ? x.stride(0) : pitch_of(x.size(1)); }
+
+Tensor scales(const Tensor& x, const char* name, at::IntArrayRef sizes, const Tensor& like) {
+  TORCH_CHECK_VALUE(x.defined() && x.scalar_type() == at::kFloat && x.sizes() == sizes && x.device() == like.device(), name,
+                    " must be FP32 ", sizes, " on the tensors' device");
+  return x.contiguous();
+}
+
+// linear_int8(q, scale, weight, weight_scale, bias, dtype, gated)
+PyObject* linear_int8(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  TORCH_CHECK_TYPE(n == 7, "linear_int8 takes 7 arguments");
+  const Tensor &q = tensor(o[0], "q"), &weight = tensor(o[2], "weight");
+  Tensor bias = tensor(o[4], "bias");
+  TORCH_CHECK_TYPE(THPDtype_Check(o[5]), "dtype must be a torch.dtype");
+  const at::ScalarType type = reinterpret_cast<THPDtype*>(o[5])->scalar_type;
+  const bool gated = truth(o[6]);
+  forward_only("linear_int8", {&tensor(o[1], "scale"), &tensor(o[3], "weight_scale"), &bias});
+  no_tangent("linear_int8", {&tensor(o[1], "scale"), &tensor(o[3], "weight_scale"), &bias});
+  TORCH_CHECK_VALUE(weight.defined() && weight.dim() == 2, "weight must be (N, K)");
+  const Tensor a = whole_rows(q, "q"), b = whole_rows(weight, "weight");
+  TORCH_CHECK_VALUE(a.device() == b.device() && a.size(1) == b.size(1), "q and weight must share a device and K, got ",
+                    q.sizes(), " and ", weight.sizes());
+  TORCH_CHECK_VALUE(b.size(0) >= 1 && a.size(1) <= MRSA_INT8_MAX_K, "weight must have rows, and at most ", MRSA_INT8_MAX_K,
+                    " columns (sums of 32 bits)");
+  TORCH_CHECK_VALUE(!gated || b.size(0) % 256 == 0, "the gated product takes weights in blocks of 256 rows, got ", b.size(0));
+  const Tensor sa = scales(tensor(o[1], "scale"), "scale", q.sizes().slice(0, q.dim() - 1), a),
+               sb = scales(tensor(o[3], "weight_scale"), "weight_scale", {b.size(0)}, a);
+  std::vector<int64_t> sizes = q.sizes().vec();
+  sizes.back() = gated ? b.size(0) / 2 : b.size(0);
+  Tensor out = at::empty(sizes, a.options().dtype(type));
+  mrsa_gemm_int8_args p = {};
+  p.dtype = type_of(out);
+  TORCH_CHECK_VALUE(p.dtype >= 0, "dtype must be BF16, FP16 or FP32, got ", type);
+  if (bias.defined()) {
+    TORCH_CHECK_VALUE(bias.dim() == 1 && bias.size(0) == b.size(0) && bias.device() == a.device(),
+                      "bias must be (", b.size(0), ") on the tensors' device");
+    p.bias_dtype = float_type(bias, "bias");
+    bias = bias.contiguous();
+    p.bias = bias.const_data_ptr();
+  }
+  p.a = a.const_data_ptr<int8_t>();
+  p.b = b.const_data_ptr<int8_t>();
+  p.a_scale = sa.const_data_ptr<float>();
+  p.b_scale = sb.const_data_ptr<float>();
+  p.c = out.mutable_data_ptr();
+  p.m = a.size(0);
+  p.n = b.size(0);
+  p.k = a.size(1);
+  p.a_stride = row_pitch(a);
+  p.b_stride = row_pitch(b);
+  p.epilogue = gated ? MRSA_GEMM_SWIGLU : MRSA_GEMM_PLAIN;
+  if (!finish(mrsa_gemm_int8(&p, stream_of(a)), "mrsa_gemm_int8")) return nullptr;
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
 // set_check(callable): what turns a negative code of the library into an exception
 PyObject* set_check(PyObject*, PyObject* f) {
   Py_INCREF(f);
@@ -604,6 +876,8 @@ PyObject* set_check(PyObject*, PyObject* f) {
 PyMethodDef kMethods[] = {FAST("rotary", rotary), FAST("free", page_free), FAST("extend", page_extend),
                           FAST("fork", page_fork), FAST("compact", page_compact), FAST("copy", page_copy),
                           FAST("append", append), FAST("attend", attend),
+                          FAST("add_rms_norm", add_rms_norm), FAST("add_rms_norm_int8", add_rms_norm_int8),
+                          FAST("quantize_int8", quantize_int8), FAST("linear_int8", linear_int8),
                           {"set_check", set_check, METH_O, nullptr}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "mrsa_b200_ext", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

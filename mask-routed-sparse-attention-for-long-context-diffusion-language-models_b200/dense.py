@@ -69,3 +69,14 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float) -> torch.Tensor:
     _lib.call("mrsa_rms_norm", _lib.ptr(a), _lib.ptr(weight.to(torch.bfloat16).contiguous()), _lib.ptr(out),
               a.shape[0], a.shape[1], float(eps), _lib.stream_of(a))
     return out.view(x.shape)
+
+
+def add_rms_norm(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor, eps: float):
+    """``(y, h)``: the residual stream ``h = x + residual`` of ``x [..., D]``,
+    rounded to their type (bf16, fp16 or fp32), and its norm ``y = h * weight /
+    sqrt(mean(h^2) + eps)`` in fp32, rounded once (:func:`rms_norm` rounds
+    before the weight too).  Without a residual ``h`` is ``x`` itself.  Any
+    width and row stride; ``eps`` at least 1e-12.  Records the gradient of x,
+    residual and weight, the same bits on every run; the gradient of that
+    gradient and forward-mode tangents are refused."""
+    return _lib.ext().add_rms_norm(x, residual, weight, eps)
