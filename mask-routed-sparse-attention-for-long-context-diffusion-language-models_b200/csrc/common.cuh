@@ -131,6 +131,7 @@ int gemm_error_flags(int clear);
 int local_bwd_error_flags(int clear);
 int paged_error_flags(int clear);
 int int8_error_flags(int clear);
+int int8_few_error_flags(int clear);
 
 // Inverted chunk -> (query, slot) index of indices [B,Lq,Hkv,K] int32: per
 // segment (b, h, c) (flattened as (b*Hkv + h)*C + c) cnt[seg] entries from
