@@ -10,13 +10,23 @@
 // does not depend on it: sum of squares and maximum come from one pass over the
 // row and are joined behind one barrier.  (h w is exact in fp32 for 16-bit types.)
 //
-// All of it is bound by memory: each element is read once into registers, in
-// 16-byte vectors where rows are aligned, and each output written once.  A row
-// belongs to the warps of one CTA (a single warp if it is short; then a CTA has
-// eight rows).  The gradient's CTAs walk rows a grid apart, so that a thread's
-// columns of dw stay in registers, and the next row's loads are under way while
-// a row is summed up; the CTAs' parts of dw are joined in a fixed order by a
-// second launch, so that every run gives the same bits.
+// All of it is bound by memory, if the instructions are kept few (about 8 an
+// element: packed fp32 arithmetic, no conversions to integers, the weights and
+// the rows to come in shared memory and not in registers) and loads are always in
+// flight.  So CTAs stay, their rows a grid apart, and each thread copies its
+// 16-byte vectors of the next rows into slots of its own while the present one is
+// summed up and written.  A row belongs to the warps of one CTA (a single warp if
+// it is short; then a CTA has eight rows), with as few warps as leave four vectors
+// to a thread, or two where the rows are too few to fill the SMs.  The gradient
+// does the same with three tensors; a thread's columns of dw stay in registers,
+// and the CTAs' parts are joined in a fixed order by a second launch, so that
+// every run gives the same bits.
+//
+// Measured (B200, bf16, us, and of the 6.55 TB/s of a copy): 16384 x 3584 norm with
+// residual 85 (84 %; 96 with a CTA per row and loads in registers), without 45
+// (79 %), with its gradient 160 (90 %; 248); 32768 x 3584 in 8 bits 135 (93 %; 192);
+// 16384 x 18944 quantized 162 (88 %; 312).  Rows off 16-byte boundaries go element
+// by element: fp32 4095 x 2561 with gradient 90 (57 %).
 #include "common.cuh"
 #include "elements.cuh"
 
@@ -24,10 +34,15 @@ using namespace mrsa;
 
 namespace {
 
-constexpr int N_MAX_THREADS = 1024, N_BWD_THREADS = 512;
+constexpr int N_MAX_THREADS = 1024;
 constexpr int N_SHORT_ROWS = 8;      // rows per CTA where one warp takes a row
+constexpr int ring_threads(int per) { return per == 4 ? 640 : 512; }     // at most, with so many vectors a thread
+constexpr int ring_ctas(int per) { return per == 1 ? 3 : per == 2 ? 2 : 1; }
+constexpr int kAhead = 2;            // rows whose copies are under way
+constexpr int N_SMEM = 227 * 1024;
 constexpr float kSmall = 7.888609e-31f, kSmallUp = 1.2676506e30f;     // 2^-100, 2^100
 constexpr float kLargeDown = 1.2621774e-29f;                          // 2^-96
+constexpr float kWhole = 12582912.f;                                  // 1.5 * 2^23
 
 struct NormArgs {
   const void *x, *residual, *weight;
@@ -36,7 +51,7 @@ struct NormArgs {
   float *scale, *rstd;
   int64_t rows, x_stride, residual_stride, q_stride;
   int dim, row_warps;
-  float eps;
+  float eps, inv_dim;
 };
 
 struct RowSums {
@@ -44,86 +59,208 @@ struct RowSums {
   uint32_t top;        // bits of the largest magnitude; NaN above infinity above numbers
 };
 
+// What the warps of a CTA hand each other: read four at a time, so up to a multiple
+// of four, and zeros beyond the last warp.
+struct alignas(16) Joined {
+  float squares[32];
+  uint32_t top[32];
+};
+
 // Over the row's warps; every thread of the row gets the sums in the same order.
-__device__ __forceinline__ RowSums join_row(RowSums v, int row_warps, RowSums* red) {
-  v.squares = warp_sum(v.squares);
-  v.top = __reduce_max_sync(0xffffffffu, v.top);
+template <bool kNorm, bool kQ8>
+__device__ __forceinline__ RowSums join_row(RowSums v, int row_warps, Joined& red) {
+  if (kNorm) v.squares = warp_sum(v.squares);
+  if (kQ8) v.top = __reduce_max_sync(0xffffffffu, v.top);
   if (row_warps == 1) return v;
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  const int warp = threadIdx.x >> 5;
+  if ((threadIdx.x & 31) == 0) {
+    if (kNorm) red.squares[warp] = v.squares;
+    if (kQ8) red.top[warp] = v.top;
+  }
   __syncthreads();
-  RowSums r = red[0];
-  for (int i = 1; i < row_warps; ++i) {
-    r.squares += red[i].squares;
-    r.top = max(r.top, red[i].top);
+  RowSums r = {0.f, 0u};
+  for (int i = 0; i < row_warps; i += 4) {
+    if (kNorm) {
+      const float4 q = *reinterpret_cast<const float4*>(red.squares + i);
+      r.squares += (q.x + q.y) + (q.z + q.w);
+    }
+    if (kQ8) {
+      const uint4 q = *reinterpret_cast<const uint4*>(red.top + i);
+      r.top = max(max(max(q.x, q.y), max(q.z, q.w)), r.top);
+    }
   }
   return r;
+}
+// Before the first row; a barrier has to follow.
+__device__ __forceinline__ void clear(Joined* red, int n) {
+  for (int i = threadIdx.x; i < 32 * n; i += blockDim.x) {
+    red[i >> 5].squares[i & 31] = 0.f;
+    red[i >> 5].top[i & 31] = 0u;
+  }
 }
 
 __device__ __forceinline__ uint32_t magnitude(float f) { return __float_as_uint(f) & 0x7fffffffu; }
 constexpr uint32_t kInfBits = 0x7f800000u;
 
-// A row's statistics from its elements in registers (or memory): get(i, h, w) gives
-// element i of this thread.  Rows whose squares (or products with w) pass the
-// largest fp32 number are summed once more, 2^-96 as large; `down` says so.
+// The larger of three magnitudes, NaN where one is none.
+__device__ __forceinline__ float top_of(float a, float b, float c) {
+  float d;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;\n" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// A thread's part of a row's statistics; with kDown of the row 2^-96 as large.
+template <bool kNorm, bool kQ8, bool kDown> struct Statistics {
+  float2 squares = {0.f, 0.f};
+  float top = 0.f;
+  __device__ __forceinline__ void add(float2 h, float2 w) {
+    if (kDown) h = fmul2(h, make_float2(kLargeDown, kLargeDown));
+    if (kNorm) squares = ffma2(h, h, squares);
+    if (kQ8) {
+      if (kNorm) h = fmul2(h, w);
+      top = top_of(top, h.x, h.y);
+    }
+  }
+  template <typename T, int V> __device__ __forceinline__ void add(const Elements<T, V>& h, const Elements<T, V>& w) {
+#pragma unroll
+    for (int p = 0; p < (V + 1) / 2; ++p) add(pair_of(h, p), pair_of(w, p));
+  }
+  __device__ __forceinline__ RowSums sums() const { return {squares.x + squares.y, magnitude(top)}; }
+};
+
+// A row's statistics from its elements in registers (or memory): each(s) adds this
+// thread's to s.  Rows whose squares (or products with w) pass the largest fp32
+// number are summed once more, 2^-96 as large; `down` says so.
 template <bool kNorm, bool kQ8, typename F>
-__device__ __forceinline__ void row_statistics(const NormArgs& a, RowSums* red, F each, float& rstd, float& top, float& down) {
-  RowSums v = {0.f, 0u};
-  each([&](float h, float w) {
-    if (kNorm) v.squares = fmaf(h, h, v.squares);
-    if (kQ8) v.top = max(v.top, magnitude(kNorm ? h * w : h));
-  });
-  v = join_row(v, a.row_warps, red);
+__device__ __forceinline__ void row_statistics(const NormArgs& a, Joined& red, F each, float& rstd, float& top, float& down) {
+  Statistics<kNorm, kQ8, false> s;
+  each(s);
+  RowSums v = join_row<kNorm, kQ8>(s.sums(), a.row_warps, red);
   down = 1.f;
   float eps = a.eps;
   if (kNorm && (magnitude(v.squares) >= kInfBits || (kQ8 && v.top >= kInfBits))) {
     down = kLargeDown;
     eps = eps * kLargeDown * kLargeDown;
-    v = {0.f, 0u};
-    each([&](float h, float w) {
-      h *= kLargeDown;
-      v.squares = fmaf(h, h, v.squares);
-      if (kQ8) v.top = max(v.top, magnitude(h * w));
-    });
+    Statistics<kNorm, kQ8, true> l;
+    each(l);
     if (a.row_warps > 1) __syncthreads();      // red is read no more
-    v = join_row(v, a.row_warps, red);
+    v = join_row<kNorm, kQ8>(l.sums(), a.row_warps, red);
   }
-  rstd = kNorm ? 1.f / sqrtf(v.squares / static_cast<float>(a.dim) + eps) : 1.f;
+  rstd = kNorm ? rsqrtf(fmaf(v.squares, a.inv_dim, eps)) : 1.f;      // to 2 units in the last place
   top = __uint_as_float(v.top);
   // an infinity makes r zero: what it leaves is not a number
   if (kNorm && kQ8 && magnitude(v.squares) >= kInfBits) top = __uint_as_float(0x7fffffffu);
 }
 
-// nearest(127 p / top) by a product with 127 / top: within one rounding of p / s,
-// so only values as near to half-way as that may go to the other neighbour.
-// Tops below 2^-100 are taken 2^100 as large, so that 127 / top stays finite.
+// nearest(127 p / top) as the low byte of fma(p, 127 / top, 1.5 * 2^23), whose one
+// rounding is to a whole number (no conversion, which runs at a quarter of the
+// rate): off from p / s by what 127 / top is, so only values as near to half-way as
+// that may go to the other neighbour.  Tops below 2^-100 are taken 2^100 as large,
+// so that 127 / top stays finite.
 struct Whole {
   float up, inv;
+  uint32_t keep;       // no bits of rows that are zeros or not numbers
   __device__ __forceinline__ explicit Whole(float top) {
+    const bool none = !(top > 0.f) || magnitude(top) >= kInfBits;
     up = top < kSmall ? kSmallUp : 1.f;
-    const bool none = !(top > 0.f) || magnitude(top) >= kInfBits;    // zeros, or not a number: whole numbers 0
-    inv = none ? 0.f : 127.f / (top * up);
-    if (none) up = 0.f;
+    inv = none ? 0.f : __fdividef(127.f, top * up);     // to 2 units in the last place
+    keep = none ? 0u : 0xffffffffu;
   }
-  __device__ __forceinline__ int operator()(float p) const {
-    // at most 127 by p <= top; the conversion takes NaN (an infinity times 0) to 0
-    return __float2int_rn(p * up * inv);
-  }
+  __device__ __forceinline__ uint32_t operator()(float p) const { return __float_as_uint(fmaf(p * up, inv, kWhole)); }
 };
 
 __device__ __forceinline__ float scale_of(float top, float rstd) {
   return magnitude(top) >= kInfBits ? __uint_as_float(0x7fffffffu) : top / 127.f * rstd;
 }
 
-template <int V> __device__ __forceinline__ void store_whole(int8_t* p, const int (&n)[V]) {
+// The low bytes of n.
+template <int V> __device__ __forceinline__ void store_whole(int8_t* p, const uint32_t (&n)[V], uint32_t keep) {
   if constexpr (V == 1) {
-    *p = static_cast<int8_t>(n[0]);
+    *p = static_cast<int8_t>(n[0] & keep);
   } else {
     uint32_t w[V / 4];
 #pragma unroll
     for (int i = 0; i < V / 4; ++i)
-      w[i] = (n[4 * i] & 255) | (n[4 * i + 1] & 255) << 8 | (n[4 * i + 2] & 255) << 16 | static_cast<uint32_t>(n[4 * i + 3]) << 24;
+      w[i] = __byte_perm(__byte_perm(n[4 * i], n[4 * i + 1], 0x0040), __byte_perm(n[4 * i + 2], n[4 * i + 3], 0x0040), 0x5410) & keep;
     if constexpr (V == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
     else *reinterpret_cast<uint32_t*>(p) = w[0];
+  }
+}
+
+// What a row's thread writes of vector v (elements v V on) once the statistics are
+// known; kPlain: neither the row nor its top was scaled.
+template <typename T, int V, bool kNorm, bool kQ8, bool kPlain>
+__device__ __forceinline__ void write_vector(const NormArgs& a, int64_t row, int v, const Elements<T, V>& h,
+                                             const Elements<T, V>& w, float rstd, float down, const Whole& whole) {
+  if constexpr (kQ8) {
+    uint32_t n[V];
+    if constexpr (V == 1) {
+      const float f = to_float(h.e[0]);
+      n[0] = whole(kNorm ? f * down * to_float(w.e[0]) : f);
+    } else {
+#pragma unroll
+      for (int p = 0; p < V / 2; ++p) {
+        float2 f = pair_of(h, p);
+        if (!kPlain) f = fmul2(f, make_float2(down, down));
+        if (kNorm) f = fmul2(f, pair_of(w, p));
+        if (!kPlain) f = fmul2(f, make_float2(whole.up, whole.up));
+        f = ffma2(f, make_float2(whole.inv, whole.inv), make_float2(kWhole, kWhole));
+        n[2 * p] = __float_as_uint(f.x);
+        n[2 * p + 1] = __float_as_uint(f.y);
+      }
+    }
+    store_whole<V>(a.q + row * a.q_stride + static_cast<int64_t>(v) * V, n, whole.keep);
+  } else {
+    Elements<T, V> o;
+    if constexpr (V == 1) {
+      o.e[0] = from_float<T>(to_float(h.e[0]) * down * rstd * to_float(w.e[0]));
+    } else {
+#pragma unroll
+      for (int p = 0; p < V / 2; ++p) {
+        float2 f = pair_of(h, p);
+        if (!kPlain) f = fmul2(f, make_float2(down, down));
+        set_pair(o, p, fmul2(fmul2(f, make_float2(rstd, rstd)), pair_of(w, p)));
+      }
+    }
+    reinterpret_cast<Elements<T, V>*>(static_cast<T*>(a.y) + row * a.dim)[v] = o;
+  }
+}
+template <typename T, int V, int kPer, bool kNorm, bool kQ8>
+__device__ __forceinline__ void write_row(const NormArgs& a, int64_t row, int t, int team, const Elements<T, V> (&h)[kPer],
+                                          const Elements<T, V>* weight, float rstd, float down, float top) {
+  const int vecs = a.dim / V;
+  const Whole whole(kQ8 ? top : 0.f);
+  if ((!kNorm || down == 1.f) && (!kQ8 || whole.up == 1.f)) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (t + i * team < vecs)
+        write_vector<T, V, kNorm, kQ8, true>(a, row, t + i * team, h[i], kNorm ? weight[t + i * team] : h[i], rstd, down, whole);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (t + i * team < vecs)
+        write_vector<T, V, kNorm, kQ8, false>(a, row, t + i * team, h[i], kNorm ? weight[t + i * team] : h[i], rstd, down, whole);
+  }
+}
+template <bool kQ8> __device__ __forceinline__ void write_statistics(const NormArgs& a, int64_t row, float rstd, float down, float top) {
+  if (kQ8) a.scale[row] = scale_of(top, rstd);
+  else if (a.rstd != nullptr) a.rstd[row] = rstd * down;
+}
+
+// x + residual, rounded: the packed addition rounds the exact sum once; fp32 would
+// round before where exponents are more than 13 apart, and both then give the larger.
+template <typename T, int V>
+__device__ __forceinline__ void add_to(Elements<T, V>& h, const Elements<T, V>& r) {
+  if constexpr (V == 8) {
+    using Two = std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>;
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      Two& x = reinterpret_cast<Two*>(h.e)[p];
+      x = __hadd2_rn(x, reinterpret_cast<const Two*>(r.e)[p]);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) h.e[e] = from_float<T>(to_float(h.e[e]) + to_float(r.e[e]));
   }
 }
 
@@ -131,7 +268,11 @@ template <int V> __device__ __forceinline__ void store_whole(int8_t* p, const in
 template <typename T, int V, int kPer, bool kNorm, bool kQ8>
 __global__ void __launch_bounds__(N_MAX_THREADS) norm_kernel(const NormArgs a) {
   using Vec = Elements<T, V>;
-  __shared__ RowSums red[32];
+  __shared__ Joined red;
+  if (a.row_warps > 1) {
+    clear(&red, 1);
+    __syncthreads();
+  }
   chain_wait();
   chain_next();
   const int team = a.row_warps * 32, t = threadIdx.x % team;
@@ -162,54 +303,96 @@ __global__ void __launch_bounds__(N_MAX_THREADS) norm_kernel(const NormArgs a) {
     for (int i = 0; i < kPer; ++i) {
       const int v = t + i * team;
       if (v >= vecs) continue;
-#pragma unroll
-      for (int e = 0; e < V; ++e) h[i].e[e] = from_float<T>(to_float(h[i].e[e]) + to_float(r[i].e[e]));
+      add_to<T, V>(h[i], r[i]);
       reinterpret_cast<Vec*>(static_cast<T*>(a.h) + row * a.dim)[v] = h[i];
     }
   }
   float rstd, top, down;
-  row_statistics<kNorm, kQ8>(a, red, [&](auto&& f) {
+  row_statistics<kNorm, kQ8>(a, red, [&](auto& s) {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i)
-#pragma unroll
-      for (int e = 0; e < V; ++e) f(to_float(h[i].e[e]), to_float(w[i].e[e]));
+    for (int i = 0; i < kPer; ++i) s.add(h[i], w[i]);
   }, rstd, top, down);
-  if (kQ8) {
-    const Whole whole(top);
+  write_row<T, V, kPer, kNorm, kQ8>(a, row, t, team, h, static_cast<const Vec*>(a.weight), rstd, down, top);
+  if (t == 0) write_statistics<kQ8>(a, row, rstd, down, top);
+}
+
+// The same for rows on 16-byte boundaries, a CTA's (or warp's) rows a grid apart:
+// each thread copies its vectors of the rows to come into slots of its own, kAhead
+// rows ahead, so that loads are always in flight while a row is summed up and
+// written.  Nobody else reads a thread's slots, so its own wait is enough.
+template <typename T, int kPer, bool kNorm, bool kQ8>
+__global__ void __launch_bounds__(ring_threads(kPer), ring_ctas(kPer)) norm_ring_kernel(const NormArgs a) {
+  constexpr int V = 16 / sizeof(T);
+  using Vec = Elements<T, V>;
+  extern __shared__ __align__(16) unsigned char slots[];
+  __shared__ Joined red[2];                    // in turn: a row's are read until the next row's barrier
+  if (a.row_warps > 1) {
+    clear(red, 2);
+    __syncthreads();
+  }
+  chain_wait();
+  chain_next();
+  const int team = a.row_warps * 32, t = threadIdx.x % team, side = blockDim.x / team;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * side;
+  int64_t row = static_cast<int64_t>(blockIdx.x) * side + threadIdx.x / team;
+  const int vecs = a.dim / V, threads = blockDim.x;
+  const bool add = kNorm && a.residual != nullptr;
+  Vec* const weight = reinterpret_cast<Vec*>(slots);     // (in shared memory: in registers it costs as many as the row)
+  Vec* const ring = weight + (kNorm ? vecs : 0) + threadIdx.x;
+  const int tensor = kPer * threads, stage = (add ? 2 : 1) * tensor;
+  auto ask = [&](int64_t r, int s) {
+    if (r < a.rows) {
+      const Vec* x = reinterpret_cast<const Vec*>(static_cast<const T*>(a.x) + r * a.x_stride);
+      const Vec* y = add ? reinterpret_cast<const Vec*>(static_cast<const T*>(a.residual) + r * a.residual_stride) : nullptr;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int v = t + i * team;
-      if (v >= vecs) continue;
-      int n[V];
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float f = to_float(h[i].e[e]);
-        n[e] = whole(kNorm ? f * down * to_float(w[i].e[e]) : f);
+      for (int i = 0; i < kPer; ++i) {
+        const int v = t + i * team;
+        if (v >= vecs) continue;
+        cp_async16(ring + s * stage + i * threads, x + v);
+        if (add) cp_async16(ring + s * stage + tensor + i * threads, y + v);
       }
-      store_whole<V>(a.q + row * a.q_stride + static_cast<int64_t>(v) * V, n);
     }
-    if (t == 0) a.scale[row] = scale_of(top, rstd);
-  } else {
-    const Vec* weight = static_cast<const Vec*>(a.weight);
-    Vec* y = reinterpret_cast<Vec*>(static_cast<T*>(a.y) + row * a.dim);
+    asm volatile("cp.async.commit_group;\n" ::: "memory");
+  };
+#pragma unroll
+  for (int s = 0; s < kAhead; ++s) ask(row + s * step, s);
+  if (kNorm) {
+    for (int v = threadIdx.x; v < vecs; v += threads) weight[v] = static_cast<const Vec*>(a.weight)[v];
+    __syncthreads();
+  }
+  int s = 0, turn = 0;
+  for (; row < a.rows; row += step, turn ^= 1) {
+    asm volatile("cp.async.wait_group %0;\n" ::"n"(kAhead - 1) : "memory");
+    Vec h[kPer];
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const int v = t + i * team;
-      if (v >= vecs) continue;
-      w[i] = weight[v];
-      Vec o;
 #pragma unroll
-      for (int e = 0; e < V; ++e) o.e[e] = from_float<T>(to_float(h[i].e[e]) * down * rstd * to_float(w[i].e[e]));
-      y[v] = o;
+      for (int e = 0; e < V; ++e) h[i].e[e] = from_float<T>(0.f);
+      if (v >= vecs) continue;
+      h[i] = ring[s * stage + i * threads];
+      if (add) {
+        add_to<T, V>(h[i], ring[s * stage + tensor + i * threads]);
+        reinterpret_cast<Vec*>(static_cast<T*>(a.h) + row * a.dim)[v] = h[i];
+      }
     }
-    if (t == 0 && a.rstd != nullptr) a.rstd[row] = rstd * down;
+    ask(row + kAhead * step, s);
+    if (++s == kAhead) s = 0;
+    float rstd, top, down;
+    row_statistics<kNorm, kQ8>(a, red[turn], [&](auto& s) {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        if (t + i * team < vecs) s.add(h[i], kNorm && kQ8 ? weight[t + i * team] : h[i]);
+    }, rstd, top, down);
+    write_row<T, V, kPer, kNorm, kQ8>(a, row, t, team, h, weight, rstd, down, top);
+    if (t == 0) write_statistics<kQ8>(a, row, rstd, down, top);
   }
 }
 
 // Rows too wide for registers: element by element, read again for the outputs.
 template <typename T, bool kNorm, bool kQ8>
 __global__ void __launch_bounds__(N_MAX_THREADS) norm_wide_kernel(const NormArgs a) {
-  __shared__ RowSums red[32];
+  __shared__ Joined red;                       // every warp writes its own
   chain_wait();
   chain_next();
   const int64_t row = blockIdx.x;
@@ -221,24 +404,36 @@ __global__ void __launch_bounds__(N_MAX_THREADS) norm_wide_kernel(const NormArgs
     return res != nullptr ? from_float<T>(to_float(v) + to_float(res[i])) : v;
   };
   float rstd, top, down;
-  row_statistics<kNorm, kQ8>(a, red, [&](auto&& f) {
-    for (int i = threadIdx.x; i < a.dim; i += N_MAX_THREADS) f(to_float(h_at(i)), kNorm && kQ8 ? to_float(weight[i]) : 0.f);
+  row_statistics<kNorm, kQ8>(a, red, [&](auto& s) {
+    for (int i = threadIdx.x; i < a.dim; i += N_MAX_THREADS) {
+      const Elements<T, 1> h = {h_at(i)}, w = {kNorm && kQ8 ? weight[i] : from_float<T>(0.f)};
+      s.add(h, w);
+    }
   }, rstd, top, down);
   const Whole whole(top);
   for (int i = threadIdx.x; i < a.dim; i += N_MAX_THREADS) {
     const T h = h_at(i);
     const float f = to_float(h) * down, w = kNorm ? to_float(weight[i]) : 1.f;
     if (kNorm && res != nullptr) static_cast<T*>(a.h)[row * a.dim + i] = h;
-    if (kQ8) a.q[row * a.q_stride + i] = static_cast<int8_t>(whole(kNorm ? f * w : f));
+    if (kQ8) a.q[row * a.q_stride + i] = static_cast<int8_t>(whole(kNorm ? f * w : f) & whole.keep);
     else static_cast<T*>(a.y)[row * a.dim + i] = from_float<T>(f * rstd * w);
   }
-  if (threadIdx.x == 0) {
-    if (kQ8) a.scale[row] = scale_of(top, rstd);
-    else if (a.rstd != nullptr) a.rstd[row] = rstd * down;
-  }
+  if (threadIdx.x == 0) write_statistics<kQ8>(a, row, rstd, down, top);
 }
 
 // ------------------------------------------------------------ gradient
+template <typename T, int V> __device__ __forceinline__ Elements<T, V> zeros() {
+  Elements<T, V> z;
+#pragma unroll
+  for (int e = 0; e < V; ++e) z.e[e] = from_float<T>(0.f);
+  return z;
+}
+template <typename Vec> __device__ __forceinline__ void copy_in(Vec* to, const Vec* from) {
+  static_assert(sizeof(Vec) == 16 || sizeof(Vec) == 4);
+  if constexpr (sizeof(Vec) == 16) cp_async16(to, from);
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;\n" ::"r"(smem_u32(to)), "l"(from));
+}
+
 struct BackwardArgs {
   const void *gy, *gh, *h, *weight;
   const float* rstd;
@@ -246,6 +441,7 @@ struct BackwardArgs {
   float* parts;          // [grid, dim]
   int64_t rows, gy_stride, gh_stride, h_stride;
   int dim, grid;
+  float inv_dim;
 };
 
 __device__ __forceinline__ float join_sum(float v, float* red) {
@@ -259,66 +455,93 @@ __device__ __forceinline__ float join_sum(float v, float* red) {
   return s;
 }
 
-template <typename T, int V, int kPer>
-__global__ void __launch_bounds__(N_BWD_THREADS) norm_backward_kernel(const BackwardArgs a) {
+// A thread's part of a row: dw and the sum of g u; then dx.
+template <typename T, int V>
+__device__ __forceinline__ void add_products(float2 (&dw)[(V + 1) / 2], float2& sum, const Elements<T, V>& g, const Elements<T, V>& h,
+                                             const Elements<T, V>& w, float rstd) {
+#pragma unroll
+  for (int p = 0; p < (V + 1) / 2; ++p) {
+    const float2 dy = pair_of(g, p), u = fmul2(pair_of(h, p), make_float2(rstd, rstd));
+    dw[p] = ffma2(dy, u, dw[p]);
+    sum = ffma2(fmul2(dy, pair_of(w, p)), u, sum);
+  }
+}
+template <typename T, int V>
+__device__ __forceinline__ Elements<T, V> gradient_of(const Elements<T, V>& g, const Elements<T, V>& h, const Elements<T, V>& w,
+                                                      const Elements<T, V>& o, float rstd, float mean) {
+  Elements<T, V> d;
+#pragma unroll
+  for (int p = 0; p < (V + 1) / 2; ++p) {
+    const float2 gw = fmul2(pair_of(g, p), pair_of(w, p)), u = fmul2(pair_of(h, p), make_float2(rstd, rstd));
+    set_pair(d, p, ffma2(make_float2(rstd, rstd), ffma2(u, make_float2(-mean, -mean), gw), pair_of(o, p)));
+  }
+  return d;
+}
+
+// Each thread copies its vectors of the rows to come into slots of its own, as in
+// the forward kernel: 16 bytes each, or single fp32 numbers where rows do not start
+// on 16-byte boundaries.  kRows: rows whose copies are under way.
+template <typename T, int V, int kPer, int kRows>
+__global__ void __launch_bounds__(ring_threads(kPer)) norm_backward_ring_kernel(const BackwardArgs a) {
   using Vec = Elements<T, V>;
+  extern __shared__ __align__(16) unsigned char slots[];
   __shared__ float red[2][32];         // in turn: a row's are read until the next row's barrier
   chain_wait();
   chain_next();
-  const int t = threadIdx.x, team = blockDim.x, vecs = a.dim / V;
-  Vec w[kPer], g[kPer], h[kPer], o[kPer];
-  float dw[kPer][V];
-  float rstd = 0.f;
+  const int t = threadIdx.x, team = blockDim.x, vecs = a.dim / V, tensor = kPer * team;
+  const bool add = a.gh != nullptr;
+  const int stage = (add ? 3 : 2) * tensor;
+  Vec* const weight = reinterpret_cast<Vec*>(slots);
+  Vec* const ring = weight + (vecs * static_cast<int>(sizeof(Vec)) + 15) / 16 * 16 / static_cast<int>(sizeof(Vec)) + t;
+  auto ask = [&](int64_t row, int s) {
+    if (row < a.rows) {
+      const Vec* gy = reinterpret_cast<const Vec*>(static_cast<const T*>(a.gy) + row * a.gy_stride);
+      const Vec* hr = reinterpret_cast<const Vec*>(static_cast<const T*>(a.h) + row * a.h_stride);
+      const Vec* gh = add ? reinterpret_cast<const Vec*>(static_cast<const T*>(a.gh) + row * a.gh_stride) : nullptr;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      dw[i][e] = 0.f;
-      w[i].e[e] = g[i].e[e] = h[i].e[e] = o[i].e[e] = from_float<T>(0.f);
+      for (int i = 0; i < kPer; ++i) {
+        const int v = t + i * team;
+        if (v >= vecs) continue;
+        Vec* at = ring + s * stage + i * team;
+        copy_in(at, gy + v);
+        copy_in(at + tensor, hr + v);
+        if (add) copy_in(at + 2 * tensor, gh + v);
+      }
     }
-    if (t + i * team < vecs) w[i] = static_cast<const Vec*>(a.weight)[t + i * team];
-  }
-  auto load = [&](int64_t row) {
-    const Vec* gy = reinterpret_cast<const Vec*>(static_cast<const T*>(a.gy) + row * a.gy_stride);
-    const Vec* hr = reinterpret_cast<const Vec*>(static_cast<const T*>(a.h) + row * a.h_stride);
-    const Vec* gh = a.gh ? reinterpret_cast<const Vec*>(static_cast<const T*>(a.gh) + row * a.gh_stride) : nullptr;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int v = t + i * team;
-      if (v >= vecs) continue;
-      g[i] = gy[v];
-      h[i] = hr[v];
-      if (gh != nullptr) o[i] = gh[v];
-    }
-    rstd = a.rstd[row];
+    asm volatile("cp.async.commit_group;\n" ::: "memory");
   };
-  if (blockIdx.x < a.rows) load(blockIdx.x);
-  int turn = 0;
+#pragma unroll
+  for (int s = 0; s < kRows; ++s) ask(blockIdx.x + static_cast<int64_t>(s) * gridDim.x, s);
+  float rstd = blockIdx.x < a.rows ? a.rstd[blockIdx.x] : 0.f;
+  for (int v = t; v < vecs; v += team) weight[v] = static_cast<const Vec*>(a.weight)[v];
+  __syncthreads();
+  float2 dw[kPer][(V + 1) / 2];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i)
+#pragma unroll
+    for (int p = 0; p < (V + 1) / 2; ++p) dw[i][p] = make_float2(0.f, 0.f);
+  int turn = 0, s = 0;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
-    float s = 0.f;
+    const int64_t next = row + gridDim.x;
+    const float next_rstd = next < a.rows ? a.rstd[next] : 0.f;
+    asm volatile("cp.async.wait_group %0;\n" ::"n"(kRows - 1) : "memory");
+    // (the row is read twice from its slots: held in registers beside dw it spills)
+    const Vec* const at = ring + s * stage;
+    float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float dy = to_float(g[i].e[e]), u = to_float(h[i].e[e]) * rstd;
-        dw[i][e] = fmaf(dy, u, dw[i][e]);
-        s = fmaf(dy * to_float(w[i].e[e]), u, s);
-      }
-    const float mean = join_sum(s, red[turn]) / static_cast<float>(a.dim);
+      if (t + i * team < vecs)
+        add_products<T, V>(dw[i], sum, at[i * team], at[tensor + i * team], weight[t + i * team], rstd);
+    const float mean = join_sum(sum.x + sum.y, red[turn]) * a.inv_dim;
     Vec* dx = reinterpret_cast<Vec*>(static_cast<T*>(a.dx) + row * a.dim);
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int v = t + i * team;
-      if (v >= vecs) continue;
-      Vec d;
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float gw = to_float(g[i].e[e]) * to_float(w[i].e[e]), u = to_float(h[i].e[e]) * rstd;
-        d.e[e] = from_float<T>(fmaf(rstd, fmaf(-u, mean, gw), to_float(o[i].e[e])));
-      }
-      dx[v] = d;
-    }
-    if (row + gridDim.x < a.rows) load(row + gridDim.x);
+    for (int i = 0; i < kPer; ++i)
+      if (t + i * team < vecs)
+        dx[t + i * team] = gradient_of<T, V>(at[i * team], at[tensor + i * team], weight[t + i * team],
+                                             add ? at[2 * tensor + i * team] : zeros<T, V>(), rstd, mean);
+    ask(row + static_cast<int64_t>(kRows) * gridDim.x, s);
+    if (++s == kRows) s = 0;
+    rstd = next_rstd;
   }
   if (a.parts == nullptr) return;
   float* part = a.parts + static_cast<int64_t>(blockIdx.x) * a.dim;
@@ -327,8 +550,75 @@ __global__ void __launch_bounds__(N_BWD_THREADS) norm_backward_kernel(const Back
     const int v = t + i * team;
     if (v >= vecs) continue;
 #pragma unroll
-    for (int e = 0; e < V; ++e) part[v * V + e] = dw[i][e];
+    for (int e = 0; e < V; ++e) part[v * V + e] = e & 1 ? dw[i][e / 2].y : dw[i][e / 2].x;
   }
+}
+
+// Rows of 16-bit elements that do not start on 16-byte boundaries: the next row's
+// elements are asked for before a row is joined.
+template <typename T, int kPer>
+__global__ void __launch_bounds__(N_MAX_THREADS) norm_backward_kernel(const BackwardArgs a) {
+  using One = Elements<T, 1>;
+  __shared__ float red[2][32];
+  chain_wait();
+  chain_next();
+  const int t = threadIdx.x, team = blockDim.x;
+  One w[kPer], g[kPer], h[kPer], o[kPer];
+  float2 dw[kPer][1];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    dw[i][0] = make_float2(0.f, 0.f);
+    w[i] = g[i] = h[i] = o[i] = zeros<T, 1>();
+    if (t + i * team < a.dim) w[i] = static_cast<const One*>(a.weight)[t + i * team];
+  }
+  auto load = [&](int64_t row, One (&g)[kPer], One (&h)[kPer], One (&o)[kPer]) {
+    const One* gy = reinterpret_cast<const One*>(static_cast<const T*>(a.gy) + row * a.gy_stride);
+    const One* hr = reinterpret_cast<const One*>(static_cast<const T*>(a.h) + row * a.h_stride);
+    const One* gh = a.gh ? reinterpret_cast<const One*>(static_cast<const T*>(a.gh) + row * a.gh_stride) : nullptr;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int v = t + i * team;
+      if (v >= a.dim) continue;
+      g[i] = gy[v];
+      h[i] = hr[v];
+      if (gh != nullptr) o[i] = gh[v];
+    }
+  };
+  float rstd = 0.f;
+  if (blockIdx.x < a.rows) {
+    load(blockIdx.x, g, h, o);
+    rstd = a.rstd[blockIdx.x];
+  }
+  int turn = 0;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
+    float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) add_products<T, 1>(dw[i], sum, g[i], h[i], w[i], rstd);
+    const int64_t next = row + gridDim.x;
+    One ng[kPer], nh[kPer], no[kPer];
+    float next_rstd = 0.f;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) ng[i] = nh[i] = no[i] = zeros<T, 1>();
+    if (next < a.rows) {
+      load(next, ng, nh, no);
+      next_rstd = a.rstd[next];
+    }
+    const float mean = join_sum(sum.x, red[turn]) * a.inv_dim;
+    One* dx = reinterpret_cast<One*>(static_cast<T*>(a.dx) + row * a.dim);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      if (t + i * team < a.dim) dx[t + i * team] = gradient_of<T, 1>(g[i], h[i], w[i], o[i], rstd, mean);
+      g[i] = ng[i];
+      h[i] = nh[i];
+      o[i] = no[i];
+    }
+    rstd = next_rstd;
+  }
+  if (a.parts == nullptr) return;
+  float* part = a.parts + static_cast<int64_t>(blockIdx.x) * a.dim;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i)
+    if (t + i * team < a.dim) part[t + i * team] = dw[i][0].x;
 }
 
 // Rows too wide for registers: dx row by row, and each CTA's part of dw in memory.
@@ -353,7 +643,7 @@ __global__ void __launch_bounds__(N_MAX_THREADS) norm_backward_wide_kernel(const
       if (part != nullptr) part[i] = fmaf(dy, u, part[i]);
       s = fmaf(dy * to_float(weight[i]), u, s);
     }
-    const float mean = join_sum(s, red[turn]) / static_cast<float>(a.dim);
+    const float mean = join_sum(s, red[turn]) * a.inv_dim;
     for (int i = threadIdx.x; i < a.dim; i += N_MAX_THREADS) {
       const float gw = to_float(gy[i]) * to_float(weight[i]), u = to_float(h[i]) * rstd;
       static_cast<T*>(a.dx)[row * a.dim + i] = from_float<T>(fmaf(rstd, fmaf(-u, mean, gw), gh ? to_float(gh[i]) : 0.f));
@@ -371,7 +661,7 @@ __global__ void __launch_bounds__(512) norm_weight_join_kernel(const BackwardArg
   const int col = blockIdx.x * 32 + lane;
   float s = 0.f;
   if (col < a.dim)
-#pragma unroll 4
+#pragma unroll 8
     for (int i = group; i < a.grid; i += 16) s += a.parts[static_cast<int64_t>(i) * a.dim + col];
   red[group][lane] = s;
   __syncthreads();
@@ -396,16 +686,46 @@ int launch_norm(NormArgs a, cudaStream_t s) {
                         a.row_warps == 1 ? 32 * N_SHORT_ROWS : 32 * a.row_warps, 0, s, a);
 }
 
+// CTAs that an SM holds at once, asked for once per size.
+template <typename K>
+int resident(K* kernel, int threads, int smem, std::atomic<int>& known) {
+  int n = known.load(std::memory_order_relaxed);
+  if (n > 0) return n;
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, static_cast<size_t>(smem)) != cudaSuccess || n < 1) {
+    (void)cudaGetLastError();
+    return 1;
+  }
+  known.store(n, std::memory_order_relaxed);
+  return n;
+}
+
+template <typename T, int kPer, bool kNorm, bool kQ8>
+int launch_ring(NormArgs a, cudaStream_t s) {
+  static std::atomic<uint64_t> allowed{0};
+  constexpr int V = 16 / sizeof(T);
+  a.row_warps = warps_for(a.dim / V, kPer);
+  const int side = a.row_warps == 1 ? N_SHORT_ROWS : 1, threads = 32 * a.row_warps * side;
+  const int smem = kAhead * (kNorm && a.residual ? 2 : 1) * kPer * threads * 16 + (kNorm ? a.dim * static_cast<int>(sizeof(T)) : 0);
+  if (!allow_smem(norm_ring_kernel<T, kPer, kNorm, kQ8>, N_SMEM - 1024, allowed)) return MRSA_ERR_LAUNCH;
+  static std::atomic<int> known[2][ring_threads(kPer) / 32 + 1];
+  const int per_sm = resident(norm_ring_kernel<T, kPer, kNorm, kQ8>, threads, smem, known[a.residual != nullptr][threads / 32]);
+  const int64_t need = (a.rows + side - 1) / side, most = static_cast<int64_t>(per_sm) * sm_count();
+  return launch_chained(norm_ring_kernel<T, kPer, kNorm, kQ8>, dim3(static_cast<unsigned>(need < most ? need : most)), threads,
+                        static_cast<size_t>(smem), s, a);
+}
+
 template <typename T, bool kNorm, bool kQ8>
 int norm_of(const NormArgs& a, cudaStream_t s) {
   constexpr int V = 16 / sizeof(T);
   const int64_t e = sizeof(T);
   const bool wide = a.dim % V == 0 && aligned_row(a.x, a.x_stride * e) && aligned_row(a.residual, a.residual_stride * e) &&
                     aligned_row(a.weight, 0) && aligned_row(a.y, 0) && aligned_row(a.h, 0) && aligned_row(a.q, a.q_stride);
-  if (wide && a.dim / V <= 4 * N_MAX_THREADS) {
-    const int vecs = a.dim / V;
-    if (vecs <= 32) return launch_norm<T, V, 1, kNorm, kQ8>(a, s);
-    if (vecs <= 1024) return launch_norm<T, V, 2, kNorm, kQ8>(a, s);
+  const int vecs = a.dim / V, smem8 = (kAhead * (kNorm && a.residual ? 2 : 1) * (vecs + 32 * 8) + (kNorm ? vecs : 0)) * 16;
+  if (wide && vecs <= 4 * N_MAX_THREADS) {
+    if (vecs <= 32) return launch_ring<T, 1, kNorm, kQ8>(a, s);
+    if (vecs <= 64 || (vecs <= 1024 && a.rows <= 4 * sm_count())) return launch_ring<T, 2, kNorm, kQ8>(a, s);
+    if (vecs <= 4 * ring_threads(4)) return launch_ring<T, 4, kNorm, kQ8>(a, s);
+    if (vecs <= 8 * ring_threads(8) && smem8 <= N_SMEM - 2048) return launch_ring<T, 8, kNorm, kQ8>(a, s);
     return launch_norm<T, V, 4, kNorm, kQ8>(a, s);
   }
   if (a.dim <= 1024) return launch_norm<T, 1, 4, kNorm, kQ8>(a, s);
@@ -422,10 +742,30 @@ int norm_of_type(const NormArgs& a, int dtype, cudaStream_t s) {
   return norm_of<float, kNorm, kQ8>(a, s);
 }
 
-// CTAs of the gradient, and so parts of dw: as many as are resident at once.
+// Parts of dw at most: CTAs of the gradient that are resident at once.
 int64_t backward_grid(int64_t rows) {
-  const int64_t most = 4LL * sm_count();
+  const int64_t most = 6LL * sm_count();
   return rows < most ? rows : most;
+}
+
+template <typename T, int V, int kPer, int kRows>
+int launch_backward_rows(BackwardArgs& a, int threads, int smem, cudaStream_t s) {
+  static std::atomic<uint64_t> allowed{0};
+  static std::atomic<int> known[2][ring_threads(kPer) / 32 + 1];
+  if (!allow_smem(norm_backward_ring_kernel<T, V, kPer, kRows>, N_SMEM - 1024, allowed)) return MRSA_ERR_LAUNCH;
+  const int64_t most = static_cast<int64_t>(resident(norm_backward_ring_kernel<T, V, kPer, kRows>, threads, smem,
+                                                     known[a.gh != nullptr][threads / 32])) * sm_count();
+  if (a.grid > most) a.grid = static_cast<int>(most);
+  return launch_chained(norm_backward_ring_kernel<T, V, kPer, kRows>, dim3(static_cast<unsigned>(a.grid)), threads,
+                        static_cast<size_t>(smem), s, a);
+}
+// kAhead rows, or one where so many do not fit (16-bit rows of more than 18000 elements).
+template <typename T, int V, int kPer>
+int launch_backward_ring(BackwardArgs& a, cudaStream_t s) {
+  const int vecs = a.dim / V, threads = 32 * warps_for(vecs, kPer), bytes = sizeof(T) * V;
+  const int row = (a.gh ? 3 : 2) * kPer * threads * bytes, weight = (vecs * bytes + 15) / 16 * 16;
+  if (kAhead * row + weight <= N_SMEM - 1024) return launch_backward_rows<T, V, kPer, kAhead>(a, threads, kAhead * row + weight, s);
+  return launch_backward_rows<T, V, kPer, 1>(a, threads, row + weight, s);
 }
 
 template <typename T>
@@ -436,16 +776,23 @@ int backward_of(BackwardArgs a, cudaStream_t s) {
                     aligned_row(a.h, a.h_stride * e) && aligned_row(a.weight, 0) && aligned_row(a.dx, 0);
   const dim3 grid(static_cast<unsigned>(a.grid));
   int rc;
-  if (wide && a.dim / V <= 1024)
-    rc = launch_chained(norm_backward_kernel<T, V, 2>, grid, 32 * warps_for(a.dim / V, 2), 0, s, a);
-  else if (wide && a.dim / V <= 4 * N_BWD_THREADS)
-    rc = launch_chained(norm_backward_kernel<T, V, 4>, grid, 32 * warps_for(a.dim / V, 4), 0, s, a);
-  else if (a.dim <= 2048)
-    rc = launch_chained(norm_backward_kernel<T, 1, 8>, grid, 32 * warps_for(a.dim, 8), 0, s, a);
-  else if (a.dim <= 16 * N_BWD_THREADS)
-    rc = launch_chained(norm_backward_kernel<T, 1, 16>, grid, 32 * warps_for(a.dim, 16), 0, s, a);
-  else
+  const int vecs = a.dim / V;
+  if (wide && vecs <= 128) {
+    rc = launch_backward_ring<T, V, 1>(a, s);
+  } else if (wide && vecs <= 1024) {
+    rc = launch_backward_ring<T, V, 2>(a, s);
+  } else if (wide && vecs <= 4 * 640) {
+    rc = launch_backward_ring<T, V, 4>(a, s);
+  } else if (a.dim <= 8192) {
+    if constexpr (sizeof(T) == 4)
+      rc = a.dim <= 4096 ? launch_backward_ring<T, 1, 8>(a, s) : launch_backward_ring<T, 1, 16>(a, s);
+    else if (a.dim <= 1024)
+      rc = launch_chained(norm_backward_kernel<T, 2>, grid, 32 * warps_for(a.dim, 2), 0, s, a);
+    else
+      rc = launch_chained(norm_backward_kernel<T, 8>, grid, 32 * warps_for(a.dim, 8), 0, s, a);
+  } else {
     rc = launch_chained(norm_backward_wide_kernel<T>, grid, N_MAX_THREADS, 0, s, a);
+  }
   if (rc || a.dw == nullptr) return rc;
   return launch_chained(norm_weight_join_kernel<T>, dim3((a.dim + 31) / 32), 512, 0, s, a);
 }
@@ -482,6 +829,7 @@ extern "C" int mrsa_add_rms_norm(const mrsa_norm_args* p, mrsa_stream_t stream) 
   a.residual_stride = p->residual_stride;
   a.q_stride = p->q_stride;
   a.dim = static_cast<int>(p->dim);
+  a.inv_dim = 1.f / static_cast<float>(p->dim);
   a.eps = p->eps;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   return p->q ? norm_of_type<true, true>(a, p->dtype, s) : norm_of_type<true, false>(a, p->dtype, s);
@@ -539,6 +887,7 @@ extern "C" int mrsa_add_rms_norm_backward(const mrsa_norm_backward_args* p, void
   a.gh_stride = p->grad_h_stride;
   a.h_stride = p->h_stride;
   a.dim = static_cast<int>(p->dim);
+  a.inv_dim = 1.f / static_cast<float>(p->dim);
   a.grid = static_cast<int>(backward_grid(p->rows));
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (p->dtype == MRSA_BF16) return backward_of<__nv_bfloat16>(a, s);
