@@ -638,6 +638,12 @@ typedef struct {
  * 8 of mrsa_device_error_flags if a CTA gave up on a bounded wait. */
 int mrsa_gemm_int8(const mrsa_gemm_int8_args* a, mrsa_stream_t stream);
 
+/* Rows of k bytes, src_stride apart, copied to rows as mrsa_gemm_int8 takes them:
+ * dst 16-byte aligned, dst_stride a multiple of 16, the bytes from k up to the
+ * next multiple of 16 zero. */
+int mrsa_align_rows_int8(const int8_t* src, int64_t src_stride, int8_t* dst, int64_t dst_stride, int64_t rows,
+                         int64_t k, mrsa_stream_t stream);
+
 /* ---------------------------------------------------------------- layers */
 typedef struct {
   /* inputs (device) */

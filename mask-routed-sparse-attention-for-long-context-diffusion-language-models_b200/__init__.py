@@ -12,6 +12,7 @@ from . import _lib
 from .chunk_pool import chunk_attn_pool_gqa, chunk_pool_backward
 from .dense import add_rms_norm
 from .dream_forward import DreamConfig, DreamForward
+from .dream_int8 import DreamInt8
 from .int8 import add_rms_norm_int8, linear_int8, quantize_int8, swiglu_int8
 from .layer import RouteLayer, RouteLayerConfig, swa_layer_forward
 from .local_attention import (bidir_local_attention, cached_local_attention, flex_attn_tl,
@@ -42,7 +43,7 @@ __all__ = [
     "route_scores_backward", "fuse_outputs_backward", "window_attention_backward",
     "rotary_embedding", "rotary_inv_freq", "PagedKVCache", "page_compact", "page_copy", "page_extend", "page_fork",
     "page_free", "paged_append", "paged_attention", "PagedDream", "add_rms_norm", "add_rms_norm_int8", "linear_int8",
-    "quantize_int8", "swiglu_int8",
+    "quantize_int8", "swiglu_int8", "DreamInt8",
 ]
 
 

@@ -97,6 +97,7 @@ _SIGS = {
     "mrsa_add_rms_norm_backward": [_vp, _vp, _sz, _vp],
     "mrsa_add_rms_norm_backward_workspace": [_i64, _i64],
     "mrsa_gemm_int8": [_vp, _vp],
+    "mrsa_align_rows_int8": [_vp, _i64, _vp, _i64, _i64, _i64, _vp],
     "mrsa_device_error_flags": [_int],
     "mrsa_wait_selftest": [_vp, _int, _vp],
     "mrsa_route_layer_workspace_size": [_vp],

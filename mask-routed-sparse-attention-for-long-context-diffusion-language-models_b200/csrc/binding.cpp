@@ -795,7 +795,7 @@ PyObject* quantize_int8(PyObject*, PyObject* const* o, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// 8-bit rows as the products read them: 16-byte boundaries, copied to such rows where they are not.
+// 8-bit rows as the products read them: on 16-byte boundaries, or copied to such rows.
 Tensor whole_rows(const Tensor& x, const char* name) {
   TORCH_CHECK_VALUE(x.defined() && x.scalar_type() == at::kChar, name, " must be INT8");
   Tensor y = as_rows(x, name);
@@ -803,9 +803,11 @@ Tensor whole_rows(const Tensor& x, const char* name) {
   const bool fit = reinterpret_cast<uintptr_t>(y.const_data_ptr()) % 16 == 0 &&
                    (y.size(0) <= 1 || (y.stride(0) % 16 == 0 && y.stride(0) >= k));
   if (fit) return y;
-  Tensor z = at::empty_strided({y.size(0), k}, {pitch_of(k), 1}, y.options());
-  z.copy_(y);
-  return z;
+  TORCH_CHECK_VALUE(k <= MRSA_INT8_MAX_K, name, " must have at most ", MRSA_INT8_MAX_K, " columns (sums of 32 bits)");
+  Tensor z = at::empty({y.size(0), pitch_of(k)}, y.options());
+  checked(mrsa_align_rows_int8(y.const_data_ptr<int8_t>(), y.stride(0), z.mutable_data_ptr<int8_t>(), pitch_of(k), y.size(0), k,
+                               stream_of(y)), "mrsa_align_rows_int8");
+  return z.narrow(1, 0, k);
 }
 int64_t row_pitch(const Tensor& x) { return x.size(0) > 1 ? x.stride(0) : pitch_of(x.size(1)); }
 

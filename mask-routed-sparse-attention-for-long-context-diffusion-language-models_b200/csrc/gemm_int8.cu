@@ -319,6 +319,35 @@ bool make_map(CUtensorMap* m, const void* base, int64_t inner, int64_t rows, int
 
 namespace {
 
+// Rows from anywhere to rows on 16-byte boundaries: a thread puts 16 bytes together
+// from the five aligned words that hold them (bytes one by one at a row's end and
+// where such a word would reach outside the tensor).
+__global__ void __launch_bounds__(256) align_rows_kernel(const int8_t* __restrict__ src, int64_t src_stride, const int8_t* end,
+                                                         int8_t* __restrict__ dst, int64_t dst_stride, int k, int pieces,
+                                                         FastDiv by_pieces, int total) {
+  chain_wait();
+  chain_next();
+  const int i = static_cast<int>(blockIdx.x) * 256 + static_cast<int>(threadIdx.x);
+  if (i >= total) return;
+  const int row = by_pieces.div(i), c = (i - row * pieces) * 16;
+  const int8_t* a = src + row * src_stride + c;
+  const int off = static_cast<int>(reinterpret_cast<uintptr_t>(a) & 3);
+  const uint32_t* p = reinterpret_cast<const uint32_t*>(a - off);
+  uint32_t o[4] = {0u, 0u, 0u, 0u};
+  if (c + 16 <= k && a - off >= src && a - off + 20 <= end) {
+    uint32_t w[5];
+#pragma unroll
+    for (int j = 0; j < 5; ++j) w[j] = p[j];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] = __funnelshift_r(w[j], w[j + 1], 8 * off);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (c + j < k) o[j / 4] |= static_cast<uint32_t>(static_cast<uint8_t>(a[j])) << (8 * (j % 4));
+  }
+  *reinterpret_cast<uint4*>(dst + row * dst_stride + c) = make_uint4(o[0], o[1], o[2], o[3]);
+}
+
 template <typename T> constexpr CUtensorMapDataType kMapType =
     sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16;     // 16 bits are 16 bits
 
@@ -394,4 +423,26 @@ extern "C" int mrsa_gemm_int8(const mrsa_gemm_int8_args* p, mrsa_stream_t stream
   if (p->dtype == MRSA_BF16) return launch_type<__nv_bfloat16>(p, a, s);
   if (p->dtype == MRSA_F16) return launch_type<__half>(p, a, s);
   return launch_type<float>(p, a, s);
+}
+
+extern "C" int mrsa_align_rows_int8(const int8_t* src, int64_t src_stride, int8_t* dst, int64_t dst_stride, int64_t rows,
+                                    int64_t k, mrsa_stream_t stream) {
+  if (rows < 0 || k < 1 || k > MRSA_INT8_MAX_K || src_stride < 0 || dst_stride < k) return MRSA_ERR_SHAPE;
+  if (rows == 0) return MRSA_OK;
+  if (!src || !dst) return MRSA_ERR_NULL;
+  if ((reinterpret_cast<uintptr_t>(dst) | static_cast<uintptr_t>(dst_stride)) & 15) return MRSA_ERR_ALIGN;
+  const mrsa::DeviceScope device_scope(src);
+  const int pieces = static_cast<int>((k + 15) / 16);
+  FastDiv by_pieces;
+  by_pieces.set(static_cast<uint32_t>(pieces));
+  const int64_t at_once = 0x7ffffe00LL / pieces;
+  const int8_t* end = src + (rows - 1) * src_stride + k;
+  for (int64_t r = 0; r < rows; r += at_once) {
+    const int total = static_cast<int>((rows - r < at_once ? rows - r : at_once) * pieces);
+    if (int rc = launch_chained(align_rows_kernel, dim3(static_cast<unsigned>((total + 255) / 256)), 256, 0,
+                                static_cast<cudaStream_t>(stream), src + r * src_stride, src_stride, end, dst + r * dst_stride,
+                                dst_stride, static_cast<int>(k), pieces, by_pieces, total))
+      return rc;
+  }
+  return MRSA_OK;
 }

@@ -117,13 +117,22 @@ class DreamForward:
         blocks = wgu.view(c.ffn // 128, 2, 128, c.hidden)
         return blocks[:, 0].reshape(c.ffn, c.hidden), blocks[:, 1].reshape(c.ffn, c.hidden)
 
-    def attention(self, idx, h, position_ids, key_valid):
-        """Attention output of layer ``idx`` before ``o_proj``: ``[B, L, Hq*D]``."""
+    def project(self, idx, h):
+        """q, k and v ``[B, L, heads, D]`` of layer ``idx`` from its normed input."""
         c, lay = self.cfg, self.layers[idx]
         b, l, _ = h.shape
-        q = linear(h, lay["wq"], lay["bq"]).view(b, l, c.q_heads, c.head_dim)
-        k = linear(h, lay["wk"], lay["bk"]).view(b, l, c.kv_heads, c.head_dim)
-        v = linear(h, lay["wv"], lay["bv"]).view(b, l, c.kv_heads, c.head_dim)
+        return (linear(h, lay["wq"], lay["bq"]).view(b, l, c.q_heads, c.head_dim),
+                linear(h, lay["wk"], lay["bk"]).view(b, l, c.kv_heads, c.head_dim),
+                linear(h, lay["wv"], lay["bv"]).view(b, l, c.kv_heads, c.head_dim))
+
+    def attention(self, idx, h, position_ids, key_valid):
+        """Attention output of layer ``idx`` before ``o_proj``: ``[B, L, Hq*D]``."""
+        return self.attend(idx, *self.project(idx, h), h, position_ids, key_valid)
+
+    def attend(self, idx, q, k, v, h, position_ids, key_valid):
+        """The same from the projections (``h``, the normed input, is read by route layers only)."""
+        c, lay = self.cfg, self.layers[idx]
+        b, l = q.shape[:2]
         if "route" in lay:
             o = lay["route"].forward(q, k, v, h, position_ids, key_valid)
         else:
@@ -132,26 +141,47 @@ class DreamForward:
                                     skip_inert=False, chunk=c.chunk, need_lse=False)
         return o.reshape(b, l, c.q_heads * c.head_dim)
 
-    def layer(self, idx, x, position_ids, key_valid):
+    # A layer is entered with the residual stream (begin makes one from embeddings)
+    # and left with it; what it is, is the model's own affair (dream_int8.py).
+    def begin(self, x):
+        return x
+
+    def stream(self, x):
+        """The residual stream as a tensor."""
+        return x
+
+    def enter(self, idx, x):
+        """``(q, k, v, h, x)``: the projections and normed input of layer ``idx``, and the stream."""
+        h = self.rms_norm(x, self.layers[idx]["in_norm"])
+        return (*self.project(idx, h), h, x)
+
+    def leave(self, idx, o, x):
+        """The stream behind layer ``idx`` with attention output ``o [B, L, Hq*D]``."""
         lay = self.layers[idx]
-        h = self.rms_norm(x, lay["in_norm"])
-        x = linear_residual(self.attention(idx, h, position_ids, key_valid), lay["wo"], x)
+        x = linear_residual(o, lay["wo"], x)
         h = self.rms_norm(x, lay["post_norm"])
         return linear_residual(swiglu(h, lay["wgu"]), lay["wd"], x)
+
+    def end(self, x, logits: bool = True):
+        """Logits, or the final hidden states, of the stream."""
+        x = self.rms_norm(x, self.final_norm)
+        return linear(x, self.lm_head) if logits else x
+
+    def layer(self, idx, x, position_ids, key_valid):
+        q, k, v, h, x = self.enter(idx, x)
+        return self.leave(idx, self.attend(idx, q, k, v, h, position_ids, key_valid), x)
 
     @torch.inference_mode()
     def forward(self, ids, position_ids, key_valid=None, *, logits: bool = True, return_layer_inputs=False):
         lmk = (torch.arange(ids.shape[1], device=ids.device) + 1) % self.cfg.chunk == 0
         x = self.embed[ids]
-        x = torch.where(lmk[None, :, None], x + self.role, x)
+        x = self.begin(torch.where(lmk[None, :, None], x + self.role, x))
         inputs = []
         for idx in range(self.cfg.layers):
             if return_layer_inputs:
-                inputs.append(x)
+                inputs.append(self.stream(x))
             x = self.layer(idx, x, position_ids, key_valid)
-        out = self.rms_norm(x, self.final_norm)
-        if logits:
-            out = linear(out, self.lm_head)
+        out = self.end(x, logits)
         return (out, inputs) if return_layer_inputs else out
 
     __call__ = forward

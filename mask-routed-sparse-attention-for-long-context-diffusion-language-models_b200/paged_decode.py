@@ -29,13 +29,13 @@ from __future__ import annotations
 
 import torch
 
-from .dense import linear, linear_residual, swiglu
 from .dream_forward import DreamForward
 from .paged_cache import PagedKVCache
 
 
 class PagedDream:
-    """``model``'s weights with full attention and a cache of ``pages`` pages
+    """``model``'s weights (:class:`DreamForward`, or :class:`DreamInt8` for
+    dense layers in 8 bits) with full attention and a cache of ``pages`` pages
     for all layers."""
 
     def __init__(self, model: DreamForward, *, pages: int, sequences: int, max_len: int, page_size: int = 64):
@@ -55,21 +55,14 @@ class PagedDream:
         ``causal`` (last positions only) the tokens up to itself."""
         m, c = self.model, self.model.cfg
         b, s = ids.shape
-        x = m.embed[ids]
+        x = m.begin(m.embed[ids])
         for idx in range(c.layers):
-            lay = m.layers[idx]
-            h = m.rms_norm(x, lay["in_norm"])
-            q = linear(h, lay["wq"], lay["bq"]).view(b, s, c.q_heads, c.head_dim)
-            k = linear(h, lay["wk"], lay["bk"]).view(b, s, c.kv_heads, c.head_dim)
-            v = linear(h, lay["wv"], lay["bv"]).view(b, s, c.kv_heads, c.head_dim)
+            q, k, v, _, x = m.enter(idx, x)
             q = self.cache.append(idx, seqs, k, v, q=q, start=start, position_ids=position_ids, inv_freq=m.inv_freq,
                                   attention_factor=m.attention_factor)
             o = self.cache.attend(idx, seqs, q, causal=causal, key_valid=key_valid)
-            x = linear_residual(o.reshape(b, s, c.q_heads * c.head_dim), lay["wo"], x)
-            h = m.rms_norm(x, lay["post_norm"])
-            x = linear_residual(swiglu(h, lay["wgu"]), lay["wd"], x)
-        x = m.rms_norm(x, m.final_norm)
-        return linear(x, m.lm_head) if logits else x
+            x = m.leave(idx, o.reshape(b, s, c.q_heads * c.head_dim), x)
+        return m.end(x, logits)
 
     def prefill(self, seqs, ids, **kw):
         """The tokens ``ids [B, S]`` appended to the sequences: room for them,

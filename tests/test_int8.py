@@ -226,6 +226,21 @@ def test_layouts(mrsa, cuda_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,k", [(1, 1), (3, 15), (2, 16), (5, 17), (1000, 31), (7, 4097), (40, 1003)])
+def test_rows_off_boundaries(mrsa, cuda_device, rows, k):
+    """Rows at every offset of a 16-byte boundary, at the very ends of their memory, at any distance."""
+    L, dev = mrsa._lib, cuda_device
+    for off in range(0, 16, 5):
+        for pad in (0, 1, 2, 13):
+            flat = torch.randint(-128, 128, (off + (rows - 1) * (k + pad) + k,), device=dev, dtype=torch.int8)
+            x = torch.as_strided(flat, (rows, k), (k + pad, 1), off)
+            pitch = (k + 15) // 16 * 16
+            y = torch.full((rows, pitch), 77, dtype=torch.int8, device=dev)
+            L.call("mrsa_align_rows_int8", L.ptr(x), k + pad, L.ptr(y), pitch, rows, k, L.stream_of(x))
+            assert torch.equal(y[:, :k], x) and not y[:, k:].any()
+
+
+@pytest.mark.gpu
 def test_streams_and_graphs(mrsa, cuda_device):
     """A layer of few rows and one of many on two streams at once, and in two graphs replayed together."""
     dev = cuda_device
@@ -359,3 +374,7 @@ def test_argument_codes(mrsa):
     assert q8(4096, 8, 4096, 16, 4096, 2, 8, 3, None) == L.ERR_ARG and q8(4097, 8, 4096, 16, 4096, 2, 8, 0, None) == L.ERR_ALIGN
     assert q8(4096, 8, 4096, 16, 4096, 0, 8, 0, None) == 0
     assert L.GEMM_INT8_ARGS.size == 104
+    al = lib.mrsa_align_rows_int8
+    assert al(0, 8, 4096, 16, 2, 8, None) == L.ERR_NULL and al(4096, 8, 4096, 16, 2, 0, None) == L.ERR_SHAPE
+    assert al(4096, 8, 4096, 16, 2, 17, None) == L.ERR_SHAPE and al(4096, 8, 4096, 24, 2, 8, None) == L.ERR_ALIGN
+    assert al(4096, -8, 4096, 16, 2, 8, None) == L.ERR_SHAPE and al(4096, 8, 4096, 16, 0, 8, None) == 0
