@@ -281,8 +281,8 @@ void note_cuda_error(cudaError_t e, const char* where);
 // Programmatic dependent launch, for chains of short kernels: a kernel launched
 // with launch_chained may be put in place while the one before it in the stream
 // still runs (once every CTA of that has called chain_next, or ended), and
-// touches no memory (nor allocates tensor memory that the one before may still
-// ask for) before chain_wait, which returns when all before it is done and seen.
+// touches no memory (but to fetch it into L2; nor allocates tensor memory that the
+// one before may still ask for) before chain_wait, which returns when all before it is done and seen.
 // Every thread of such a kernel calls chain_wait, so that the end of a grid
 // implies the end of those before it, and calls chain_next after it, so that a
 // kernel put in place early finds everything but the one before it done.

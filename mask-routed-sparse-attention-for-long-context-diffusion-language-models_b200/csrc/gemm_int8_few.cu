@@ -9,10 +9,17 @@
 // rate unused.  Each CTA streams its K blocks of both operands by TMA; then the
 // clusters' CTAs put their sums in shared memory, and each adds up its share of
 // the tokens over all of them (32-bit integers: the order does not matter),
-// scales them and writes them out, channels along a warp.
+// scales them and writes them out, channels along a warp.  Many tokens under long
+// sums take tiles of 256 channels by 256 tokens, a pair of CTAs (cta_group::2) to
+// each share of K.
 //
-// Every wait is bounded; a CTA that gives up drains its copies and MMAs, still
-// meets its cluster, and sets bit 8 of mrsa_device_error_flags.
+// Measured (B200, us; a launch among others, the weights not in L2; floor by bytes):
+// one token x 4608 x 3584 7.0 (2.5; about 2.5 of it is any launch, 1 the cluster's),
+// x 152064 x 3584 81 (83), x 3584 x 18944 14.8 (10.4), gated x 37888 x 3584 22.7
+// (20.7); 32 tokens 7.9, 15.1 and 23.8; 256 x 3584 x 18944 21.7 (11.4).
+//
+// Every wait is bounded; a CTA that gives up tells its pair, drains its copies and
+// MMAs, still meets its cluster, and sets bit 8 of mrsa_device_error_flags.
 #include "gemm_int8.cuh"
 
 using namespace mrsa;
@@ -22,20 +29,21 @@ namespace {
 
 constexpr int F_THREADS = 256, BC = 128;         // channels of an MMA
 constexpr int F_MAX_CLUSTER = 8;        // the portable most
+constexpr int F_AHEAD = 8;              // K blocks of weights fetched into L2 before the launch's turn
 
 __device__ int g_few_error;
 
-constexpr int stage_bytes(int tokens, bool gated) { return ((gated ? 2 : 1) * BC + tokens) * BK; }
+constexpr int stage_bytes(int tokens, bool gated, bool pair) { return ((gated ? 2 : 1) * BC + tokens / (pair ? 2 : 1)) * BK; }
 // One CTA per SM with a deep pipeline, or two with half of it each, so that one's
 // copies run while the other sums up.
-constexpr int stages(int tokens, bool gated, int per_sm) {
-  const int n = (per_sm == 2 ? 110 : 222) * 1024 / stage_bytes(tokens, gated);
+constexpr int stages(int tokens, bool gated, int per_sm, bool pair = false) {
+  const int n = (per_sm == 2 ? 110 : 222) * 1024 / stage_bytes(tokens, gated, pair);
   return n < 8 ? n : 8;
 }
 
-template <int kTokens, bool kGated, int kPerSm>
+template <int kTokens, bool kGated, int kPerSm, bool kPair>
 struct __align__(1024) FewSmem {
-  static constexpr int ST = stages(kTokens, kGated, kPerSm), BYTES = stage_bytes(kTokens, kGated);
+  static constexpr int ST = stages(kTokens, kGated, kPerSm, kPair), BYTES = stage_bytes(kTokens, kGated, kPair);
   static constexpr int SUMS = (kGated ? 2 : 1) * kTokens * BC * 4;         // the CTA's sums [accumulator][token][channel]
   unsigned char tiles[ST * BYTES > SUMS ? ST * BYTES : SUMS];
   float a_scale[kTokens];
@@ -44,30 +52,28 @@ struct __align__(1024) FewSmem {
   int abort_flag;
 };
 
-__device__ __forceinline__ void cluster_barrier() {
-  asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;\n" ::: "memory");
-}
-// Four sums in the shared memory of the cluster's CTA `rank`, at this CTA's address p.
-__device__ __forceinline__ int4 peer_sums(const void* p, int rank) {
-  uint32_t at;
+// Four sums at an address of the cluster's window.
+__device__ __forceinline__ int4 peer_sums(uint32_t at) {
   int4 v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
-  asm volatile("ld.shared::cluster.v4.s32 {%0,%1,%2,%3}, [%4];\n"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  asm volatile("ld.shared::cluster.v4.s32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
   return v;
 }
 
-template <typename T, int kTokens, bool kGated, int kPerSm>
+template <typename T, int kTokens, bool kGated, int kPerSm, bool kPair>
 __global__ void __launch_bounds__(F_THREADS, kPerSm) gemm_int8_few_kernel(const __grid_constant__ CUtensorMap tm_a,
                                                                   const __grid_constant__ CUtensorMap tm_b, const Args a,
                                                                   const int share) {
-  using Smem = FewSmem<kTokens, kGated, kPerSm>;
+  using Smem = FewSmem<kTokens, kGated, kPerSm, kPair>;
   constexpr int ST = Smem::ST, kAcc = kGated ? 2 : 1;
   constexpr int kColumns = kAcc * kTokens < 32 ? 32 : kAcc * kTokens;
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   Smem& sm = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = static_cast<int>(blockIdx.x) % share, tn = static_cast<int>(blockIdx.x) / share, tm = blockIdx.y;
+  // this CTA's share of K, its half of the pair's channels (and of the copies of the tokens), its tile
+  constexpr int kHalves = kPair ? 2 : 1;
+  const int in_cluster = static_cast<int>(blockIdx.x) % (share * kHalves), tm = blockIdx.y;
+  const int rank = in_cluster / kHalves, half = in_cluster % kHalves, first_half = in_cluster - half;
+  const int tn = static_cast<int>(blockIdx.x) / (share * kHalves) * kHalves + half;      // of 128 channels (gated: 256)
   const int k0 = static_cast<int>(static_cast<int64_t>(a.k_blocks) * rank / share);
   const int k1 = static_cast<int>(static_cast<int64_t>(a.k_blocks) * (rank + 1) / share);
   if (threadIdx.x == 0) {
@@ -81,14 +87,25 @@ __global__ void __launch_bounds__(F_THREADS, kPerSm) gemm_int8_few_kernel(const 
     tc::prefetch_tensormap(&tm_a);
     tc::prefetch_tensormap(&tm_b);
   }
+  // While the launch before still runs: nothing is read here, and should that launch
+  // write the weights, L2 is where it writes them.  0, 4, 8, 16 and all K blocks: a
+  // decode step of one token 2.19, 2.14, 2.12, 2.15, 2.32 ms.
+  if (threadIdx.x == 0)
+    for (int kb = k0; kb < min(k1, k0 + F_AHEAD); ++kb) tc::tma_prefetch_2d(&tm_b, kb * BK, tn * kAcc * BC);
   chain_wait();
   chain_next();
   if (warp == 1) {
-    tc::tmem_alloc(tc::smem_addr(&sm.tmem_base), kColumns);
-    tc::tmem_relinquish();
+    if (kPair) {
+      tc::pair_tmem_alloc(tc::smem_addr(&sm.tmem_base), kColumns);
+      tc::pair_tmem_relinquish();
+    } else {
+      tc::tmem_alloc(tc::smem_addr(&sm.tmem_base), kColumns);
+      tc::tmem_relinquish();
+    }
   }
   tc::fence_before_sync();
   __syncthreads();
+  if (kPair) tc::cluster_sync();         // both CTAs' barriers and tensor memory are there
   tc::fence_after_sync();
   const uint32_t tbase = sm.tmem_base;
   volatile int* ab = &sm.abort_flag;
@@ -100,18 +117,26 @@ __global__ void __launch_bounds__(F_THREADS, kPerSm) gemm_int8_few_kernel(const 
         const int s = it % ST;
         if (it >= ST && !tc::wait_bounded(tc::smem_addr(&sm.empty[s]), static_cast<uint32_t>((it / ST - 1) & 1), ab)) break;
         const uint32_t bar = tc::smem_addr(&sm.full[s]), at = tc::smem_addr(sm.tiles + s * Smem::BYTES);
-        tc::mbar_arrive_expect_tx(bar, Smem::BYTES);
-        tc::tma_load_2d(at, &tm_b, kb * BK, tn * kAcc * BC, bar);            // kAcc * 128 channels
-        tc::tma_load_2d(at + kAcc * BC * BK, &tm_a, kb * BK, tm * kTokens, bar);
+        if (kPair) {                       // both CTAs' copies count on the even one's barrier
+          const uint32_t shared_bar = tc::peer_addr(bar, first_half);
+          if (half == 0) tc::mbar_arrive_expect_tx(bar, 2 * Smem::BYTES);
+          tc::pair_tma_load_2d(at, &tm_b, kb * BK, tn * BC, shared_bar);
+          tc::pair_tma_load_2d(at + BC * BK, &tm_a, kb * BK, tm * kTokens + half * (kTokens / 2), shared_bar);
+        } else {
+          tc::mbar_arrive_expect_tx(bar, Smem::BYTES);
+          tc::tma_load_2d(at, &tm_b, kb * BK, tn * kAcc * BC, bar);            // kAcc * 128 channels
+          tc::tma_load_2d(at + kAcc * BC * BK, &tm_a, kb * BK, tm * kTokens, bar);
+        }
       }
-      // copies still in flight after an abort: the last one issued into each stage
-      if (*ab)
+      // copies still in flight after an abort: the last one issued into each stage (the
+      // odd CTA of a pair stays until the even one has seen its copies land too)
+      if (*ab && half == 0)
         for (int j = it > ST ? it - ST : 0; j < it; ++j)
           tc::mbar_wait(tc::smem_addr(&sm.full[j % ST]), static_cast<uint32_t>((j / ST) & 1), 4000000u);
     }
     __syncwarp();
-  } else if (warp == 1) {
-    constexpr uint32_t idesc = tc::idesc_s8_s32(BC, kTokens);
+  } else if (warp == 1 && half == 0) {
+    constexpr uint32_t idesc = tc::idesc_s8_s32(kHalves * BC, kTokens);
     const uint64_t dw = tc::smem_desc_sw128(tc::smem_addr(sm.tiles), 16, 1024);
     const uint64_t dt = tc::desc_adv(dw, kAcc * BC * BK);
     for (int kb = k0, it = 0; kb < k1; ++kb, ++it) {
@@ -123,16 +148,22 @@ __global__ void __launch_bounds__(F_THREADS, kPerSm) gemm_int8_few_kernel(const 
 #pragma unroll
         for (int acc = 0; acc < kAcc; ++acc)
 #pragma unroll
-          for (int kk = 0; kk < BK / 32; ++kk)
-            tc::mma_s8_ss(tbase + acc * kTokens, tc::desc_adv(dw, so + acc * BC * BK + kk * 32), tc::desc_adv(dt, so + kk * 32),
-                          idesc, it > 0 || kk > 0);
-        tc::mma_commit(tc::smem_addr(&sm.empty[s]));
+          for (int kk = 0; kk < BK / 32; ++kk) {
+            const uint64_t w = tc::desc_adv(dw, so + acc * BC * BK + kk * 32), x = tc::desc_adv(dt, so + kk * 32);
+            if (kPair) tc::pair_mma_s8_ss(tbase, w, x, idesc, it > 0 || kk > 0);
+            else tc::mma_s8_ss(tbase + acc * kTokens, w, x, idesc, it > 0 || kk > 0);
+          }
+        if (kPair) tc::pair_commit(tc::smem_addr(&sm.empty[s]), first_half);
+        else tc::mma_commit(tc::smem_addr(&sm.empty[s]));
       }
       __syncwarp();
     }
-    if (tc::elect_one()) tc::mma_commit(tc::smem_addr(&sm.done));
+    if (tc::elect_one()) {
+      if (kPair) tc::pair_commit(tc::smem_addr(&sm.done), first_half);
+      else tc::mma_commit(tc::smem_addr(&sm.done));
+    }
     __syncwarp();
-  } else {
+  } else if (warp >= 2) {
     for (int i = threadIdx.x - 64; i < kTokens; i += F_THREADS - 64)
       sm.a_scale[i] = tm * kTokens + i < a.M ? a.a_scale[tm * kTokens + i] : 0.f;
   }
@@ -168,35 +199,34 @@ __global__ void __launch_bounds__(F_THREADS, kPerSm) gemm_int8_few_kernel(const 
   }
   tc::fence_before_sync();
   __syncthreads();
-  if (share > 1) cluster_barrier();
+  if (share > 1) tc::cluster_sync();
   // This CTA's share of the tokens, a warp to a token, four channels to a lane.
   const int tokens = min(kTokens, a.M - tm * kTokens), per = (tokens + share - 1) / share, first = rank * per, last = min(first + per, tokens);
   T* c = static_cast<T*>(a.c);
   const int col = tn * BC + lane * 4, cols = kGated ? a.N / 2 : a.N;
   const bool four = a.ldc % 4 == 0 && reinterpret_cast<uintptr_t>(c) % (4 * sizeof(T)) == 0;
   constexpr int kWarps = F_THREADS / 32, kAtOnce = kGated ? 2 : 4;
-  for (int t0 = first + warp; t0 < last; t0 += kWarps * kAtOnce) {
-    // kAtOnce tokens' loads from each CTA in flight together
-    int4 s[kAtOnce][kAcc];
+  const bool whole = four && col + 4 <= cols;
+  // kTok tokens, kWarps apart: their loads from each CTA in flight together
+  auto write_tokens = [&](int tok, auto count) {
+    constexpr int kTok = decltype(count)::value;
+    int4 s[kTok][kAcc];
+    const int* own = sums + tok * BC + lane * 4;
 #pragma unroll
-    for (int i = 0; i < kAtOnce; ++i)
+    for (int i = 0; i < kTok; ++i)
 #pragma unroll
-      for (int acc = 0; acc < kAcc; ++acc) s[i][acc] = make_int4(0, 0, 0, 0);
-    for (int r = 0; r < share; ++r) {
-      int peer = rank + r;                       // each CTA begins with its own sums
+      for (int acc = 0; acc < kAcc; ++acc) s[i][acc] = *reinterpret_cast<const int4*>(own + (acc * kTokens + i * kWarps) * BC);
+    for (int r = 1; r < share; ++r) {
+      int peer = rank + r;                       // each CTA begins elsewhere
       if (peer >= share) peer -= share;
-      int4 v[kAtOnce][kAcc];
+      const uint32_t at = tc::peer_addr(smem_u32(own), peer * kHalves + half);
+      int4 v[kTok][kAcc];
 #pragma unroll
-      for (int i = 0; i < kAtOnce; ++i)
+      for (int i = 0; i < kTok; ++i)
 #pragma unroll
-        for (int acc = 0; acc < kAcc; ++acc) {
-          v[i][acc] = make_int4(0, 0, 0, 0);
-          if (t0 + i * kWarps >= last) continue;
-          const int* at = sums + (acc * kTokens + t0 + i * kWarps) * BC + lane * 4;
-          v[i][acc] = r == 0 ? *reinterpret_cast<const int4*>(at) : peer_sums(at, peer);
-        }
+        for (int acc = 0; acc < kAcc; ++acc) v[i][acc] = peer_sums(at + (acc * kTokens + i * kWarps) * BC * 4);
 #pragma unroll
-      for (int i = 0; i < kAtOnce; ++i)
+      for (int i = 0; i < kTok; ++i)
 #pragma unroll
         for (int acc = 0; acc < kAcc; ++acc) {
           s[i][acc].x += v[i][acc].x;
@@ -205,22 +235,30 @@ __global__ void __launch_bounds__(F_THREADS, kPerSm) gemm_int8_few_kernel(const 
           s[i][acc].w += v[i][acc].w;
         }
     }
+    T* dst = c + (static_cast<int64_t>(tm) * kTokens + tok) * a.ldc + col;
 #pragma unroll
-    for (int i = 0; i < kAtOnce; ++i) {
-      const int tok = t0 + i * kWarps;
-      if (tok >= last) break;
-      const float as = sm.a_scale[tok];
-      const int n0[4] = {s[i][0].x, s[i][0].y, s[i][0].z, s[i][0].w};
-      const int n1[4] = {s[i][kAcc - 1].x, s[i][kAcc - 1].y, s[i][kAcc - 1].z, s[i][kAcc - 1].w};
+    for (int i = 0; i < kTok; ++i, dst += kWarps * a.ldc) {
+      const float as = sm.a_scale[tok + i * kWarps];
+      const float2 as2 = make_float2(as, as);
+      auto scaled = [&](int4 n, const float (&b)[4], int p) {
+        const float2 f = p == 0 ? make_float2(static_cast<float>(n.x), static_cast<float>(n.y))
+                                : make_float2(static_cast<float>(n.z), static_cast<float>(n.w));
+        return fmul2(fmul2(f, as2), make_float2(b[2 * p], b[2 * p + 1]));
+      };
       struct alignas(4 * sizeof(T)) Four { T e[4]; } o;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float v = static_cast<float>(n0[e]) * as;
-        if (kGated) o.e[e] = from_float<T>(silu<T>(v * bs[0][e]) * (static_cast<float>(n1[e]) * as * bs[kAcc - 1][e]));
-        else o.e[e] = from_float<T>(fmaf(v, bs[0][e], bias[e]));
+      for (int p = 0; p < 2; ++p) {
+        float2 v = scaled(s[i][0], bs[0], p);
+        if (kGated) {
+          const float2 u = scaled(s[i][kAcc - 1], bs[kAcc - 1], p);
+          v = make_float2(silu<T>(v.x) * u.x, silu<T>(v.y) * u.y);
+        } else {
+          v = fadd2(v, make_float2(bias[2 * p], bias[2 * p + 1]));
+        }
+        o.e[2 * p] = from_float<T>(v.x);
+        o.e[2 * p + 1] = from_float<T>(v.y);
       }
-      T* dst = c + (static_cast<int64_t>(tm) * kTokens + tok) * a.ldc + col;
-      if (four && col + 4 <= cols) {
+      if (whole) {
         *reinterpret_cast<Four*>(dst) = o;
       } else {
 #pragma unroll
@@ -228,10 +266,18 @@ __global__ void __launch_bounds__(F_THREADS, kPerSm) gemm_int8_few_kernel(const 
           if (col + e < cols) dst[e] = o.e[e];
       }
     }
-  }
-  if (share > 1) cluster_barrier();      // no CTA leaves while another reads its memory
+  };
+  int tok = first + warp;
+  for (; tok + (kAtOnce - 1) * kWarps < last; tok += kWarps * kAtOnce) write_tokens(tok, std::integral_constant<int, kAtOnce>());
+  for (; tok < last; tok += kWarps) write_tokens(tok, std::integral_constant<int, 1>());
+  if (kPair && *ab) tc::peer_store(tc::peer_addr(tc::smem_addr(&sm.abort_flag), in_cluster ^ 1), 1);
+  if (share > 1 || kPair) tc::cluster_sync();      // no CTA leaves while another reads its memory
   if (threadIdx.x == 0 && *ab) atomicOr(&g_few_error, 1);
-  if (warp == 1) tc::tmem_dealloc(tbase, kColumns);
+  if (warp == 1) {
+    tc::fence_after_sync();
+    if (kPair) tc::pair_tmem_dealloc(tbase, kColumns);
+    else tc::tmem_dealloc(tbase, kColumns);
+  }
 }
 
 // How many clusters of `cluster` CTAs the device holds at once (GPCs have no whole
@@ -261,18 +307,18 @@ int resident_clusters(int cluster, int smem) {
   return n;
 }
 
-template <typename T, int kTokens, bool kGated, int kPerSm>
+template <typename T, int kTokens, bool kGated, int kPerSm, bool kPair = false>
 int launch(const mrsa_gemm_int8_args* p, Args a, cudaStream_t s) {
   static std::atomic<uint64_t> allowed{0};
-  constexpr int smem = sizeof(FewSmem<kTokens, kGated, kPerSm>) + 1024;
-  constexpr int kChannels = (kGated ? 2 : 1) * BC;
+  constexpr int smem = sizeof(FewSmem<kTokens, kGated, kPerSm, kPair>) + 1024;
+  constexpr int kChannels = (kGated ? 2 : 1) * BC, kHalves = kPair ? 2 : 1;
   CUtensorMap tma, tmb;
-  if (!make_map(&tma, p->a, p->k, p->m, p->a_stride, kTokens) || !make_map(&tmb, p->b, p->k, p->n, p->b_stride, kChannels)) {
+  if (!make_map(&tma, p->a, p->k, p->m, p->a_stride, kTokens / kHalves) || !make_map(&tmb, p->b, p->k, p->n, p->b_stride, kChannels)) {
     note_cuda_error(cudaErrorInvalidValue, "mrsa_gemm_int8: tensor map encoding");
     return MRSA_ERR_LAUNCH;
   }
-  if (!allow_smem(gemm_int8_few_kernel<T, kTokens, kGated, kPerSm>, smem, allowed)) return MRSA_ERR_LAUNCH;
-  a.n_tiles = (a.N + kChannels - 1) / kChannels;
+  if (!allow_smem(gemm_int8_few_kernel<T, kTokens, kGated, kPerSm, kPair>, smem, allowed)) return MRSA_ERR_LAUNCH;
+  a.n_tiles = (a.N + kHalves * kChannels - 1) / (kHalves * kChannels);
   a.m_tiles = (a.M + kTokens - 1) / kTokens;
   const int64_t tiles = static_cast<int64_t>(a.n_tiles) * a.m_tiles;
   // As many CTAs to a tile as leave all clusters resident at once, each with four K
@@ -280,12 +326,12 @@ int launch(const mrsa_gemm_int8_args* p, Args a, cudaStream_t s) {
   // a second turn of clusters costs as much as the first.
   int64_t share = 1;
   if (kPerSm == 1) {
-    share = a.k_blocks / 4 < F_MAX_CLUSTER ? a.k_blocks / 4 : F_MAX_CLUSTER;
-    while (share > 1 && resident_clusters<gemm_int8_few_kernel<T, kTokens, kGated, kPerSm>>(static_cast<int>(share), smem) < tiles) --share;
+    share = a.k_blocks / 4 < F_MAX_CLUSTER / kHalves ? a.k_blocks / 4 : F_MAX_CLUSTER / kHalves;
+    while (share > 1 && resident_clusters<gemm_int8_few_kernel<T, kTokens, kGated, kPerSm, kPair>>(static_cast<int>(share) * kHalves, smem) < tiles) --share;
     if (share < 1) share = 1;
   }
-  return launch_clusters(gemm_int8_few_kernel<T, kTokens, kGated, kPerSm>, dim3(static_cast<unsigned>(a.n_tiles * share), a.m_tiles),
-                         static_cast<unsigned>(share), F_THREADS, smem, s, tma, tmb, a, static_cast<int>(share));
+  return launch_clusters(gemm_int8_few_kernel<T, kTokens, kGated, kPerSm, kPair>, dim3(static_cast<unsigned>(a.n_tiles * share * kHalves), a.m_tiles),
+                         static_cast<unsigned>(share * kHalves), F_THREADS, smem, s, tma, tmb, a, static_cast<int>(share));
 }
 
 template <typename T, int kTokens, bool kGated>
@@ -301,13 +347,19 @@ int launch_tokens(const mrsa_gemm_int8_args* p, const Args& a, cudaStream_t s) {
   return launch<T, kTokens, kGated, 1>(p, a, s);
 }
 
-// Tiles of 128 tokens at most: of 256, where they would all be in use, no faster
-// (256 tokens x 4608 channels 10.5 us, in tiles of 256 13.2; 512 13.2 and 14.3).
+// Tiles of 256 tokens by a pair of CTAs for long sums of many tokens: half the
+// shared-memory traffic of tiles of 128 (which holds those up), but fewer CTAs share
+// K, and each has more to add up.  In us, tiles of 128 and pairs: K 18944, 256 tokens
+// x 3584 channels 24.0 and 21.7, 512 38.0 and 30.2, 1024 65 and 51; K 3584, 256 x 4608
+// 10.2 and 13.3, 512 11.2 and 14.9, 1024 x 3584 16.8 and 15.6.
 template <typename T, bool kGated>
 int launch_type(const mrsa_gemm_int8_args* p, const Args& a, cudaStream_t s) {
   if (p->m <= 16) return launch_tokens<T, 16, kGated>(p, a, s);
   if (p->m <= 32) return launch_tokens<T, 32, kGated>(p, a, s);
   if (p->m <= 64) return launch_tokens<T, 64, kGated>(p, a, s);
+  if constexpr (!kGated) {
+    if (p->m > 128 && p->m * a.k_blocks >= 28000) return launch<T, 256, false, 1, true>(p, a, s);
+  }
   return launch_tokens<T, 128, kGated>(p, a, s);
 }
 

@@ -217,6 +217,12 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst_smem, const void* map, 
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
       : "memory");
 }
+// The box into L2 only.
+__device__ __forceinline__ void tma_prefetch_2d(const void* map, int x, int y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];\n" ::"l"(reinterpret_cast<uint64_t>(map)),
+               "r"(x), "r"(y)
+               : "memory");
+}
 // The box of shared memory to global memory (what lies outside the tensor is left
 // out); `x` as above, no coordinate negative.  One group per store.
 __device__ __forceinline__ void tma_store_2d(const void* map, int x, int y, uint32_t src_smem) {
@@ -304,11 +310,11 @@ __device__ __forceinline__ void pair_mma_s8_ss(uint32_t d_tmem, uint64_t a_desc,
       "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
       "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate ? 1 : 0));
 }
-// Arrive on the barrier at offset `bar` of both CTAs once the MMAs issued so far complete.
-__device__ __forceinline__ void pair_commit(uint32_t bar) {
+// Arrive on the barrier at offset `bar` of both CTAs (`first`: the even one's rank) once the MMAs issued so far complete.
+__device__ __forceinline__ void pair_commit(uint32_t bar, uint32_t first = 0) {
   asm volatile(
       "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n" ::"r"(bar),
-      "h"(static_cast<uint16_t>(3)));
+      "h"(static_cast<uint16_t>(3u << first)));
 }
 // The same on this CTA's barrier alone.
 __device__ __forceinline__ void pair_commit_own(uint32_t bar) {
