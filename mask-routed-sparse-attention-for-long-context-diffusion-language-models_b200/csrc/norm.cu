@@ -722,6 +722,17 @@ int norm_of(const NormArgs& a, cudaStream_t s) {
                     aligned_row(a.weight, 0) && aligned_row(a.y, 0) && aligned_row(a.h, 0) && aligned_row(a.q, a.q_stride);
   const int vecs = a.dim / V, smem8 = (kAhead * (kNorm && a.residual ? 2 : 1) * (vecs + 32 * 8) + (kNorm ? vecs : 0)) * 16;
   if (wide && vecs <= 4 * N_MAX_THREADS) {
+    // No row behind another on an SM: straight to registers, with as many threads as
+    // there are vectors (one row of 3584: 1.8 us, by the copies ahead 2.3; 18944
+    // quantized 1.9 and 2.4).
+    if (a.rows <= sm_count()) {
+      if (vecs <= N_MAX_THREADS) return launch_norm<T, V, 1, kNorm, kQ8>(a, s);
+      return launch_norm<T, V, 4, kNorm, kQ8>(a, s);
+    }
+    // Four vectors to a thread (a warp to a row of up to 1024 elements of 16 bits), two
+    // where the rows would leave SMs short of warps (256 rows of 3584 in 8 bits 3.2 us,
+    // with four 4.3; 32768 rows 139, with four 135), one for rows of a warp, eight past
+    // 640 threads.
     if (vecs <= 32) return launch_ring<T, 1, kNorm, kQ8>(a, s);
     if (vecs <= 64 || (vecs <= 1024 && a.rows <= 4 * sm_count())) return launch_ring<T, 2, kNorm, kQ8>(a, s);
     if (vecs <= 4 * ring_threads(4)) return launch_ring<T, 4, kNorm, kQ8>(a, s);

@@ -12,8 +12,9 @@ form without a pass of its own::
     q, scale, x = add_rms_norm_int8(delta, x, norm_weight, eps)
     y = linear_int8(q, scale, wq, ws, bias)
 
-The sums are exact, so a result does not depend on how many rows a call has.
-Forward only: each raises under autograd rather than lose a gradient.
+The products' sums are exact, so their rows do not depend on how many a call
+has.  Forward only: each operator raises under autograd rather than lose a
+gradient.
 """
 
 from __future__ import annotations

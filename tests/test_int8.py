@@ -12,8 +12,9 @@ import pytest
 import torch
 
 TYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+# one element; odd; a warp; a CTA; wide; past the registers; more rows than one, and than four, to an SM
 ROWS = [(1, 1), (3, 17), (9, 40), (5, 256), (2, 1000), (7, 896), (33, 3584), (4, 4097), (3, 18944), (2, 33000), (2, 65536),
-        (700, 64)]
+        (700, 64), (300, 896), (200, 18944), (1000, 1000)]
 
 
 def half(dtype):
@@ -238,6 +239,24 @@ def test_rows_off_boundaries(mrsa, cuda_device, rows, k):
             y = torch.full((rows, pitch), 77, dtype=torch.int8, device=dev)
             L.call("mrsa_align_rows_int8", L.ptr(x), k + pad, L.ptr(y), pitch, rows, k, L.stream_of(x))
             assert torch.equal(y[:, :k], x) and not y[:, k:].any()
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits(mrsa, cuda_device):
+    """More than 2^31 elements in, and out of a product: the last rows as by themselves."""
+    dev, n = cuda_device, 530_000
+    x = torch.empty(n, 4096, device=dev, dtype=torch.bfloat16).normal_()
+    q, scale = mrsa.quantize_int8(x)
+    few, fs = mrsa.quantize_int8(x[-3:].clone())
+    assert torch.equal(q[-3:], few) and torch.equal(scale[-3:], fs)
+    w, ws = mrsa.quantize_int8(torch.randn(4608, 4096, device=dev))
+    y = mrsa.linear_int8(q, scale, w, ws)
+    assert y.numel() > 2 ** 31 and torch.equal(y[-3:], mrsa.linear_int8(few, fs, w, ws))
+    del y
+    off = x.view(-1)[1:1 + 529_000 * 4095].view(529_000, 4095)
+    q, scale = mrsa.quantize_int8(off)
+    few, fs = mrsa.quantize_int8(off[-3:].clone())
+    assert torch.equal(q[-3:], few) and torch.equal(scale[-3:], fs)
 
 
 @pytest.mark.gpu

@@ -14,7 +14,7 @@ import torch
 TYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
 # one element; odd; a warp; a CTA; unaligned and wide rows; past the registers
 SIZES = [(1, 1), (3, 17), (9, 40), (5, 256), (2, 1000), (7, 896), (33, 3584), (4, 4097), (3, 18944), (2, 20001), (2, 33000),
-         (2, 65536), (700, 64)]
+         (2, 65536), (700, 64), (300, 896), (1000, 3584), (160, 12000)]
 EPS = 1e-6
 
 
