@@ -480,9 +480,10 @@ __device__ __forceinline__ Elements<T, V> gradient_of(const Elements<T, V>& g, c
 
 // Each thread copies its vectors of the rows to come into slots of its own, as in
 // the forward kernel: 16 bytes each, or single fp32 numbers where rows do not start
-// on 16-byte boundaries.  kRows: rows whose copies are under way.
+// on 16-byte boundaries.  kRows: rows whose copies are under way.  (Without the bound of
+// one CTA the compiler saves registers that nothing else needs: 160 against 179 us.)
 template <typename T, int V, int kPer, int kRows>
-__global__ void __launch_bounds__(ring_threads(kPer)) norm_backward_ring_kernel(const BackwardArgs a) {
+__global__ void __launch_bounds__(ring_threads(kPer), 1) norm_backward_ring_kernel(const BackwardArgs a) {
   using Vec = Elements<T, V>;
   extern __shared__ __align__(16) unsigned char slots[];
   __shared__ float red[2][32];         // in turn: a row's are read until the next row's barrier
