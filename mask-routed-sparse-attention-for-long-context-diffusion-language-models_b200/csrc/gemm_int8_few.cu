@@ -384,8 +384,12 @@ int int8_few_error_flags(int clear) {
 namespace int8 {
 bool few_rows(const mrsa_gemm_int8_args* p) {
   if (p->m <= 128) return true;
-  // tiles of the other kernel (128 tokens by 256 channels) that leave SMs idle
-  return p->epilogue != MRSA_GEMM_SWIGLU && ((p->m + 127) / 128) * ((p->n + 255) / 256) < sm_count();
+  // more rows, where tiles of 128 tokens by 256 channels would not fill the SMs; gated,
+  // where that leaves two CTAs to share a long K (us, here and there: 200 x 2048 x 18944
+  // 20 and 50, 500 x 2048 x 3584 12.5 and 14.8; 500 x 8192 x 3584 19 and 16, 500 x 2048
+  // x 896 9.4 and 8.7)
+  const int64_t tiles = (p->m + 127) / 128 * ((p->n + 255) / 256);
+  return p->epilogue == MRSA_GEMM_SWIGLU ? 2 * tiles <= sm_count() && p->k >= 2048 : tiles < sm_count();
 }
 
 int launch_few(const mrsa_gemm_int8_args* p, const Args& a, cudaStream_t s) {

@@ -130,7 +130,8 @@ def test_linear(mrsa, cuda_device, m, n, k):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("m,f,k", [(1, 128, 16), (1, 18944, 3584), (3, 256, 129), (17, 384, 896), (32, 1024, 300),
-                                   (70, 128, 4000), (130, 640, 256), (257, 512, 1000), (1025, 256, 64)])
+                                   (70, 128, 4000), (130, 640, 256), (257, 512, 1000), (1025, 256, 64),
+                                   (300, 256, 5000)])
 def test_swiglu(mrsa, cuda_device, m, f, k):
     q, scale, w, ws, _ = operands(cuda_device, m, 2 * f, k, 1)
     ws = ws * 20 * k ** 0.5 / 74           # gates of a few units
