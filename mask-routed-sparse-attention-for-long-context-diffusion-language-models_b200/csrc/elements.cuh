@@ -18,8 +18,8 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_float(float v) { retur
 template <> __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ float from_float(float v) { return v; }
 
-// V elements of T: one access where they are 16 bytes, else one per element.
-template <typename T, int V> struct alignas(V * sizeof(T) == 16 ? 16 : sizeof(T)) Elements { T e[V]; };
+// V elements of T, read and written in one access.
+template <typename T, int V> struct alignas(V * sizeof(T)) Elements { T e[V]; };
 
 // Elements 2p and 2p + 1 as a pair of fp32 numbers (of a single element, it and 0).
 template <typename T, int V> __device__ __forceinline__ float2 pair_of(const Elements<T, V>& x, int p) {

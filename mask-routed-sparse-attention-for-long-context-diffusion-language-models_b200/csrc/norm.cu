@@ -25,8 +25,8 @@
 // Measured (B200, bf16, us, and of the 6.55 TB/s of a copy): 16384 x 3584 norm with
 // residual 85 (84 %; 96 with a CTA per row and loads in registers), without 45
 // (79 %), with its gradient 160 (90 %; 248); 32768 x 3584 in 8 bits 135 (93 %; 192);
-// 16384 x 18944 quantized 162 (88 %; 312).  Rows off 16-byte boundaries go element
-// by element: fp32 4095 x 2561 with gradient 90 (57 %).
+// 16384 x 18944 quantized 162 (88 %; 312).  Rows off 16-byte boundaries go by
+// words: 4095 x 3585 36 (49 %), with gradient 84 (43 %), fp32 4095 x 2561 90 (57 %).
 #include "common.cuh"
 #include "elements.cuh"
 
@@ -316,6 +316,108 @@ __global__ void __launch_bounds__(N_MAX_THREADS) norm_kernel(const NormArgs a) {
   if (t == 0) write_statistics<kQ8>(a, row, rstd, down, top);
 }
 
+// Rows of 16-bit elements at any address: the aligned words inside a row, a word to a
+// thread at a time, and the elements before and behind them (`odd`, `tail`: whether
+// there are such), which the row's first thread has as a pair of their own.
+template <typename T> struct Words {
+  using Two = Elements<T, 2>;
+  int odd, count, tail, last;
+  __device__ __forceinline__ Words(const T* row, int dim)
+      : odd((reinterpret_cast<uintptr_t>(row) >> 1) & 1), count((dim - odd) / 2), tail((dim - odd) & 1), last(dim - 1) {}
+  __device__ __forceinline__ Two word(const T* row, int i) const { return reinterpret_cast<const Two*>(row + odd)[i]; }
+  __device__ __forceinline__ Two any(const T* row, int i) const { return {row[odd + 2 * i], row[odd + 2 * i + 1]}; }
+  __device__ __forceinline__ Two ends(const T* row, int t) const {
+    return {t == 0 && odd ? row[0] : from_float<T>(0.f), t == 0 && tail ? row[last] : from_float<T>(0.f)};
+  }
+  __device__ __forceinline__ void set_word(T* row, int i, const Two& v) const { reinterpret_cast<Two*>(row + odd)[i] = v; }
+  __device__ __forceinline__ void set_ends(T* row, int t, const Two& v) const {
+    if (t == 0 && odd) row[0] = v.e[0];
+    if (t == 0 && tail) row[last] = v.e[1];
+  }
+};
+
+template <typename T, int kPer, bool kNorm, bool kQ8>
+__global__ void __launch_bounds__(N_MAX_THREADS) norm_words_kernel(const NormArgs a) {
+  using Two = Elements<T, 2>;
+  __shared__ Joined red;
+  if (a.row_warps > 1) {
+    clear(&red, 1);
+    __syncthreads();
+  }
+  chain_wait();
+  chain_next();
+  const int team = a.row_warps * 32, t = threadIdx.x % team;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (blockDim.x / team) + threadIdx.x / team;
+  if (row >= a.rows) return;                   // whole warps of short rows: no barrier follows for them
+  const T *x = static_cast<const T*>(a.x) + row * a.x_stride, *weight = static_cast<const T*>(a.weight);
+  const T* res = kNorm && a.residual ? static_cast<const T*>(a.residual) + row * a.residual_stride : nullptr;
+  const Words<T> at(x, a.dim);
+  Two h[kPer + 1];                             // the last: the ends
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    h[i].e[0] = h[i].e[1] = from_float<T>(0.f);
+    if (t + i * team < at.count) h[i] = at.word(x, t + i * team);
+  }
+  h[kPer] = at.ends(x, t);
+  if (res != nullptr) {
+    Two r[kPer + 1];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (t + i * team < at.count) r[i] = at.word(res, t + i * team);
+    r[kPer] = at.ends(res, t);
+    T* out = static_cast<T*>(a.h) + row * a.dim;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      if (t + i * team >= at.count) continue;
+      add_to<T, 2>(h[i], r[i]);
+      at.set_word(out, t + i * team, h[i]);
+    }
+    add_to<T, 2>(h[kPer], r[kPer]);
+    at.set_ends(out, t, h[kPer]);
+  }
+  float rstd, top, down;
+  row_statistics<kNorm, kQ8>(a, red, [&](auto& s) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (t + i * team < at.count) s.add(h[i], kNorm && kQ8 ? at.any(weight, t + i * team) : h[i]);
+    s.add(h[kPer], kNorm && kQ8 ? at.ends(weight, t) : h[kPer]);
+  }, rstd, top, down);
+  const Whole whole(kQ8 ? top : 0.f);
+  auto result = [&](const Two& v, const Two& w) {
+    float2 f = fmul2(pair_of(v, 0), make_float2(down, down));
+    if (kNorm && !kQ8) f = fmul2(f, make_float2(rstd, rstd));
+    if (kNorm) f = fmul2(f, pair_of(w, 0));
+    if (kQ8) f = ffma2(fmul2(f, make_float2(whole.up, whole.up)), make_float2(whole.inv, whole.inv), make_float2(kWhole, kWhole));
+    return f;
+  };
+  auto byte = [&](float f) { return static_cast<int8_t>(__float_as_uint(f) & whole.keep); };
+  T* y = static_cast<T*>(a.y) + row * a.dim;
+  int8_t* q = a.q + row * a.q_stride;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    if (t + i * team >= at.count) continue;
+    const float2 f = result(h[i], kNorm ? at.any(weight, t + i * team) : h[i]);
+    if (kQ8) {
+      q[at.odd + 2 * (t + i * team)] = byte(f.x);
+      q[at.odd + 2 * (t + i * team) + 1] = byte(f.y);
+    } else {
+      Two o;
+      set_pair(o, 0, f);
+      at.set_word(y, t + i * team, o);
+    }
+  }
+  const float2 f = result(h[kPer], kNorm ? at.ends(weight, t) : h[kPer]);
+  if (kQ8) {
+    if (t == 0 && at.odd) q[0] = byte(f.x);
+    if (t == 0 && at.tail) q[at.last] = byte(f.y);
+  } else {
+    Two o;
+    set_pair(o, 0, f);
+    at.set_ends(y, t, o);
+  }
+  if (t == 0) write_statistics<kQ8>(a, row, rstd, down, top);
+}
+
 // The same for rows on 16-byte boundaries, a CTA's (or warp's) rows a grid apart:
 // each thread copies its vectors of the rows to come into slots of its own, kAhead
 // rows ahead, so that loads are always in flight while a row is summed up and
@@ -479,44 +581,69 @@ __device__ __forceinline__ Elements<T, V> gradient_of(const Elements<T, V>& g, c
 }
 
 // Each thread copies its vectors of the rows to come into slots of its own, as in
-// the forward kernel: 16 bytes each, or single fp32 numbers where rows do not start
-// on 16-byte boundaries.  kRows: rows whose copies are under way.  (Without the bound of
-// one CTA the compiler saves registers that nothing else needs: 160 against 179 us.)
+// the forward kernel: 16 bytes each, or where rows do not start on 16-byte boundaries
+// single fp32 numbers, or the words inside rows of 16-bit elements (V = 2; all tensors'
+// rows alike, and a CTA's rows an even number apart, so that they all begin in the
+// middle of a word or none does; the ends go through registers of the first thread).
+// kRows: rows whose copies are under way.  (Without the bound of one CTA the compiler
+// saves registers that nothing else needs: 160 against 179 us.)
 template <typename T, int V, int kPer, int kRows>
 __global__ void __launch_bounds__(ring_threads(kPer), 1) norm_backward_ring_kernel(const BackwardArgs a) {
   using Vec = Elements<T, V>;
+  constexpr bool kWords = V == 2 && sizeof(T) == 2;
   extern __shared__ __align__(16) unsigned char slots[];
   __shared__ float red[2][32];         // in turn: a row's are read until the next row's barrier
   chain_wait();
   chain_next();
-  const int t = threadIdx.x, team = blockDim.x, vecs = a.dim / V, tensor = kPer * team;
+  const Words<T> at(static_cast<const T*>(a.h) + static_cast<int64_t>(blockIdx.x) * a.h_stride, a.dim);
+  const int t = threadIdx.x, team = blockDim.x, tensor = kPer * team;
+  const int vecs = kWords ? at.count : a.dim / V, skip = kWords ? at.odd : 0;
   const bool add = a.gh != nullptr;
   const int stage = (add ? 3 : 2) * tensor;
   Vec* const weight = reinterpret_cast<Vec*>(slots);
-  Vec* const ring = weight + (vecs * static_cast<int>(sizeof(Vec)) + 15) / 16 * 16 / static_cast<int>(sizeof(Vec)) + t;
+  Vec* const ring = weight + (a.dim / V * static_cast<int>(sizeof(Vec)) + 15) / 16 * 16 / static_cast<int>(sizeof(Vec)) + t;
+  auto row_of = [&](const void* p, int64_t row, int64_t stride) { return static_cast<const T*>(p) + row * stride; };
   auto ask = [&](int64_t row, int s) {
     if (row < a.rows) {
-      const Vec* gy = reinterpret_cast<const Vec*>(static_cast<const T*>(a.gy) + row * a.gy_stride);
-      const Vec* hr = reinterpret_cast<const Vec*>(static_cast<const T*>(a.h) + row * a.h_stride);
-      const Vec* gh = add ? reinterpret_cast<const Vec*>(static_cast<const T*>(a.gh) + row * a.gh_stride) : nullptr;
+      const Vec* gy = reinterpret_cast<const Vec*>(row_of(a.gy, row, a.gy_stride) + skip);
+      const Vec* hr = reinterpret_cast<const Vec*>(row_of(a.h, row, a.h_stride) + skip);
+      const Vec* gh = add ? reinterpret_cast<const Vec*>(row_of(a.gh, row, a.gh_stride) + skip) : nullptr;
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
         const int v = t + i * team;
         if (v >= vecs) continue;
-        Vec* at = ring + s * stage + i * team;
-        copy_in(at, gy + v);
-        copy_in(at + tensor, hr + v);
-        if (add) copy_in(at + 2 * tensor, gh + v);
+        Vec* to = ring + s * stage + i * team;
+        copy_in(to, gy + v);
+        copy_in(to + tensor, hr + v);
+        if (add) copy_in(to + 2 * tensor, gh + v);
       }
     }
     asm volatile("cp.async.commit_group;\n" ::: "memory");
   };
+  struct Ends { Elements<T, 2> g, h, o; };
+  auto ends_of = [&](int64_t row) {
+    Ends e = {zeros<T, 2>(), zeros<T, 2>(), zeros<T, 2>()};
+    if (kWords && row < a.rows) {
+      e.g = at.ends(row_of(a.gy, row, a.gy_stride), t);
+      e.h = at.ends(row_of(a.h, row, a.h_stride), t);
+      if (add) e.o = at.ends(row_of(a.gh, row, a.gh_stride), t);
+    }
+    return e;
+  };
 #pragma unroll
   for (int s = 0; s < kRows; ++s) ask(blockIdx.x + static_cast<int64_t>(s) * gridDim.x, s);
   float rstd = blockIdx.x < a.rows ? a.rstd[blockIdx.x] : 0.f;
-  for (int v = t; v < vecs; v += team) weight[v] = static_cast<const Vec*>(a.weight)[v];
+  Ends ends;                           // (constant conditions, so that nothing of it is left where there are none)
+  if constexpr (kWords) ends = ends_of(blockIdx.x);
+  const T* const w = static_cast<const T*>(a.weight);
+  const Elements<T, 2> weight_ends = kWords ? at.ends(w, t) : zeros<T, 2>();
+  for (int v = t; v < vecs; v += team) {
+    if constexpr (kWords) weight[v] = at.any(w, v);
+    else weight[v] = reinterpret_cast<const Vec*>(w)[v];
+  }
   __syncthreads();
-  float2 dw[kPer][(V + 1) / 2];
+  float2 dw[kPer][(V + 1) / 2], dw_ends[1];
+  dw_ends[0] = make_float2(0.f, 0.f);
 #pragma unroll
   for (int i = 0; i < kPer; ++i)
 #pragma unroll
@@ -525,24 +652,30 @@ __global__ void __launch_bounds__(ring_threads(kPer), 1) norm_backward_ring_kern
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
     const int64_t next = row + gridDim.x;
     const float next_rstd = next < a.rows ? a.rstd[next] : 0.f;
+    Ends next_ends;
+    if constexpr (kWords) next_ends = ends_of(next);
     asm volatile("cp.async.wait_group %0;\n" ::"n"(kRows - 1) : "memory");
     // (the row is read twice from its slots: held in registers beside dw it spills)
-    const Vec* const at = ring + s * stage;
+    const Vec* const from = ring + s * stage;
     float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
       if (t + i * team < vecs)
-        add_products<T, V>(dw[i], sum, at[i * team], at[tensor + i * team], weight[t + i * team], rstd);
+        add_products<T, V>(dw[i], sum, from[i * team], from[tensor + i * team], weight[t + i * team], rstd);
+    if constexpr (kWords) add_products<T, 2>(dw_ends, sum, ends.g, ends.h, weight_ends, rstd);
     const float mean = join_sum(sum.x + sum.y, red[turn]) * a.inv_dim;
-    Vec* dx = reinterpret_cast<Vec*>(static_cast<T*>(a.dx) + row * a.dim);
+    T* const out = static_cast<T*>(a.dx) + row * a.dim;
+    Vec* dx = reinterpret_cast<Vec*>(out + skip);
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
       if (t + i * team < vecs)
-        dx[t + i * team] = gradient_of<T, V>(at[i * team], at[tensor + i * team], weight[t + i * team],
-                                             add ? at[2 * tensor + i * team] : zeros<T, V>(), rstd, mean);
+        dx[t + i * team] = gradient_of<T, V>(from[i * team], from[tensor + i * team], weight[t + i * team],
+                                             add ? from[2 * tensor + i * team] : zeros<T, V>(), rstd, mean);
+    if constexpr (kWords) at.set_ends(out, t, gradient_of<T, 2>(ends.g, ends.h, weight_ends, ends.o, rstd, mean));
     ask(row + static_cast<int64_t>(kRows) * gridDim.x, s);
     if (++s == kRows) s = 0;
     rstd = next_rstd;
+    if constexpr (kWords) ends = next_ends;
   }
   if (a.parts == nullptr) return;
   float* part = a.parts + static_cast<int64_t>(blockIdx.x) * a.dim;
@@ -551,8 +684,10 @@ __global__ void __launch_bounds__(ring_threads(kPer), 1) norm_backward_ring_kern
     const int v = t + i * team;
     if (v >= vecs) continue;
 #pragma unroll
-    for (int e = 0; e < V; ++e) part[v * V + e] = e & 1 ? dw[i][e / 2].y : dw[i][e / 2].x;
+    for (int e = 0; e < V; ++e) part[skip + v * V + e] = e & 1 ? dw[i][e / 2].y : dw[i][e / 2].x;
   }
+  if (kWords && t == 0 && at.odd) part[0] = dw_ends[0].x;
+  if (kWords && t == 0 && at.tail) part[at.last] = dw_ends[0].y;
 }
 
 // Rows of 16-bit elements that do not start on 16-byte boundaries: the next row's
@@ -700,6 +835,21 @@ int resident(K* kernel, int threads, int smem, std::atomic<int>& known) {
   return n;
 }
 
+// Whether a row begins in the middle of a word in both tensors or in neither, on
+// every row (16-bit elements; strides in elements).  No tensor agrees with any.
+bool words_alike(const void* p, int64_t p_stride, const void* q, int64_t q_stride, int64_t rows) {
+  if (p == nullptr || q == nullptr) return true;
+  return ((reinterpret_cast<uintptr_t>(p) ^ reinterpret_cast<uintptr_t>(q)) & 2) == 0 && (rows == 1 || ((p_stride ^ q_stride) & 1) == 0);
+}
+
+template <typename T, int kPer, bool kNorm, bool kQ8>
+int launch_words(NormArgs a, cudaStream_t s) {
+  a.row_warps = a.dim > 1 ? warps_for(a.dim / 2, kPer) : 1;
+  const int64_t ctas = a.row_warps == 1 ? (a.rows + N_SHORT_ROWS - 1) / N_SHORT_ROWS : a.rows;
+  return launch_chained(norm_words_kernel<T, kPer, kNorm, kQ8>, dim3(static_cast<unsigned>(ctas)),
+                        a.row_warps == 1 ? 32 * N_SHORT_ROWS : 32 * a.row_warps, 0, s, a);
+}
+
 template <typename T, int kPer, bool kNorm, bool kQ8>
 int launch_ring(NormArgs a, cudaStream_t s) {
   static std::atomic<uint64_t> allowed{0};
@@ -740,6 +890,14 @@ int norm_of(const NormArgs& a, cudaStream_t s) {
     if (vecs <= 8 * ring_threads(8) && smem8 <= N_SMEM - 2048) return launch_ring<T, 8, kNorm, kQ8>(a, s);
     return launch_norm<T, V, 4, kNorm, kQ8>(a, s);
   }
+  if constexpr (sizeof(T) == 2) {
+    if (a.dim <= 16384 && words_alike(a.x, a.x_stride, a.residual, a.residual_stride, a.rows) &&
+        words_alike(a.x, a.x_stride, a.y, a.dim, a.rows) && words_alike(a.x, a.x_stride, a.h, a.dim, a.rows)) {
+      if (a.dim <= 1024) return launch_words<T, 2, kNorm, kQ8>(a, s);
+      if (a.dim <= 4096) return launch_words<T, 4, kNorm, kQ8>(a, s);
+      return launch_words<T, 8, kNorm, kQ8>(a, s);
+    }
+  }
   if (a.dim <= 1024) return launch_norm<T, 1, 4, kNorm, kQ8>(a, s);
   if (a.dim <= 16 * N_MAX_THREADS) return launch_norm<T, 1, 16, kNorm, kQ8>(a, s);
   NormArgs b = a;
@@ -768,13 +926,14 @@ int launch_backward_rows(BackwardArgs& a, int threads, int smem, cudaStream_t s)
   const int64_t most = static_cast<int64_t>(resident(norm_backward_ring_kernel<T, V, kPer, kRows>, threads, smem,
                                                      known[a.gh != nullptr][threads / 32])) * sm_count();
   if (a.grid > most) a.grid = static_cast<int>(most);
+  if (V == 2 && sizeof(T) == 2 && a.grid > 1) a.grid &= ~1;
   return launch_chained(norm_backward_ring_kernel<T, V, kPer, kRows>, dim3(static_cast<unsigned>(a.grid)), threads,
                         static_cast<size_t>(smem), s, a);
 }
 // kAhead rows, or one where so many do not fit (16-bit rows of more than 18000 elements).
 template <typename T, int V, int kPer>
 int launch_backward_ring(BackwardArgs& a, cudaStream_t s) {
-  const int vecs = a.dim / V, threads = 32 * warps_for(vecs, kPer), bytes = sizeof(T) * V;
+  const int vecs = a.dim / V, threads = vecs > 0 ? 32 * warps_for(vecs, kPer) : 32, bytes = sizeof(T) * V;
   const int row = (a.gh ? 3 : 2) * kPer * threads * bytes, weight = (vecs * bytes + 15) / 16 * 16;
   if (kAhead * row + weight <= N_SMEM - 1024) return launch_backward_rows<T, V, kPer, kAhead>(a, threads, kAhead * row + weight, s);
   return launch_backward_rows<T, V, kPer, 1>(a, threads, row + weight, s);
@@ -798,6 +957,9 @@ int backward_of(BackwardArgs a, cudaStream_t s) {
   } else if (a.dim <= 8192) {
     if constexpr (sizeof(T) == 4)
       rc = a.dim <= 4096 ? launch_backward_ring<T, 1, 8>(a, s) : launch_backward_ring<T, 1, 16>(a, s);
+    else if (words_alike(a.h, a.h_stride, a.gy, a.gy_stride, a.rows) && words_alike(a.h, a.h_stride, a.gh, a.gh_stride, a.rows) &&
+             words_alike(a.h, a.h_stride, a.dx, a.dim, a.rows))
+      rc = a.dim <= 4096 ? launch_backward_ring<T, 2, 8>(a, s) : launch_backward_ring<T, 2, 16>(a, s);
     else if (a.dim <= 1024)
       rc = launch_chained(norm_backward_kernel<T, 2>, grid, 32 * warps_for(a.dim, 2), 0, s, a);
     else

@@ -142,6 +142,42 @@ def test_strides_broadcasts_and_shapes(mrsa, cuda_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["bf16", "fp16"])
+@pytest.mark.parametrize("dim,pitch,first", [(96, 300, 3), (97, 300, 1), (97, 301, 2), (98, 301, 1), (31, 31, 1), (8, 9, 1), (1000, 1001, 5),
+                                             (2503, 2503, 0), (4001, 4002, 1), (6001, 6001, 3), (7999, 8001, 0), (12001, 12001, 1),
+                                             (15999, 15999, 0)])
+def test_views_of_16_bits(mrsa, cuda_device, dim, pitch, first, kind):
+    """Rows that begin in the middle of a word, all, some or none of them, in tensors that agree in it or do not."""
+    dev, dtype, rows = cuda_device, TYPES[kind], 13
+    g = torch.Generator(device=dev).manual_seed(8)
+
+    def view(p, f):
+        flat = torch.randn(f + rows * p + 8, device=dev, generator=g).to(dtype)
+        return torch.as_strided(flat, (rows, dim), (p, 1), f)
+
+    w = view(pitch, first)[0]
+    for r, gy, gh in ((view(pitch, first), view(pitch, first), view(pitch, first)), (view(dim, 0), view(dim, 0), view(dim, 0)),
+                      (view(pitch, first + 1), view(dim, 0), None), (None, view(pitch + 1, 0), None)):
+        x = view(pitch, first)
+        leaves = [v.requires_grad_() for v in (x, r, w) if v is not None]
+        y, h = mrsa.add_rms_norm(x, r, w, EPS)
+        with torch.no_grad():
+            assert torch.equal(h, x if r is None else x + r)
+            check(y, h, w)
+        outs, grads = ((y, h), (gy, gh)) if gh is not None else ((y,), (gy,))
+        got = torch.autograd.grad(outs, leaves, grads)
+        check_gradient((got[0], got[-1]), gy, gh, h.detach(), w.detach(), dtype)
+        with torch.no_grad():
+            q, scale = mrsa.quantize_int8(x)
+            p = x.double()
+            n = 127 * p / p.abs().amax(-1, keepdim=True)
+            assert ((q.double() - n).abs() <= 0.5 + 4e-5).all()
+            q, scale, h8 = mrsa.add_rms_norm_int8(x, r, w, EPS)
+            p = h.double() * w.double()
+            assert torch.equal(h8, h) and ((q.double() - 127 * p / p.abs().amax(-1, keepdim=True)).abs() <= 0.5 + 4e-5).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dim", [64, 999])
 def test_extreme_values(mrsa, cuda_device, dim):
     """Squares past fp32's range, zeros, NaN and infinities: each row by itself."""
