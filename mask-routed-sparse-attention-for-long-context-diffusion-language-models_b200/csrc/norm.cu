@@ -289,7 +289,8 @@ __global__ void __launch_bounds__(N_MAX_THREADS) norm_kernel(const NormArgs a) {
     for (int e = 0; e < V; ++e) h[i].e[e] = w[i].e[e] = from_float<T>(0.f);
     if (v < vecs) h[i] = x[v];
   }
-  if (kNorm && kQ8) {
+  // with more vectors to a thread the norm reads its weights where it uses them: held they spill
+  if (kNorm && (kQ8 || kPer == 1)) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
       if (t + i * team < vecs) w[i] = static_cast<const Vec*>(a.weight)[t + i * team];
@@ -312,7 +313,12 @@ __global__ void __launch_bounds__(N_MAX_THREADS) norm_kernel(const NormArgs a) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) s.add(h[i], w[i]);
   }, rstd, top, down);
-  write_row<T, V, kPer, kNorm, kQ8>(a, row, t, team, h, static_cast<const Vec*>(a.weight), rstd, down, top);
+  if constexpr (kPer == 1) {
+    const Whole whole(kQ8 ? top : 0.f);
+    if (t < vecs) write_vector<T, V, kNorm, kQ8, false>(a, row, t, h[0], w[0], rstd, down, whole);
+  } else {
+    write_row<T, V, kPer, kNorm, kQ8>(a, row, t, team, h, static_cast<const Vec*>(a.weight), rstd, down, top);
+  }
   if (t == 0) write_statistics<kQ8>(a, row, rstd, down, top);
 }
 
@@ -874,7 +880,7 @@ int norm_of(const NormArgs& a, cudaStream_t s) {
   const int vecs = a.dim / V, smem8 = (kAhead * (kNorm && a.residual ? 2 : 1) * (vecs + 32 * 8) + (kNorm ? vecs : 0)) * 16;
   if (wide && vecs <= 4 * N_MAX_THREADS) {
     // No row behind another on an SM: straight to registers, with as many threads as
-    // there are vectors (one row of 3584: 1.8 us, by the copies ahead 2.3; 18944
+    // there are vectors (one row of 3584: 1.6 us, by the copies ahead 2.3; 18944
     // quantized 1.9 and 2.4).
     if (a.rows <= sm_count()) {
       if (vecs <= N_MAX_THREADS) return launch_norm<T, V, 1, kNorm, kQ8>(a, s);
@@ -898,7 +904,9 @@ int norm_of(const NormArgs& a, cudaStream_t s) {
       return launch_words<T, 8, kNorm, kQ8>(a, s);
     }
   }
+  // (4095 x 2561 fp32: norm 35 us by eight elements a thread, 40 by sixteen; quantized 22 and 15)
   if (a.dim <= 1024) return launch_norm<T, 1, 4, kNorm, kQ8>(a, s);
+  if (kNorm && a.dim <= 4096) return launch_norm<T, 1, 8, kNorm, kQ8>(a, s);
   if (a.dim <= 16 * N_MAX_THREADS) return launch_norm<T, 1, 16, kNorm, kQ8>(a, s);
   NormArgs b = a;
   b.row_warps = N_MAX_THREADS / 32;
@@ -912,9 +920,10 @@ int norm_of_type(const NormArgs& a, int dtype, cudaStream_t s) {
   return norm_of<float, kNorm, kQ8>(a, s);
 }
 
-// Parts of dw at most: CTAs of the gradient that are resident at once.
-int64_t backward_grid(int64_t rows) {
-  const int64_t most = 6LL * sm_count();
+// Parts of dw at most: CTAs of the gradient that are resident at once, and 256 MB of them.
+int64_t backward_grid(int64_t rows, int64_t dim) {
+  int64_t most = 6LL * sm_count();
+  if (most > (1 << 26) / dim) most = (1 << 26) / dim;
   return rows < most ? rows : most;
 }
 
@@ -1030,7 +1039,7 @@ extern "C" int mrsa_quantize_int8(const void* x, int64_t x_stride, int8_t* q, in
 
 extern "C" size_t mrsa_add_rms_norm_backward_workspace(int64_t rows, int64_t dim) {
   if (!sizes_ok(rows, dim) || rows == 0) return 0;
-  return static_cast<size_t>(backward_grid(rows)) * static_cast<size_t>(dim) * sizeof(float);
+  return static_cast<size_t>(backward_grid(rows, dim)) * static_cast<size_t>(dim) * sizeof(float);
 }
 
 extern "C" int mrsa_add_rms_norm_backward(const mrsa_norm_backward_args* p, void* workspace, size_t ws_bytes,
@@ -1062,7 +1071,7 @@ extern "C" int mrsa_add_rms_norm_backward(const mrsa_norm_backward_args* p, void
   a.h_stride = p->h_stride;
   a.dim = static_cast<int>(p->dim);
   a.inv_dim = 1.f / static_cast<float>(p->dim);
-  a.grid = static_cast<int>(backward_grid(p->rows));
+  a.grid = static_cast<int>(backward_grid(p->rows, p->dim));
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (p->dtype == MRSA_BF16) return backward_of<__nv_bfloat16>(a, s);
   if (p->dtype == MRSA_F16) return backward_of<__half>(a, s);

@@ -113,7 +113,7 @@ def check_linear(y, q, scale, w, ws, bias):
 SHAPES = [(1, 1, 1), (1, 8, 16), (2, 7, 15), (1, 4608, 3584), (3, 130, 129), (5, 33, 4000), (16, 256, 128), (17, 264, 127),
           (31, 512, 896), (33, 1001, 517), (64, 640, 1024), (65, 128, 18944), (100, 4608, 896), (128, 384, 130),
           (129, 257, 257), (256, 3584, 1000), (300, 515, 96), (511, 72, 640), (1000, 2000, 333), (2049, 300, 256),
-          (1, 40000, 64), (700, 8, 20000)]
+          (1, 40000, 64), (700, 8, 20000), (300, 515, 12999), (520, 130, 7000)]
 
 
 @pytest.mark.gpu
