@@ -13,8 +13,14 @@
 // N reads as zeros); the even CTA issues UMMA M=256 N=256 K=32 (four per stage) into
 // one of two 256-column TMEM accumulators, while warps 4-11 of both CTAs drain the
 // other (an output row per thread, stored by TMA through 128 bytes of each row in
-// shared memory).  One CTA by itself (128 x 256 tiles) is held up by
-// shared memory: it reads and writes 96 bytes each per cycle of the MMA, the pair 64.
+// shared memory).  One CTA by itself (128 x 256 tiles) is held up by shared memory:
+// it reads and writes 96 bytes each per cycle of the MMA, the pair 64.  (Rows of C off
+// 16-byte boundaries are turned in shared memory and stored along the row.)
+//
+// Measured (B200, us): 8191 x 4608 x 3584 87 cold, 103 in a long run, 2620 to 3110
+// TOP/s (one CTA per tile 121); gated 16384 x 37888 x 3584 1460 to 1600 (1824), the
+// tensor pipe 90 to 93 % active at the 1.56 GHz that the power cap leaves.
+//
 // Every wait is bounded; a CTA that gives up tells its pair, drains its copies and
 // MMAs, and sets bit 8 of mrsa_device_error_flags.
 #include <mutex>
