@@ -9,7 +9,7 @@
 //
 // Persistent: a pair of CTAs on two SMs (cta_group::2) walks 256 x 256 output tiles,
 // each CTA with 128 of the rows.  A CTA copies its half of both operands' 128-byte K
-// blocks by TMA into six stages (32 KB each, 128-byte swizzle; what lies past K, M or
+// blocks by TMA into five stages (32 KB each, 128-byte swizzle; what lies past K, M or
 // N reads as zeros); the even CTA issues UMMA M=256 N=256 K=32 (four per stage) into
 // one of two 256-column TMEM accumulators, while warps 4-11 of both CTAs drain the
 // other (an output row per thread, stored by TMA through 128 bytes of each row in

@@ -155,22 +155,25 @@ __device__ __forceinline__ void row_statistics(const NormArgs& a, Joined& red, F
 // nearest(127 p / top) as the low byte of fma(p, 127 / top, 1.5 * 2^23), whose one
 // rounding is to a whole number (no conversion, which runs at a quarter of the
 // rate): off from p / s by what 127 / top is, so only values as near to half-way as
-// that may go to the other neighbour.  Tops below 2^-100 are taken 2^100 as large,
-// so that 127 / top stays finite.
+// that may go to the other neighbour.  Tops below 2^-100 are taken 2^100 as large, so
+// that 127 / top stays finite, and those above 2^100 2^-100 as large (the fast
+// division gives zero for divisors past 2^126).
 struct Whole {
   float up, inv;
   uint32_t keep;       // no bits of rows that are zeros or not numbers
   __device__ __forceinline__ explicit Whole(float top) {
     const bool none = !(top > 0.f) || magnitude(top) >= kInfBits;
-    up = top < kSmall ? kSmallUp : 1.f;
+    up = top < kSmall ? kSmallUp : top > kSmallUp ? kSmall : 1.f;
     inv = none ? 0.f : __fdividef(127.f, top * up);     // to 2 units in the last place
     keep = none ? 0u : 0xffffffffu;
   }
   __device__ __forceinline__ uint32_t operator()(float p) const { return __float_as_uint(fmaf(p * up, inv, kWhole)); }
 };
 
+// (Small tops times r first: their quotients may be below the smallest normal number.)
 __device__ __forceinline__ float scale_of(float top, float rstd) {
-  return magnitude(top) >= kInfBits ? __uint_as_float(0x7fffffffu) : top / 127.f * rstd;
+  if (magnitude(top) >= kInfBits) return __uint_as_float(0x7fffffffu);
+  return top < kSmall ? top * rstd / 127.f : top / 127.f * rstd;
 }
 
 // The low bytes of n.

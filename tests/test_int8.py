@@ -27,7 +27,8 @@ def check_whole(q, scale, p, want_scale, off=0.0):
     n = torch.where(top > 0, 127 * p / top, torch.zeros_like(p))
     assert q.dtype == torch.int8 and scale.dtype == torch.float32
     assert ((q.double() - n).abs() <= 0.5 + 4e-5).all()
-    assert ((scale.double() - want_scale).abs() <= want_scale * (4 * 2 ** -24 + off)).all()
+    # a scale below the smallest normal number 2^-126 is a multiple of 2^-149 and rounds by half of that
+    assert ((scale.double() - want_scale).abs() <= want_scale * (4 * 2 ** -24 + off) + 2.0 ** -150).all()
 
 
 @pytest.mark.gpu
@@ -59,6 +60,26 @@ def test_norm_int8(mrsa, cuda_device, rows, dim, kind):
         d = h.double()
         p = d * w.double()
         check_whole(q, scale, p, p.abs().amax(-1) / 127 / (d.square().mean(-1) + 1e-6).sqrt(), 5e-6)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [1, 7, 64, 999, 18944])
+@pytest.mark.parametrize("rows", [3, 400])
+@pytest.mark.parametrize("size", [2.0 ** -120, 2.0 ** -101, 2.0 ** -99, 2.0 ** 99, 2.0 ** 101, 2.0 ** 125, 2.0 ** 126])
+def test_rows_of_any_size(mrsa, cuda_device, rows, dim, size):
+    """From numbers whose quotients pass fp32's range to the largest there are (below 2^128)."""
+    dev = cuda_device
+    g = torch.Generator(device=dev).manual_seed(3)
+    x = torch.randn(rows, dim, device=dev, generator=g).clamp(-3.9, 3.9) * size
+    w = torch.rand(dim, device=dev, generator=g) + 0.5
+    for kind in ("fp32", "bf16"):
+        a, b = x.to(TYPES[kind]), w.to(TYPES[kind])
+        q, scale = mrsa.quantize_int8(a)
+        p = a.double()
+        check_whole(q, scale, p, p.abs().amax(-1) / 127)
+        q, scale, _ = mrsa.add_rms_norm_int8(a, None, b, 1e-6)
+        p = p * b.double()
+        check_whole(q, scale, p, p.abs().amax(-1) / 127 / (a.double().square().mean(-1) + 1e-6).sqrt(), 5e-6)
 
 
 @pytest.mark.gpu
