@@ -201,7 +201,8 @@ __global__ void __launch_bounds__(F_THREADS, kPerSm) gemm_int8_few_kernel(const 
   __syncthreads();
   if (share > 1) tc::cluster_sync();
   // This CTA's share of the tokens, a warp to a token, four channels to a lane.
-  const int tokens = min(kTokens, a.M - tm * kTokens), per = (tokens + share - 1) / share, first = rank * per, last = min(first + per, tokens);
+  const int tokens = min(kTokens, a.M - tm * kTokens), per = (tokens + share - 1) / share;
+  const int first = rank * per, last = min(first + per, tokens);
   T* c = static_cast<T*>(a.c);
   const int col = tn * BC + lane * 4, cols = kGated ? a.N / 2 : a.N;
   const bool four = a.ldc % 4 == 0 && reinterpret_cast<uintptr_t>(c) % (4 * sizeof(T)) == 0;
@@ -310,14 +311,17 @@ int resident_clusters(int cluster, int smem) {
 template <typename T, int kTokens, bool kGated, int kPerSm, bool kPair = false>
 int launch(const mrsa_gemm_int8_args* p, Args a, cudaStream_t s) {
   static std::atomic<uint64_t> allowed{0};
+  constexpr auto kernel = gemm_int8_few_kernel<T, kTokens, kGated, kPerSm, kPair>;
   constexpr int smem = sizeof(FewSmem<kTokens, kGated, kPerSm, kPair>) + 1024;
+  static_assert(smem <= 232448 && kPerSm * (smem + 1024) <= 233472, "shared memory over budget");
   constexpr int kChannels = (kGated ? 2 : 1) * BC, kHalves = kPair ? 2 : 1;
   CUtensorMap tma, tmb;
-  if (!make_map(&tma, p->a, p->k, p->m, p->a_stride, kTokens / kHalves) || !make_map(&tmb, p->b, p->k, p->n, p->b_stride, kChannels)) {
+  if (!make_map(&tma, p->a, p->k, p->m, p->a_stride, kTokens / kHalves) ||
+      !make_map(&tmb, p->b, p->k, p->n, p->b_stride, kChannels)) {
     note_cuda_error(cudaErrorInvalidValue, "mrsa_gemm_int8: tensor map encoding");
     return MRSA_ERR_LAUNCH;
   }
-  if (!allow_smem(gemm_int8_few_kernel<T, kTokens, kGated, kPerSm, kPair>, smem, allowed)) return MRSA_ERR_LAUNCH;
+  if (!allow_smem(kernel, smem, allowed)) return MRSA_ERR_LAUNCH;
   a.n_tiles = (a.N + kHalves * kChannels - 1) / (kHalves * kChannels);
   a.m_tiles = (a.M + kTokens - 1) / kTokens;
   const int64_t tiles = static_cast<int64_t>(a.n_tiles) * a.m_tiles;
@@ -327,11 +331,12 @@ int launch(const mrsa_gemm_int8_args* p, Args a, cudaStream_t s) {
   int64_t share = 1;
   if (kPerSm == 1) {
     share = a.k_blocks / 4 < F_MAX_CLUSTER / kHalves ? a.k_blocks / 4 : F_MAX_CLUSTER / kHalves;
-    while (share > 1 && resident_clusters<gemm_int8_few_kernel<T, kTokens, kGated, kPerSm, kPair>>(static_cast<int>(share) * kHalves, smem) < tiles) --share;
+    while (share > 1 && resident_clusters<kernel>(static_cast<int>(share) * kHalves, smem) < tiles) --share;
     if (share < 1) share = 1;
   }
-  return launch_clusters(gemm_int8_few_kernel<T, kTokens, kGated, kPerSm, kPair>, dim3(static_cast<unsigned>(a.n_tiles * share * kHalves), a.m_tiles),
-                         static_cast<unsigned>(share * kHalves), F_THREADS, smem, s, tma, tmb, a, static_cast<int>(share));
+  const unsigned cluster = static_cast<unsigned>(share) * kHalves;
+  return launch_clusters(kernel, dim3(a.n_tiles * cluster, a.m_tiles), cluster, F_THREADS, smem, s, tma, tmb, a,
+                         static_cast<int>(share));
 }
 
 template <typename T, int kTokens, bool kGated>
