@@ -26,7 +26,7 @@
 // residual 85 (84 %; 96 with a CTA per row and loads in registers), without 45
 // (79 %), with its gradient 160 (90 %; 248); 32768 x 3584 in 8 bits 135 (93 %; 192);
 // 16384 x 18944 quantized 162 (88 %; 312).  Rows off 16-byte boundaries go by
-// words: 4095 x 3585 36 (49 %), with gradient 84 (43 %), fp32 4095 x 2561 90 (57 %).
+// words: 4095 x 3585 36 (49 %), with gradient 84 (43 %), fp32 4095 x 2561 86 (60 %).
 #include "common.cuh"
 #include "elements.cuh"
 
