@@ -590,12 +590,13 @@ typedef struct {
 
 /* Norm with the residual's addition: h = x + residual, rounded to the type; v =
  * h * weight / sqrt(mean(h^2) + eps) in fp32; y = v, rounded once, or v in 8 bits:
- * scale = max|v| / 127 and q = the whole number nearest v / scale (either
- * neighbour where fp32 does not tell).  A row of zeros has scale 0; a row with a
- * NaN or an infinity has scale NaN and q 0. */
+ * scale = max|v| / 127 and, with p = h * weight (in fp32: exact for 16-bit types),
+ * q = the whole number nearest p * ((1 / max|p|) * 127), each step in 64 bits, of two
+ * the even one.  A row of zeros has scale 0; a row with a NaN or an infinity
+ * has scale NaN and q 0. */
 int mrsa_add_rms_norm(const mrsa_norm_args* a, mrsa_stream_t stream);
 
-/* Rows of x in 8 bits, as there: scale = max|x| / 127, q = nearest(x / scale). */
+/* Rows of x in 8 bits, as there with p = x. */
 int mrsa_quantize_int8(const void* x, int64_t x_stride, int8_t* q, int64_t q_stride, float* scale, int64_t rows,
                        int64_t dim, int dtype, mrsa_stream_t stream);
 

@@ -24,8 +24,8 @@
 //
 // Measured (B200, bf16, us, and of the 6.55 TB/s of a copy): 16384 x 3584 norm with
 // residual 85 (84 %; 96 with a CTA per row and loads in registers), without 45
-// (79 %), with its gradient 160 (90 %; 248); 32768 x 3584 in 8 bits 135 (93 %; 192);
-// 16384 x 18944 quantized 162 (88 %; 312).  Rows off 16-byte boundaries go by
+// (79 %), with its gradient 160 (90 %; 248); 32768 x 3584 in 8 bits 139 (90 %; 192);
+// 16384 x 18944 quantized 175 (81 %; 312).  Rows off 16-byte boundaries go by
 // words: 4095 x 3585 36 (49 %), with gradient 84 (43 %), fp32 4095 x 2561 86 (60 %).
 #include "common.cuh"
 #include "elements.cuh"
@@ -40,7 +40,7 @@ constexpr int ring_threads(int per) { return per == 4 ? 640 : 512; }     // at m
 constexpr int ring_ctas(int per) { return per == 1 ? 3 : per == 2 ? 2 : 1; }
 constexpr int kAhead = 2;            // rows whose copies are under way
 constexpr int N_SMEM = 227 * 1024;
-constexpr float kSmall = 7.888609e-31f, kSmallUp = 1.2676506e30f;     // 2^-100, 2^100
+constexpr float kSmall = 0x1p-100f, kSmallUp = 0x1p100f;
 constexpr float kLargeDown = 1.2621774e-29f;                          // 2^-96
 constexpr float kWhole = 12582912.f;                                  // 1.5 * 2^23
 
@@ -153,22 +153,78 @@ __device__ __forceinline__ void row_statistics(const NormArgs& a, Joined& red, F
 }
 
 // nearest(127 p / top) as the low byte of fma(p, 127 / top, 1.5 * 2^23), whose one
-// rounding is to a whole number (no conversion, which runs at a quarter of the
-// rate): off from p / s by what 127 / top is, so only values as near to half-way as
-// that may go to the other neighbour.  Tops below 2^-100 are taken 2^100 as large, so
-// that 127 / top stays finite, and those above 2^100 2^-100 as large (the fast
-// division gives zero for divisors past 2^126).
+// rounding is to a whole number (no conversion, which runs at a quarter of the rate).
+// 127 / top is off by 2^-24 of itself, so the quotient by 127 * 2^-24 < 7.7e-6 at most:
+// nearer to half-way than that, fp32 does not tell which whole number is the nearest,
+// and it is taken in 64 bits, p * ((1 / top) * 127), of two the even one.  That is one
+// quotient in 60000, and half-way itself is common in 16-bit rows: p = top / 2 alone is
+// one number in 700 of a normal row of bf16.  (With the fast division, off by 2^-22,
+// four times as many are taken twice: 32768 x 3584 144 us, so 139.)  Tops below 2^-100
+// are taken 2^100 as large, so that 127 / top stays finite.
+constexpr float kSure = 0.5f - 8e-6f;
 struct Whole {
-  float up, inv;
+  float top, up, inv;
   uint32_t keep;       // no bits of rows that are zeros or not numbers
-  __device__ __forceinline__ explicit Whole(float top) {
+  __device__ __forceinline__ explicit Whole(float t) : top(t) {
     const bool none = !(top > 0.f) || magnitude(top) >= kInfBits;
-    up = top < kSmall ? kSmallUp : top > kSmallUp ? kSmall : 1.f;
-    inv = none ? 0.f : __fdividef(127.f, top * up);     // to 2 units in the last place
+    up = top < kSmall ? kSmallUp : 1.f;
+    inv = none ? 0.f : 127.f / (top * up);
     keep = none ? 0u : 0xffffffffu;
   }
-  __device__ __forceinline__ uint32_t operator()(float p) const { return __float_as_uint(fmaf(p * up, inv, kWhole)); }
+  // A pair's whole numbers in the low bytes; `far` (where it counts): the farthest that a quotient was from its own.
+  template <bool kPlain, bool kCount = true> __device__ __forceinline__ uint2 near(float2 p, float& far) const {
+    if (!kPlain) p = fmul2(p, make_float2(up, up));
+    const float2 by = make_float2(inv, inv), m = ffma2(p, by, make_float2(kWhole, kWhole));
+    if (kCount) {
+      const float2 off = ffma2(p, by, ffma2(m, make_float2(-1.f, -1.f), make_float2(kWhole, kWhole)));
+      far = top_of(far, off.x, off.y);         // (no number: neither is top, and nothing is kept)
+    }
+    return make_uint2(__float_as_uint(m.x), __float_as_uint(m.y));
+  }
+  static __device__ __forceinline__ double quotient(float top) { return 1.0 / static_cast<double>(top) * 127.0; }
+  static __device__ __forceinline__ uint32_t decided(float p, double by) {
+    return static_cast<uint32_t>(__double2int_rn(static_cast<double>(p) * by));
+  }
+  // A pair that may be nearer to half-way than fp32 tells.
+  __device__ __forceinline__ uint2 nearest(float2 p, double by) const {
+    float far = 0.f;
+    uint2 n = near<false>(p, far);
+    if (far > kSure) n = make_uint2(decided(p.x, by), decided(p.y, by));
+    return n;
+  }
+  __device__ __forceinline__ uint2 nearest(float2 p) const {
+    float far = 0.f;
+    const uint2 n = near<false>(p, far);
+    return far > kSure ? nearest(p, quotient(top)) : n;
+  }
 };
+
+// Rows of 16-bit numbers themselves: 254 p = (2 k + 1) top, half-way, asks that 127, a
+// prime, divides 2 k + 1 (then it is 127, and p = top / 2) or top's significand, and
+// any other quotient is 1 / (253 * 2047) of itself or more from half-way.  So unless
+// 127 divides the significand, 127 / top taken 2^-21 too large or too small, to the
+// side where 64 bits put top / 2, gives every whole number; and if it is 127 (times a
+// power of two), 127 / top is a power of two, and the fma rounds the quotient itself.
+// All this goes by the significand alone: a CTA of many rows works it out for all of
+// them while its first rows are on their way.
+enum Side : unsigned char { kBelow, kAbove, kExact, kUnsure };
+template <typename T> constexpr int SIDES = std::is_same_v<T, __half> ? 1024 : 128;
+template <typename T> __device__ __forceinline__ void set_sides(unsigned char* sides) {
+  for (int i = threadIdx.x; i < SIDES<T>; i += blockDim.x) {
+    const int digits = SIDES<T> + i;
+    const float top = static_cast<float>(digits);
+    if (digits % 127 != 0) sides[i] = Whole::decided(0.5f * top, Whole::quotient(top)) == 64u ? kAbove : kBelow;
+    else sides[i] = (digits / 127 & (digits / 127 - 1)) == 0 ? kExact : kUnsure;
+  }
+}
+// Whether `whole` is now such that no quotient has to be looked at twice.
+template <typename T> __device__ __forceinline__ bool take_side(Whole& whole, const unsigned char* sides) {
+  const unsigned char side = sides[(__float_as_uint(whole.top) & 0x7fffffu) / (0x800000u / SIDES<T>)];
+  if (side == kUnsure || whole.up != 1.f) return false;
+  if (side == kExact) whole.inv = __uint_as_float((__float_as_uint(whole.inv) + 0x400000u) & 0x7f800000u);
+  else whole.inv *= side == kAbove ? 1.f + 0x1p-21f : 1.f - 0x1p-21f;
+  return true;
+}
 
 // (Small tops times r first: their quotients may be below the smallest normal number.)
 __device__ __forceinline__ float scale_of(float top, float rstd) {
@@ -190,28 +246,28 @@ template <int V> __device__ __forceinline__ void store_whole(int8_t* p, const ui
   }
 }
 
+template <int V> __device__ __forceinline__ void set_two(uint32_t (&n)[V], int p, uint2 two) {
+  n[2 * p] = two.x;
+  if constexpr (V > 1) n[2 * p + 1] = two.y;
+}
+
+// A pair of h w (or of the row itself).
+template <typename T, int V, bool kNorm, bool kPlain>
+__device__ __forceinline__ float2 product_of(const Elements<T, V>& h, const Elements<T, V>& w, int p, float down) {
+  float2 f = pair_of(h, p);
+  if (!kPlain) f = fmul2(f, make_float2(down, down));
+  return kNorm ? fmul2(f, pair_of(w, p)) : f;
+}
 // What a row's thread writes of vector v (elements v V on) once the statistics are
 // known; kPlain: neither the row nor its top was scaled.
-template <typename T, int V, bool kNorm, bool kQ8, bool kPlain>
+template <typename T, int V, bool kNorm, bool kQ8, bool kPlain, bool kCount = true>
 __device__ __forceinline__ void write_vector(const NormArgs& a, int64_t row, int v, const Elements<T, V>& h,
-                                             const Elements<T, V>& w, float rstd, float down, const Whole& whole) {
+                                             const Elements<T, V>& w, float rstd, float down, const Whole& whole, float& far) {
   if constexpr (kQ8) {
     uint32_t n[V];
-    if constexpr (V == 1) {
-      const float f = to_float(h.e[0]);
-      n[0] = whole(kNorm ? f * down * to_float(w.e[0]) : f);
-    } else {
 #pragma unroll
-      for (int p = 0; p < V / 2; ++p) {
-        float2 f = pair_of(h, p);
-        if (!kPlain) f = fmul2(f, make_float2(down, down));
-        if (kNorm) f = fmul2(f, pair_of(w, p));
-        if (!kPlain) f = fmul2(f, make_float2(whole.up, whole.up));
-        f = ffma2(f, make_float2(whole.inv, whole.inv), make_float2(kWhole, kWhole));
-        n[2 * p] = __float_as_uint(f.x);
-        n[2 * p + 1] = __float_as_uint(f.y);
-      }
-    }
+    for (int p = 0; p < (V + 1) / 2; ++p)
+      set_two<V>(n, p, whole.template near<kPlain, kCount>(product_of<T, V, kNorm, kPlain>(h, w, p, down), far));
     store_whole<V>(a.q + row * a.q_stride + static_cast<int64_t>(v) * V, n, whole.keep);
   } else {
     Elements<T, V> o;
@@ -228,21 +284,48 @@ __device__ __forceinline__ void write_vector(const NormArgs& a, int64_t row, int
     reinterpret_cast<Elements<T, V>*>(static_cast<T*>(a.y) + row * a.dim)[v] = o;
   }
 }
+// Its whole numbers once more, where a quotient was too near to half-way.
+template <typename T, int V, bool kNorm>
+__device__ __forceinline__ void write_nearest(const NormArgs& a, int64_t row, int v, const Elements<T, V>& h,
+                                              const Elements<T, V>& w, float down, const Whole& whole, double by) {
+  uint32_t n[V];
+#pragma unroll
+  for (int p = 0; p < (V + 1) / 2; ++p) set_two<V>(n, p, whole.nearest(product_of<T, V, kNorm, false>(h, w, p, down), by));
+  store_whole<V>(a.q + row * a.q_stride + static_cast<int64_t>(v) * V, n, whole.keep);
+}
+// `sides`: those of set_sides, or none.
 template <typename T, int V, int kPer, bool kNorm, bool kQ8>
 __device__ __forceinline__ void write_row(const NormArgs& a, int64_t row, int t, int team, const Elements<T, V> (&h)[kPer],
-                                          const Elements<T, V>* weight, float rstd, float down, float top) {
+                                          const Elements<T, V>* weight, float rstd, float down, float top,
+                                          const unsigned char* sides = nullptr) {
   const int vecs = a.dim / V;
-  const Whole whole(kQ8 ? top : 0.f);
-  if ((!kNorm || down == 1.f) && (!kQ8 || whole.up == 1.f)) {
+  Whole whole(kQ8 ? top : 0.f);
+  float far = 0.f;
+  const bool halves = kQ8 && !kNorm && sizeof(T) == 2 && sides != nullptr;
+  if (halves && take_side<T>(whole, sides)) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
       if (t + i * team < vecs)
-        write_vector<T, V, kNorm, kQ8, true>(a, row, t + i * team, h[i], kNorm ? weight[t + i * team] : h[i], rstd, down, whole);
+        write_vector<T, V, kNorm, kQ8, true, false>(a, row, t + i * team, h[i], h[i], rstd, down, whole, far);
+    return;
+  }
+  if (!halves && (!kNorm || down == 1.f) && (!kQ8 || whole.up == 1.f)) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (t + i * team < vecs)
+        write_vector<T, V, kNorm, kQ8, true>(a, row, t + i * team, h[i], kNorm ? weight[t + i * team] : h[i], rstd, down, whole, far);
   } else {
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
       if (t + i * team < vecs)
-        write_vector<T, V, kNorm, kQ8, false>(a, row, t + i * team, h[i], kNorm ? weight[t + i * team] : h[i], rstd, down, whole);
+        write_vector<T, V, kNorm, kQ8, false>(a, row, t + i * team, h[i], kNorm ? weight[t + i * team] : h[i], rstd, down, whole, far);
+  }
+  if (kQ8 && far > kSure) {
+    const double by = Whole::quotient(top);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (t + i * team < vecs)
+        write_nearest<T, V, kNorm>(a, row, t + i * team, h[i], kNorm ? weight[t + i * team] : h[i], down, whole, by);
   }
 }
 template <bool kQ8> __device__ __forceinline__ void write_statistics(const NormArgs& a, int64_t row, float rstd, float down, float top) {
@@ -318,7 +401,9 @@ __global__ void __launch_bounds__(N_MAX_THREADS) norm_kernel(const NormArgs a) {
   }, rstd, top, down);
   if constexpr (kPer == 1) {
     const Whole whole(kQ8 ? top : 0.f);
-    if (t < vecs) write_vector<T, V, kNorm, kQ8, false>(a, row, t, h[0], w[0], rstd, down, whole);
+    float far = 0.f;
+    if (t < vecs) write_vector<T, V, kNorm, kQ8, false>(a, row, t, h[0], w[0], rstd, down, whole, far);
+    if (kQ8 && far > kSure) write_nearest<T, V, kNorm>(a, row, t, h[0], w[0], down, whole, Whole::quotient(top));
   } else {
     write_row<T, V, kPer, kNorm, kQ8>(a, row, t, team, h, static_cast<const Vec*>(a.weight), rstd, down, top);
   }
@@ -396,10 +481,9 @@ __global__ void __launch_bounds__(N_MAX_THREADS) norm_words_kernel(const NormArg
     float2 f = fmul2(pair_of(v, 0), make_float2(down, down));
     if (kNorm && !kQ8) f = fmul2(f, make_float2(rstd, rstd));
     if (kNorm) f = fmul2(f, pair_of(w, 0));
-    if (kQ8) f = ffma2(fmul2(f, make_float2(whole.up, whole.up)), make_float2(whole.inv, whole.inv), make_float2(kWhole, kWhole));
     return f;
   };
-  auto byte = [&](float f) { return static_cast<int8_t>(__float_as_uint(f) & whole.keep); };
+  auto byte = [&](uint32_t n) { return static_cast<int8_t>(n & whole.keep); };
   T* y = static_cast<T*>(a.y) + row * a.dim;
   int8_t* q = a.q + row * a.q_stride;
 #pragma unroll
@@ -407,8 +491,9 @@ __global__ void __launch_bounds__(N_MAX_THREADS) norm_words_kernel(const NormArg
     if (t + i * team >= at.count) continue;
     const float2 f = result(h[i], kNorm ? at.any(weight, t + i * team) : h[i]);
     if (kQ8) {
-      q[at.odd + 2 * (t + i * team)] = byte(f.x);
-      q[at.odd + 2 * (t + i * team) + 1] = byte(f.y);
+      const uint2 n = whole.nearest(f);
+      q[at.odd + 2 * (t + i * team)] = byte(n.x);
+      q[at.odd + 2 * (t + i * team) + 1] = byte(n.y);
     } else {
       Two o;
       set_pair(o, 0, f);
@@ -417,8 +502,9 @@ __global__ void __launch_bounds__(N_MAX_THREADS) norm_words_kernel(const NormArg
   }
   const float2 f = result(h[kPer], kNorm ? at.ends(weight, t) : h[kPer]);
   if (kQ8) {
-    if (t == 0 && at.odd) q[0] = byte(f.x);
-    if (t == 0 && at.tail) q[at.last] = byte(f.y);
+    const uint2 n = whole.nearest(f);
+    if (t == 0 && at.odd) q[0] = byte(n.x);
+    if (t == 0 && at.tail) q[at.last] = byte(n.y);
   } else {
     Two o;
     set_pair(o, 0, f);
@@ -437,6 +523,8 @@ __global__ void __launch_bounds__(ring_threads(kPer), ring_ctas(kPer)) norm_ring
   using Vec = Elements<T, V>;
   extern __shared__ __align__(16) unsigned char slots[];
   __shared__ Joined red[2];                    // in turn: a row's are read until the next row's barrier
+  constexpr bool kSides = kQ8 && !kNorm && sizeof(T) == 2;
+  __shared__ unsigned char sides[kSides ? SIDES<T> : 1];
   if (a.row_warps > 1) {
     clear(red, 2);
     __syncthreads();
@@ -470,6 +558,9 @@ __global__ void __launch_bounds__(ring_threads(kPer), ring_ctas(kPer)) norm_ring
   if (kNorm) {
     for (int v = threadIdx.x; v < vecs; v += threads) weight[v] = static_cast<const Vec*>(a.weight)[v];
     __syncthreads();
+  } else if (kSides) {
+    set_sides<T>(sides);
+    __syncthreads();
   }
   int s = 0, turn = 0;
   for (; row < a.rows; row += step, turn ^= 1) {
@@ -495,7 +586,7 @@ __global__ void __launch_bounds__(ring_threads(kPer), ring_ctas(kPer)) norm_ring
       for (int i = 0; i < kPer; ++i)
         if (t + i * team < vecs) s.add(h[i], kNorm && kQ8 ? weight[t + i * team] : h[i]);
     }, rstd, top, down);
-    write_row<T, V, kPer, kNorm, kQ8>(a, row, t, team, h, weight, rstd, down, top);
+    write_row<T, V, kPer, kNorm, kQ8>(a, row, t, team, h, weight, rstd, down, top, kSides ? sides : nullptr);
     if (t == 0) write_statistics<kQ8>(a, row, rstd, down, top);
   }
 }
@@ -526,7 +617,7 @@ __global__ void __launch_bounds__(N_MAX_THREADS) norm_wide_kernel(const NormArgs
     const T h = h_at(i);
     const float f = to_float(h) * down, w = kNorm ? to_float(weight[i]) : 1.f;
     if (kNorm && res != nullptr) static_cast<T*>(a.h)[row * a.dim + i] = h;
-    if (kQ8) a.q[row * a.q_stride + i] = static_cast<int8_t>(whole(kNorm ? f * w : f) & whole.keep);
+    if (kQ8) a.q[row * a.q_stride + i] = static_cast<int8_t>(whole.nearest(make_float2(kNorm ? f * w : f, 0.f)).x & whole.keep);
     else static_cast<T*>(a.y)[row * a.dim + i] = from_float<T>(f * rstd * w);
   }
   if (threadIdx.x == 0) write_statistics<kQ8>(a, row, rstd, down, top);
@@ -866,7 +957,7 @@ int launch_ring(NormArgs a, cudaStream_t s) {
   a.row_warps = warps_for(a.dim / V, kPer);
   const int side = a.row_warps == 1 ? N_SHORT_ROWS : 1, threads = 32 * a.row_warps * side;
   const int smem = kAhead * (kNorm && a.residual ? 2 : 1) * kPer * threads * 16 + (kNorm ? a.dim * static_cast<int>(sizeof(T)) : 0);
-  if (!allow_smem(norm_ring_kernel<T, kPer, kNorm, kQ8>, N_SMEM - 1024, allowed)) return MRSA_ERR_LAUNCH;
+  if (!allow_smem(norm_ring_kernel<T, kPer, kNorm, kQ8>, N_SMEM - 2048, allowed)) return MRSA_ERR_LAUNCH;
   static std::atomic<int> known[2][ring_threads(kPer) / 32 + 1];
   const int per_sm = resident(norm_ring_kernel<T, kPer, kNorm, kQ8>, threads, smem, known[a.residual != nullptr][threads / 32]);
   const int64_t need = (a.rows + side - 1) / side, most = static_cast<int64_t>(per_sm) * sm_count();
@@ -891,7 +982,7 @@ int norm_of(const NormArgs& a, cudaStream_t s) {
     }
     // Four vectors to a thread (a warp to a row of up to 1024 elements of 16 bits), two
     // where the rows would leave SMs short of warps (256 rows of 3584 in 8 bits 3.2 us,
-    // with four 4.3; 32768 rows 139, with four 135), one for rows of a warp, eight past
+    // with four 4.3; 32768 rows 139, with four 135; before quotients were looked at twice), one for rows of a warp, eight past
     // 640 threads.
     if (vecs <= 32) return launch_ring<T, 1, kNorm, kQ8>(a, s);
     if (vecs <= 64 || (vecs <= 1024 && a.rows <= 4 * sm_count())) return launch_ring<T, 2, kNorm, kQ8>(a, s);

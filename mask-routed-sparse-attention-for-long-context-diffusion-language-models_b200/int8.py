@@ -27,16 +27,17 @@ from . import _lib
 def quantize_int8(x: torch.Tensor):
     """``(q, scale)``: each row (last dimension) of ``x`` (bf16, fp16 or fp32)
     as int8 whole numbers and an fp32 scale, ``scale = max|x| / 127`` and ``q``
-    the whole number nearest ``x / scale`` (where that is half-way to within
-    fp32's rounding, either neighbour).  Zeros have scale 0; a row with a NaN
-    or an infinity has scale NaN, and so has what is computed from it.  ``q``
-    has ``x``'s shape, its rows on 16-byte boundaries."""
+    the whole number nearest ``x * (127 / max|x|)`` in 64 bits (the reciprocal of
+    ``max|x|`` times 127, as torch divides), of two the even one.  Zeros have scale 0; a row with a NaN or an
+    infinity has scale NaN, and so has what is computed from it.  ``q`` has
+    ``x``'s shape, its rows on 16-byte boundaries."""
     return _lib.ext().quantize_int8(x)
 
 
 def add_rms_norm_int8(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor, eps: float):
     """``(q, scale, h)``: :func:`add_rms_norm` with its norm in 8 bits, as
-    :func:`quantize_int8` gives it (of the norm in fp32, not rounded before)."""
+    :func:`quantize_int8` gives it (of the norm in fp32, not rounded before;
+    ``q`` is that of ``h * weight``, products of fp32 numbers rounded to fp32)."""
     return _lib.ext().add_rms_norm_int8(x, residual, weight, eps)
 
 

@@ -62,6 +62,36 @@ def test_norm_int8(mrsa, cuda_device, rows, dim, kind):
         check_whole(q, scale, p, p.abs().amax(-1) / 127 / (d.square().mean(-1) + 1e-6).sqrt(), 5e-6)
 
 
+def nearest(p):
+    """The whole numbers of rows p, in 64 bits, of two the even one."""
+    return torch.round(p * (127.0 / p.abs().amax(-1, keepdim=True)))
+
+
+# a few rows, more than one and than four to an SM; by words, by elements, past the registers
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("rows,dim", [(2, 40), (300, 256), (2, 999), (1000, 1000), (700, 3584), (3, 4097), (3, 18944), (700, 18944),
+                                      (2, 20001), (2, 65536)])
+def test_whole_numbers_are_the_nearest(mrsa, cuda_device, rows, dim, kind):
+    """Every one of them, with as many half-way as a row can have."""
+    dev, dtype = cuda_device, TYPES[kind]
+    g = torch.Generator(device=dev).manual_seed(9)
+    # k + 1/2 times 1 / 64, and 127 / 64 once: half-way exactly, as are the bounds' quotients in 64 bits
+    half_way = (torch.randint(-127, 127, (rows, dim), device=dev, generator=g).double() + 0.5) / 64
+    half_way[torch.arange(rows, device=dev), torch.randint(0, dim, (rows,), device=dev, generator=g)] = 127 / 64
+    x = half_way.to(dtype)
+    sign = torch.where(torch.rand(dim, device=dev, generator=g) < 0.5, -1.0, 1.0).to(dtype)
+    want = torch.round(half_way * 64)
+    assert torch.equal(mrsa.quantize_int8(x)[0].double(), want)
+    assert torch.equal(mrsa.add_rms_norm_int8(x, None, sign, 1e-6)[0].double(), want * sign.double())
+    x, r = (torch.randn(rows, dim, device=dev, generator=g).to(dtype) for _ in range(2))
+    w = (1 + 0.3 * torch.randn(dim, device=dev, generator=g)).to(dtype)
+    assert torch.equal(mrsa.quantize_int8(x)[0].double(), nearest(x.double()))
+    q, _, h = mrsa.add_rms_norm_int8(x, r, w, 1e-6)
+    # (products of 16-bit numbers are exact in fp32; those of fp32 numbers are rounded to it)
+    assert torch.equal(q.double(), nearest((h.float() * w.float()).double()))
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dim", [1, 7, 64, 999, 18944])
 @pytest.mark.parametrize("rows", [3, 400])
