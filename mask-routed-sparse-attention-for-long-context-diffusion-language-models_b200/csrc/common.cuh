@@ -145,7 +145,8 @@ int build_chunk_index(const int32_t* indices, int64_t batch, int64_t q_len, int 
                       void* workspace, cudaStream_t s, ChunkIndex* out);
 
 // ---- sm_100 paired fp32 arithmetic (one instruction for two lanes of work)
-// fma/add/mul on a register pair, each half rounded as the scalar op would be.
+// fma/add/mul on a register pair, each half rounded as the scalar op would be (but
+// that the assembler may join an fmul2 and the fadd2 of its result to one fma).
 __device__ __forceinline__ float2 ffma2(float2 a, float2 b, float2 c) {
   float2 d;
   asm("{\n\t.reg .b64 ra, rb, rc, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"

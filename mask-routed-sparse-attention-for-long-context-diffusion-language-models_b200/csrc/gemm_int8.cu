@@ -253,16 +253,19 @@ __global__ void __launch_bounds__(G8_THREADS, 1) gemm_int8_kernel(const __grid_c
           if (lane == 0) tc::peer_arrive(tc::peer_addr(tc::smem_addr(&sm.acc_empty[buf]), 0));
         }
         if (col0 + j >= cols) continue;
+        // each product and the sum rounded by itself, as the kernel for few rows does: a row
+        // has the same bits from both
         float v[32];
 #pragma unroll
         for (int e = 0; e < 32; ++e) {
-          const float x = static_cast<float>(static_cast<int>(r[e])) * as;
-          if constexpr (kSwiglu) v[e] = silu<T>(x * bs[j + e]) * (static_cast<float>(static_cast<int>(u[e])) * as * bs[kOut + j + e]);
-          else v[e] = x * bs[j + e];
+          const float x = __fmul_rn(static_cast<float>(static_cast<int>(r[e])), as);
+          v[e] = __fmul_rn(x, bs[j + e]);
+          if constexpr (kSwiglu)
+            v[e] = silu<T>(v[e]) * __fmul_rn(__fmul_rn(static_cast<float>(static_cast<int>(u[e])), as), bs[kOut + j + e]);
         }
         if (add) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] += bias[j + e];
+          for (int e = 0; e < 32; ++e) v[e] = __fadd_rn(v[e], bias[j + e]);
         }
         if (a.rows16) {
           if (j % kStep == 0) {                // the store before has read the staged rows

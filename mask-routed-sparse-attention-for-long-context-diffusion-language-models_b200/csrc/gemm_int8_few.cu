@@ -242,9 +242,9 @@ __global__ void __launch_bounds__(F_THREADS, kPerSm) gemm_int8_few_kernel(const 
       const float as = sm.a_scale[tok + i * kWarps];
       const float2 as2 = make_float2(as, as);
       auto scaled = [&](int4 n, const float (&b)[4], int p) {
-        const float2 f = p == 0 ? make_float2(static_cast<float>(n.x), static_cast<float>(n.y))
-                                : make_float2(static_cast<float>(n.z), static_cast<float>(n.w));
-        return fmul2(fmul2(f, as2), make_float2(b[2 * p], b[2 * p + 1]));
+        const float2 f = fmul2(p == 0 ? make_float2(static_cast<float>(n.x), static_cast<float>(n.y))
+                                      : make_float2(static_cast<float>(n.z), static_cast<float>(n.w)), as2);
+        return make_float2(__fmul_rn(f.x, b[2 * p]), __fmul_rn(f.y, b[2 * p + 1]));
       };
       struct alignas(4 * sizeof(T)) Four { T e[4]; } o;
 #pragma unroll
@@ -254,7 +254,9 @@ __global__ void __launch_bounds__(F_THREADS, kPerSm) gemm_int8_few_kernel(const 
           const float2 u = scaled(s[i][kAcc - 1], bs[kAcc - 1], p);
           v = make_float2(silu<T>(v.x) * u.x, silu<T>(v.y) * u.y);
         } else {
-          v = fadd2(v, make_float2(bias[2 * p], bias[2 * p + 1]));
+          // (not fadd2, which the assembler joins with the product to one fma: the kernel for
+          // many rows rounds both, and a row has the same bits from either)
+          v = make_float2(__fadd_rn(v.x, bias[2 * p]), __fadd_rn(v.y, bias[2 * p + 1]));
         }
         o.e[2 * p] = from_float<T>(v.x);
         o.e[2 * p + 1] = from_float<T>(v.y);

@@ -232,6 +232,19 @@ def test_rows_do_not_depend_on_the_others(mrsa, cuda_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("n", [4001, 4608])
+def test_rows_with_bias_do_not_depend_on_the_others(mrsa, cuda_device, n, kind):
+    """Rows of the kernels for many rows and for few, their outputs' last bits and the bias's rounding."""
+    m = 2500
+    assert (m + 127) // 128 * ((n + 255) // 256) > 2 * torch.cuda.get_device_properties(cuda_device).multi_processor_count
+    q, scale, w, ws, bias = operands(cuda_device, m, n, 333, 12)
+    y = mrsa.linear_int8(q, scale, w, ws, bias, dtype=TYPES[kind])
+    for rows in (slice(0, 1), slice(3, 40), slice(100, 228), slice(2400, 2500), slice(500, 1100)):
+        assert torch.equal(mrsa.linear_int8(q[rows], scale[rows], w, ws, bias, dtype=TYPES[kind]), y[rows])
+
+
+@pytest.mark.gpu
 def test_layouts(mrsa, cuda_device):
     """Leading dimensions, strides, unaligned rows, one row, none."""
     dev = cuda_device
