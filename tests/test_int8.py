@@ -206,6 +206,33 @@ def test_swiglu(mrsa, cuda_device, m, f, k):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(2500, 4001, 333), (4097, 2600, 1000), (8191, 4608, 130), (2048, 5000, 640)])
+def test_linear_of_many_rows(mrsa, cuda_device, m, n, k):
+    """Products that the kernel for many rows takes (a tile of 128 x 256 to each SM), two and more tiles of 256 x 256 to each
+    pair of SMs: all types and biases, rows of C on and off 16-byte boundaries, ragged edges."""
+    assert (m + 127) // 128 * ((n + 255) // 256) > 2 * torch.cuda.get_device_properties(cuda_device).multi_processor_count
+    q, scale, w, ws, bias = operands(cuda_device, m, n, k, 10)
+    for i, dtype in enumerate(TYPES.values()):
+        check_linear(mrsa.linear_int8(q, scale, w, ws, dtype=dtype), q, scale, w, ws, None)
+        b = bias.to(list(TYPES.values())[(i + 1) % 3])
+        check_linear(mrsa.linear_int8(q, scale, w, ws, b, dtype=dtype), q, scale, w, ws, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", TYPES)
+def test_swiglu_of_many_rows(mrsa, cuda_device, kind):
+    """Three tiles of 256 x 256 and more to each pair of SMs; the rows as calls of a few give them, which
+    test_swiglu compares with 64 bits."""
+    m, f, k = 4000, 2048, 700
+    assert (m + 255) // 256 * (2 * f // 256) > 3 * torch.cuda.get_device_properties(cuda_device).multi_processor_count // 2
+    q, scale, w, ws, _ = operands(cuda_device, m, 2 * f, k, 11)
+    ws = ws * 20 * k ** 0.5 / 74
+    y = mrsa.swiglu_int8(q, scale, w, ws, dtype=TYPES[kind])
+    for at in range(0, m, 128):
+        assert torch.equal(mrsa.swiglu_int8(q[at:at + 128], scale[at:at + 128], w, ws, dtype=TYPES[kind]), y[at:at + 128])
+
+
+@pytest.mark.gpu
 def test_sums_are_exact(mrsa, cuda_device):
     """The longest sum that 32 bits hold, and single ones among zeros."""
     dev = cuda_device
