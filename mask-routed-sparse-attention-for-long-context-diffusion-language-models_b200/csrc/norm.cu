@@ -922,16 +922,19 @@ int launch_norm(NormArgs a, cudaStream_t s) {
                         a.row_warps == 1 ? 32 * N_SHORT_ROWS : 32 * a.row_warps, 0, s, a);
 }
 
-// CTAs that an SM holds at once, asked for once per size.
+// CTAs that an SM holds at once, asked for once per number of threads as long as the
+// shared memory stays the same: that goes by the row's width too, and so does the
+// answer, on which the parts of dw and with them its bits depend.  `known`: both.
 template <typename K>
-int resident(K* kernel, int threads, int smem, std::atomic<int>& known) {
-  int n = known.load(std::memory_order_relaxed);
-  if (n > 0) return n;
+int resident(K* kernel, int threads, int smem, std::atomic<uint64_t>& known) {
+  const uint64_t k = known.load(std::memory_order_relaxed);
+  if (k >> 32 == static_cast<uint64_t>(smem) && k != 0) return static_cast<int>(k & 0xffffffffu);
+  int n = 0;
   if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, static_cast<size_t>(smem)) != cudaSuccess || n < 1) {
     (void)cudaGetLastError();
     return 1;
   }
-  known.store(n, std::memory_order_relaxed);
+  known.store(static_cast<uint64_t>(smem) << 32 | static_cast<uint64_t>(n), std::memory_order_relaxed);
   return n;
 }
 
@@ -958,7 +961,7 @@ int launch_ring(NormArgs a, cudaStream_t s) {
   const int side = a.row_warps == 1 ? N_SHORT_ROWS : 1, threads = 32 * a.row_warps * side;
   const int smem = kAhead * (kNorm && a.residual ? 2 : 1) * kPer * threads * 16 + (kNorm ? a.dim * static_cast<int>(sizeof(T)) : 0);
   if (!allow_smem(norm_ring_kernel<T, kPer, kNorm, kQ8>, N_SMEM - 2048, allowed)) return MRSA_ERR_LAUNCH;
-  static std::atomic<int> known[2][ring_threads(kPer) / 32 + 1];
+  static std::atomic<uint64_t> known[2][ring_threads(kPer) / 32 + 1];
   const int per_sm = resident(norm_ring_kernel<T, kPer, kNorm, kQ8>, threads, smem, known[a.residual != nullptr][threads / 32]);
   const int64_t need = (a.rows + side - 1) / side, most = static_cast<int64_t>(per_sm) * sm_count();
   return launch_chained(norm_ring_kernel<T, kPer, kNorm, kQ8>, dim3(static_cast<unsigned>(need < most ? need : most)), threads,
@@ -1024,7 +1027,7 @@ int64_t backward_grid(int64_t rows, int64_t dim) {
 template <typename T, int V, int kPer, int kRows>
 int launch_backward_rows(BackwardArgs& a, int threads, int smem, cudaStream_t s) {
   static std::atomic<uint64_t> allowed{0};
-  static std::atomic<int> known[2][ring_threads(kPer) / 32 + 1];
+  static std::atomic<uint64_t> known[2][ring_threads(kPer) / 32 + 1];
   if (!allow_smem(norm_backward_ring_kernel<T, V, kPer, kRows>, N_SMEM - 1024, allowed)) return MRSA_ERR_LAUNCH;
   const int64_t most = static_cast<int64_t>(resident(norm_backward_ring_kernel<T, V, kPer, kRows>, threads, smem,
                                                      known[a.gh != nullptr][threads / 32])) * sm_count();

@@ -8,8 +8,13 @@ half of 138 * 2^-24 at most, y by 5e-6 and a rounding to its type.  The
 gradient's sums are such chains too, so they are off by 1e-5 of the sums of
 their terms' magnitudes."""
 
+import subprocess
+import sys
+
 import pytest
 import torch
+
+from conftest import ROOT
 
 TYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
 # one element; odd; a warp; a CTA; unaligned and wide rows; past the registers
@@ -87,6 +92,29 @@ def test_gradient(mrsa, cuda_device, rows, dim, kind):
     check_gradient((dx, None), gy, None, h.detach(), w.detach(), dtype)
     y, _ = mrsa.add_rms_norm(x, None, w, EPS)
     check_gradient(torch.autograd.grad(y, (x, w), gy), gy, None, x.detach(), w.detach(), dtype)
+
+
+_DWEIGHT = """
+import hashlib, sys
+import torch
+import __graft_entry__
+m = __graft_entry__.load_package()
+for dim in map(int, sys.argv[1:]):
+    g = torch.Generator(device="cuda").manual_seed(0)
+    x, r, gy, gh = (torch.randn(1000, dim, device="cuda", generator=g) for _ in range(4))
+    w = torch.ones(dim, device="cuda", requires_grad=True)
+    dw, = torch.autograd.grad(m.add_rms_norm(x, r, w, 1e-6), w, (gy, gh))
+print(hashlib.sha256(dw.cpu().view(torch.uint8).numpy().tobytes()).hexdigest())
+"""
+
+
+@pytest.mark.gpu
+def test_gradient_does_not_depend_on_calls_before(cuda_device):
+    """The same bits of dw in a process that took another width before, of as many threads, whose rows leave room for
+    another CTA."""
+    out = [subprocess.run([sys.executable, "-c", _DWEIGHT, *dims], cwd=ROOT, capture_output=True, text=True, check=True,
+                          timeout=300).stdout.strip() for dims in (("2048",), ("1800", "2048"))]
+    assert len(out[0]) == 64 and out[0] == out[1]
 
 
 @pytest.mark.gpu
