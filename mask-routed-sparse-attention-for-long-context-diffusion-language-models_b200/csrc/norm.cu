@@ -41,7 +41,7 @@ constexpr int ring_ctas(int per) { return per == 1 ? 3 : per == 2 ? 2 : 1; }
 constexpr int kAhead = 2;            // rows whose copies are under way
 constexpr int N_SMEM = 227 * 1024;
 constexpr float kSmall = 0x1p-100f, kSmallUp = 0x1p100f;
-constexpr float kLargeDown = 1.2621774e-29f;                          // 2^-96
+constexpr float kLargeDown = 0x1p-96f;
 constexpr float kWhole = 12582912.f;                                  // 1.5 * 2^23
 
 struct NormArgs {
@@ -130,7 +130,8 @@ template <bool kNorm, bool kQ8, bool kDown> struct Statistics {
 
 // A row's statistics from its elements in registers (or memory): each(s) adds this
 // thread's to s.  Rows whose squares (or products with w) pass the largest fp32
-// number are summed once more, 2^-96 as large; `down` says so.
+// number are summed once more, 2^-96 as large; `down` says so of top (rstd is the
+// row's own, to 2^-22 where it is below the smallest normal number).
 template <bool kNorm, bool kQ8, typename F>
 __device__ __forceinline__ void row_statistics(const NormArgs& a, Joined& red, F each, float& rstd, float& top, float& down) {
   Statistics<kNorm, kQ8, false> s;
@@ -146,7 +147,7 @@ __device__ __forceinline__ void row_statistics(const NormArgs& a, Joined& red, F
     if (a.row_warps > 1) __syncthreads();      // red is read no more
     v = join_row<kNorm, kQ8>(l.sums(), a.row_warps, red);
   }
-  rstd = kNorm ? rsqrtf(fmaf(v.squares, a.inv_dim, eps)) : 1.f;      // to 2 units in the last place
+  rstd = kNorm ? rsqrtf(fmaf(v.squares, a.inv_dim, eps)) * down : 1.f;      // to 2 units in the last place
   top = __uint_as_float(v.top);
   // an infinity makes r zero: what it leaves is not a number
   if (kNorm && kQ8 && magnitude(v.squares) >= kInfBits) top = __uint_as_float(0x7fffffffu);
@@ -259,7 +260,7 @@ __device__ __forceinline__ float2 product_of(const Elements<T, V>& h, const Elem
   return kNorm ? fmul2(f, pair_of(w, p)) : f;
 }
 // What a row's thread writes of vector v (elements v V on) once the statistics are
-// known; kPlain: neither the row nor its top was scaled.
+// known; kPlain: neither the row nor its top was scaled (whole numbers).
 template <typename T, int V, bool kNorm, bool kQ8, bool kPlain, bool kCount = true>
 __device__ __forceinline__ void write_vector(const NormArgs& a, int64_t row, int v, const Elements<T, V>& h,
                                              const Elements<T, V>& w, float rstd, float down, const Whole& whole, float& far) {
@@ -271,16 +272,8 @@ __device__ __forceinline__ void write_vector(const NormArgs& a, int64_t row, int
     store_whole<V>(a.q + row * a.q_stride + static_cast<int64_t>(v) * V, n, whole.keep);
   } else {
     Elements<T, V> o;
-    if constexpr (V == 1) {
-      o.e[0] = from_float<T>(to_float(h.e[0]) * down * rstd * to_float(w.e[0]));
-    } else {
 #pragma unroll
-      for (int p = 0; p < V / 2; ++p) {
-        float2 f = pair_of(h, p);
-        if (!kPlain) f = fmul2(f, make_float2(down, down));
-        set_pair(o, p, fmul2(fmul2(f, make_float2(rstd, rstd)), pair_of(w, p)));
-      }
-    }
+    for (int p = 0; p < (V + 1) / 2; ++p) set_pair(o, p, fmul2(fmul2(pair_of(h, p), make_float2(rstd, rstd)), pair_of(w, p)));
     reinterpret_cast<Elements<T, V>*>(static_cast<T*>(a.y) + row * a.dim)[v] = o;
   }
 }
@@ -309,7 +302,7 @@ __device__ __forceinline__ void write_row(const NormArgs& a, int64_t row, int t,
         write_vector<T, V, kNorm, kQ8, true, false>(a, row, t + i * team, h[i], h[i], rstd, down, whole, far);
     return;
   }
-  if (!halves && (!kNorm || down == 1.f) && (!kQ8 || whole.up == 1.f)) {
+  if (!kQ8 || (!halves && (!kNorm || down == 1.f) && whole.up == 1.f)) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
       if (t + i * team < vecs)
@@ -329,8 +322,8 @@ __device__ __forceinline__ void write_row(const NormArgs& a, int64_t row, int t,
   }
 }
 template <bool kQ8> __device__ __forceinline__ void write_statistics(const NormArgs& a, int64_t row, float rstd, float down, float top) {
-  if (kQ8) a.scale[row] = scale_of(top, rstd);
-  else if (a.rstd != nullptr) a.rstd[row] = rstd * down;
+  if (kQ8) a.scale[row] = scale_of(top, rstd * (1.f / down));
+  else if (a.rstd != nullptr) a.rstd[row] = rstd;
 }
 
 // x + residual, rounded: the packed addition rounds the exact sum once; fp32 would
@@ -478,8 +471,8 @@ __global__ void __launch_bounds__(N_MAX_THREADS) norm_words_kernel(const NormArg
   }, rstd, top, down);
   const Whole whole(kQ8 ? top : 0.f);
   auto result = [&](const Two& v, const Two& w) {
-    float2 f = fmul2(pair_of(v, 0), make_float2(down, down));
-    if (kNorm && !kQ8) f = fmul2(f, make_float2(rstd, rstd));
+    const float by = kQ8 ? down : rstd;
+    float2 f = fmul2(pair_of(v, 0), make_float2(by, by));
     if (kNorm) f = fmul2(f, pair_of(w, 0));
     return f;
   };
@@ -615,10 +608,10 @@ __global__ void __launch_bounds__(N_MAX_THREADS) norm_wide_kernel(const NormArgs
   const Whole whole(top);
   for (int i = threadIdx.x; i < a.dim; i += N_MAX_THREADS) {
     const T h = h_at(i);
-    const float f = to_float(h) * down, w = kNorm ? to_float(weight[i]) : 1.f;
+    const float f = to_float(h) * (kQ8 ? down : rstd), w = kNorm ? to_float(weight[i]) : 1.f;
     if (kNorm && res != nullptr) static_cast<T*>(a.h)[row * a.dim + i] = h;
     if (kQ8) a.q[row * a.q_stride + i] = static_cast<int8_t>(whole.nearest(make_float2(kNorm ? f * w : f, 0.f)).x & whole.keep);
-    else static_cast<T*>(a.y)[row * a.dim + i] = from_float<T>(f * rstd * w);
+    else static_cast<T*>(a.y)[row * a.dim + i] = from_float<T>(f * w);
   }
   if (threadIdx.x == 0) write_statistics<kQ8>(a, row, rstd, down, top);
 }

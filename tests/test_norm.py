@@ -227,6 +227,26 @@ def test_extreme_values(mrsa, cuda_device, dim):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["bf16", "fp32"])
+@pytest.mark.parametrize("rows,dim", [(5, 64), (5, 999), (300, 1000), (300, 4096), (3, 40000)])
+def test_rows_past_the_squares(mrsa, cuda_device, rows, dim, kind):
+    """Rows whose squares pass fp32's largest number: small elements beside large ones, and the gradient."""
+    dev, dtype = cuda_device, TYPES[kind]
+    x, r, w, gy, gh = make(dev, rows, dim, dtype, 9)
+    x[:, 1:] *= 2.0 ** -40
+    x[:, 0] = 2.0 ** 66
+    check(mrsa.add_rms_norm(x, None, w, EPS)[0], x, w)
+    x, r = x * 2.0 ** 30, r * 2.0 ** 95
+    for t in (x, r, w):
+        t.requires_grad_()
+    y, h = mrsa.add_rms_norm(x, r, w, EPS)
+    check(y.detach(), h.detach(), w.detach())
+    # gradients of y near one are 2^-96 as large here: so is the stream's own
+    got = torch.autograd.grad((y, h), (x, w), (gy, gh * 2.0 ** -96))
+    check_gradient(got, gy, gh * 2.0 ** -96, h.detach(), w.detach(), dtype)
+
+
+@pytest.mark.gpu
 def test_empty_other_stream_and_graph(mrsa, cuda_device):
     dev = cuda_device
     w = torch.ones(64, device=dev)
