@@ -24,7 +24,7 @@
 //
 // Measured (B200, bf16, us, and of the 6.55 TB/s of a copy): 16384 x 3584 norm with
 // residual 85 (84 %; 96 with a CTA per row and loads in registers), without 45
-// (79 %), with its gradient 160 (90 %; 248); 32768 x 3584 in 8 bits 139 (90 %; 192);
+// (79 %), with its gradient 160 (90 %; 248); 32768 x 3584 in 8 bits 142 (88 %; 192);
 // 16384 x 18944 quantized 175 (81 %; 312).  Rows off 16-byte boundaries go by
 // words: 4095 x 3585 36 (49 %), with gradient 84 (43 %), fp32 4095 x 2561 86 (60 %).
 #include "common.cuh"
@@ -37,7 +37,9 @@ namespace {
 constexpr int N_MAX_THREADS = 1024;
 constexpr int N_SHORT_ROWS = 8;      // rows per CTA where one warp takes a row
 constexpr int ring_threads(int per) { return per == 4 ? 640 : 512; }     // at most, with so many vectors a thread
-constexpr int ring_ctas(int per) { return per == 1 ? 3 : per == 2 ? 2 : 1; }
+// (a vector a thread is eight rows to a CTA of 256 threads; 8-bit rows by themselves spill at six CTAs: 16384 x 200
+// quantized 5.6 us, at five 5.0)
+constexpr int ring_ctas(int per, bool itself) { return per == 1 ? (itself ? 5 : 6) : per == 2 ? 2 : 1; }
 constexpr int kAhead = 2;            // rows whose copies are under way
 constexpr int N_SMEM = 227 * 1024;
 constexpr float kSmall = 0x1p-100f, kSmallUp = 0x1p100f;
@@ -109,12 +111,21 @@ __device__ __forceinline__ float top_of(float a, float b, float c) {
   return d;
 }
 
-// A thread's part of a row's statistics; with kDown of the row 2^-96 as large.
-template <bool kNorm, bool kQ8, bool kDown> struct Statistics {
+// 2^e.
+__device__ __forceinline__ double power(int e) { return __hiloint2double((e + 1023) << 20, 0); }
+
+// A pair of h w 2^shift as large, rounded to fp32 once.
+__device__ __forceinline__ float2 products(float2 h, float2 w, int shift) {
+  const double by = power(shift);
+  return make_float2(static_cast<float>(static_cast<double>(h.x) * static_cast<double>(w.x) * by),
+                     static_cast<float>(static_cast<double>(h.y) * static_cast<double>(w.y) * by));
+}
+
+// A thread's part of a row's statistics.
+template <bool kNorm, bool kQ8> struct Statistics {
   float2 squares = {0.f, 0.f};
   float top = 0.f;
   __device__ __forceinline__ void add(float2 h, float2 w) {
-    if (kDown) h = fmul2(h, make_float2(kLargeDown, kLargeDown));
     if (kNorm) squares = ffma2(h, h, squares);
     if (kQ8) {
       if (kNorm) h = fmul2(h, w);
@@ -127,27 +138,61 @@ template <bool kNorm, bool kQ8, bool kDown> struct Statistics {
   }
   __device__ __forceinline__ RowSums sums() const { return {squares.x + squares.y, magnitude(top)}; }
 };
+// The squares alone, of a row 2^-96 as large.
+struct SquaresDown {
+  float2 squares = {0.f, 0.f};
+  template <typename T, int V> __device__ __forceinline__ void add(const Elements<T, V>& h, const Elements<T, V>&) {
+#pragma unroll
+    for (int p = 0; p < (V + 1) / 2; ++p) {
+      const float2 f = fmul2(pair_of(h, p), make_float2(kLargeDown, kLargeDown));
+      squares = ffma2(f, f, squares);
+    }
+  }
+  __device__ __forceinline__ RowSums sums() const { return {squares.x + squares.y, 0u}; }
+};
+// The largest product alone, 2^shift as large.
+struct TopShifted {
+  int shift;
+  float top = 0.f;
+  template <typename T, int V> __device__ __forceinline__ void add(const Elements<T, V>& h, const Elements<T, V>& w) {
+#pragma unroll
+    for (int p = 0; p < (V + 1) / 2; ++p) {
+      const float2 f = products(pair_of(h, p), pair_of(w, p), shift);
+      top = top_of(top, f.x, f.y);
+    }
+  }
+  __device__ __forceinline__ RowSums sums() const { return {0.f, magnitude(top)}; }
+};
 
 // A row's statistics from its elements in registers (or memory): each(s) adds this
-// thread's to s.  Rows whose squares (or products with w) pass the largest fp32
-// number are summed once more, 2^-96 as large; `down` says so of top (rstd is the
-// row's own, to 2^-22 where it is below the smallest normal number).
+// thread's to s.  A row whose squares pass the largest fp32 number has them summed once
+// more, 2^-96 as large (rstd is the row's own all the same, to 2^-22 where it is below
+// the smallest normal number).  Products of h and w have twice the exponents of fp32: a
+// row whose largest is past its range, or below 2^-100, where the others lose digits,
+// has its products in 64 bits, 2^-144 or 2^200 as large; `shift` says so of top.
 template <bool kNorm, bool kQ8, typename F>
-__device__ __forceinline__ void row_statistics(const NormArgs& a, Joined& red, F each, float& rstd, float& top, float& down) {
-  Statistics<kNorm, kQ8, false> s;
+__device__ __forceinline__ void row_statistics(const NormArgs& a, Joined& red, F each, float& rstd, float& top, int& shift) {
+  Statistics<kNorm, kQ8> s;
   each(s);
   RowSums v = join_row<kNorm, kQ8>(s.sums(), a.row_warps, red);
-  down = 1.f;
-  float eps = a.eps;
-  if (kNorm && (magnitude(v.squares) >= kInfBits || (kQ8 && v.top >= kInfBits))) {
+  float down = 1.f, eps = a.eps;
+  if (kNorm && magnitude(v.squares) >= kInfBits) {
     down = kLargeDown;
     eps = eps * kLargeDown * kLargeDown;
-    Statistics<kNorm, kQ8, true> l;
+    SquaresDown l;
     each(l);
     if (a.row_warps > 1) __syncthreads();      // red is read no more
-    v = join_row<kNorm, kQ8>(l.sums(), a.row_warps, red);
+    v.squares = join_row<true, false>(l.sums(), a.row_warps, red).squares;
   }
   rstd = kNorm ? rsqrtf(fmaf(v.squares, a.inv_dim, eps)) * down : 1.f;      // to 2 units in the last place
+  shift = 0;
+  if (kNorm && kQ8 && (v.top >= kInfBits || v.top < __float_as_uint(kSmall))) {
+    shift = v.top >= kInfBits ? -144 : 200;
+    TopShifted l = {shift};
+    each(l);
+    if (a.row_warps > 1) __syncthreads();
+    v.top = join_row<false, true>(l.sums(), a.row_warps, red).top;
+  }
   top = __uint_as_float(v.top);
   // an infinity makes r zero: what it leaves is not a number
   if (kNorm && kQ8 && magnitude(v.squares) >= kInfBits) top = __uint_as_float(0x7fffffffu);
@@ -160,7 +205,7 @@ __device__ __forceinline__ void row_statistics(const NormArgs& a, Joined& red, F
 // and it is taken in 64 bits, p * ((1 / top) * 127), of two the even one.  That is one
 // quotient in 60000, and half-way itself is common in 16-bit rows: p = top / 2 alone is
 // one number in 700 of a normal row of bf16.  (With the fast division, off by 2^-22,
-// four times as many are taken twice: 32768 x 3584 144 us, so 139.)  Tops below 2^-100
+// four times as many are taken twice: 32768 x 3584 6 us longer.)  Tops below 2^-100
 // are taken 2^100 as large, so that 127 / top stays finite.
 constexpr float kSure = 0.5f - 8e-6f;
 struct Whole {
@@ -187,16 +232,16 @@ struct Whole {
     return static_cast<uint32_t>(__double2int_rn(static_cast<double>(p) * by));
   }
   // A pair that may be nearer to half-way than fp32 tells.
-  __device__ __forceinline__ uint2 nearest(float2 p, double by) const {
+  template <bool kPlain> __device__ __forceinline__ uint2 nearest(float2 p, double by) const {
     float far = 0.f;
-    uint2 n = near<false>(p, far);
+    uint2 n = near<kPlain>(p, far);
     if (far > kSure) n = make_uint2(decided(p.x, by), decided(p.y, by));
     return n;
   }
   __device__ __forceinline__ uint2 nearest(float2 p) const {
     float far = 0.f;
     const uint2 n = near<false>(p, far);
-    return far > kSure ? nearest(p, quotient(top)) : n;
+    return far > kSure ? nearest<false>(p, quotient(top)) : n;
   }
 };
 
@@ -227,10 +272,10 @@ template <typename T> __device__ __forceinline__ bool take_side(Whole& whole, co
   return true;
 }
 
-// (Small tops times r first: their quotients may be below the smallest normal number.)
-__device__ __forceinline__ float scale_of(float top, float rstd) {
+__device__ __forceinline__ float scale_of(float top, float rstd, int shift) {
   if (magnitude(top) >= kInfBits) return __uint_as_float(0x7fffffffu);
-  return top < kSmall ? top * rstd / 127.f : top / 127.f * rstd;
+  if (shift != 0) return static_cast<float>(static_cast<double>(top) * power(-shift) * static_cast<double>(rstd) / 127.0);
+  return top / 127.f * rstd;
 }
 
 // The low bytes of n.
@@ -254,21 +299,20 @@ template <int V> __device__ __forceinline__ void set_two(uint32_t (&n)[V], int p
 
 // A pair of h w (or of the row itself).
 template <typename T, int V, bool kNorm, bool kPlain>
-__device__ __forceinline__ float2 product_of(const Elements<T, V>& h, const Elements<T, V>& w, int p, float down) {
-  float2 f = pair_of(h, p);
-  if (!kPlain) f = fmul2(f, make_float2(down, down));
-  return kNorm ? fmul2(f, pair_of(w, p)) : f;
+__device__ __forceinline__ float2 product_of(const Elements<T, V>& h, const Elements<T, V>& w, int p, int shift) {
+  if (!kNorm) return pair_of(h, p);
+  return kPlain || shift == 0 ? fmul2(pair_of(h, p), pair_of(w, p)) : products(pair_of(h, p), pair_of(w, p), shift);
 }
 // What a row's thread writes of vector v (elements v V on) once the statistics are
 // known; kPlain: neither the row nor its top was scaled (whole numbers).
 template <typename T, int V, bool kNorm, bool kQ8, bool kPlain, bool kCount = true>
 __device__ __forceinline__ void write_vector(const NormArgs& a, int64_t row, int v, const Elements<T, V>& h,
-                                             const Elements<T, V>& w, float rstd, float down, const Whole& whole, float& far) {
+                                             const Elements<T, V>& w, float rstd, int shift, const Whole& whole, float& far) {
   if constexpr (kQ8) {
     uint32_t n[V];
 #pragma unroll
     for (int p = 0; p < (V + 1) / 2; ++p)
-      set_two<V>(n, p, whole.template near<kPlain, kCount>(product_of<T, V, kNorm, kPlain>(h, w, p, down), far));
+      set_two<V>(n, p, whole.template near<kPlain, kCount>(product_of<T, V, kNorm, kPlain>(h, w, p, shift), far));
     store_whole<V>(a.q + row * a.q_stride + static_cast<int64_t>(v) * V, n, whole.keep);
   } else {
     Elements<T, V> o;
@@ -278,51 +322,51 @@ __device__ __forceinline__ void write_vector(const NormArgs& a, int64_t row, int
   }
 }
 // Its whole numbers once more, where a quotient was too near to half-way.
-template <typename T, int V, bool kNorm>
+template <typename T, int V, bool kNorm, bool kPlain>
 __device__ __forceinline__ void write_nearest(const NormArgs& a, int64_t row, int v, const Elements<T, V>& h,
-                                              const Elements<T, V>& w, float down, const Whole& whole, double by) {
+                                              const Elements<T, V>& w, int shift, const Whole& whole, double quotient) {
   uint32_t n[V];
 #pragma unroll
-  for (int p = 0; p < (V + 1) / 2; ++p) set_two<V>(n, p, whole.nearest(product_of<T, V, kNorm, false>(h, w, p, down), by));
+  for (int p = 0; p < (V + 1) / 2; ++p)
+    set_two<V>(n, p, whole.template nearest<kPlain>(product_of<T, V, kNorm, kPlain>(h, w, p, shift), quotient));
   store_whole<V>(a.q + row * a.q_stride + static_cast<int64_t>(v) * V, n, whole.keep);
+}
+// (Looking twice has a form of its own without the products in 64 bits: with them in
+// it, a path that one row in ten takes, 32768 x 3584 in 8 bits takes 145 us, so 142.)
+template <typename T, int V, int kPer, bool kNorm, bool kQ8, bool kPlain, bool kCount>
+__device__ __forceinline__ void write_vectors(const NormArgs& a, int64_t row, int t, int team, const Elements<T, V> (&h)[kPer],
+                                              const Elements<T, V>* weight, float rstd, int shift, const Whole& whole) {
+  const int vecs = a.dim / V;
+  float far = 0.f;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i)
+    if (t + i * team < vecs)
+      write_vector<T, V, kNorm, kQ8, kPlain, kCount>(a, row, t + i * team, h[i], kNorm ? weight[t + i * team] : h[i], rstd, shift,
+                                                     whole, far);
+  if (kQ8 && kCount && far > kSure) {
+    const double quotient = Whole::quotient(whole.top);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (t + i * team < vecs)
+        write_nearest<T, V, kNorm, kPlain>(a, row, t + i * team, h[i], kNorm ? weight[t + i * team] : h[i], shift, whole, quotient);
+  }
 }
 // `sides`: those of set_sides, or none.
 template <typename T, int V, int kPer, bool kNorm, bool kQ8>
 __device__ __forceinline__ void write_row(const NormArgs& a, int64_t row, int t, int team, const Elements<T, V> (&h)[kPer],
-                                          const Elements<T, V>* weight, float rstd, float down, float top,
+                                          const Elements<T, V>* weight, float rstd, int shift, float top,
                                           const unsigned char* sides = nullptr) {
-  const int vecs = a.dim / V;
   Whole whole(kQ8 ? top : 0.f);
-  float far = 0.f;
   const bool halves = kQ8 && !kNorm && sizeof(T) == 2 && sides != nullptr;
-  if (halves && take_side<T>(whole, sides)) {
-#pragma unroll
-    for (int i = 0; i < kPer; ++i)
-      if (t + i * team < vecs)
-        write_vector<T, V, kNorm, kQ8, true, false>(a, row, t + i * team, h[i], h[i], rstd, down, whole, far);
-    return;
-  }
-  if (!kQ8 || (!halves && (!kNorm || down == 1.f) && whole.up == 1.f)) {
-#pragma unroll
-    for (int i = 0; i < kPer; ++i)
-      if (t + i * team < vecs)
-        write_vector<T, V, kNorm, kQ8, true>(a, row, t + i * team, h[i], kNorm ? weight[t + i * team] : h[i], rstd, down, whole, far);
-  } else {
-#pragma unroll
-    for (int i = 0; i < kPer; ++i)
-      if (t + i * team < vecs)
-        write_vector<T, V, kNorm, kQ8, false>(a, row, t + i * team, h[i], kNorm ? weight[t + i * team] : h[i], rstd, down, whole, far);
-  }
-  if (kQ8 && far > kSure) {
-    const double by = Whole::quotient(top);
-#pragma unroll
-    for (int i = 0; i < kPer; ++i)
-      if (t + i * team < vecs)
-        write_nearest<T, V, kNorm>(a, row, t + i * team, h[i], kNorm ? weight[t + i * team] : h[i], down, whole, by);
-  }
+  if (halves && take_side<T>(whole, sides))
+    write_vectors<T, V, kPer, kNorm, kQ8, true, false>(a, row, t, team, h, weight, rstd, shift, whole);
+  else if (!kQ8 || (!halves && (!kNorm || shift == 0) && whole.up == 1.f))
+    write_vectors<T, V, kPer, kNorm, kQ8, true, true>(a, row, t, team, h, weight, rstd, shift, whole);
+  else
+    write_vectors<T, V, kPer, kNorm, kQ8, false, true>(a, row, t, team, h, weight, rstd, shift, whole);
 }
-template <bool kQ8> __device__ __forceinline__ void write_statistics(const NormArgs& a, int64_t row, float rstd, float down, float top) {
-  if (kQ8) a.scale[row] = scale_of(top, rstd * (1.f / down));
+template <bool kQ8> __device__ __forceinline__ void write_statistics(const NormArgs& a, int64_t row, float rstd, int shift, float top) {
+  if (kQ8) a.scale[row] = scale_of(top, rstd, shift);
   else if (a.rstd != nullptr) a.rstd[row] = rstd;
 }
 
@@ -387,20 +431,26 @@ __global__ void __launch_bounds__(N_MAX_THREADS) norm_kernel(const NormArgs a) {
       reinterpret_cast<Vec*>(static_cast<T*>(a.h) + row * a.dim)[v] = h[i];
     }
   }
-  float rstd, top, down;
+  float rstd, top;
+  int shift;
   row_statistics<kNorm, kQ8>(a, red, [&](auto& s) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) s.add(h[i], w[i]);
-  }, rstd, top, down);
+  }, rstd, top, shift);
   if constexpr (kPer == 1) {
     const Whole whole(kQ8 ? top : 0.f);
-    float far = 0.f;
-    if (t < vecs) write_vector<T, V, kNorm, kQ8, false>(a, row, t, h[0], w[0], rstd, down, whole, far);
-    if (kQ8 && far > kSure) write_nearest<T, V, kNorm>(a, row, t, h[0], w[0], down, whole, Whole::quotient(top));
+    auto write = [&](auto plain) {
+      constexpr bool kPlain = decltype(plain)::value;
+      float far = 0.f;
+      if (t < vecs) write_vector<T, V, kNorm, kQ8, kPlain>(a, row, t, h[0], w[0], rstd, shift, whole, far);
+      if (kQ8 && far > kSure) write_nearest<T, V, kNorm, kPlain>(a, row, t, h[0], w[0], shift, whole, Whole::quotient(top));
+    };
+    if (!kQ8 || (shift == 0 && whole.up == 1.f)) write(std::true_type());
+    else write(std::false_type());
   } else {
-    write_row<T, V, kPer, kNorm, kQ8>(a, row, t, team, h, static_cast<const Vec*>(a.weight), rstd, down, top);
+    write_row<T, V, kPer, kNorm, kQ8>(a, row, t, team, h, static_cast<const Vec*>(a.weight), rstd, shift, top);
   }
-  if (t == 0) write_statistics<kQ8>(a, row, rstd, down, top);
+  if (t == 0) write_statistics<kQ8>(a, row, rstd, shift, top);
 }
 
 // Rows of 16-bit elements at any address: the aligned words inside a row, a word to a
@@ -462,19 +512,18 @@ __global__ void __launch_bounds__(N_MAX_THREADS) norm_words_kernel(const NormArg
     add_to<T, 2>(h[kPer], r[kPer]);
     at.set_ends(out, t, h[kPer]);
   }
-  float rstd, top, down;
+  float rstd, top;
+  int shift;
   row_statistics<kNorm, kQ8>(a, red, [&](auto& s) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
       if (t + i * team < at.count) s.add(h[i], kNorm && kQ8 ? at.any(weight, t + i * team) : h[i]);
     s.add(h[kPer], kNorm && kQ8 ? at.ends(weight, t) : h[kPer]);
-  }, rstd, top, down);
+  }, rstd, top, shift);
   const Whole whole(kQ8 ? top : 0.f);
   auto result = [&](const Two& v, const Two& w) {
-    const float by = kQ8 ? down : rstd;
-    float2 f = fmul2(pair_of(v, 0), make_float2(by, by));
-    if (kNorm) f = fmul2(f, pair_of(w, 0));
-    return f;
+    if (kQ8) return product_of<T, 2, kNorm, false>(v, w, 0, shift);
+    return fmul2(fmul2(pair_of(v, 0), make_float2(rstd, rstd)), pair_of(w, 0));
   };
   auto byte = [&](uint32_t n) { return static_cast<int8_t>(n & whole.keep); };
   T* y = static_cast<T*>(a.y) + row * a.dim;
@@ -503,7 +552,7 @@ __global__ void __launch_bounds__(N_MAX_THREADS) norm_words_kernel(const NormArg
     set_pair(o, 0, f);
     at.set_ends(y, t, o);
   }
-  if (t == 0) write_statistics<kQ8>(a, row, rstd, down, top);
+  if (t == 0) write_statistics<kQ8>(a, row, rstd, shift, top);
 }
 
 // The same for rows on 16-byte boundaries, a CTA's (or warp's) rows a grid apart:
@@ -511,7 +560,7 @@ __global__ void __launch_bounds__(N_MAX_THREADS) norm_words_kernel(const NormArg
 // rows ahead, so that loads are always in flight while a row is summed up and
 // written.  Nobody else reads a thread's slots, so its own wait is enough.
 template <typename T, int kPer, bool kNorm, bool kQ8>
-__global__ void __launch_bounds__(ring_threads(kPer), ring_ctas(kPer)) norm_ring_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(kPer == 1 ? 32 * N_SHORT_ROWS : ring_threads(kPer), ring_ctas(kPer, kQ8 && !kNorm)) norm_ring_kernel(const NormArgs a) {
   constexpr int V = 16 / sizeof(T);
   using Vec = Elements<T, V>;
   extern __shared__ __align__(16) unsigned char slots[];
@@ -573,14 +622,15 @@ __global__ void __launch_bounds__(ring_threads(kPer), ring_ctas(kPer)) norm_ring
     }
     ask(row + kAhead * step, s);
     if (++s == kAhead) s = 0;
-    float rstd, top, down;
+    float rstd, top;
+  int shift;
     row_statistics<kNorm, kQ8>(a, red[turn], [&](auto& s) {
 #pragma unroll
       for (int i = 0; i < kPer; ++i)
         if (t + i * team < vecs) s.add(h[i], kNorm && kQ8 ? weight[t + i * team] : h[i]);
-    }, rstd, top, down);
-    write_row<T, V, kPer, kNorm, kQ8>(a, row, t, team, h, weight, rstd, down, top, kSides ? sides : nullptr);
-    if (t == 0) write_statistics<kQ8>(a, row, rstd, down, top);
+    }, rstd, top, shift);
+    write_row<T, V, kPer, kNorm, kQ8>(a, row, t, team, h, weight, rstd, shift, top, kSides ? sides : nullptr);
+    if (t == 0) write_statistics<kQ8>(a, row, rstd, shift, top);
   }
 }
 
@@ -598,22 +648,23 @@ __global__ void __launch_bounds__(N_MAX_THREADS) norm_wide_kernel(const NormArgs
     const T v = x[i];
     return res != nullptr ? from_float<T>(to_float(v) + to_float(res[i])) : v;
   };
-  float rstd, top, down;
+  float rstd, top;
+  int shift;
   row_statistics<kNorm, kQ8>(a, red, [&](auto& s) {
     for (int i = threadIdx.x; i < a.dim; i += N_MAX_THREADS) {
       const Elements<T, 1> h = {h_at(i)}, w = {kNorm && kQ8 ? weight[i] : from_float<T>(0.f)};
       s.add(h, w);
     }
-  }, rstd, top, down);
+  }, rstd, top, shift);
   const Whole whole(top);
   for (int i = threadIdx.x; i < a.dim; i += N_MAX_THREADS) {
     const T h = h_at(i);
-    const float f = to_float(h) * (kQ8 ? down : rstd), w = kNorm ? to_float(weight[i]) : 1.f;
+    const Elements<T, 1> one = {h}, w = {kNorm ? weight[i] : h};
     if (kNorm && res != nullptr) static_cast<T*>(a.h)[row * a.dim + i] = h;
-    if (kQ8) a.q[row * a.q_stride + i] = static_cast<int8_t>(whole.nearest(make_float2(kNorm ? f * w : f, 0.f)).x & whole.keep);
-    else static_cast<T*>(a.y)[row * a.dim + i] = from_float<T>(f * w);
+    if (kQ8) a.q[row * a.q_stride + i] = static_cast<int8_t>(whole.nearest(product_of<T, 1, kNorm, false>(one, w, 0, shift)).x & whole.keep);
+    else static_cast<T*>(a.y)[row * a.dim + i] = from_float<T>(to_float(h) * rstd * to_float(w.e[0]));
   }
-  if (threadIdx.x == 0) write_statistics<kQ8>(a, row, rstd, down, top);
+  if (threadIdx.x == 0) write_statistics<kQ8>(a, row, rstd, shift, top);
 }
 
 // ------------------------------------------------------------ gradient

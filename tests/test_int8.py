@@ -113,6 +113,28 @@ def test_rows_of_any_size(mrsa, cuda_device, rows, dim, size):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 999, 5000, 18944, 40000])
+@pytest.mark.parametrize("rows", [6, 400])
+@pytest.mark.parametrize("kind", ["bf16", "fp32"])
+def test_products_of_any_size(mrsa, cuda_device, rows, dim, kind):
+    """Rows and weights whose products are past fp32's largest number, below its smallest normal one, or
+    both in turn, while the norm itself is not."""
+    dev, dtype = cuda_device, TYPES[kind]
+    g = torch.Generator(device=dev).manual_seed(13)
+    x = torch.randn(rows, dim, device=dev, generator=g).clamp(-3.9, 3.9)
+    w = torch.rand(dim, device=dev, generator=g) + 0.5
+    w[torch.rand(dim, device=dev, generator=g) < 0.1] = 0
+    sizes = torch.tensor([2.0 ** -140, 2.0 ** -75, 2.0 ** -20, 1.0, 2.0 ** 70, 2.0 ** 125], device=dev, dtype=torch.float64)
+    for size in (2.0 ** -130, 2.0 ** -60, 2.0 ** 40, 2.0 ** 126):
+        for eps in (1e-6, 1e-12):
+            h = (x.double() * sizes[torch.arange(rows, device=dev) % 6, None]).to(dtype)
+            b = (w.double() * size).to(dtype)
+            q, scale, _ = mrsa.add_rms_norm_int8(h, None, b, eps)
+            p = h.double() * b.double()
+            check_whole(q, scale, p, p.abs().amax(-1) / 127 / (h.double().square().mean(-1) + eps).sqrt(), 5e-6)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dim", [64, 999])
 def test_extreme_rows(mrsa, cuda_device, dim):
     dev = cuda_device
