@@ -168,8 +168,8 @@ class DreamForward:
         return linear(x, self.lm_head) if logits else x
 
     def layer(self, idx, x, position_ids, key_valid):
-        q, k, v, h, x = self.enter(idx, x)
-        return self.leave(idx, self.attend(idx, q, k, v, h, position_ids, key_valid), x)
+        h = self.rms_norm(x, self.layers[idx]["in_norm"])
+        return self.leave(idx, self.attention(idx, h, position_ids, key_valid), x)
 
     @torch.inference_mode()
     def forward(self, ids, position_ids, key_valid=None, *, logits: bool = True, return_layer_inputs=False):

@@ -71,6 +71,10 @@ class DreamInt8(DreamForward):
             q, k, v = self._split(idx, q8, scale)
         return q, k, v, h, x
 
+    def layer(self, idx, x, position_ids, key_valid):
+        q, k, v, h, x = self.enter(idx, x)
+        return self.leave(idx, self.attend(idx, q, k, v, h, position_ids, key_valid), x)
+
     def leave(self, idx, o, x):
         lay = self.layers[idx]
         delta = linear_int8(*quantize_int8(o), *lay["wo"])
