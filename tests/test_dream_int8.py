@@ -141,3 +141,55 @@ def test_forward_with_route_layers(models, mrsa, cuda_device):
     cos = F.cosine_similarity(logits.float().flatten(), model(ids, pos).float().flatten(), dim=0)
     assert cos > 0.99, float(cos)
     assert "wq" not in m.layers[0] and m.embed is model.embed
+
+
+def test_norm_weights_by_layer(mrsa, cuda_device):
+    """Norm weights of their own for every norm: each where it belongs, in the forward and over pages."""
+    from mrsa_b200.dream_forward import DreamConfig, DreamForward
+    from mrsa_b200.paged_decode import PagedDream
+
+    dev = cuda_device
+    cfg = DreamConfig(layers=4, hidden=896, ffn=1024, q_heads=7, kv_heads=1, vocab=520, swa_window=300)
+    model = DreamForward(cfg, seed=5, device=dev)
+    g = torch.Generator(device=dev).manual_seed(6)
+    for where, k in [(lay, k) for lay in model.layers for k in ("in_norm", "post_norm")] + [(vars(model), "final_norm")]:
+        where[k] = (torch.rand(cfg.hidden, device=dev, generator=g) * 2 + 0.2).bfloat16()
+    m = mrsa.DreamInt8(model)
+    ids = torch.randint(0, 520, (1, 512), device=dev, generator=g)
+    pos = torch.arange(512, device=dev)[None]
+    lmk = (pos[0] + 1) % cfg.chunk == 0
+
+    def layer(i, delta, x, attention):
+        """The layer by the public operators; attention(q, k, v, normed input)."""
+        h, x = mrsa.add_rms_norm(delta, x, model.layers[i]["in_norm"], cfg.rms_eps)
+        q8 = mrsa.quantize_int8(h) if "route" in model.layers[i] else None
+        if q8 is None:
+            q8 = mrsa.add_rms_norm_int8(x, None, model.layers[i]["in_norm"], cfg.rms_eps)[:2]
+        qkv = mrsa.linear_int8(*q8, *m.layers[i]["wqkv"], m.layers[i]["bqkv"]).view(1, 512, 9, 128)
+        o = attention(i, qkv[:, :, :7], qkv[:, :, 7:8], qkv[:, :, 8:], h)
+        delta = mrsa.linear_int8(*mrsa.quantize_int8(o), *m.layers[i]["wo"])
+        q8, s8, x = mrsa.add_rms_norm_int8(delta, x, model.layers[i]["post_norm"], cfg.rms_eps)
+        return mrsa.linear_int8(*mrsa.quantize_int8(mrsa.swiglu_int8(q8, s8, *m.layers[i]["wgu"])), *m.layers[i]["wd"]), x
+
+    def model_by(first, attention):
+        delta, x = first, None
+        for i in range(cfg.layers):
+            delta, x = layer(i, delta, x, attention)
+        q8, s8, _ = mrsa.add_rms_norm_int8(delta, x, model.final_norm, cfg.rms_eps)
+        return mrsa.linear_int8(q8, s8, *m.lm_head), mrsa.add_rms_norm(delta, x, model.final_norm, cfg.rms_eps)[0]
+
+    with torch.inference_mode():
+        first = torch.where(lmk[None, :, None], m.embed[ids] + m.role, m.embed[ids])
+        logits, hidden = model_by(first, lambda i, q, k, v, h: m.attend(i, q, k, v, h, pos, None))
+        assert torch.equal(m(ids, pos), logits) and torch.equal(m(ids, pos, logits=False), hidden)
+        # over pages: the model's own cache holds what the steps append to theirs
+        dec, own = (PagedDream(m, pages=12, sequences=2, max_len=512) for _ in range(2))
+        got = dec.prefill(dec.cache.seqs(0), ids)
+        seqs = own.cache.seqs(0)
+        own.cache.extend(seqs, 512)
+
+        def paged(i, q, k, v, h):
+            q = own.cache.append(i, seqs, k, v, q=q, inv_freq=m.inv_freq, attention_factor=m.attention_factor)
+            return own.cache.attend(i, seqs, q).reshape(1, 512, -1)
+
+        assert torch.equal(model_by(m.embed[ids], paged)[0], got)

@@ -118,6 +118,19 @@ def test_gradient_does_not_depend_on_calls_before(cuda_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind,rows,dim", [("fp32", 950, 18944), ("bf16", 950, 24000), ("bf16", 900, 9001)])
+def test_gradient_of_many_wide_rows(mrsa, cuda_device, kind, rows, dim):
+    """Past the registers, more rows than CTAs: parts of dw that take several rows each."""
+    dtype = TYPES[kind]
+    x, r, w, gy, gh = make(cuda_device, rows, dim, dtype, 10)
+    for t in (x, r, w):
+        t.requires_grad_()
+    y, h = mrsa.add_rms_norm(x, r, w, EPS)
+    dx, dw = torch.autograd.grad((y, h), (x, w), (gy, gh))
+    check_gradient((dx, dw), gy, gh, h.detach(), w.detach(), dtype)
+
+
+@pytest.mark.gpu
 def test_gradient_against_differences(mrsa, cuda_device):
     x, r, w, gy, gh = make(cuda_device, 5, 48, torch.float32, 2)
     for t in (x, r, w):
