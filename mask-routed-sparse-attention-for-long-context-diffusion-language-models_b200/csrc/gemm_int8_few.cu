@@ -178,6 +178,7 @@ __global__ void __launch_bounds__(F_THREADS, kPerSm) gemm_int8_few_kernel(const 
   }
   // The last MMA done: the copies have landed and been read, and their memory takes the sums.
   const bool ok = tc::wait_bounded_warp(tc::smem_addr(&sm.done), 0, ab);
+  if (!ok && warp == 1 && half == 0) tc::mbar_wait(tc::smem_addr(&sm.done), 0);      // the MMAs of a CTA that gives up end first
   tc::fence_after_sync();
   __syncthreads();                       // (an aborted CTA's producer has seen its copies land)
   int* sums = reinterpret_cast<int*>(sm.tiles);
