@@ -23,10 +23,13 @@
 // every run gives the same bits.
 //
 // Measured (B200, bf16, us, and of the 6.55 TB/s of a copy): 16384 x 3584 norm with
-// residual 85 (84 %; 96 with a CTA per row and loads in registers), without 45
-// (79 %), with its gradient 160 (90 %; 248); 32768 x 3584 in 8 bits 142 (88 %; 192);
+// residual 84 (85 %; 96 with a CTA per row and loads in registers), without 44
+// (82 %), with its gradient 160 (90 %; 248); 32768 x 3584 in 8 bits 142 (88 %; 192);
 // 16384 x 18944 quantized 175 (81 %; 312).  Rows off 16-byte boundaries go by
-// words: 4095 x 3585 36 (49 %), with gradient 84 (43 %), fp32 4095 x 2561 86 (60 %).
+// words: 4095 x 3585 36 (50 %), with gradient 83 (43 %), fp32 4095 x 2561 with gradient
+// 85 (60 %).  fp32 on boundaries: 4096 x 3584 42 (86 %), with gradient 83 (87 %), in 8
+// bits 32.  Rows past the registers, an element at a time: 4095 x 18944 fp32 345 (55 %),
+// with gradient 1006 (38 %), 25 of them 14 and 40.
 #include "common.cuh"
 #include "elements.cuh"
 
@@ -251,11 +254,16 @@ struct Whole {
 // 127 divides the significand, 127 / top taken 2^-21 too large or too small, to the
 // side where 64 bits put top / 2, gives every whole number; and if it is 127 (times a
 // power of two), 127 / top is a power of two, and the fma rounds the quotient itself.
-// All this goes by the significand alone: a CTA of many rows works it out for all of
-// them while its first rows are on their way.
+// All this goes by the significand alone: a CTA works it out for all of them while its
+// first rows are on their way, or the launch before it ends.  (One row of 18944 2.1 us,
+// 3.4 without; 16384 of them 175 and 229.  Rows by words do without: 4095 x 3585 25.2
+// us, with their own row's side found by every thread 26.3.)
 enum Side : unsigned char { kBelow, kAbove, kExact, kUnsure };
 template <typename T> constexpr int SIDES = std::is_same_v<T, __half> ? 1024 : 128;
-template <typename T> __device__ __forceinline__ void set_sides(unsigned char* sides) {
+template <typename T> __device__ __forceinline__ int digits_of(float top) {
+  return static_cast<int>((__float_as_uint(top) & 0x7fffffu) / (0x800000u / SIDES<T>));       // less SIDES
+}
+template <typename T> __device__ __forceinline__ void set_sides(Side* sides) {
   for (int i = threadIdx.x; i < SIDES<T>; i += blockDim.x) {
     const int digits = SIDES<T> + i;
     const float top = static_cast<float>(digits);
@@ -264,8 +272,7 @@ template <typename T> __device__ __forceinline__ void set_sides(unsigned char* s
   }
 }
 // Whether `whole` is now such that no quotient has to be looked at twice.
-template <typename T> __device__ __forceinline__ bool take_side(Whole& whole, const unsigned char* sides) {
-  const unsigned char side = sides[(__float_as_uint(whole.top) & 0x7fffffu) / (0x800000u / SIDES<T>)];
+__device__ __forceinline__ bool take_side(Whole& whole, Side side) {
   if (side == kUnsure || whole.up != 1.f) return false;
   if (side == kExact) whole.inv = __uint_as_float((__float_as_uint(whole.inv) + 0x400000u) & 0x7f800000u);
   else whole.inv *= side == kAbove ? 1.f + 0x1p-21f : 1.f - 0x1p-21f;
@@ -355,10 +362,10 @@ __device__ __forceinline__ void write_vectors(const NormArgs& a, int64_t row, in
 template <typename T, int V, int kPer, bool kNorm, bool kQ8>
 __device__ __forceinline__ void write_row(const NormArgs& a, int64_t row, int t, int team, const Elements<T, V> (&h)[kPer],
                                           const Elements<T, V>* weight, float rstd, int shift, float top,
-                                          const unsigned char* sides = nullptr) {
+                                          const Side* sides = nullptr) {
   Whole whole(kQ8 ? top : 0.f);
   const bool halves = kQ8 && !kNorm && sizeof(T) == 2 && sides != nullptr;
-  if (halves && take_side<T>(whole, sides))
+  if (halves && take_side(whole, sides[digits_of<T>(top)]))
     write_vectors<T, V, kPer, kNorm, kQ8, true, false>(a, row, t, team, h, weight, rstd, shift, whole);
   else if (!kQ8 || (!halves && (!kNorm || shift == 0) && whole.up == 1.f))
     write_vectors<T, V, kPer, kNorm, kQ8, true, true>(a, row, t, team, h, weight, rstd, shift, whole);
@@ -391,9 +398,12 @@ __device__ __forceinline__ void add_to(Elements<T, V>& h, const Elements<T, V>& 
 template <typename T, int V, int kPer, bool kNorm, bool kQ8>
 __global__ void __launch_bounds__(N_MAX_THREADS) norm_kernel(const NormArgs a) {
   using Vec = Elements<T, V>;
+  constexpr bool kSides = kQ8 && !kNorm && sizeof(T) == 2 && V > 1;
   __shared__ Joined red;
-  if (a.row_warps > 1) {
+  __shared__ Side sides[kSides ? SIDES<T> : 1];
+  if (kSides || a.row_warps > 1) {
     clear(&red, 1);
+    if (kSides) set_sides<T>(sides);
     __syncthreads();
   }
   chain_wait();
@@ -413,6 +423,7 @@ __global__ void __launch_bounds__(N_MAX_THREADS) norm_kernel(const NormArgs a) {
     if (v < vecs) h[i] = x[v];
   }
   // with more vectors to a thread the norm reads its weights where it uses them: held they spill
+  // (in 8 bits they are used twice, and held although some spill)
   if (kNorm && (kQ8 || kPer == 1)) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
@@ -438,17 +449,19 @@ __global__ void __launch_bounds__(N_MAX_THREADS) norm_kernel(const NormArgs a) {
     for (int i = 0; i < kPer; ++i) s.add(h[i], w[i]);
   }, rstd, top, shift);
   if constexpr (kPer == 1) {
-    const Whole whole(kQ8 ? top : 0.f);
-    auto write = [&](auto plain) {
-      constexpr bool kPlain = decltype(plain)::value;
+    Whole whole(kQ8 ? top : 0.f);
+    auto write = [&](auto plain, auto count) {
+      constexpr bool kPlain = decltype(plain)::value, kCount = decltype(count)::value;
       float far = 0.f;
-      if (t < vecs) write_vector<T, V, kNorm, kQ8, kPlain>(a, row, t, h[0], w[0], rstd, shift, whole, far);
-      if (kQ8 && far > kSure) write_nearest<T, V, kNorm, kPlain>(a, row, t, h[0], w[0], shift, whole, Whole::quotient(top));
+      if (t < vecs) write_vector<T, V, kNorm, kQ8, kPlain, kCount>(a, row, t, h[0], w[0], rstd, shift, whole, far);
+      if (kQ8 && kCount && far > kSure)
+        write_nearest<T, V, kNorm, kPlain>(a, row, t, h[0], w[0], shift, whole, Whole::quotient(top));
     };
-    if (!kQ8 || (shift == 0 && whole.up == 1.f)) write(std::true_type());
-    else write(std::false_type());
+    if (kSides && take_side(whole, sides[kSides ? digits_of<T>(top) : 0])) write(std::true_type(), std::false_type());
+    else if (!kQ8 || (!kSides && shift == 0 && whole.up == 1.f)) write(std::true_type(), std::true_type());
+    else write(std::false_type(), std::true_type());
   } else {
-    write_row<T, V, kPer, kNorm, kQ8>(a, row, t, team, h, static_cast<const Vec*>(a.weight), rstd, shift, top);
+    write_row<T, V, kPer, kNorm, kQ8>(a, row, t, team, h, static_cast<const Vec*>(a.weight), rstd, shift, top, kSides ? sides : nullptr);
   }
   if (t == 0) write_statistics<kQ8>(a, row, rstd, shift, top);
 }
@@ -566,7 +579,7 @@ __global__ void __launch_bounds__(kPer == 1 ? 32 * N_SHORT_ROWS : ring_threads(k
   extern __shared__ __align__(16) unsigned char slots[];
   __shared__ Joined red[2];                    // in turn: a row's are read until the next row's barrier
   constexpr bool kSides = kQ8 && !kNorm && sizeof(T) == 2;
-  __shared__ unsigned char sides[kSides ? SIDES<T> : 1];
+  __shared__ Side sides[kSides ? SIDES<T> : 1];
   if (a.row_warps > 1) {
     clear(red, 2);
     __syncthreads();
@@ -1022,14 +1035,14 @@ int norm_of(const NormArgs& a, cudaStream_t s) {
   if (wide && vecs <= 4 * N_MAX_THREADS) {
     // No row behind another on an SM: straight to registers, with as many threads as
     // there are vectors (one row of 3584: 1.6 us, by the copies ahead 2.3; 18944
-    // quantized 1.9 and 2.4).
+    // quantized 2.1 and 2.7).
     if (a.rows <= sm_count()) {
       if (vecs <= N_MAX_THREADS) return launch_norm<T, V, 1, kNorm, kQ8>(a, s);
       return launch_norm<T, V, 4, kNorm, kQ8>(a, s);
     }
     // Four vectors to a thread (a warp to a row of up to 1024 elements of 16 bits), two
-    // where the rows would leave SMs short of warps (256 rows of 3584 in 8 bits 3.2 us,
-    // with four 4.3; 32768 rows 139, with four 135; before quotients were looked at twice), one for rows of a warp, eight past
+    // where the rows would leave SMs short of warps (256 rows of 3584 in 8 bits 4.5 us,
+    // with four 5.2; 32768 rows 167, with four 142), one for rows of a warp, eight past
     // 640 threads.
     if (vecs <= 32) return launch_ring<T, 1, kNorm, kQ8>(a, s);
     if (vecs <= 64 || (vecs <= 1024 && a.rows <= 4 * sm_count())) return launch_ring<T, 2, kNorm, kQ8>(a, s);
@@ -1045,7 +1058,7 @@ int norm_of(const NormArgs& a, cudaStream_t s) {
       return launch_words<T, 8, kNorm, kQ8>(a, s);
     }
   }
-  // (4095 x 2561 fp32: norm 35 us by eight elements a thread, 40 by sixteen; quantized 22 and 15)
+  // (4095 x 2561 fp32: norm 35 us by eight elements a thread, 40 by sixteen; quantized 25 and 19)
   if (a.dim <= 1024) return launch_norm<T, 1, 4, kNorm, kQ8>(a, s);
   if (kNorm && a.dim <= 4096) return launch_norm<T, 1, 8, kNorm, kQ8>(a, s);
   if (a.dim <= 16 * N_MAX_THREADS) return launch_norm<T, 1, 16, kNorm, kQ8>(a, s);
