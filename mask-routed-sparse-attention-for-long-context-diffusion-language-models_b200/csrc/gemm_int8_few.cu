@@ -359,7 +359,9 @@ int launch_tokens(const mrsa_gemm_int8_args* p, const Args& a, cudaStream_t s) {
 // shared-memory traffic of tiles of 128 (which holds those up), but fewer CTAs share
 // K, and each has more to add up.  In us, tiles of 128 and pairs: K 18944, 256 tokens
 // x 3584 channels 24.0 and 21.7, 512 38.0 and 30.2, 1024 65 and 51; K 3584, 256 x 4608
-// 10.2 and 13.3, 512 11.2 and 14.9, 1024 x 3584 16.8 and 15.6.
+// 10.2 and 13.3, 512 11.2 and 14.9, 1024 x 3584 16.8 and 15.6.  (Nothing was measured
+// between 512 x 28 and 1024 x 28 K blocks, where the rule puts its bound, and the
+// channels, on which the CTAs that share K depend, are not in it.)
 template <typename T, bool kGated>
 int launch_type(const mrsa_gemm_int8_args* p, const Args& a, cudaStream_t s) {
   if (p->m <= 16) return launch_tokens<T, 16, kGated>(p, a, s);

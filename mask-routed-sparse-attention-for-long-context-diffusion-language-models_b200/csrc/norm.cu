@@ -573,7 +573,8 @@ __global__ void __launch_bounds__(N_MAX_THREADS) norm_words_kernel(const NormArg
 // rows ahead, so that loads are always in flight while a row is summed up and
 // written.  Nobody else reads a thread's slots, so its own wait is enough.
 template <typename T, int kPer, bool kNorm, bool kQ8>
-__global__ void __launch_bounds__(kPer == 1 ? 32 * N_SHORT_ROWS : ring_threads(kPer), ring_ctas(kPer, kQ8 && !kNorm)) norm_ring_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(kPer == 1 ? 32 * N_SHORT_ROWS : ring_threads(kPer), ring_ctas(kPer, kQ8 && !kNorm))
+    norm_ring_kernel(const NormArgs a) {
   constexpr int V = 16 / sizeof(T);
   using Vec = Elements<T, V>;
   extern __shared__ __align__(16) unsigned char slots[];

@@ -76,7 +76,10 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.T
     rounded to their type (bf16, fp16 or fp32), and its norm ``y = h * weight /
     sqrt(mean(h^2) + eps)`` in fp32, rounded once (:func:`rms_norm` rounds
     before the weight too).  Without a residual ``h`` is ``x`` itself.  Any
-    width and row stride; ``eps`` at least 1e-12.  Records the gradient of x,
-    residual and weight, the same bits on every run; the gradient of that
-    gradient and forward-mode tangents are refused."""
+    width and row stride; ``eps`` at least 1e-12.  The sum of squares is added up
+    in an order that goes by the number of rows (up to one to an SM, up to four,
+    more) and by alignment: a row's last bits may differ from one batch to
+    another, not from one run to the next.  Records the gradient of x, residual
+    and weight, the same bits on every run; the gradient of that gradient and
+    forward-mode tangents are refused."""
     return _lib.ext().add_rms_norm(x, residual, weight, eps)

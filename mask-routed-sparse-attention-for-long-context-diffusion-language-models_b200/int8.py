@@ -12,8 +12,10 @@ form without a pass of its own::
     q, scale, x = add_rms_norm_int8(delta, x, norm_weight, eps)
     y = linear_int8(q, scale, wq, ws, bias)
 
-The products' sums are exact, so their rows do not depend on how many a call
-has.  Forward only: each operator raises under autograd rather than lose a
+The products' sums are exact and their outputs rounded alike, so their rows do
+not depend on how many a call has; nor do quantized rows.  The scales of
+:func:`add_rms_norm_int8` do in their last bits, as :func:`add_rms_norm` says:
+a sequence's values may differ by that from one batch to another.  Forward only: each operator raises under autograd rather than lose a
 gradient.
 """
 
