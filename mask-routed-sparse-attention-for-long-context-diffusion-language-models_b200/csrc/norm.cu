@@ -25,7 +25,7 @@
 // Measured (B200, bf16, us, and of the 6.55 TB/s of a copy): 16384 x 3584 norm with
 // residual 84 (85 %; 96 with a CTA per row and loads in registers), without 44
 // (82 %), with its gradient 160 (90 %; 248); 32768 x 3584 in 8 bits 142 (88 %; 192);
-// 16384 x 18944 quantized 175 (81 %; 312).  Rows off 16-byte boundaries go by
+// 16384 x 18944 quantized 170 (84 %; 312).  Rows off 16-byte boundaries go by
 // words: 4095 x 3585 36 (50 %), with gradient 83 (43 %), fp32 4095 x 2561 with gradient
 // 85 (60 %).  fp32 on boundaries: 4096 x 3584 42 (86 %), with gradient 83 (87 %), in 8
 // bits 32.  Rows past the registers, an element at a time: 4095 x 18944 fp32 345 (55 %),
@@ -160,7 +160,10 @@ struct TopShifted {
   template <typename T, int V> __device__ __forceinline__ void add(const Elements<T, V>& h, const Elements<T, V>& w) {
 #pragma unroll
     for (int p = 0; p < (V + 1) / 2; ++p) {
-      const float2 f = products(pair_of(h, p), pair_of(w, p), shift);
+      const float2 x = pair_of(h, p);
+      // rows of zeros come this way, a batch's padding (and no weight of theirs is other than finite)
+      if (shift > 0 && x.x == 0.f && x.y == 0.f) continue;
+      const float2 f = products(x, pair_of(w, p), shift);
       top = top_of(top, f.x, f.y);
     }
   }
@@ -195,6 +198,7 @@ __device__ __forceinline__ void row_statistics(const NormArgs& a, Joined& red, F
     each(l);
     if (a.row_warps > 1) __syncthreads();
     v.top = join_row<false, true>(l.sums(), a.row_warps, red).top;
+    if (v.top == 0u) shift = 0;
   }
   top = __uint_as_float(v.top);
   // an infinity makes r zero: what it leaves is not a number
@@ -216,7 +220,7 @@ struct Whole {
   uint32_t keep;       // no bits of rows that are zeros or not numbers
   __device__ __forceinline__ explicit Whole(float t) : top(t) {
     const bool none = !(top > 0.f) || magnitude(top) >= kInfBits;
-    up = top < kSmall ? kSmallUp : 1.f;
+    up = !none && top < kSmall ? kSmallUp : 1.f;
     inv = none ? 0.f : 127.f / (top * up);
     keep = none ? 0u : 0xffffffffu;
   }
@@ -256,7 +260,7 @@ struct Whole {
 // power of two), 127 / top is a power of two, and the fma rounds the quotient itself.
 // All this goes by the significand alone: a CTA works it out for all of them while its
 // first rows are on their way, or the launch before it ends.  (One row of 18944 2.1 us,
-// 3.4 without; 16384 of them 175 and 229.  Rows by words do without: 4095 x 3585 25.2
+// 3.4 without; 16384 of them 170 and 229.  Rows by words do without: 4095 x 3585 25.2
 // us, with their own row's side found by every thread 26.3.)
 enum Side : unsigned char { kBelow, kAbove, kExact, kUnsure };
 template <typename T> constexpr int SIDES = std::is_same_v<T, __half> ? 1024 : 128;

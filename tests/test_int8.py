@@ -135,6 +135,22 @@ def test_products_of_any_size(mrsa, cuda_device, rows, dim, kind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,dim", [(3, 64), (400, 999), (400, 3584), (3, 40000)])
+def test_weights_that_are_not_finite(mrsa, cuda_device, rows, dim):
+    """A row times a weight that is not finite has no scale, a zero in its place neither; rows of zeros beside others."""
+    dev = cuda_device
+    x = torch.randn(rows, dim, device=dev, generator=torch.Generator(device=dev).manual_seed(14))
+    x[1], x[2, 5] = 0, 0
+    w = torch.ones(dim, device=dev)
+    q, scale, _ = mrsa.add_rms_norm_int8(x, None, w, 1e-6)
+    assert scale[1] == 0 and not q[1].any() and torch.equal(scale == 0, (x == 0).all(-1))
+    for bad in ("inf", "nan"):
+        w[5] = float(bad)
+        q, scale, _ = mrsa.add_rms_norm_int8(x, None, w, 1e-6)
+        assert scale.isnan().all() and not q.any()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dim", [64, 999])
 def test_extreme_rows(mrsa, cuda_device, dim):
     dev = cuda_device
